@@ -559,6 +559,101 @@ typedef struct nrl_readout_args {
 uint64_t nrl_readout_workspace_bytes(uint64_t rows, uint32_t V, uint32_t d, uint32_t flags);
 int nrl_readout_fwd(const nrl_readout_args* args, nrl_stream stream);
 
+/* ---------------------------------------------------------------------------------------------
+ * Backward of the readout: from the per-token upstreams of the log-prob and entropy terms to the
+ * gradients of the hidden states and of the weight, the [rows, V] logits and their gradient never
+ * kept. The reference's tape goes through d(logits) (log_softmax, src/tensor/activation.rs:30-35;
+ * gather, src/nn/rl.rs:134-141; entropy, src/nn/rl.rs:405-414) and two generic products
+ * (`Linear`, src/nn/linear.rs:51-58). With z = hidden · W / τ, excluded tokens at −inf, and the
+ * forward's row statistics (m, ln Z) and entropy H:
+ *   π_j = exp(z_j − m − ln Z)
+ *   ∂/∂z_j = g_logp·(1[j = token] − π_j) − g_ent·π_j·(ln π_j + H)     (0 at excluded tokens)
+ *   d_hidden = ∂/∂z · Wᵀ / τ,  d_weights = hiddenᵀ · ∂/∂z / τ.
+ * The vocabulary is taken in pieces: a piece's logits are computed again (tcgen05.mma), its ∂/∂z is
+ * written as bf16 to the workspace by that product's epilogue, and two more products read it. ∂/∂z is
+ * divided by the call's largest |upstream| before it is rounded to bf16 (2^-8 relative per entry at most, as the
+ * operands of every bf16 product) and the factor is put back in f32; all sums are f32 in a fixed order, so
+ * results are bitwise reproducible. A row whose upstreams are all 0 is not scored: nothing of it is
+ * read, it costs no products and its d_hidden is 0 (left as it is with ADD). A row the forward refused
+ * (NaN statistics) with a non-zero upstream makes its d_hidden and d_weights NaN. An upstream whose token
+ * lies outside [0, V) has no one-hot term.
+ *
+ * `hidden` may be an 8-bit checkpoint of the hidden states (NRL_READOUT_BWD_HIDDEN_I8): integers and one
+ * scale per row as nrl_i8_quantize_rows writes them. The logits are then those of values·scale (products of
+ * the exact integers, scaled in f32), normalised by the given row statistics — the forward's on the
+ * unrounded states — and d_weights is taken with values·scale.
+ *
+ * Limits as nrl_readout_fwd: d and V multiples of 8, 16-byte aligned matrices, compute capability 10.x.
+ * A product that gives up a bounded wait (an internal error) writes NaN for what it did not reach. */
+enum {
+    /* NRL_READOUT_W_VD, NRL_READOUT_ROUND_BF16 and NRL_READOUT_MASK_BITS as in the forward call, and */
+    NRL_READOUT_BWD_HIDDEN_I8 = 1u << 8,      /* `hidden` is int8 [rows, hidden_pitch] with `hidden_scales` */
+    NRL_READOUT_BWD_D_HIDDEN_F32 = 1u << 9,   /* d_hidden is f32 instead of bf16 */
+    NRL_READOUT_BWD_D_WEIGHTS_F32 = 1u << 10, /* d_weights is f32 instead of bf16 */
+    NRL_READOUT_BWD_ADD_D_HIDDEN = 1u << 11,  /* add to what d_hidden holds (the tape's `new + old`, src/tensor/autodiff.rs:198-201) */
+    NRL_READOUT_BWD_ADD_D_WEIGHTS = 1u << 12  /* add to what d_weights holds */
+};
+
+typedef struct nrl_readout_bwd_args {
+    uint32_t struct_size;
+    uint32_t flags;
+    uint32_t V;
+    uint32_t d;
+    uint64_t rows;             /* at most 2^30 */
+    nrl_devptr hidden;         /* bf16 [rows, d], or int8 [rows, hidden_pitch] */
+    nrl_devptr hidden_scales;  /* f32 [rows] with HIDDEN_I8, else 0 */
+    uint64_t hidden_pitch;     /* bytes between int8 rows, a multiple of 16; 0 or d for bf16 */
+    nrl_devptr weights;        /* bf16 [d, V], or [V, d] with W_VD */
+    nrl_devptr tokens;         /* i32 [rows], with g_logp */
+    nrl_devptr rowstats;       /* f32 [rows, 4] of the forward */
+    nrl_devptr entropy;        /* f32 [rows] of the forward, with g_ent */
+    nrl_devptr g_logp;         /* f32 [rows] or 0 */
+    nrl_devptr g_ent;          /* f32 [rows] or 0 */
+    nrl_devptr d_hidden;       /* out [rows, d] or 0 */
+    nrl_devptr d_weights;      /* out, the layout of `weights`, or 0 */
+    nrl_devptr allow_mask;     /* as in the forward call, or 0 */
+    uint64_t allow_row_stride;
+    nrl_devptr workspace;      /* 256-byte aligned */
+    uint64_t workspace_bytes;
+    float temperature;         /* as in the forward call; 0 means 1 */
+    uint32_t reserved;         /* 0 */
+} nrl_readout_bwd_args;
+
+uint64_t nrl_readout_bwd_workspace_bytes(uint64_t rows, uint32_t V, uint32_t d);
+int nrl_readout_bwd(const nrl_readout_bwd_args* args, nrl_stream stream);
+
+/* ---------------------------------------------------------------------------------------------
+ * 8-bit integers with a scale per row (no counterpart in the reference, whose half product rounds to
+ * bf16, src/tensor/cuda/half_gemm.rs:32-40): q = rint(127·x / max|x|) in [-127, 127], ties to even,
+ * scale = max|x| / 127 in f32, x ≈ q·scale. A row of zeros has scale 0; a row with an infinity or a NaN
+ * has a non-finite scale and zeros, so everything computed from it is NaN. `values` is int8 [rows, pitch],
+ * 16-byte aligned, pitch >= d a multiple of 16; the bytes behind d are set to 0.
+ *   nrl_i8_quantize_rows     x F32 or BF16 [rows, d]: hidden states (a scale per token), or a [V, d] weight
+ *   nrl_i8_quantize_columns  a BF16 [d, V] weight as int8 [V, pitch] with a scale per vocabulary entry
+ *   nrl_i8_dequantize_rows   q·scale as F32, or rounded to BF16, [rows, d]
+ *   nrl_i8_matmul            out[r, v] = (Σ_k x[r, k]·w[v, k]) · x_scales[r] · w_scales[v] as F32 or BF16
+ *                            [rows, n]: `Decoder::head` (src/nn/decoder.rs:270-279) in 8 bits. The sums are
+ *                            exact (32-bit integers, k <= 131072); needs compute capability 10.x */
+int nrl_i8_quantize_rows(uint32_t dtype, uint64_t rows, uint32_t d, nrl_devptr x, nrl_devptr values, uint64_t pitch, nrl_devptr scales, nrl_stream stream);
+int nrl_i8_quantize_columns(uint32_t d, uint32_t V, nrl_devptr weights, nrl_devptr values, uint64_t pitch, nrl_devptr scales, nrl_stream stream);
+int nrl_i8_dequantize_rows(uint32_t dtype, uint64_t rows, uint32_t d, nrl_devptr values, uint64_t pitch, nrl_devptr scales, nrl_devptr out, nrl_stream stream);
+
+typedef struct nrl_i8_matmul_args {
+    uint32_t struct_size;
+    uint32_t dtype;       /* of `out` */
+    uint64_t rows;        /* tokens */
+    uint32_t n;           /* rows of w (the vocabulary) */
+    uint32_t k;
+    nrl_devptr x;         /* int8 [rows, x_pitch] */
+    uint64_t x_pitch;
+    nrl_devptr x_scales;  /* f32 [rows] */
+    nrl_devptr w;         /* int8 [n, w_pitch] */
+    uint64_t w_pitch;
+    nrl_devptr w_scales;  /* f32 [n] */
+    nrl_devptr out;       /* [rows, n] */
+} nrl_i8_matmul_args;
+int nrl_i8_matmul(const nrl_i8_matmul_args* args, nrl_stream stream);
+
 /* check_scored_finite (src/nn/rl.rs:204-211), the check the reference's losses run in debug
  * builds (debug_check, :213-221, called from policy_gradient_loss :230, clipped_policy_loss
  * :268-269 and kl_estimate :386-387): every scored log-probability is finite. `logp` is f32 [n]

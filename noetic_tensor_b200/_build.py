@@ -8,8 +8,8 @@ import sys
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libnrl.so")
-SOURCES = ["nrl_api.cu", "nrl_bits.cu"]  # the second compiles the row kernels again for bit-packed masks
-HEADERS = ["common.cuh", "row_fwd.cuh", "row_fwd_kernels.cuh", "row_fwd_group.cuh", "row_bwd.cuh", "token_ops.cuh", "ce_ops.cuh", "gumbel.cuh", "host_pack.cuh", "lane_ops.cuh", "readout.cuh", "row_api.inl"]
+SOURCES = ["nrl_api.cu", "nrl_bits.cu", "nrl_head.cu"]  # the second compiles the row kernels again for bit-packed masks, the third holds the readout's backward and 8-bit forms
+HEADERS = ["common.cuh", "row_fwd.cuh", "row_fwd_kernels.cuh", "row_fwd_group.cuh", "row_bwd.cuh", "token_ops.cuh", "ce_ops.cuh", "gumbel.cuh", "host_pack.cuh", "lane_ops.cuh", "tcgen05.cuh", "readout.cuh", "head_gemm.cuh", "head_ops.cuh", "row_api.inl"]
 INCLUDE = os.path.join(os.path.dirname(HERE), "include", "nrl.h")
 
 

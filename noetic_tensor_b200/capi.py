@@ -103,7 +103,23 @@ class ReadoutArgs(C.Structure):
     ]
 
 
+class ReadoutBwdArgs(C.Structure):
+    _fields_ = [
+        ("struct_size", u32), ("flags", u32), ("V", u32), ("d", u32), ("rows", u64),
+        ("hidden", ptr), ("hidden_scales", ptr), ("hidden_pitch", u64), ("weights", ptr), ("tokens", ptr), ("rowstats", ptr), ("entropy", ptr), ("g_logp", ptr), ("g_ent", ptr),
+        ("d_hidden", ptr), ("d_weights", ptr), ("allow_mask", ptr), ("allow_row_stride", u64), ("workspace", ptr), ("workspace_bytes", u64), ("temperature", f32), ("reserved", u32),
+    ]
+
+
+class I8MatmulArgs(C.Structure):
+    _fields_ = [
+        ("struct_size", u32), ("dtype", u32), ("rows", u64), ("n", u32), ("k", u32),
+        ("x", ptr), ("x_pitch", u64), ("x_scales", ptr), ("w", ptr), ("w_pitch", u64), ("w_scales", ptr), ("out", ptr),
+    ]
+
+
 READOUT_W_VD, READOUT_ROUND_BF16, READOUT_ONE_CTA, READOUT_SAMPLE, READOUT_GREEDY, READOUT_MASK_BITS = 1, 2, 4, 8, 16, 32
+READOUT_BWD_HIDDEN_I8, READOUT_BWD_D_HIDDEN_F32, READOUT_BWD_D_WEIGHTS_F32, READOUT_BWD_ADD_D_HIDDEN, READOUT_BWD_ADD_D_WEIGHTS = 256, 512, 1024, 2048, 4096
 
 LANE_SOFTMAX, LANE_LOG_SOFTMAX, LANE_LOGSUMEXP, LANE_ARGMAX, LANE_SUM, LANE_SOFTMAX_BWD, LANE_LOG_SOFTMAX_BWD, LANE_LOGSUMEXP_BWD = range(8)
 
@@ -138,6 +154,12 @@ SYMBOLS = {
     "nrl_unpack_rows": (C.c_int, [C.POINTER(UnpackArgs), C.c_void_p]),
     "nrl_readout_workspace_bytes": (u64, [u64, u32, u32, u32]),
     "nrl_readout_fwd": (C.c_int, [C.POINTER(ReadoutArgs), C.c_void_p]),
+    "nrl_readout_bwd_workspace_bytes": (u64, [u64, u32, u32]),
+    "nrl_readout_bwd": (C.c_int, [C.POINTER(ReadoutBwdArgs), C.c_void_p]),
+    "nrl_i8_quantize_rows": (C.c_int, [u32, u64, u32, ptr, ptr, u64, ptr, C.c_void_p]),
+    "nrl_i8_quantize_columns": (C.c_int, [u32, u32, ptr, ptr, u64, ptr, C.c_void_p]),
+    "nrl_i8_dequantize_rows": (C.c_int, [u32, u64, u32, ptr, u64, ptr, ptr, C.c_void_p]),
+    "nrl_i8_matmul": (C.c_int, [C.POINTER(I8MatmulArgs), C.c_void_p]),
     "nrl_check_status": (C.c_int, [ptr, u64, C.c_void_p, C.POINTER(u64), C.POINTER(u32)]),
     "nrl_check_scored_finite": (C.c_int, [ptr, ptr, u64, ptr, C.c_void_p, C.POINTER(u64), C.POINTER(f32)]),
 }

@@ -642,27 +642,8 @@ static uint64_t readout_workspace_one(uint64_t rows, uint32_t V, uint32_t d, uin
     return n;
 }
 
-typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-// cuTensorMapEncodeTiled through the runtime's driver entry point lookup: the library links no libcuda.
 static int encode_bf16_2d(CUtensorMap* map, uint64_t base, uint64_t inner, uint64_t outer, uint32_t box_inner, uint32_t box_outer) {
-    static std::atomic<void*> fn{nullptr};
-    void* f = fn.load(std::memory_order_acquire);
-    if (!f) {
-        cudaDriverEntryPointQueryResult q;
-        cudaError_t e = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q);
-        if (e != cudaSuccess) return (int)e;
-        if (q != cudaDriverEntryPointSuccess || !f) return NRL_E_UNSUPPORTED;
-        fn.store(f, std::memory_order_release);
-    }
-    const cuuint64_t dims[2] = {inner, outer};
-    const cuuint64_t strides[1] = {inner * 2};
-    const cuuint32_t box[2] = {box_inner, box_outer};
-    const cuuint32_t estr[2] = {1, 1};
-    CUresult r = ((EncodeTiledFn)f)(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, (void*)base, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                                    CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    return r == CUDA_SUCCESS ? NRL_OK : NRL_E_BAD_ARG;
+    return encode_2d(map, false, base, inner, outer, inner, box_inner, box_outer);
 }
 
 static int readout_fwd_one(const nrl_readout_args* a, nrl_stream stream);

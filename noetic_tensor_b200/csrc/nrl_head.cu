@@ -1,0 +1,296 @@
+// The C ABI of the readout's backward pass and of its 8-bit forms: argument checks, the
+// decomposition of a call into pieces of the vocabulary, and launches. No allocation, no synchronisation.
+#include <atomic>
+#include <cstring>
+
+#include "head_ops.cuh"
+
+using namespace nrl;
+
+extern std::atomic<uint64_t> nrl_g_launches;
+
+static inline int after_launch(int n = 1) {
+    nrl_g_launches.fetch_add((uint64_t)n, std::memory_order_relaxed);
+    cudaError_t e = cudaGetLastError();
+    return e == cudaSuccess ? NRL_OK : (int)e;
+}
+
+static int need_cc10() {
+    int dev = 0, cc_major = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e == cudaSuccess) e = cudaDeviceGetAttribute(&cc_major, cudaDevAttrComputeCapabilityMajor, dev);
+    if (e != cudaSuccess) return (int)e;
+    return cc_major == 10 ? NRL_OK : NRL_E_UNSUPPORTED;  // tcgen05 / tensor memory
+}
+
+constexpr uint32_t kPairs = 74;  // CTA pairs that run side by side (148 SMs)
+
+template <int EPI>
+static int launch_gemm(const CUtensorMap& ma, const CUtensorMap& mb, HeadGemm p, uint64_t tiles, cudaStream_t st) {
+    p.stages = kHgSmemTiles / (kHgABytes + (p.bn / 2) * 128);
+    if (p.stages > kHgMaxStages) p.stages = kHgMaxStages;
+    if (tiles > 0x7fffffffull) return NRL_E_UNSUPPORTED;
+    cudaError_t e = cudaFuncSetAttribute(head_gemm_kernel<EPI>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kHgSmemBytes);
+    if (e != cudaSuccess) return (int)e;
+    const unsigned grid = 2u * (unsigned)(tiles < kPairs ? (tiles ? tiles : 1) : kPairs);
+    head_gemm_kernel<EPI><<<grid, kHgThreads, kHgSmemBytes, st>>>(ma, mb, p);
+    return after_launch();
+}
+
+static inline uint64_t up(uint64_t x, uint64_t to) { return (x + to - 1) / to * to; }
+static inline uint32_t tiles256(uint64_t x) { return (uint32_t)((x + 255) / 256); }
+
+// How a backward call is cut: pieces of `vc` vocabulary columns (their dz is what exists of [rows, V] at any time) and
+// `nsplit` ranges of a piece's columns in dx = dz·Wᵀ. A function of (rows, V, d) only.
+struct BwdPlan {
+    uint64_t rows_pad;
+    uint32_t vc, pieces, nsplit;
+    uint64_t off_coef, off_more, off_rows, off_x, off_dz, off_acc, bytes;
+};
+static BwdPlan bwd_plan(uint64_t rows, uint32_t V, uint32_t d) {
+    BwdPlan b;
+    b.rows_pad = up(rows, 256);
+    // dz of a piece is at most 512 MB, but not narrower than 4096 columns: dx's f32 sums are read and written once per piece
+    uint64_t vc = (512ull << 20) / (b.rows_pad * 2) / 256 * 256;
+    if (vc < 4096) vc = 4096;
+    if (vc > up(V, 256)) vc = up(V, 256);
+    b.pieces = (uint32_t)((V + vc - 1) / vc);
+    b.vc = (uint32_t)up((V + b.pieces - 1) / b.pieces, 256);  // pieces of about the same width
+    b.pieces = (V + b.vc - 1) / b.vc;
+    // few tiles of dx: the columns of a piece go to several pairs
+    const uint64_t tiles = (uint64_t)tiles256(rows) * tiles256(d);
+    const uint32_t chunks = (b.vc + 63) / 64;
+    double best = 0.0;
+    b.nsplit = 1;
+    for (uint32_t s = 1; s <= 64 && (s == 1 || chunks / s >= 8); s++) {
+        const uint64_t units = tiles * s, waves = (units + kPairs - 1) / kPairs;
+        const double eff = (double)units / (double)(waves * kPairs);
+        if (eff > best + 0.08) { best = eff; b.nsplit = s; }
+        if (waves > 4) break;
+    }
+    uint64_t at = 256;
+    b.off_coef = at; at += up(rows * 16, 256);
+    b.off_more = at; at += up(rows * 16, 256);
+    b.off_rows = at; at += up(rows * 4, 256);
+    b.off_x = at; at += b.rows_pad * d * 2;
+    b.off_dz = at; at += b.rows_pad * b.vc * 2;
+    b.off_acc = at;
+    if (b.pieces > 1 || b.nsplit > 1) at += (uint64_t)b.nsplit * b.rows_pad * d * 4;
+    b.bytes = at;
+    return b;
+}
+
+extern "C" uint64_t nrl_readout_bwd_workspace_bytes(uint64_t rows, uint32_t V, uint32_t d) {
+    if (rows == 0 || V == 0 || d == 0) return 0;
+    return bwd_plan(rows, V, d).bytes;
+}
+
+extern "C" int nrl_readout_bwd(const nrl_readout_bwd_args* a, nrl_stream stream) {
+    if (!a || a->struct_size != sizeof(nrl_readout_bwd_args)) return NRL_E_BAD_ARG;
+    if (a->rows == 0 || a->V == 0 || a->d == 0 || !a->hidden || !a->weights || !a->rowstats || (!a->d_hidden && !a->d_weights)) return NRL_E_BAD_ARG;
+    const uint32_t known = NRL_READOUT_W_VD | NRL_READOUT_ROUND_BF16 | NRL_READOUT_MASK_BITS | NRL_READOUT_BWD_HIDDEN_I8 | NRL_READOUT_BWD_D_HIDDEN_F32 | NRL_READOUT_BWD_D_WEIGHTS_F32 |
+                           NRL_READOUT_BWD_ADD_D_HIDDEN | NRL_READOUT_BWD_ADD_D_WEIGHTS;
+    if (a->flags & ~known) return NRL_E_BAD_ARG;
+    if (a->V % 8 != 0 || a->d % 8 != 0 || ((a->hidden | a->weights | a->d_hidden | a->d_weights) & 15u)) return NRL_E_UNSUPPORTED;
+    if (a->V > 0x40000000u || a->d > 0x40000000u || a->rows > 0x40000000ull) return NRL_E_UNSUPPORTED;  // TMA coordinates are 32-bit
+    if (!a->g_logp && !a->g_ent) return NRL_E_BAD_ARG;
+    if ((a->g_logp && !a->tokens) || (a->g_ent && !a->entropy)) return NRL_E_BAD_ARG;
+    if ((a->rowstats & 15u) || ((a->tokens | a->entropy | a->g_logp | a->g_ent | a->hidden_scales) & 3u) || (a->workspace & 255u)) return NRL_E_BAD_ARG;
+    if (a->reserved != 0 || !(a->temperature >= 0.f) || !isfinite(a->temperature)) return NRL_E_BAD_ARG;
+    const bool i8 = (a->flags & NRL_READOUT_BWD_HIDDEN_I8) != 0;
+    if (i8 ? (!a->hidden_scales || a->hidden_pitch < a->d || a->hidden_pitch % 16 != 0) : (a->hidden_scales || (a->hidden_pitch != 0 && a->hidden_pitch != a->d))) return NRL_E_BAD_ARG;
+    if (a->flags & NRL_READOUT_MASK_BITS) {
+        if (!a->allow_mask || (a->allow_mask & 3u) || (a->allow_row_stride != 0 && a->allow_row_stride < (a->V + 31u) / 32u)) return NRL_E_BAD_ARG;
+    } else if (a->allow_mask && a->allow_row_stride != 0 && a->allow_row_stride != a->V) {
+        return NRL_E_BAD_ARG;
+    }
+    int rc = need_cc10();
+    if (rc) return rc;
+    const BwdPlan b = bwd_plan(a->rows, a->V, a->d);
+    if (!a->workspace || a->workspace_bytes < b.bytes) return NRL_E_WORKSPACE;
+    const cudaStream_t st = (cudaStream_t)stream;
+    const uint64_t ws = a->workspace;
+    const bool vd = (a->flags & NRL_READOUT_W_VD) != 0;
+    const float tau = a->temperature == 0.f ? 1.f : a->temperature;
+
+    HeadRows hr;
+    memset(&hr, 0, sizeof hr);
+    hr.rows = a->rows;
+    hr.d = a->d;
+    hr.g_logp = (const float*)a->g_logp;
+    hr.g_ent = (const float*)a->g_ent;
+    hr.rowstats = (const float*)a->rowstats;
+    hr.entropy = (const float*)a->entropy;
+    hr.tokens = (const int32_t*)a->tokens;
+    hr.tau = tau;
+    hr.hidden = (const void*)a->hidden;
+    hr.pitch = a->hidden_pitch;
+    hr.scales = i8 ? (const float*)a->hidden_scales : nullptr;
+    hr.count = (uint32_t*)ws;
+    hr.alpha = (float*)(ws + 4);
+    hr.coef = (float4*)(ws + b.off_coef);
+    hr.more = (float4*)(ws + b.off_more);
+    hr.rows_at = (uint32_t*)(ws + b.off_rows);
+    hr.x = (uint16_t*)(ws + b.off_x);
+    hr.d_hidden = (a->flags & NRL_READOUT_BWD_ADD_D_HIDDEN) ? nullptr : (void*)a->d_hidden;
+    hr.d_hidden_f32 = (a->flags & NRL_READOUT_BWD_D_HIDDEN_F32) ? 1u : 0u;
+    head_rows_kernel<<<1, 1024, 0, st>>>(hr);
+    rc = after_launch();
+    if (rc) return rc;
+    head_gather_kernel<<<(unsigned)b.rows_pad, 128, 0, st>>>(hr);
+    rc = after_launch();
+    if (rc) return rc;
+
+    HeadGemm g;
+    memset(&g, 0, sizeof g);
+    g.bn = 256;
+    g.nsplit = 1;
+    g.group_m = 16;
+    g.coef = hr.coef;
+    g.more = hr.more;
+    g.rows_at = hr.rows_at;
+    g.tau = tau;
+    g.round_bf16 = (a->flags & NRL_READOUT_ROUND_BF16) ? 1u : 0u;
+    g.entropy_term = a->g_ent ? 1u : 0u;
+    g.allow = (const uint8_t*)a->allow_mask;
+    g.allow_stride = a->allow_row_stride;
+    g.allow_bits = (a->flags & NRL_READOUT_MASK_BITS) ? 1u : 0u;
+    g.vocab = a->V;
+    g.dz = (uint16_t*)(ws + b.off_dz);
+    g.dz_pitch = b.vc;
+    g.alpha = hr.alpha;
+    g.acc_rows = b.rows_pad;
+
+    const uint64_t x = ws + b.off_x, dz = ws + b.off_dz;
+    CUtensorMap x_k, x_mn, w_k, w_mn, dz_k, dz_mn;
+    // boxes of 64 elements of K × 128 rows, or of 64 columns × 64 elements of K
+    if ((rc = encode_2d(&x_k, false, x, a->d, b.rows_pad, a->d, 64, 128)) || (rc = encode_2d(&x_mn, false, x, a->d, b.rows_pad, a->d, 64, 64)) ||
+        (rc = encode_2d(&dz_k, false, dz, b.vc, b.rows_pad, b.vc, 64, 128)) || (rc = encode_2d(&dz_mn, false, dz, b.vc, b.rows_pad, b.vc, 64, 64)) ||
+        (rc = encode_2d(&w_k, false, a->weights, vd ? a->d : a->V, vd ? a->V : a->d, vd ? a->d : a->V, 64, 128)) ||
+        (rc = encode_2d(&w_mn, false, a->weights, vd ? a->d : a->V, vd ? a->V : a->d, vd ? a->d : a->V, 64, 64)))
+        return rc;
+
+    for (uint32_t piece = 0; piece < b.pieces; piece++) {
+        const uint32_t v0 = piece * b.vc, cols = a->V - v0 < b.vc ? a->V - v0 : b.vc;
+        {  // dz of this piece: x [count, d] · W[:, v0 …]
+            HeadGemm p = g;
+            p.m = (uint32_t)a->rows;
+            p.m_count = hr.count;
+            p.n = cols;
+            p.k = a->d;
+            p.b_mn = vd ? 0u : 1u;
+            p.b_n0 = v0;
+            p.v0 = v0;
+            rc = launch_gemm<kEpiGrad>(x_k, vd ? w_k : w_mn, p, (uint64_t)tiles256(a->rows) * tiles256(cols), st);
+            if (rc) return rc;
+        }
+        if (a->d_hidden) {  // dx += dz · Wᵀ
+            HeadGemm p = g;
+            p.m = (uint32_t)a->rows;
+            p.m_count = hr.count;
+            p.n = a->d;
+            p.k = cols;
+            p.b_mn = vd ? 1u : 0u;
+            p.b_k0 = v0;
+            p.nsplit = b.nsplit;
+            p.acc = b.pieces > 1 || b.nsplit > 1 ? (float*)(ws + b.off_acc) : nullptr;
+            p.acc_in = piece > 0 ? 1u : 0u;
+            p.acc_out = b.nsplit > 1 || piece + 1 < b.pieces ? 1u : 0u;
+            p.out = (void*)a->d_hidden;
+            p.out_pitch = a->d;
+            p.out_f32 = hr.d_hidden_f32;
+            p.out_add = (a->flags & NRL_READOUT_BWD_ADD_D_HIDDEN) ? 1u : 0u;
+            p.wide = (a->d_hidden % 32 == 0 && (p.out_f32 || a->d % 16 == 0)) ? 1u : 0u;
+            rc = launch_gemm<kEpiHidden>(dz_k, vd ? w_mn : w_k, p, (uint64_t)tiles256(a->rows) * tiles256(a->d) * b.nsplit, st);
+            if (rc) return rc;
+            if (b.nsplit > 1 && piece + 1 == b.pieces) {
+                head_fold_kernel<<<(unsigned)a->rows, 128, 0, st>>>(hr.count, hr.alpha, hr.more, hr.rows_at, p.acc, b.rows_pad, b.nsplit, a->d, (void*)a->d_hidden, p.out_f32, p.out_add);
+                rc = after_launch();
+                if (rc) return rc;
+            }
+        }
+        if (a->d_weights) {  // dW[:, v0 …] = xᵀ · dz, or its transpose
+            HeadGemm p = g;
+            p.m = vd ? cols : a->d;
+            p.n = vd ? a->d : cols;
+            p.k = (uint32_t)a->rows;
+            p.k_count = hr.count;
+            p.a_mn = p.b_mn = 1u;
+            p.out = (void*)a->d_weights;
+            p.out_pitch = vd ? a->d : a->V;
+            p.out_row0 = vd ? v0 : 0u;
+            p.out_col0 = vd ? 0u : v0;
+            p.out_f32 = (a->flags & NRL_READOUT_BWD_D_WEIGHTS_F32) ? 1u : 0u;
+            p.out_add = (a->flags & NRL_READOUT_BWD_ADD_D_WEIGHTS) ? 1u : 0u;
+            p.wide = (a->d_weights % 32 == 0 && (p.out_f32 || p.out_pitch % 16 == 0)) ? 1u : 0u;
+            rc = launch_gemm<kEpiWeight>(vd ? dz_mn : x_mn, vd ? x_mn : dz_mn, p, (uint64_t)tiles256(p.m) * tiles256(p.n), st);
+            if (rc) return rc;
+        }
+    }
+    return NRL_OK;
+}
+
+// ---- 8-bit integers -----------------------------------------------------------------------------------
+
+extern "C" int nrl_i8_quantize_rows(uint32_t dtype, uint64_t rows, uint32_t d, nrl_devptr x, nrl_devptr values, uint64_t pitch, nrl_devptr scales, nrl_stream stream) {
+    if (rows == 0 || d == 0 || !x || !values || !scales || (scales & 3u)) return NRL_E_BAD_ARG;
+    if (dtype != NRL_F32 && dtype != NRL_BF16) return NRL_E_UNSUPPORTED;
+    if (pitch < d || pitch % 16 != 0 || (values & 15u) || (x & (dtype == NRL_F32 ? 3u : 1u))) return NRL_E_BAD_ARG;
+    if (rows > 0x7fffffffull) return NRL_E_UNSUPPORTED;
+    const bool vec = d % 8 == 0 && (x & 15u) == 0;
+    const cudaStream_t st = (cudaStream_t)stream;
+    if (dtype == NRL_BF16) quantise_rows_kernel<NRL_BF16><<<(unsigned)rows, 256, 0, st>>>((const void*)x, d, pitch, (int8_t*)values, (float*)scales, vec);
+    else quantise_rows_kernel<NRL_F32><<<(unsigned)rows, 256, 0, st>>>((const void*)x, d, pitch, (int8_t*)values, (float*)scales, vec);
+    return after_launch();
+}
+
+extern "C" int nrl_i8_quantize_columns(uint32_t d, uint32_t V, nrl_devptr weights, nrl_devptr values, uint64_t pitch, nrl_devptr scales, nrl_stream stream) {
+    if (d == 0 || V == 0 || !weights || !values || !scales || (scales & 3u) || (weights & 1u)) return NRL_E_BAD_ARG;
+    if (pitch < d || pitch % 16 != 0 || (values & 15u)) return NRL_E_BAD_ARG;
+    quantise_columns_kernel<<<(V + 63) / 64, 256, 0, (cudaStream_t)stream>>>((const uint16_t*)weights, d, V, pitch, (int8_t*)values, (float*)scales);
+    return after_launch();
+}
+
+extern "C" int nrl_i8_dequantize_rows(uint32_t dtype, uint64_t rows, uint32_t d, nrl_devptr values, uint64_t pitch, nrl_devptr scales, nrl_devptr out, nrl_stream stream) {
+    if (rows == 0 || d == 0 || !values || !scales || !out || (scales & 3u)) return NRL_E_BAD_ARG;
+    if (dtype != NRL_F32 && dtype != NRL_BF16) return NRL_E_UNSUPPORTED;
+    if (pitch < d || (out & (dtype == NRL_F32 ? 3u : 1u))) return NRL_E_BAD_ARG;
+    if (rows > 0x7fffffffull) return NRL_E_UNSUPPORTED;
+    dequantise_rows_kernel<<<(unsigned)rows, 256, 0, (cudaStream_t)stream>>>((const int8_t*)values, (const float*)scales, d, pitch, (void*)out, dtype == NRL_F32 ? 1u : 0u);
+    return after_launch();
+}
+
+extern "C" int nrl_i8_matmul(const nrl_i8_matmul_args* a, nrl_stream stream) {
+    if (!a || a->struct_size != sizeof(nrl_i8_matmul_args)) return NRL_E_BAD_ARG;
+    if (a->rows == 0 || a->n == 0 || a->k == 0 || !a->x || !a->x_scales || !a->w || !a->w_scales || !a->out) return NRL_E_BAD_ARG;
+    if (a->dtype != NRL_F32 && a->dtype != NRL_BF16) return NRL_E_UNSUPPORTED;
+    if (a->x_pitch < a->k || a->w_pitch < a->k || a->x_pitch % 16 != 0 || a->w_pitch % 16 != 0 || ((a->x | a->w) & 15u) || ((a->x_scales | a->w_scales) & 3u) ||
+        (a->out & (a->dtype == NRL_F32 ? 3u : 1u)))
+        return NRL_E_BAD_ARG;
+    if (a->rows > 0x40000000ull || a->n > 0x40000000u) return NRL_E_UNSUPPORTED;  // TMA coordinates are 32-bit
+    if (a->k > 131072u) return NRL_E_UNSUPPORTED;                                  // 127·127·k must fit 31 bits
+    int rc = need_cc10();
+    if (rc) return rc;
+    // M = the weight's rows, N = the tokens: few tokens make a narrow tile, and the weight streams through it
+    HeadGemm p;
+    memset(&p, 0, sizeof p);
+    const uint64_t tiles_n = (a->rows + 255) / 256;
+    p.bn = (uint32_t)up((a->rows + tiles_n - 1) / tiles_n, 32);
+    p.m = a->n;
+    p.n = (uint32_t)a->rows;
+    p.k = a->k;
+    p.nsplit = 1;
+    p.group_m = 16;
+    p.m_scale = (const float*)a->w_scales;
+    p.n_scale = (const float*)a->x_scales;
+    p.out = (void*)a->out;
+    p.out_pitch = a->n;
+    p.out_f32 = a->dtype == NRL_F32 ? 1u : 0u;
+    CUtensorMap mw, mx;
+    // the extent along K is k, not the pitch: what lies behind a row's k integers is read as zeros
+    rc = encode_2d(&mw, true, a->w, a->k, a->n, a->w_pitch, 128, 128);
+    if (rc) return rc;
+    rc = encode_2d(&mx, true, a->x, a->k, a->rows, a->x_pitch, 128, p.bn / 2);
+    if (rc) return rc;
+    return launch_gemm<kEpiInt8>(mw, mx, p, (uint64_t)tiles256(a->n) * ((a->rows + p.bn - 1) / p.bn), (cudaStream_t)stream);
+}

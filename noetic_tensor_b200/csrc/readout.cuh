@@ -28,9 +28,7 @@
 // again bounded, for its copies in flight, tensor memory is released and the rows of the CTA get
 // status bit 2 ("gave up"). Nothing spins forever.
 #pragma once
-#include <cuda.h>
-
-#include "common.cuh"
+#include "tcgen05.cuh"
 
 namespace nrl {
 
@@ -43,7 +41,6 @@ constexpr uint32_t kRoABytes = kRoBM * kRoBK * 2;  // 16 KB
 constexpr uint32_t kRoBBytes = kRoBN * kRoBK * 2;  // 32 KB
 constexpr uint32_t kRoStageBytes = kRoABytes + kRoBBytes;
 constexpr uint32_t kRoSmemBytes = kRoStages * kRoStageBytes + 1024 /* alignment slack */ + 256 /* barriers */;
-constexpr unsigned long long kWaitLimitNs = 2000000000ull;  // 2 s: far beyond any legitimate wait here
 constexpr int kRoPartFloats = 4;  // (m, S, W, token logit) per row and column range
 
 struct ReadoutParams {
@@ -67,61 +64,6 @@ struct ReadoutParams {
     float2* slog;          // optional sampling log [rows, tiles, 4]: per 64 columns (mass at the running maximum, that maximum)
 };
 constexpr int kRoLogCols = 64;  // columns per sampling-log entry
-
-// ---- raw PTX wrappers -----------------------------------------------------------------------------
-// Bounded wait: false when the CTA aborted or the limit passed (then the abort flag is raised).
-__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile uint32_t* abort_flag, unsigned long long limit_ns = kWaitLimitNs) {
-    if (mbar_try_wait(bar, parity)) return true;
-    const unsigned long long t0 = global_ns();
-    for (uint32_t i = 1;; i++) {
-        if (mbar_try_wait(bar, parity)) return true;
-        if ((i & 63u) == 0u) {
-            if (*abort_flag) return false;
-            if (global_ns() - t0 > limit_ns) {
-                *abort_flag = 1u;
-                return false;
-            }
-        }
-    }
-}
-__device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map, int32_t x, int32_t y, uint32_t bar) {
-    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(bar)
-                 : "memory");
-}
-__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void tc_commit(uint32_t bar) { asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory"); }
-__device__ __forceinline__ void tc_mma_bf16(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
-        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
-        : "memory");
-}
-// 32 consecutive f32 columns of this thread's lane
-__device__ __forceinline__ void tc_ld32(uint32_t taddr, uint32_t r[32]) {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
-          "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]),
-          "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-        : "r"(taddr)
-        : "memory");
-}
-__device__ __forceinline__ void tc_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
-
-// Shared-memory matrix descriptor of a 128-byte-swizzled tile (version 1, layout type 2), offsets in bytes.
-__device__ __forceinline__ uint64_t smem_desc_sw128(uint32_t addr, uint32_t lbo_bytes, uint32_t sbo_bytes) {
-    return (uint64_t)((addr >> 4) & 0x3fffu) | ((uint64_t)((lbo_bytes >> 4) & 0x3fffu) << 16) | ((uint64_t)((sbo_bytes >> 4) & 0x3fffu) << 32) | (1ull << 46) | (2ull << 61);
-}
-
-__device__ __forceinline__ float round_through_bf16(float x) {
-    uint32_t u = __float_as_uint(x);
-    if ((u & 0x7fffffffu) > 0x7f800000u) return x;  // NaN stays NaN
-    u = (u + 0x7fffu + ((u >> 16) & 1u)) & 0xffff0000u;  // nearest, ties to even (src/tensor/half.rs:16-27)
-    return __uint_as_float(u);
-}
 
 // the range of vocabulary tiles of column range `split`
 __device__ __forceinline__ void readout_tile_range(const ReadoutParams& p, uint32_t split, uint32_t& t0, uint32_t& t1) {
@@ -424,33 +366,6 @@ constexpr int kRoStages2 = 6;  // a seventh stage fits the 227 KB and measured t
 constexpr uint32_t kRoBBytes2 = kRoBBytes / 2;                 // 16 KB: this CTA's half of the W tile
 constexpr uint32_t kRoStageBytes2 = kRoABytes + kRoBBytes2;    // 32 KB
 constexpr uint32_t kRoSmemBytes2 = kRoStages2 * kRoStageBytes2 + 1024 + 256;
-// a shared-memory address of this CTA -> the address of the same offset in the cluster's first CTA
-__device__ __forceinline__ uint32_t in_first_cta(uint32_t addr) {
-    uint32_t r;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(0u));
-    return r;
-}
-
-__device__ __forceinline__ void tma_load_2d_pair(uint32_t dst, const CUtensorMap* map, int32_t x, int32_t y, uint32_t bar_in_first_cta) {
-    asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst), "l"(map), "r"(x), "r"(y),
-                 "r"(bar_in_first_cta)
-                 : "memory");
-}
-__device__ __forceinline__ void tc_commit_pair(uint32_t bar) {  // arrives on `bar` in both CTAs of the pair
-    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar), "h"((uint16_t)3) : "memory");
-}
-__device__ __forceinline__ void tc_mma_bf16_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
-        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
-        : "memory");
-}
-__device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar_cluster_addr) {
-    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar_cluster_addr) : "memory");
-}
-
 // Work items are (256-row block, column range) pairs laid out in groups as above; the grid holds
 // `gridDim.x / 2 / (group_blocks · nsplit)` groups' worth of clusters and a cluster walks the groups
 // with that stride (one cluster per item when the grid covers every group).

@@ -4,12 +4,14 @@ fused row kernels: same names, argument meanings, per-seed results `[S]` and err
 Where the reference runs log_softmax, builds a dense one-hot `[S, N, V]`, multiplies and sums
 (three `[rows, V]` f32 intermediates plus the saved log-softmax), this reads the logits once
 forward (twice with label smoothing) and once backward. Each function returns an `rl.Loss`:
-`.value` and `.backward(upstream)` → d(logits) `[S, B, T, V]` f32 (kl_div: a pair).
+`.value` and `.backward(upstream)` → d(logits) `[S, B, T, V]` f32 (kl_div: a pair). Given an `rl.Head`
+instead of logits, nll and the cross-entropies (without label smoothing) go through the fused readout
+and `.backward` returns (d_hidden, d_weight).
 """
 import torch
 
 from . import capi, ops
-from .rl import Loss
+from .rl import Head, Loss
 
 
 class CeOptions:
@@ -23,10 +25,10 @@ class CeOptions:
 
 
 def _rows(logits):
-    if logits.dim() != 4:
+    if len(logits.shape) != 4:
         raise ValueError("logits [S, B, T, V]")
     S, B, T, V = logits.shape
-    return S, B * T, V, logits.reshape(S * B * T, V)
+    return S, B * T, V, logits if isinstance(logits, Head) else logits.reshape(S * B * T, V)
 
 
 def _targets(targets, S, N, V, ignore_index=None):
@@ -53,7 +55,12 @@ def _ce(logits, targets, keep, smoothing, reduce):
         keep = keep * not_ignored
     elif not_ignored is not None:
         keep = not_ignored
-    fwd = ops.row_forward(flat, tokens=tok, want_entropy=False)
+    head, shape = None, logits.shape
+    if isinstance(flat, Head):
+        if smoothing > 0.0:
+            raise ValueError("label smoothing needs the sum of a row's logits: a Head has none")
+        head, flat = flat.run(tok), None  # the run holds what the backward needs, which with a checkpoint is not the hidden states
+    fwd = head.fwd if head is not None else ops.row_forward(flat, tokens=tok, want_entropy=False)
     zsum = ops.row_sum(flat) if smoothing > 0.0 else None
     per, _, _ = ops.ce_tokens(V, fwd.logp, smoothing=smoothing, rowstats=fwd.rowstats, logit_sum=zsum, keep=keep)
     per3 = per.reshape(S, 1, N)
@@ -67,7 +74,9 @@ def _ce(logits, targets, keep, smoothing, reduce):
             d_per = up
         _, g_lp, g_un = ops.ce_tokens(V, fwd.logp, smoothing=smoothing, rowstats=fwd.rowstats, logit_sum=zsum, keep=keep,
                                       upstream=d_per.reshape(-1).contiguous(), want_loss=False)
-        return ops.row_backward(flat, fwd, g_logp=g_lp, g_uniform=g_un).reshape(logits.shape)
+        if head is not None:
+            return head.backward(g_logp=g_lp)
+        return ops.row_backward(flat, fwd, g_logp=g_lp, g_uniform=g_un).reshape(shape)
 
     return Loss(value, backward)
 

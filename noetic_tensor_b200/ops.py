@@ -421,6 +421,22 @@ class Readout:
     __slots__ = ("logp", "entropy", "rowstats", "status", "logits", "tokens")
 
 
+def _readout_masks(a, V, rows, allow, allow_bits, dev):
+    """The allow-mask fields of a readout call; returns the byte mask as the call reads it (keep it alive until the launch)."""
+    if allow is not None and allow_bits is not None:
+        raise ValueError("give `allow` or `allow_bits`, not both")
+    if allow is not None:
+        allow, a.allow_row_stride, _, _ = _masks(V, rows, allow, None, dev)
+        a.allow_mask = _p(allow)
+    if allow_bits is not None:
+        words = (V + 31) // 32
+        if allow_bits.dtype != torch.int32 or allow_bits.dim() != 2 or allow_bits.shape[0] not in (1, rows) or allow_bits.shape[1] < words or allow_bits.device != dev or not allow_bits.is_contiguous():
+            raise ValueError("allow_bits: contiguous int32 [rows, >= ceil(V/32)] or [1, ...] on the logits' device")
+        a.allow_mask, a.allow_row_stride = _p(allow_bits), (0 if allow_bits.shape[0] == 1 else allow_bits.shape[1])
+        a.flags |= capi.READOUT_MASK_BITS
+    return allow
+
+
 def readout_forward(hidden, weights, *, tokens=None, weights_are_vd=False, round_bf16=False, want_logits=False, workspace=None, one_cta=False, uniforms=None, allow=None, greedy=False, temperature=1.0, allow_bits=None):
     """Row statistics of logits = hidden [rows, d] · W without writing the logits (nrl_readout_fwd):
     `hidden` bf16 [rows, d]; `weights` bf16 [d, V] (the reference's Linear layout) or, with
@@ -460,17 +476,7 @@ def readout_forward(hidden, weights, *, tokens=None, weights_are_vd=False, round
     if tokens is not None:
         a.tokens = _p(tokens)
         out.logp = torch.empty(rows, dtype=torch.float32, device=dev)
-    if allow is not None and allow_bits is not None:
-        raise ValueError("give `allow` or `allow_bits`, not both")
-    if allow is not None:
-        allow, a.allow_row_stride, _, _ = _masks(V, rows, allow, None, dev)
-        a.allow_mask = _p(allow)
-    if allow_bits is not None:
-        words = (V + 31) // 32
-        if allow_bits.dtype != torch.int32 or allow_bits.dim() != 2 or allow_bits.shape[0] not in (1, rows) or allow_bits.shape[1] < words or allow_bits.device != dev or not allow_bits.is_contiguous():
-            raise ValueError("allow_bits: contiguous int32 [rows, >= ceil(V/32)] or [1, ...] on the logits' device")
-        a.allow_mask, a.allow_row_stride = _p(allow_bits), (0 if allow_bits.shape[0] == 1 else allow_bits.shape[1])
-        a.flags |= capi.READOUT_MASK_BITS
+    allow = _readout_masks(a, V, rows, allow, allow_bits, dev)
     out.entropy = torch.empty(rows, dtype=torch.float32, device=dev)
     out.rowstats = torch.empty(rows, 4, dtype=torch.float32, device=dev)
     out.status = torch.empty(rows, dtype=torch.uint8, device=dev)
@@ -482,6 +488,150 @@ def readout_forward(hidden, weights, *, tokens=None, weights_are_vd=False, round
     with torch.cuda.device(dev):
         capi.check(capi.lib().nrl_readout_fwd(C.byref(a), _stream(dev)), "nrl_readout_fwd")
     return out
+
+
+class Int8Rows:
+    """Rows as 8-bit integers with an f32 scale each: `values` int8 [rows, pitch] (pitch: `d` rounded up
+    to a multiple of 16), `scales` f32 [rows], x ≈ values[:, :d] · scales[:, None]."""
+
+    __slots__ = ("values", "scales", "d")
+
+    def __init__(self, values, scales, d):
+        dev = values.device
+        if values.dim() != 2 or not 0 < d <= values.shape[1] or values.shape[1] % 16:
+            raise ValueError("values: int8 [rows, pitch], pitch >= d and a multiple of 16")
+        _need(values, torch.int8, tuple(values.shape), "values", dev)
+        _need(scales, torch.float32, (values.shape[0],), "scales", dev)
+        self.values, self.scales, self.d = values, scales, d
+
+
+def quantize_rows(x):
+    """`x` [rows, d] (float32 or bfloat16) as Int8Rows: q = rint(127 x / max|x|), scale max|x| / 127
+    (nrl_i8_quantize_rows). A row with an infinity or a NaN gets a non-finite scale."""
+    dev = x.device
+    if dev.type != "cuda":
+        raise ValueError("quantize_rows needs CUDA tensors: this library has no CPU path")
+    rows, d = x.shape
+    if not x.is_contiguous():
+        raise ValueError("x must be contiguous")
+    q = Int8Rows(torch.empty(rows, (d + 15) // 16 * 16, dtype=torch.int8, device=dev), torch.empty(rows, dtype=torch.float32, device=dev), d)
+    with torch.cuda.device(dev):
+        capi.check(capi.lib().nrl_i8_quantize_rows(_dt(x), rows, d, _p(x), _p(q.values), q.values.shape[1], _p(q.scales), _stream(dev)), "nrl_i8_quantize_rows")
+    return q
+
+
+def quantize_weight(weights, weights_are_vd=False):
+    """A readout weight, bf16 [d, V] (or [V, d] with `weights_are_vd`), as Int8Rows [V, d]: a scale per
+    vocabulary entry (nrl_i8_quantize_columns / nrl_i8_quantize_rows)."""
+    if weights_are_vd:
+        return quantize_rows(weights)
+    dev = weights.device
+    if dev.type != "cuda":
+        raise ValueError("quantize_weight needs CUDA tensors: this library has no CPU path")
+    d, V = weights.shape
+    _need(weights, torch.bfloat16, (d, V), "weights", dev)
+    q = Int8Rows(torch.empty(V, (d + 15) // 16 * 16, dtype=torch.int8, device=dev), torch.empty(V, dtype=torch.float32, device=dev), d)
+    with torch.cuda.device(dev):
+        capi.check(capi.lib().nrl_i8_quantize_columns(d, V, _p(weights), _p(q.values), q.values.shape[1], _p(q.scales), _stream(dev)), "nrl_i8_quantize_columns")
+    return q
+
+
+def dequantize_rows(q, dtype=torch.bfloat16):
+    """values · scale as [rows, d] of `dtype` (nrl_i8_dequantize_rows)."""
+    dev = q.values.device
+    if dev.type != "cuda":
+        raise ValueError("dequantize_rows needs CUDA tensors: this library has no CPU path")
+    out = torch.empty(q.values.shape[0], q.d, dtype=dtype, device=dev)
+    with torch.cuda.device(dev):
+        capi.check(capi.lib().nrl_i8_dequantize_rows(_dt(out), out.shape[0], q.d, _p(q.values), q.values.shape[1], _p(q.scales), _p(out), _stream(dev)), "nrl_i8_dequantize_rows")
+    return out
+
+
+def int8_matmul(x, w, dtype=torch.float32):
+    """out[r, v] = Σ_k x[r, k] w[v, k] (exact) · x.scales[r] · w.scales[v], [rows, V] of `dtype`
+    (nrl_i8_matmul); `x`, `w`: Int8Rows of the same d."""
+    dev = x.values.device
+    if dev.type != "cuda":
+        raise ValueError("int8_matmul needs CUDA tensors: this library has no CPU path")
+    if x.d != w.d or w.values.device != dev:
+        raise ValueError(f"int8_matmul: rows of {x.d} and of {w.d} integers on {dev} and {w.values.device}")
+    out = torch.empty(x.values.shape[0], w.values.shape[0], dtype=dtype, device=dev)
+    a = capi.I8MatmulArgs()
+    a.struct_size = C.sizeof(a)
+    a.dtype, a.rows, a.n, a.k = _dt(out), out.shape[0], out.shape[1], x.d
+    a.x, a.x_pitch, a.x_scales = _p(x.values), x.values.shape[1], _p(x.scales)
+    a.w, a.w_pitch, a.w_scales = _p(w.values), w.values.shape[1], _p(w.scales)
+    a.out = _p(out)
+    with torch.cuda.device(dev):
+        capi.check(capi.lib().nrl_i8_matmul(C.byref(a), _stream(dev)), "nrl_i8_matmul")
+    return out
+
+
+def readout_backward(hidden, weights, fwd, *, tokens=None, g_logp=None, g_ent=None, weights_are_vd=False, round_bf16=False, allow=None, allow_bits=None, temperature=1.0, want_hidden=True,
+                     want_weights=True, grad_dtype=torch.bfloat16, add_hidden=None, add_weights=None, workspace=None):
+    """(d_hidden, d_weights) of Σ g_logp·logp + Σ g_ent·entropy of `readout_forward`'s results `fwd` (its
+    `rowstats` and, with `g_ent`, `entropy`), the logits computed again in pieces (nrl_readout_bwd).
+    `hidden`: the bf16 [rows, d] of the forward call, or an Int8Rows checkpoint of it. Gradients are
+    `grad_dtype` (bfloat16 or float32); `add_hidden` / `add_weights` are tensors they are added to in place
+    (their own dtype counts). Rows whose upstreams are 0 are not read."""
+    quant = hidden if isinstance(hidden, Int8Rows) else None
+    x = quant.values if quant else hidden
+    dev = x.device
+    if dev.type != "cuda":
+        raise ValueError("readout_backward needs CUDA tensors: this library has no CPU path")
+    rows, d = x.shape[0], (quant.d if quant else x.shape[1])
+    V = weights.shape[0] if weights_are_vd else weights.shape[1]
+    wshape = (V, d) if weights_are_vd else (d, V)
+    _need(weights, torch.bfloat16, wshape, "weights", dev)
+    if grad_dtype not in (torch.bfloat16, torch.float32):
+        raise TypeError(f"gradients must be bfloat16 or float32, got {grad_dtype}")
+    if g_logp is None and g_ent is None:
+        raise ValueError("give `g_logp`, `g_ent` or both")
+    a = capi.ReadoutBwdArgs()
+    a.struct_size = C.sizeof(a)
+    a.flags = (capi.READOUT_W_VD if weights_are_vd else 0) | (capi.READOUT_ROUND_BF16 if round_bf16 else 0)
+    a.V, a.d, a.rows, a.temperature = V, d, rows, float(temperature)
+    if quant:
+        a.flags |= capi.READOUT_BWD_HIDDEN_I8
+        a.hidden_scales, a.hidden_pitch = _p(quant.scales), x.shape[1]
+    else:
+        _need(x, torch.bfloat16, (rows, d), "hidden", dev)
+    a.hidden, a.weights = _p(x), _p(weights)
+    _need(fwd.rowstats, torch.float32, (rows, 4), "rowstats", dev)
+    a.rowstats = _p(fwd.rowstats)
+    if g_logp is not None:
+        _need(g_logp, torch.float32, (rows,), "g_logp", dev)
+        if tokens is None:
+            raise ValueError("`g_logp` needs the tokens")
+        _need(tokens, torch.int32, (rows,), "tokens", dev)
+        a.g_logp, a.tokens = _p(g_logp), _p(tokens)
+    if g_ent is not None:
+        _need(g_ent, torch.float32, (rows,), "g_ent", dev)
+        _need(fwd.entropy, torch.float32, (rows,), "entropy", dev)
+        a.g_ent, a.entropy = _p(g_ent), _p(fwd.entropy)
+    allow = _readout_masks(a, V, rows, allow, allow_bits, dev)
+
+    def out(add, want, shape, f32_flag, add_flag, what):
+        if add is not None:
+            if add.dtype not in (torch.bfloat16, torch.float32):
+                raise TypeError(f"{what}: bfloat16 or float32, got {add.dtype}")
+            _need(add, add.dtype, shape, what, dev)
+            a.flags |= add_flag
+        elif want:
+            add = torch.empty(shape, dtype=grad_dtype, device=dev)
+        if add is not None and add.dtype == torch.float32:
+            a.flags |= f32_flag
+        return add
+
+    d_hidden = out(add_hidden, want_hidden, (rows, d), capi.READOUT_BWD_D_HIDDEN_F32, capi.READOUT_BWD_ADD_D_HIDDEN, "add_hidden")
+    d_weights = out(add_weights, want_weights, wshape, capi.READOUT_BWD_D_WEIGHTS_F32, capi.READOUT_BWD_ADD_D_WEIGHTS, "add_weights")
+    a.d_hidden, a.d_weights = _p(d_hidden), _p(d_weights)
+    if workspace is None:
+        workspace = torch.empty(capi.lib().nrl_readout_bwd_workspace_bytes(rows, V, d), dtype=torch.uint8, device=dev)
+    a.workspace, a.workspace_bytes = _p(workspace), workspace.numel() * workspace.element_size()
+    with torch.cuda.device(dev):
+        capi.check(capi.lib().nrl_readout_bwd(C.byref(a), _stream(dev)), "nrl_readout_bwd")
+    return d_hidden, d_weights
 
 
 def row_sum(logits):

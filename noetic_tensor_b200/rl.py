@@ -85,8 +85,74 @@ class Tempered:
         return dict(allow=self.allow, add_mask=self.add, temperature=self.temperature)
 
 
+class Head:
+    """`Decoder::head(hidden)` (src/nn/decoder.rs:270-279) in place of logits, without computing them:
+    every function here and in `loss` that takes logits [S, B, T, V] and returns a `Loss` takes a Head,
+    runs the fused readout instead (the logits are never kept, forward or backward), and its
+    `.backward(upstream)` returns the pair (d_hidden [S, B, T, d], d_weight in the weight's layout).
+
+    `hidden` bf16 [S, B, T, d]; `weight` bf16 [d, V] (the Linear's [in, out] layout) or, with
+    `weight_is_vd`, [V, d]; d and V multiples of 8. `temperature` and `vocab_mask` make the logits the
+    tempered ones (src/nn/rl.rs:475-486); the mask is a uint8/bool allow-mask [..., V] or [1, V], or int32
+    words of one bit per token. With `checkpoint` a loss keeps the hidden states for its backward as 8-bit
+    integers with a scale per position (half the memory) instead of keeping `hidden`. `grad_dtype`:
+    bfloat16 or float32."""
+
+    def __init__(self, hidden, weight, temperature=1.0, vocab_mask=None, weight_is_vd=False, checkpoint=False, grad_dtype=torch.bfloat16):
+        if not (0.0 < temperature < float("inf")):
+            raise ValueError(f"tempered_logits: temperature {temperature} (must be positive)")
+        self.d, self.V = hidden.shape[-1], weight.shape[0 if weight_is_vd else 1]
+        self.shape = tuple(hidden.shape[:-1]) + (self.V,)
+        self.flat = hidden.reshape(-1, self.d).contiguous()
+        if vocab_mask is not None and vocab_mask.dtype not in (torch.uint8, torch.bool, torch.int32):
+            raise ValueError("Head: vocab_mask is a uint8/bool allow-mask or int32 words of bits")
+        self.allow, self.bits = _vocab_mask_args(vocab_mask, self.V)
+        self.weight, self.weight_is_vd, self.temperature, self.checkpoint, self.grad_dtype = weight, weight_is_vd, float(temperature), checkpoint, grad_dtype
+
+    def run(self, tokens=None):
+        return _HeadRun(self, tokens)
+
+
+class _HeadRun:
+    """A forward of a Head and what its backward needs (not the hidden states when they are checkpointed)."""
+
+    def __init__(self, head, tokens):
+        self.tokens = None if tokens is None else tokens.reshape(-1).to(torch.int32).contiguous()
+        self.kw = dict(weights_are_vd=head.weight_is_vd, allow=head.allow, allow_bits=head.bits, temperature=head.temperature)
+        self.weight, self.grad_dtype, self.shape = head.weight, head.grad_dtype, head.shape[:-1] + (head.d,)
+        self.fwd = ops.readout_forward(head.flat, head.weight, tokens=self.tokens, **self.kw)
+        self.saved = ops.quantize_rows(head.flat) if head.checkpoint else head.flat
+
+    def backward(self, g_logp=None, g_ent=None):
+        flat = lambda g: None if g is None else g.reshape(-1).contiguous()  # noqa: E731
+        d_hidden, d_weight = ops.readout_backward(self.saved, self.weight, self.fwd, tokens=self.tokens, g_logp=flat(g_logp), g_ent=flat(g_ent), grad_dtype=self.grad_dtype, **self.kw)
+        return d_hidden.reshape(self.shape), d_weight
+
+
+class Int8Weight(ops.Int8Rows):
+    """A readout weight laid out once as 8-bit integers [V, pitch] with a scale per vocabulary entry
+    (pitch: d rounded up to a multiple of 16). `Int8Weight.of(weight)` makes it from bf16 [d, V], or
+    [V, d] with `weight_is_vd`."""
+
+    __slots__ = ()
+
+    @staticmethod
+    def of(weight, weight_is_vd=False):
+        q = ops.quantize_weight(weight, weight_is_vd)
+        return Int8Weight(q.values, q.scales, q.d)
+
+
+def head_logits(hidden, weight, dtype=torch.float32):
+    """`head(x)` (src/nn/decoder.rs:270-279) in 8-bit integers: `hidden` [..., d] (bf16 or f32) is
+    quantised with a scale per position, `weight` is an Int8Weight; logits [..., V] of `dtype` (float32 or
+    bfloat16), ready for `sample_categorical` and the other functions here that take logits."""
+    lead = hidden.shape[:-1]
+    q = ops.quantize_rows(hidden.reshape(-1, hidden.shape[-1]).contiguous())
+    return ops.int8_matmul(q, weight, dtype).reshape(*lead, weight.values.shape[0])
+
+
 def _tempered(x):
-    return x if isinstance(x, Tempered) else Tempered(x)
+    return x if isinstance(x, (Tempered, Head)) else Tempered(x)
 
 
 class Loss:
@@ -153,10 +219,17 @@ class _TokenLogProbs:
     def __init__(self, logits, tokens):
         self.z = _tempered(logits)
         self.lead = self.z.shape[:-1]
+        if isinstance(self.z, Head):
+            self.run, self.z = self.z.run(tokens), None
+            self.logp = self.run.fwd.logp.reshape(self.lead)
+            return
         self.fwd = ops.row_forward(self.z.flat, tokens=tokens.reshape(-1).to(torch.int32).contiguous(), want_entropy=False, **self.z.kw())
         self.logp = self.fwd.logp.reshape(self.lead)
 
     def grad_logits(self, g_logp):
+        """d(logits), or (d_hidden, d_weight) of a Head."""
+        if self.z is None:
+            return self.run.backward(g_logp=g_logp)
         d = ops.row_backward(self.z.flat, self.fwd, g_logp=g_logp.reshape(-1).contiguous(), **self.z.kw())
         return d.reshape(self.z.shape)
 
@@ -230,6 +303,12 @@ def _row_level(which, logits, ref_logits, mask, reduction):
     if len(z.shape) != 4:
         raise ValueError("logits [S, B, T, V]")
     lead = z.shape[:-1]
+    if isinstance(z, Head):
+        if which != "entropy":
+            raise ValueError("the exact KL to a reference needs both sides' logits: a Head has none (kl_estimate takes one)")
+        run = z.run()
+        per = run.fwd.entropy.reshape(lead) if mask is None else ops.mask_rows(run.fwd.entropy.reshape(lead), mask)
+        return Loss(ops.reduce_tokens(per, mask, reduction), lambda up: run.backward(g_ent=ops.reduce_tokens_backward(lead, mask, reduction, up)))
     ref = None if ref_logits is None else ref_logits.reshape(-1, z.V)
     f = ops.row_forward(z.flat, ref_logits=ref, want_entropy=(which == "entropy"), want_kl=(which == "kl"), want_ref_logp=False, **z.kw())
     raw = (f.kl if which == "kl" else f.entropy).reshape(lead)
