@@ -560,6 +560,44 @@ uint64_t nrl_readout_workspace_bytes(uint64_t rows, uint32_t V, uint32_t d, uint
 int nrl_readout_fwd(const nrl_readout_args* args, nrl_stream stream);
 
 /* ---------------------------------------------------------------------------------------------
+ * Forward of the readout over the scored positions of a training batch, for a loss of the given tokens'
+ * log-probs and entropies whose backward is nrl_readout_bwd: what nrl_readout_fwd computes without drawing
+ * (f32 logits, the logits never written), with three differences. `scored` (f32 [rows], or 0: all) says
+ * which positions enter the loss (src/nn/rl.rs:9-14): the others are not read, cost no products, and get
+ * log-prob, entropy, statistics and status 0. The rows are spread over the whole device however few they
+ * are. And the logits make up for the accumulators' truncation toward zero (1.6e-8 of a logit per 16 terms
+ * on average). A given token outside [0, V) has log-prob NaN. Limits, masks, temperature and status as
+ * nrl_readout_fwd; rows <= 2^30. */
+typedef struct nrl_readout_scored_args {
+    uint32_t struct_size;
+    uint32_t flags;          /* NRL_READOUT_W_VD, NRL_READOUT_MASK_BITS */
+    uint32_t V;
+    uint32_t d;
+    uint64_t rows;
+    nrl_devptr hidden;       /* bf16 [rows, d] */
+    nrl_devptr weights;      /* bf16 [d, V], or [V, d] */
+    nrl_devptr tokens;       /* i32 [rows], or 0 */
+    nrl_devptr scored;       /* f32 [rows], or 0 */
+    nrl_devptr logp;         /* out f32 [rows] (needs tokens), or 0 */
+    nrl_devptr entropy;      /* out f32 [rows], or 0 */
+    nrl_devptr rowstats;     /* out f32 [rows, 4] */
+    nrl_devptr status;       /* out u8 [rows], or 0 */
+    nrl_devptr allow_mask;
+    uint64_t allow_row_stride;
+    nrl_devptr workspace;    /* 256-byte aligned */
+    uint64_t workspace_bytes;
+    float temperature;       /* 0 means 1 */
+    uint32_t reserved;       /* 0 */
+} nrl_readout_scored_args;
+uint64_t nrl_readout_scored_workspace_bytes(uint64_t rows, uint32_t V, uint32_t d, uint32_t has_scored);
+int nrl_readout_scored_fwd(const nrl_readout_scored_args* args, nrl_stream stream);
+
+/* masked_cross_entropy (src/nn/loss.rs:27-34) of given log-probs [s, n] and its gradient in one launch, a
+ * block per seed: out[s] = sum(-logp · keep) / max(sum(keep), 1), g_logp = upstream[s] · d out / d logp.
+ * `keep` 0: ones; `upstream` 0: ones; `out` or `g_logp` 0: not wanted. Positions with keep = 0 are not read. */
+int nrl_ce_mean(uint64_t s, uint64_t n, nrl_devptr logp, nrl_devptr keep, nrl_devptr upstream, nrl_devptr out, nrl_devptr g_logp, nrl_stream stream);
+
+/* ---------------------------------------------------------------------------------------------
  * Backward of the readout: from the per-token upstreams of the log-prob and entropy terms to the
  * gradients of the hidden states and of the weight, the [rows, V] logits and their gradient never
  * kept. The reference's tape goes through d(logits) (log_softmax, src/tensor/activation.rs:30-35;
@@ -586,7 +624,7 @@ int nrl_readout_fwd(const nrl_readout_args* args, nrl_stream stream);
  * Limits as nrl_readout_fwd: d and V multiples of 8, 16-byte aligned matrices, compute capability 10.x.
  * A product that gives up a bounded wait (an internal error) writes NaN for what it did not reach. */
 enum {
-    /* NRL_READOUT_W_VD, NRL_READOUT_ROUND_BF16 and NRL_READOUT_MASK_BITS as in the forward call, and */
+    /* NRL_READOUT_W_VD and NRL_READOUT_MASK_BITS as in the forward call, and */
     NRL_READOUT_BWD_HIDDEN_I8 = 1u << 8,      /* `hidden` is int8 [rows, hidden_pitch] with `hidden_scales` */
     NRL_READOUT_BWD_D_HIDDEN_F32 = 1u << 9,   /* d_hidden is f32 instead of bf16 */
     NRL_READOUT_BWD_D_WEIGHTS_F32 = 1u << 10, /* d_weights is f32 instead of bf16 */

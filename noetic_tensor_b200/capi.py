@@ -111,6 +111,14 @@ class ReadoutBwdArgs(C.Structure):
     ]
 
 
+class ReadoutScoredArgs(C.Structure):
+    _fields_ = [
+        ("struct_size", u32), ("flags", u32), ("V", u32), ("d", u32), ("rows", u64),
+        ("hidden", ptr), ("weights", ptr), ("tokens", ptr), ("scored", ptr), ("logp", ptr), ("entropy", ptr), ("rowstats", ptr), ("status", ptr),
+        ("allow_mask", ptr), ("allow_row_stride", u64), ("workspace", ptr), ("workspace_bytes", u64), ("temperature", f32), ("reserved", u32),
+    ]
+
+
 class I8MatmulArgs(C.Structure):
     _fields_ = [
         ("struct_size", u32), ("dtype", u32), ("rows", u64), ("n", u32), ("k", u32),
@@ -156,6 +164,9 @@ SYMBOLS = {
     "nrl_readout_fwd": (C.c_int, [C.POINTER(ReadoutArgs), C.c_void_p]),
     "nrl_readout_bwd_workspace_bytes": (u64, [u64, u32, u32]),
     "nrl_readout_bwd": (C.c_int, [C.POINTER(ReadoutBwdArgs), C.c_void_p]),
+    "nrl_readout_scored_workspace_bytes": (u64, [u64, u32, u32, u32]),
+    "nrl_readout_scored_fwd": (C.c_int, [C.POINTER(ReadoutScoredArgs), C.c_void_p]),
+    "nrl_ce_mean": (C.c_int, [u64, u64, ptr, ptr, ptr, ptr, ptr, C.c_void_p]),
     "nrl_i8_quantize_rows": (C.c_int, [u32, u64, u32, ptr, ptr, u64, ptr, C.c_void_p]),
     "nrl_i8_quantize_columns": (C.c_int, [u32, u32, ptr, ptr, u64, ptr, C.c_void_p]),
     "nrl_i8_dequantize_rows": (C.c_int, [u32, u64, u32, ptr, u64, ptr, ptr, C.c_void_p]),

@@ -25,20 +25,44 @@ static int need_cc10() {
 
 constexpr uint32_t kPairs = 74;  // CTA pairs that run side by side (148 SMs)
 
-template <int EPI>
-static int launch_gemm(const CUtensorMap& ma, const CUtensorMap& mb, HeadGemm p, uint64_t tiles, cudaStream_t st) {
+template <int EPI, int MASK = kMaskNone>
+static int launch_gemm(const CUtensorMap& ma, const CUtensorMap& mb, const CUtensorMap& mo, HeadGemm p, uint64_t tiles, cudaStream_t st) {
     p.stages = kHgSmemTiles / (kHgABytes + (p.bn / 2) * 128);
     if (p.stages > kHgMaxStages) p.stages = kHgMaxStages;
     if (tiles > 0x7fffffffull) return NRL_E_UNSUPPORTED;
-    cudaError_t e = cudaFuncSetAttribute(head_gemm_kernel<EPI>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kHgSmemBytes);
+    cudaError_t e = cudaFuncSetAttribute(head_gemm_kernel<EPI, MASK>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kHgSmemBytes);
     if (e != cudaSuccess) return (int)e;
     const unsigned grid = 2u * (unsigned)(tiles < kPairs ? (tiles ? tiles : 1) : kPairs);
-    head_gemm_kernel<EPI><<<grid, kHgThreads, kHgSmemBytes, st>>>(ma, mb, p);
+    head_gemm_kernel<EPI, MASK><<<grid, kHgThreads, kHgSmemBytes, st>>>(ma, mb, mo, p);
     return after_launch();
+}
+template <int EPI>
+static int launch_masked(const CUtensorMap& ma, const CUtensorMap& mb, const CUtensorMap& mo, const HeadGemm& p, uint32_t allow_bits, uint64_t tiles, cudaStream_t st) {
+    if (!p.allow) return launch_gemm<EPI, kMaskNone>(ma, mb, mo, p, tiles, st);
+    return allow_bits ? launch_gemm<EPI, kMaskBits>(ma, mb, mo, p, tiles, st) : launch_gemm<EPI, kMaskBytes>(ma, mb, mo, p, tiles, st);
 }
 
 static inline uint64_t up(uint64_t x, uint64_t to) { return (x + to - 1) / to * to; }
 static inline uint32_t tiles256(uint64_t x) { return (uint32_t)((x + 255) / 256); }
+
+static int launch_rows(HeadRows& hr, cudaStream_t st) {
+    // a block owns 16 rows; more when there would be over 1024 blocks, since each looks at every row's upstream
+    hr.per_block = (uint32_t)((hr.rows + 1023) / 1024);
+    if (hr.per_block < 16) hr.per_block = 16;
+    head_rows_kernel<<<(unsigned)((hr.rows + hr.per_block - 1) / hr.per_block), kRowsThreads, 0, st>>>(hr);
+    return after_launch();
+}
+
+// the mask fields that the forward and the backward share: what a call may give
+static bool bad_mask(uint32_t flags, nrl_devptr mask, uint64_t stride, uint32_t V) {
+    if (flags & NRL_READOUT_MASK_BITS) return !mask || (mask & 3u) || (stride != 0 && stride < (V + 31u) / 32u);
+    return mask && stride != 0 && stride != V;
+}
+static void set_mask(HeadGemm& g, nrl_devptr mask, uint64_t stride) {
+    g.allow = (const uint8_t*)mask;
+    g.allow_stride = stride;
+    g.allow_wide = (mask | stride) % 8 == 0 ? 1u : 0u;
+}
 
 // How a backward call is cut: pieces of `vc` vocabulary columns (their dz is what exists of [rows, V] at any time) and
 // `nsplit` ranges of a piece's columns in dx = dz·Wᵀ. A function of (rows, V, d) only.
@@ -88,7 +112,7 @@ extern "C" uint64_t nrl_readout_bwd_workspace_bytes(uint64_t rows, uint32_t V, u
 extern "C" int nrl_readout_bwd(const nrl_readout_bwd_args* a, nrl_stream stream) {
     if (!a || a->struct_size != sizeof(nrl_readout_bwd_args)) return NRL_E_BAD_ARG;
     if (a->rows == 0 || a->V == 0 || a->d == 0 || !a->hidden || !a->weights || !a->rowstats || (!a->d_hidden && !a->d_weights)) return NRL_E_BAD_ARG;
-    const uint32_t known = NRL_READOUT_W_VD | NRL_READOUT_ROUND_BF16 | NRL_READOUT_MASK_BITS | NRL_READOUT_BWD_HIDDEN_I8 | NRL_READOUT_BWD_D_HIDDEN_F32 | NRL_READOUT_BWD_D_WEIGHTS_F32 |
+    const uint32_t known = NRL_READOUT_W_VD | NRL_READOUT_MASK_BITS | NRL_READOUT_BWD_HIDDEN_I8 | NRL_READOUT_BWD_D_HIDDEN_F32 | NRL_READOUT_BWD_D_WEIGHTS_F32 |
                            NRL_READOUT_BWD_ADD_D_HIDDEN | NRL_READOUT_BWD_ADD_D_WEIGHTS;
     if (a->flags & ~known) return NRL_E_BAD_ARG;
     if (a->V % 8 != 0 || a->d % 8 != 0 || ((a->hidden | a->weights | a->d_hidden | a->d_weights) & 15u)) return NRL_E_UNSUPPORTED;
@@ -99,11 +123,7 @@ extern "C" int nrl_readout_bwd(const nrl_readout_bwd_args* a, nrl_stream stream)
     if (a->reserved != 0 || !(a->temperature >= 0.f) || !isfinite(a->temperature)) return NRL_E_BAD_ARG;
     const bool i8 = (a->flags & NRL_READOUT_BWD_HIDDEN_I8) != 0;
     if (i8 ? (!a->hidden_scales || a->hidden_pitch < a->d || a->hidden_pitch % 16 != 0) : (a->hidden_scales || (a->hidden_pitch != 0 && a->hidden_pitch != a->d))) return NRL_E_BAD_ARG;
-    if (a->flags & NRL_READOUT_MASK_BITS) {
-        if (!a->allow_mask || (a->allow_mask & 3u) || (a->allow_row_stride != 0 && a->allow_row_stride < (a->V + 31u) / 32u)) return NRL_E_BAD_ARG;
-    } else if (a->allow_mask && a->allow_row_stride != 0 && a->allow_row_stride != a->V) {
-        return NRL_E_BAD_ARG;
-    }
+    if (bad_mask(a->flags, a->allow_mask, a->allow_row_stride, a->V)) return NRL_E_BAD_ARG;
     int rc = need_cc10();
     if (rc) return rc;
     const BwdPlan b = bwd_plan(a->rows, a->V, a->d);
@@ -134,11 +154,7 @@ extern "C" int nrl_readout_bwd(const nrl_readout_bwd_args* a, nrl_stream stream)
     hr.x = (uint16_t*)(ws + b.off_x);
     hr.d_hidden = (a->flags & NRL_READOUT_BWD_ADD_D_HIDDEN) ? nullptr : (void*)a->d_hidden;
     hr.d_hidden_f32 = (a->flags & NRL_READOUT_BWD_D_HIDDEN_F32) ? 1u : 0u;
-    head_rows_kernel<<<1, 1024, 0, st>>>(hr);
-    rc = after_launch();
-    if (rc) return rc;
-    head_gather_kernel<<<(unsigned)b.rows_pad, 128, 0, st>>>(hr);
-    rc = after_launch();
+    rc = launch_rows(hr, st);
     if (rc) return rc;
 
     HeadGemm g;
@@ -149,26 +165,29 @@ extern "C" int nrl_readout_bwd(const nrl_readout_bwd_args* a, nrl_stream stream)
     g.coef = hr.coef;
     g.more = hr.more;
     g.rows_at = hr.rows_at;
-    g.tau = tau;
-    g.round_bf16 = (a->flags & NRL_READOUT_ROUND_BF16) ? 1u : 0u;
+    g.zscale = logit_scale(a->d, tau);
     g.entropy_term = a->g_ent ? 1u : 0u;
-    g.allow = (const uint8_t*)a->allow_mask;
-    g.allow_stride = a->allow_row_stride;
-    g.allow_bits = (a->flags & NRL_READOUT_MASK_BITS) ? 1u : 0u;
+    set_mask(g, a->allow_mask, a->allow_row_stride);
+    const uint32_t allow_bits = a->flags & NRL_READOUT_MASK_BITS;
     g.vocab = a->V;
-    g.dz = (uint16_t*)(ws + b.off_dz);
-    g.dz_pitch = b.vc;
     g.alpha = hr.alpha;
     g.acc_rows = b.rows_pad;
 
     const uint64_t x = ws + b.off_x, dz = ws + b.off_dz;
-    CUtensorMap x_k, x_mn, w_k, w_mn, dz_k, dz_mn;
+    CUtensorMap x_k, x_mn, w_k, w_mn, dz_k, dz_mn, dz_out, dw_out;
+    const bool dw32 = (a->flags & NRL_READOUT_BWD_D_WEIGHTS_F32) != 0;
+    memset(&dw_out, 0, sizeof dw_out);
     // boxes of 64 elements of K × 128 rows, or of 64 columns × 64 elements of K
     if ((rc = encode_2d(&x_k, false, x, a->d, b.rows_pad, a->d, 64, 128)) || (rc = encode_2d(&x_mn, false, x, a->d, b.rows_pad, a->d, 64, 64)) ||
         (rc = encode_2d(&dz_k, false, dz, b.vc, b.rows_pad, b.vc, 64, 128)) || (rc = encode_2d(&dz_mn, false, dz, b.vc, b.rows_pad, b.vc, 64, 64)) ||
+        (rc = encode_2d(&dz_out, false, dz, b.vc, b.rows_pad, b.vc, 64, 32)) ||
         (rc = encode_2d(&w_k, false, a->weights, vd ? a->d : a->V, vd ? a->V : a->d, vd ? a->d : a->V, 64, 128)) ||
         (rc = encode_2d(&w_mn, false, a->weights, vd ? a->d : a->V, vd ? a->V : a->d, vd ? a->d : a->V, 64, 64)))
         return rc;
+    if (a->d_weights) {
+        rc = dw32 ? encode_2d_f32(&dw_out, a->d_weights, vd ? a->d : a->V, vd ? a->V : a->d, 32, 32) : encode_2d(&dw_out, false, a->d_weights, vd ? a->d : a->V, vd ? a->V : a->d, vd ? a->d : a->V, 64, 32);
+        if (rc) return rc;
+    }
 
     for (uint32_t piece = 0; piece < b.pieces; piece++) {
         const uint32_t v0 = piece * b.vc, cols = a->V - v0 < b.vc ? a->V - v0 : b.vc;
@@ -181,7 +200,7 @@ extern "C" int nrl_readout_bwd(const nrl_readout_bwd_args* a, nrl_stream stream)
             p.b_mn = vd ? 0u : 1u;
             p.b_n0 = v0;
             p.v0 = v0;
-            rc = launch_gemm<kEpiGrad>(x_k, vd ? w_k : w_mn, p, (uint64_t)tiles256(a->rows) * tiles256(cols), st);
+            rc = launch_masked<kEpiGrad>(x_k, vd ? w_k : w_mn, dz_out, p, allow_bits, (uint64_t)tiles256(a->rows) * tiles256(cols), st);
             if (rc) return rc;
         }
         if (a->d_hidden) {  // dx += dz · Wᵀ
@@ -201,7 +220,7 @@ extern "C" int nrl_readout_bwd(const nrl_readout_bwd_args* a, nrl_stream stream)
             p.out_f32 = hr.d_hidden_f32;
             p.out_add = (a->flags & NRL_READOUT_BWD_ADD_D_HIDDEN) ? 1u : 0u;
             p.wide = (a->d_hidden % 32 == 0 && (p.out_f32 || a->d % 16 == 0)) ? 1u : 0u;
-            rc = launch_gemm<kEpiHidden>(dz_k, vd ? w_mn : w_k, p, (uint64_t)tiles256(a->rows) * tiles256(a->d) * b.nsplit, st);
+            rc = launch_gemm<kEpiHidden>(dz_k, vd ? w_mn : w_k, dz_out, p, (uint64_t)tiles256(a->rows) * tiles256(a->d) * b.nsplit, st);
             if (rc) return rc;
             if (b.nsplit > 1 && piece + 1 == b.pieces) {
                 head_fold_kernel<<<(unsigned)a->rows, 128, 0, st>>>(hr.count, hr.alpha, hr.more, hr.rows_at, p.acc, b.rows_pad, b.nsplit, a->d, (void*)a->d_hidden, p.out_f32, p.out_add);
@@ -220,14 +239,135 @@ extern "C" int nrl_readout_bwd(const nrl_readout_bwd_args* a, nrl_stream stream)
             p.out_pitch = vd ? a->d : a->V;
             p.out_row0 = vd ? v0 : 0u;
             p.out_col0 = vd ? 0u : v0;
-            p.out_f32 = (a->flags & NRL_READOUT_BWD_D_WEIGHTS_F32) ? 1u : 0u;
+            p.out_f32 = dw32 ? 1u : 0u;
             p.out_add = (a->flags & NRL_READOUT_BWD_ADD_D_WEIGHTS) ? 1u : 0u;
             p.wide = (a->d_weights % 32 == 0 && (p.out_f32 || p.out_pitch % 16 == 0)) ? 1u : 0u;
-            rc = launch_gemm<kEpiWeight>(vd ? dz_mn : x_mn, vd ? x_mn : dz_mn, p, (uint64_t)tiles256(p.m) * tiles256(p.n), st);
+            p.staged = p.out_add ? 0u : 1u;  // sums into what is there go through registers
+            rc = launch_gemm<kEpiWeight>(vd ? dz_mn : x_mn, vd ? x_mn : dz_mn, dw_out, p, (uint64_t)tiles256(p.m) * tiles256(p.n), st);
             if (rc) return rc;
         }
     }
     return NRL_OK;
+}
+
+// ---- forward over the scored rows -----------------------------------------------------------------------
+
+constexpr uint64_t kScoredChunk = 16384;  // rows per launch: what bounds the partial statistics' scratch (16 bytes per row and 128 columns)
+
+struct ScoredPlan {
+    bool gather;  // the scored rows are brought together first
+    uint64_t rows_pad, off_rows, off_x, off_parts, bytes;
+};
+static ScoredPlan scored_plan(uint64_t rows, uint32_t V, uint32_t d, bool scored) {
+    ScoredPlan s;
+    s.gather = scored && rows > 256;  // up to one row block nothing is saved by leaving rows out
+    s.rows_pad = up(rows, 256);
+    uint64_t at = 256;
+    s.off_rows = at; at += s.gather ? up(rows * 4, 256) : 0;
+    s.off_x = at; at += s.gather ? s.rows_pad * d * 2 : 0;
+    s.off_parts = at; at += (s.rows_pad < kScoredChunk ? s.rows_pad : kScoredChunk) * tiles256(V) * 2 * 16;
+    s.bytes = at;
+    return s;
+}
+
+extern "C" uint64_t nrl_readout_scored_workspace_bytes(uint64_t rows, uint32_t V, uint32_t d, uint32_t has_scored) {
+    if (rows == 0 || V == 0 || d == 0) return 0;
+    return scored_plan(rows, V, d, has_scored != 0).bytes;
+}
+
+extern "C" int nrl_readout_scored_fwd(const nrl_readout_scored_args* a, nrl_stream stream) {
+    if (!a || a->struct_size != sizeof(nrl_readout_scored_args)) return NRL_E_BAD_ARG;
+    if (a->rows == 0 || a->V == 0 || a->d == 0 || !a->hidden || !a->weights || !a->rowstats) return NRL_E_BAD_ARG;
+    if (a->flags & ~(uint32_t)(NRL_READOUT_W_VD | NRL_READOUT_MASK_BITS)) return NRL_E_BAD_ARG;
+    if (a->V % 8 != 0 || a->d % 8 != 0 || ((a->hidden | a->weights) & 15u)) return NRL_E_UNSUPPORTED;
+    if (a->V > 0x40000000u || a->d > 0x40000000u || a->rows > 0x40000000ull) return NRL_E_UNSUPPORTED;  // TMA coordinates are 32-bit
+    if (((a->tokens | a->scored | a->logp | a->entropy) & 3u) || (a->rowstats & 15u) || (a->workspace & 255u)) return NRL_E_BAD_ARG;
+    if (a->logp && !a->tokens) return NRL_E_BAD_ARG;
+    if (a->reserved != 0 || !(a->temperature >= 0.f) || !isfinite(a->temperature)) return NRL_E_BAD_ARG;
+    if (bad_mask(a->flags, a->allow_mask, a->allow_row_stride, a->V)) return NRL_E_BAD_ARG;
+    int rc = need_cc10();
+    if (rc) return rc;
+    const ScoredPlan s = scored_plan(a->rows, a->V, a->d, a->scored != 0);
+    if (!a->workspace || a->workspace_bytes < s.bytes) return NRL_E_WORKSPACE;
+    const cudaStream_t st = (cudaStream_t)stream;
+    const uint64_t ws = a->workspace;
+    const bool vd = (a->flags & NRL_READOUT_W_VD) != 0;
+    if (s.gather) {
+        HeadRows hr;
+        memset(&hr, 0, sizeof hr);
+        hr.rows = a->rows;
+        hr.d = a->d;
+        hr.scored = (const float*)a->scored;
+        hr.tau = 1.f;
+        hr.hidden = (const void*)a->hidden;
+        hr.count = (uint32_t*)ws;
+        hr.rows_at = (uint32_t*)(ws + s.off_rows);
+        hr.x = (uint16_t*)(ws + s.off_x);
+        hr.logp = (float*)a->logp;
+        hr.out_entropy = (float*)a->entropy;
+        hr.out_rowstats = (float4*)a->rowstats;
+        hr.status = (uint8_t*)a->status;
+        rc = launch_rows(hr, st);
+        if (rc) return rc;
+    }
+    CUtensorMap mx, mw;
+    rc = encode_2d(&mx, false, s.gather ? ws + s.off_x : a->hidden, a->d, s.gather ? s.rows_pad : a->rows, a->d, 64, 128);
+    if (rc) return rc;
+    rc = vd ? encode_2d(&mw, false, a->weights, a->d, a->V, a->d, 64, 128) : encode_2d(&mw, false, a->weights, a->V, a->d, a->V, 64, 64);
+    if (rc) return rc;
+    for (uint64_t r0 = 0; r0 < a->rows; r0 += kScoredChunk) {
+        const uint64_t n = a->rows - r0 < kScoredChunk ? a->rows - r0 : kScoredChunk;
+        HeadGemm p;
+        memset(&p, 0, sizeof p);
+        p.bn = 256;
+        p.nsplit = 1;
+        p.group_m = 16;
+        p.m = (uint32_t)n;
+        p.m_count = s.gather ? (const uint32_t*)ws : nullptr;
+        p.m_first = (uint32_t)r0;
+        p.a_m0 = (uint32_t)r0;
+        p.n = a->V;
+        p.k = a->d;
+        p.b_mn = vd ? 0u : 1u;
+        p.rows_at = s.gather ? (const uint32_t*)(ws + s.off_rows) + r0 : nullptr;
+        p.tokens = a->tokens ? (const int32_t*)a->tokens + (s.gather ? 0 : r0) : nullptr;
+        p.zscale = logit_scale(a->d, a->temperature == 0.f ? 1.f : a->temperature);
+        p.entropy_term = a->entropy ? 1u : 0u;
+        set_mask(p, a->allow_mask, a->allow_row_stride);
+        if (!s.gather && a->allow_mask) p.allow += r0 * a->allow_row_stride * ((a->flags & NRL_READOUT_MASK_BITS) ? 4u : 1u);
+        p.vocab = a->V;
+        p.parts = (float4*)(ws + s.off_parts);
+        p.parts_pitch = tiles256(a->V) * 2;
+        rc = launch_masked<kEpiStats>(mx, mw, mx, p, a->flags & NRL_READOUT_MASK_BITS, (uint64_t)tiles256(n) * tiles256(a->V), st);
+        if (rc) return rc;
+        HeadFinish f;
+        memset(&f, 0, sizeof f);
+        f.rows = (uint32_t)n;
+        f.count = p.m_count;
+        f.first = (uint32_t)r0;
+        f.rows_at = p.rows_at;
+        const uint64_t at = s.gather ? 0 : r0;
+        f.scored = a->scored ? (const float*)a->scored + at : nullptr;
+        f.parts = p.parts;
+        f.nparts = p.parts_pitch;
+        f.tokens = p.tokens;
+        f.logp = a->logp ? (float*)a->logp + at : nullptr;
+        f.entropy = a->entropy ? (float*)a->entropy + at : nullptr;
+        f.rowstats = (float4*)a->rowstats + at;
+        f.status = a->status ? (uint8_t*)a->status + at : nullptr;
+        head_finish_kernel<<<(unsigned)((n + 7) / 8), 256, 0, st>>>(f);
+        rc = after_launch();
+        if (rc) return rc;
+    }
+    return NRL_OK;
+}
+
+extern "C" int nrl_ce_mean(uint64_t s, uint64_t n, nrl_devptr logp, nrl_devptr keep, nrl_devptr upstream, nrl_devptr out, nrl_devptr g_logp, nrl_stream stream) {
+    if (s == 0 || n == 0 || (!out && !g_logp) || (out && !logp)) return NRL_E_BAD_ARG;
+    if ((logp | keep | upstream | out | g_logp) & 3u) return NRL_E_BAD_ARG;
+    if (s > 0x7fffffffull) return NRL_E_UNSUPPORTED;
+    ce_mean_kernel<<<(unsigned)s, 512, 0, (cudaStream_t)stream>>>(n, (const float*)logp, (const float*)keep, (const float*)upstream, (float*)out, (float*)g_logp);
+    return after_launch();
 }
 
 // ---- 8-bit integers -----------------------------------------------------------------------------------
@@ -292,5 +432,5 @@ extern "C" int nrl_i8_matmul(const nrl_i8_matmul_args* a, nrl_stream stream) {
     if (rc) return rc;
     rc = encode_2d(&mx, true, a->x, a->k, a->rows, a->x_pitch, 128, p.bn / 2);
     if (rc) return rc;
-    return launch_gemm<kEpiInt8>(mw, mx, p, (uint64_t)tiles256(a->n) * ((a->rows + p.bn - 1) / p.bn), (cudaStream_t)stream);
+    return launch_gemm<kEpiInt8>(mw, mx, mw, p, (uint64_t)tiles256(a->n) * ((a->rows + p.bn - 1) / p.bn), (cudaStream_t)stream);
 }

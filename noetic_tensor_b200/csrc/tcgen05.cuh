@@ -106,10 +106,10 @@ __device__ __forceinline__ float round_through_bf16(float x) {
 typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
                                   CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 
-// A row-major matrix of `outer` rows of `inner` elements, rows `pitch` elements apart, read in boxes of box_outer rows of
-// box_inner elements (128 bytes) in the 128-byte swizzle; reads outside the matrix give zeros. Through the runtime's driver
-// entry point lookup: the library links no libcuda.
-inline int encode_2d(CUtensorMap* map, bool bytes, uint64_t base, uint64_t inner, uint64_t outer, uint64_t pitch, uint32_t box_inner, uint32_t box_outer) {
+// A row-major matrix of `outer` rows of `inner` elements, rows `pitch` elements apart, as boxes of box_outer rows of
+// box_inner elements (128 bytes) in the 128-byte swizzle; reads outside the matrix give zeros, writes outside are dropped. Through
+// the runtime's driver entry point lookup: the library links no libcuda.
+inline int encode_2d_as(CUtensorMap* map, CUtensorMapDataType type, uint32_t bytes, uint64_t base, uint64_t inner, uint64_t outer, uint64_t pitch, uint32_t box_inner, uint32_t box_outer) {
     static std::atomic<void*> fn{nullptr};
     void* f = fn.load(std::memory_order_acquire);
     if (!f) {
@@ -120,12 +120,19 @@ inline int encode_2d(CUtensorMap* map, bool bytes, uint64_t base, uint64_t inner
         fn.store(f, std::memory_order_release);
     }
     const cuuint64_t dims[2] = {inner, outer};
-    const cuuint64_t strides[1] = {pitch * (bytes ? 1 : 2)};
+    const cuuint64_t strides[1] = {pitch * bytes};
     const cuuint32_t box[2] = {box_inner, box_outer};
     const cuuint32_t estr[2] = {1, 1};
-    CUresult r = ((EncodeTiledFn)f)(map, bytes ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, (void*)base, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                                    CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    CUresult r = ((EncodeTiledFn)f)(map, type, 2, (void*)base, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                                    CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     return r == CUDA_SUCCESS ? NRL_OK : NRL_E_BAD_ARG;
+}
+// bf16, or bytes
+inline int encode_2d(CUtensorMap* map, bool bytes, uint64_t base, uint64_t inner, uint64_t outer, uint64_t pitch, uint32_t box_inner, uint32_t box_outer) {
+    return encode_2d_as(map, bytes ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, bytes ? 1 : 2, base, inner, outer, pitch, box_inner, box_outer);
+}
+inline int encode_2d_f32(CUtensorMap* map, uint64_t base, uint64_t inner, uint64_t outer, uint32_t box_inner, uint32_t box_outer) {
+    return encode_2d_as(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, base, inner, outer, inner, box_inner, box_outer);
 }
 
 }  // namespace nrl

@@ -6,7 +6,8 @@ Where the reference runs log_softmax, builds a dense one-hot `[S, N, V]`, multip
 forward (twice with label smoothing) and once backward. Each function returns an `rl.Loss`:
 `.value` and `.backward(upstream)` → d(logits) `[S, B, T, V]` f32 (kl_div: a pair). Given an `rl.Head`
 instead of logits, nll and the cross-entropies (without label smoothing) go through the fused readout
-and `.backward` returns (d_hidden, d_weight).
+and `.backward` returns (d_hidden, d_weight); nothing is then read back to the host, and a target outside
+the vocabulary makes the loss NaN instead of raising.
 """
 import torch
 
@@ -31,10 +32,10 @@ def _rows(logits):
     return S, B * T, V, logits if isinstance(logits, Head) else logits.reshape(S * B * T, V)
 
 
-def _targets(targets, S, N, V, ignore_index=None):
+def _targets(targets, S, N, V, ignore_index=None, check=True):
     """Targets as device I32 rows and the not-ignored weights; ignored targets read class 0
     (src/nn/loss.rs:60-65). An out-of-range target is the reference's one_hot error."""
-    t = targets.reshape(-1).to(torch.int64)
+    t = targets.reshape(-1).to(torch.int64) if check else targets.reshape(-1)
     if t.numel() != S * N:
         raise ValueError("targets [S, B, T]")
     keep = None
@@ -42,9 +43,10 @@ def _targets(targets, S, N, V, ignore_index=None):
         ignored = t == ignore_index
         keep = (~ignored).to(torch.float32)
         t = torch.where(ignored, torch.zeros_like(t), t)
-    bad = (t < 0) | (t >= V)
-    if bad.any():
-        raise IndexError(f"one_hot: {int(t[bad][0])} is outside 0..{V}")
+    if check:
+        bad = (t < 0) | (t >= V)
+        if bad.any():
+            raise IndexError(f"one_hot: {int(t[bad][0])} is outside 0..{V}")
     return t.to(torch.int32).contiguous(), keep
 
 
@@ -55,12 +57,9 @@ def _ce(logits, targets, keep, smoothing, reduce):
         keep = keep * not_ignored
     elif not_ignored is not None:
         keep = not_ignored
-    head, shape = None, logits.shape
     if isinstance(flat, Head):
-        if smoothing > 0.0:
-            raise ValueError("label smoothing needs the sum of a row's logits: a Head has none")
-        head, flat = flat.run(tok), None  # the run holds what the backward needs, which with a checkpoint is not the hidden states
-    fwd = head.fwd if head is not None else ops.row_forward(flat, tokens=tok, want_entropy=False)
+        return _head_ce(flat, S, N, tok, keep, smoothing, reduce)
+    fwd = ops.row_forward(flat, tokens=tok, want_entropy=False)
     zsum = ops.row_sum(flat) if smoothing > 0.0 else None
     per, _, _ = ops.ce_tokens(V, fwd.logp, smoothing=smoothing, rowstats=fwd.rowstats, logit_sum=zsum, keep=keep)
     per3 = per.reshape(S, 1, N)
@@ -74,30 +73,39 @@ def _ce(logits, targets, keep, smoothing, reduce):
             d_per = up
         _, g_lp, g_un = ops.ce_tokens(V, fwd.logp, smoothing=smoothing, rowstats=fwd.rowstats, logit_sum=zsum, keep=keep,
                                       upstream=d_per.reshape(-1).contiguous(), want_loss=False)
-        if head is not None:
-            return head.backward(g_logp=g_lp)
-        return ops.row_backward(flat, fwd, g_logp=g_lp, g_uniform=g_un).reshape(shape)
+        return ops.row_backward(flat, fwd, g_logp=g_lp, g_uniform=g_un).reshape(logits.shape)
 
     return Loss(value, backward)
+
+
+def _head_ce(head, S, N, tok, keep, smoothing, reduce):
+    if smoothing > 0.0:
+        raise ValueError("label smoothing needs the sum of a row's logits: a Head has none")
+    run = head.run(tok, keep)
+    logp, keep = run.fwd.logp.reshape(S, N), None if keep is None else keep.reshape(S, N)
+    if not reduce:
+        return Loss(-logp, lambda up: run.backward(g_logp=-up))
+    value, unit = ops.ce_mean(logp, keep)
+    return Loss(value, lambda up: run.backward(g_logp=ops.ce_mean(logp, keep, up.reshape(S), want_loss=False)[1]), lambda: run.backward(g_logp=unit))
 
 
 def nll(logits, targets):
     """Per-token negative log-likelihood `[S, B·T]` (src/nn/loss.rs:10-16)."""
     S, N, V, _ = _rows(logits)
-    return _ce(logits, _targets(targets, S, N, V), None, 0.0, reduce=False)
+    return _ce(logits, _targets(targets, S, N, V, check=not isinstance(logits, Head)), None, 0.0, reduce=False)
 
 
 def cross_entropy(logits, targets):
     """Per-seed mean cross-entropy over every position, `[S]` (src/nn/loss.rs:19-22)."""
     S, N, V, _ = _rows(logits)
-    return _ce(logits, _targets(targets, S, N, V), None, 0.0, reduce=True)
+    return _ce(logits, _targets(targets, S, N, V, check=not isinstance(logits, Head)), None, 0.0, reduce=True)
 
 
 def masked_cross_entropy(logits, targets, mask):
     """`sum(nll · mask) / max(count, 1)` per seed (src/nn/loss.rs:27-34)."""
     S, N, V, _ = _rows(logits)
     keep = mask.reshape(S * N).to(torch.float32).contiguous()
-    return _ce(logits, _targets(targets, S, N, V), keep, 0.0, reduce=True)
+    return _ce(logits, _targets(targets, S, N, V, check=not isinstance(logits, Head)), keep, 0.0, reduce=True)
 
 
 def cross_entropy_with(logits, targets, mask=None, opts=None):
@@ -109,7 +117,7 @@ def cross_entropy_with(logits, targets, mask=None, opts=None):
         raise ValueError(f"label smoothing {opts.smoothing} outside [0, 1]")
     S, N, V, _ = _rows(logits)
     keep = None if mask is None else mask.reshape(S * N).to(torch.float32).contiguous()
-    return _ce(logits, _targets(targets, S, N, V, opts.ignore_index), keep, float(opts.smoothing), reduce=True)
+    return _ce(logits, _targets(targets, S, N, V, opts.ignore_index, check=not isinstance(logits, Head)), keep, float(opts.smoothing), reduce=True)
 
 
 def kl_div(pred_logits, target_logits):

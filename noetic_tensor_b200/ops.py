@@ -490,6 +490,64 @@ def readout_forward(hidden, weights, *, tokens=None, weights_are_vd=False, round
     return out
 
 
+def readout_scored_forward(hidden, weights, *, tokens=None, scored=None, want_entropy=False, weights_are_vd=False, allow=None, allow_bits=None, temperature=1.0, workspace=None):
+    """`readout_forward` of given tokens over the positions of a training batch that `scored` (float32
+    [rows], 0: not scored; None: all) lets into the loss (nrl_readout_scored_fwd): a Readout with `logp`
+    (with `tokens`), `entropy` (with `want_entropy`), `rowstats` and `status`, all 0 at the other positions,
+    which are not read. A token outside the vocabulary has log-prob NaN. `readout_backward` is its backward."""
+    dev = hidden.device
+    if dev.type != "cuda":
+        raise ValueError("readout_scored_forward needs CUDA tensors: this library has no CPU path")
+    rows, d = hidden.shape
+    V = weights.shape[0] if weights_are_vd else weights.shape[1]
+    _need(hidden, torch.bfloat16, (rows, d), "hidden", dev)
+    _need(weights, torch.bfloat16, (V, d) if weights_are_vd else (d, V), "weights", dev)
+    a = capi.ReadoutScoredArgs()
+    a.struct_size = C.sizeof(a)
+    a.flags = capi.READOUT_W_VD if weights_are_vd else 0
+    a.V, a.d, a.rows, a.temperature = V, d, rows, float(temperature)
+    a.hidden, a.weights = _p(hidden), _p(weights)
+    out = Readout()
+    out.logits = out.tokens = out.logp = out.entropy = None
+    if tokens is not None:
+        _need(tokens, torch.int32, (rows,), "tokens", dev)
+        out.logp = torch.empty(rows, dtype=torch.float32, device=dev)
+        a.tokens, a.logp = _p(tokens), _p(out.logp)
+    if scored is not None:
+        _need(scored, torch.float32, (rows,), "scored", dev)
+        a.scored = _p(scored)
+    allow = _readout_masks(a, V, rows, allow, allow_bits, dev)
+    if want_entropy:
+        out.entropy = torch.empty(rows, dtype=torch.float32, device=dev)
+        a.entropy = _p(out.entropy)
+    out.rowstats = torch.empty(rows, 4, dtype=torch.float32, device=dev)
+    out.status = torch.empty(rows, dtype=torch.uint8, device=dev)
+    a.rowstats, a.status = _p(out.rowstats), _p(out.status)
+    if workspace is None:
+        workspace = torch.empty(capi.lib().nrl_readout_scored_workspace_bytes(rows, V, d, scored is not None), dtype=torch.uint8, device=dev)
+    a.workspace, a.workspace_bytes = _p(workspace), workspace.numel() * workspace.element_size()
+    with torch.cuda.device(dev):
+        capi.check(capi.lib().nrl_readout_scored_fwd(C.byref(a), _stream(dev)), "nrl_readout_scored_fwd")
+    return out
+
+
+def ce_mean(logp, keep=None, upstream=None, want_loss=True):
+    """masked_cross_entropy of given log-probs [S, N]: (value [S] or None, d(Σ value · upstream) / d(logp)
+    [S, N]) in one launch (nrl_ce_mean); `upstream` None: ones."""
+    dev = logp.device
+    S, N = logp.shape
+    _need(logp, torch.float32, (S, N), "logp", dev)
+    if keep is not None:
+        _need(keep, torch.float32, (S, N), "keep", dev)
+    if upstream is not None:
+        _need(upstream, torch.float32, (S,), "upstream", dev)
+    value = torch.empty(S, dtype=torch.float32, device=dev) if want_loss else None
+    g = torch.empty_like(logp)
+    with torch.cuda.device(dev):
+        capi.check(capi.lib().nrl_ce_mean(S, N, _p(logp), _p(keep), _p(upstream), _p(value), _p(g), _stream(dev)), "nrl_ce_mean")
+    return value, g
+
+
 class Int8Rows:
     """Rows as 8-bit integers with an f32 scale each: `values` int8 [rows, pitch] (pitch: `d` rounded up
     to a multiple of 16), `scales` f32 [rows], x ≈ values[:, :d] · scales[:, None]."""
@@ -567,10 +625,10 @@ def int8_matmul(x, w, dtype=torch.float32):
     return out
 
 
-def readout_backward(hidden, weights, fwd, *, tokens=None, g_logp=None, g_ent=None, weights_are_vd=False, round_bf16=False, allow=None, allow_bits=None, temperature=1.0, want_hidden=True,
+def readout_backward(hidden, weights, fwd, *, tokens=None, g_logp=None, g_ent=None, weights_are_vd=False, allow=None, allow_bits=None, temperature=1.0, want_hidden=True,
                      want_weights=True, grad_dtype=torch.bfloat16, add_hidden=None, add_weights=None, workspace=None):
-    """(d_hidden, d_weights) of Σ g_logp·logp + Σ g_ent·entropy of `readout_forward`'s results `fwd` (its
-    `rowstats` and, with `g_ent`, `entropy`), the logits computed again in pieces (nrl_readout_bwd).
+    """(d_hidden, d_weights) of Σ g_logp·logp + Σ g_ent·entropy of the results `fwd` of
+    `readout_scored_forward` or `readout_forward` (their `rowstats` and, with `g_ent`, `entropy`), the logits computed again in pieces (nrl_readout_bwd).
     `hidden`: the bf16 [rows, d] of the forward call, or an Int8Rows checkpoint of it. Gradients are
     `grad_dtype` (bfloat16 or float32); `add_hidden` / `add_weights` are tensors they are added to in place
     (their own dtype counts). Rows whose upstreams are 0 are not read."""
@@ -589,7 +647,7 @@ def readout_backward(hidden, weights, fwd, *, tokens=None, g_logp=None, g_ent=No
         raise ValueError("give `g_logp`, `g_ent` or both")
     a = capi.ReadoutBwdArgs()
     a.struct_size = C.sizeof(a)
-    a.flags = (capi.READOUT_W_VD if weights_are_vd else 0) | (capi.READOUT_ROUND_BF16 if round_bf16 else 0)
+    a.flags = capi.READOUT_W_VD if weights_are_vd else 0
     a.V, a.d, a.rows, a.temperature = V, d, rows, float(temperature)
     if quant:
         a.flags |= capi.READOUT_BWD_HIDDEN_I8

@@ -96,7 +96,11 @@ class Head:
     tempered ones (src/nn/rl.rs:475-486); the mask is a uint8/bool allow-mask [..., V] or [1, V], or int32
     words of one bit per token. With `checkpoint` a loss keeps the hidden states for its backward as 8-bit
     integers with a scale per position (half the memory) instead of keeping `hidden`. `grad_dtype`:
-    bfloat16 or float32."""
+    bfloat16 or float32.
+
+    Positions that a loss's `mask` leaves out are not read and cost nothing: their d_hidden is 0 whatever
+    they hold. Nothing is read back to the host: a token outside the vocabulary makes its log-prob, and with
+    it the loss, NaN, as does a position with no allowed token."""
 
     def __init__(self, hidden, weight, temperature=1.0, vocab_mask=None, weight_is_vd=False, checkpoint=False, grad_dtype=torch.bfloat16):
         if not (0.0 < temperature < float("inf")):
@@ -109,23 +113,27 @@ class Head:
         self.allow, self.bits = _vocab_mask_args(vocab_mask, self.V)
         self.weight, self.weight_is_vd, self.temperature, self.checkpoint, self.grad_dtype = weight, weight_is_vd, float(temperature), checkpoint, grad_dtype
 
-    def run(self, tokens=None):
-        return _HeadRun(self, tokens)
+    def run(self, tokens=None, scored=None, want_entropy=False):
+        return _HeadRun(self, tokens, scored, want_entropy)
+
+
+def _flat(t, dtype):
+    return None if t is None else t.reshape(-1).to(dtype).contiguous()
 
 
 class _HeadRun:
     """A forward of a Head and what its backward needs (not the hidden states when they are checkpointed)."""
 
-    def __init__(self, head, tokens):
-        self.tokens = None if tokens is None else tokens.reshape(-1).to(torch.int32).contiguous()
+    def __init__(self, head, tokens, scored, want_entropy):
+        self.tokens = _flat(tokens, torch.int32)
         self.kw = dict(weights_are_vd=head.weight_is_vd, allow=head.allow, allow_bits=head.bits, temperature=head.temperature)
         self.weight, self.grad_dtype, self.shape = head.weight, head.grad_dtype, head.shape[:-1] + (head.d,)
-        self.fwd = ops.readout_forward(head.flat, head.weight, tokens=self.tokens, **self.kw)
+        self.fwd = ops.readout_scored_forward(head.flat, head.weight, tokens=self.tokens, scored=_flat(scored, torch.float32), want_entropy=want_entropy, **self.kw)
         self.saved = ops.quantize_rows(head.flat) if head.checkpoint else head.flat
 
     def backward(self, g_logp=None, g_ent=None):
-        flat = lambda g: None if g is None else g.reshape(-1).contiguous()  # noqa: E731
-        d_hidden, d_weight = ops.readout_backward(self.saved, self.weight, self.fwd, tokens=self.tokens, g_logp=flat(g_logp), g_ent=flat(g_ent), grad_dtype=self.grad_dtype, **self.kw)
+        d_hidden, d_weight = ops.readout_backward(self.saved, self.weight, self.fwd, tokens=self.tokens, g_logp=_flat(g_logp, torch.float32), g_ent=_flat(g_ent, torch.float32),
+                                                  grad_dtype=self.grad_dtype, **self.kw)
         return d_hidden.reshape(self.shape), d_weight
 
 
@@ -156,11 +164,14 @@ def _tempered(x):
 
 
 class Loss:
-    def __init__(self, value, backward):
+    def __init__(self, value, backward, unit=None):
         self.value = value
         self._backward = backward
+        self._unit = unit  # the backward for an upstream of ones, where the forward has left its gradient already
 
     def backward(self, upstream=None):
+        if upstream is None and self._unit is not None:
+            return self._unit()
         if upstream is None:
             upstream = torch.ones_like(self.value)
         return self._backward(upstream.to(torch.float32).contiguous())
@@ -216,11 +227,11 @@ def sample_categorical_reference(logits, temperature, vocab_mask, rng):
 class _TokenLogProbs:
     """token_log_probs (src/nn/rl.rs:134-141) and its backward to the logits."""
 
-    def __init__(self, logits, tokens):
+    def __init__(self, logits, tokens, mask=None):
         self.z = _tempered(logits)
         self.lead = self.z.shape[:-1]
         if isinstance(self.z, Head):
-            self.run, self.z = self.z.run(tokens), None
+            self.run, self.z = self.z.run(tokens, mask), None
             self.logp = self.run.fwd.logp.reshape(self.lead)
             return
         self.fwd = ops.row_forward(self.z.flat, tokens=tokens.reshape(-1).to(torch.int32).contiguous(), want_entropy=False, **self.z.kw())
@@ -235,7 +246,7 @@ class _TokenLogProbs:
 
 
 def token_log_probs(logits, tokens, mask=None):
-    t = _TokenLogProbs(logits, tokens)
+    t = _TokenLogProbs(logits, tokens, mask)
     value = t.logp if mask is None else ops.mask_rows(t.logp, mask)
 
     def backward(up):
@@ -255,7 +266,7 @@ _CHECK_NAMES = {
 
 
 def _token_level(kind, logits, tokens, mask, reduction, **kw):
-    t = _TokenLogProbs(logits, tokens)
+    t = _TokenLogProbs(logits, tokens, mask)
     lp = t.logp.reshape(t.lead) if len(t.lead) == 3 else None
     if lp is None:
         raise ValueError("logp must be [S, B, T]")
@@ -264,6 +275,9 @@ def _token_level(kind, logits, tokens, mask, reduction, **kw):
     debug_check(what, lp, mask)
     if what_other is not None:
         debug_check(what_other, kw["other"], mask)
+    if t.z is None and reduction in (SUM, TOKEN_MEAN, SEQUENCE_MEAN):
+        o = ops.token_objective(kind, lp, reduction, mask=mask, **kw)  # the value and its gradient in one launch
+        return Loss(o.policy, lambda up: t.grad_logits(ops.token_objective(kind, lp, reduction, mask=mask, up_policy=up, **kw).g_logp), lambda: t.grad_logits(o.g_logp))
     per, _ = ops.token_loss(kind, lp, mask=mask, want_grad=False, **kw)
     value = ops.reduce_tokens(per, mask, reduction)
 
@@ -306,7 +320,7 @@ def _row_level(which, logits, ref_logits, mask, reduction):
     if isinstance(z, Head):
         if which != "entropy":
             raise ValueError("the exact KL to a reference needs both sides' logits: a Head has none (kl_estimate takes one)")
-        run = z.run()
+        run = z.run(scored=mask, want_entropy=True)
         per = run.fwd.entropy.reshape(lead) if mask is None else ops.mask_rows(run.fwd.entropy.reshape(lead), mask)
         return Loss(ops.reduce_tokens(per, mask, reduction), lambda up: run.backward(g_ent=ops.reduce_tokens_backward(lead, mask, reduction, up)))
     ref = None if ref_logits is None else ref_logits.reshape(-1, z.V)
