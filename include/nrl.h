@@ -588,6 +588,9 @@ typedef struct nrl_readout_scored_args {
     uint64_t workspace_bytes;
     float temperature;       /* 0 means 1 */
     uint32_t reserved;       /* 0 */
+    uint64_t seeds;          /* > 0: also nrl_ce_mean of the log-probs as [seeds, rows / seeds] with keep = scored and upstreams of 1, or 0 */
+    nrl_devptr ce_loss;      /* out f32 [seeds], or 0 */
+    nrl_devptr ce_g_logp;    /* out f32 [rows], or 0 */
 } nrl_readout_scored_args;
 uint64_t nrl_readout_scored_workspace_bytes(uint64_t rows, uint32_t V, uint32_t d, uint32_t has_scored);
 int nrl_readout_scored_fwd(const nrl_readout_scored_args* args, nrl_stream stream);
@@ -691,6 +694,10 @@ typedef struct nrl_i8_matmul_args {
     nrl_devptr out;       /* [rows, n] */
 } nrl_i8_matmul_args;
 int nrl_i8_matmul(const nrl_i8_matmul_args* args, nrl_stream stream);
+/* nrl_i8_quantize_rows into the workspace (256-byte aligned) and nrl_i8_matmul in one call: `x` is F32 or BF16
+ * [rows, k] (x_dtype), `x_pitch` and `x_scales` are 0. */
+uint64_t nrl_i8_linear_workspace_bytes(uint64_t rows, uint32_t k);
+int nrl_i8_linear(uint32_t x_dtype, const nrl_i8_matmul_args* args, nrl_devptr workspace, uint64_t workspace_bytes, nrl_stream stream);
 
 /* check_scored_finite (src/nn/rl.rs:204-211), the check the reference's losses run in debug
  * builds (debug_check, :213-221, called from policy_gradient_loss :230, clipped_policy_loss

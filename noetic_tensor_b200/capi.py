@@ -116,6 +116,7 @@ class ReadoutScoredArgs(C.Structure):
         ("struct_size", u32), ("flags", u32), ("V", u32), ("d", u32), ("rows", u64),
         ("hidden", ptr), ("weights", ptr), ("tokens", ptr), ("scored", ptr), ("logp", ptr), ("entropy", ptr), ("rowstats", ptr), ("status", ptr),
         ("allow_mask", ptr), ("allow_row_stride", u64), ("workspace", ptr), ("workspace_bytes", u64), ("temperature", f32), ("reserved", u32),
+        ("seeds", u64), ("ce_loss", ptr), ("ce_g_logp", ptr),
     ]
 
 
@@ -171,6 +172,8 @@ SYMBOLS = {
     "nrl_i8_quantize_columns": (C.c_int, [u32, u32, ptr, ptr, u64, ptr, C.c_void_p]),
     "nrl_i8_dequantize_rows": (C.c_int, [u32, u64, u32, ptr, u64, ptr, ptr, C.c_void_p]),
     "nrl_i8_matmul": (C.c_int, [C.POINTER(I8MatmulArgs), C.c_void_p]),
+    "nrl_i8_linear_workspace_bytes": (u64, [u64, u32]),
+    "nrl_i8_linear": (C.c_int, [u32, C.POINTER(I8MatmulArgs), ptr, u64, C.c_void_p]),
     "nrl_check_status": (C.c_int, [ptr, u64, C.c_void_p, C.POINTER(u64), C.POINTER(u32)]),
     "nrl_check_scored_finite": (C.c_int, [ptr, ptr, u64, ptr, C.c_void_p, C.POINTER(u64), C.POINTER(f32)]),
 }

@@ -30,10 +30,13 @@ constexpr int kHgBM = 128;           // rows per CTA (256 per pair)
 constexpr int kHgEpiWarps = 8;       // two per quarter of tensor memory: each takes half of the columns
 constexpr int kHgThreads = 64 + 32 * kHgEpiWarps;
 constexpr uint32_t kHgABytes = kHgBM * 128;      // one stage of A: 128 rows × 128 bytes of K
-constexpr uint32_t kHgSmemTiles = 6 * 2 * kHgABytes;  // 192 KB of stages: six of 32 KB at bn = 256, more when B is narrower
 constexpr uint32_t kHgMaxStages = 10;
-constexpr uint32_t kHgStageOut = 4096;  // per epilogue warp: 32 rows × 128 bytes on their way out
-constexpr uint32_t kHgSmemBytes = kHgSmemTiles + kHgEpiWarps * kHgStageOut + 1024 + 256;
+constexpr uint32_t kHgStageOut = 4096;           // 32 rows × 128 bytes of an epilogue warp's results on their way out
+// staging tiles per epilogue warp and bytes of input stages: 192 KB (six stages of 32 KB at bn = 256, more when B is narrower), one
+// stage less where two staging tiles let a warp fill one while the other leaves
+__host__ __device__ constexpr uint32_t stage_tiles(int epi) { return epi == 2 ? 2u : 1u; }
+__host__ __device__ constexpr uint32_t smem_tiles(int epi) { return (epi == 2 ? 5u : 6u) * 2 * kHgABytes; }
+__host__ __device__ constexpr uint32_t smem_bytes(int epi) { return smem_tiles(epi) + kHgEpiWarps * stage_tiles(epi) * kHgStageOut + 1024 + 256; }
 
 enum { kEpiGrad = 0, kEpiHidden = 1, kEpiWeight = 2, kEpiInt8 = 3, kEpiStats = 4 };
 enum { kMaskNone = 0, kMaskBytes = 1, kMaskBits = 2 };
@@ -43,6 +46,21 @@ enum { kMaskNone = 0, kMaskBytes = 1, kMaskBits = 2 };
 // d = 256, 1024, 2048, 4096, the expectation for partial sums that grow in proportion to the step). The logits are scaled back.
 constexpr float kAccumulatorLoss = 1.6e-8f;
 inline float logit_scale(uint32_t d, float tau) { return (1.f + kAccumulatorLoss * (float)((d + 15) / 16)) / tau; }
+
+// Ranges of K in dx = dz·Wᵀ for `tiles` tiles of dx and `chunks` steps of K: with few tiles the steps of a tile go to several
+// pairs, whose sums are added afterwards. The count that takes the fewest waves' worth of steps, ceil(tiles·s / 74) / s, with at most
+// two waves and at least 24 steps a range (10 us of products: adding up is a launch of 3 us); a split has to gain 5 %. Decided where the number
+// of scored rows is known, on the device, and the same there and in the kernel that adds up.
+constexpr uint32_t kPairs = 74;  // CTA pairs that run side by side (148 SMs)
+__host__ __device__ inline uint32_t hidden_split(uint32_t tiles, uint32_t chunks) {
+    uint32_t best = 1;
+    float least = (float)((tiles + kPairs - 1) / kPairs);
+    for (uint32_t s = 2; tiles * s <= 2 * kPairs && chunks >= 24 * s; s++) {
+        const float t = (float)((tiles * s + kPairs - 1) / kPairs) / (float)s;
+        if (t < 0.95f * least) { least = t; best = s; }
+    }
+    return best;
+}
 
 struct HeadGemm {
     uint32_t m, n, k;          // extents of the product
@@ -54,7 +72,7 @@ struct HeadGemm {
     uint32_t a_mn, b_mn;       // A / B contiguous along M / N instead of K
     uint32_t b_n0, b_k0;       // where this piece of the vocabulary begins in B, along N / along K
     uint32_t a_m0;             // … in A, along M
-    uint32_t nsplit;           // ranges of K, each with its own output buffer
+    uint32_t split;            // kEpiHidden: ranges of K, each with its own output buffer, where that fills the device better (hidden_split); the steps of K that rule is given, 0: never
     uint32_t group_m;          // 256-row blocks that are walked side by side (L2 reuse of B)
     // kEpiGrad, kEpiStats
     const float4* coef;        // kEpiGrad [rows] of the scored rows: (a·xs, b·xs, (m + ln Z)·log2 e, a·xs + b·xs·H)
@@ -63,18 +81,18 @@ struct HeadGemm {
     const int32_t* tokens;     // kEpiStats [rows in the caller's order] or null
     float zscale;              // logit = accumulator · zscale (· xs)
     uint32_t entropy_term;     // kEpiGrad: some b ≠ 0 is possible; kEpiStats: the entropy sum is wanted
+    uint32_t* zero;            // kEpiStats: a counter that the kernel behind this one starts from
     const uint8_t* allow;
     uint64_t allow_stride;
-    uint32_t allow_wide;       // every row of the byte mask is 8-byte aligned
+    uint32_t allow_wide;       // every row of the byte mask is 4-byte aligned
     uint32_t vocab;            // V
     uint32_t v0;               // first column of this piece
     float4* parts;             // kEpiStats [rows, parts_pitch]: (max, sum, entropy sum, token's logit) per 128 columns
     uint32_t parts_pitch;
     // kEpiHidden, kEpiWeight
     const float* alpha;        // device scalar
-    float* acc;                // f32 sums between pieces / ranges of K: [nsplit, acc_rows, n]
-    uint64_t acc_rows;
-    uint32_t acc_in, acc_out;  // start from acc; end in acc (otherwise in out)
+    float* acc;                // f32 sums between pieces / ranges of K: [ranges, rows in use rounded up to 256, n]
+    uint32_t acc_in, acc_out;  // start from acc; end in acc (otherwise in out, unless K is split)
     void* out;
     uint64_t out_pitch;
     uint32_t out_f32, out_add; // type of `out`; add to what it holds
@@ -109,9 +127,10 @@ __device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, uint32_t sr
     asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];" ::"l"(map), "r"(x), "r"(y), "r"(src) : "memory");
     asm volatile("cp.async.bulk.commit_group;" ::: "memory");
 }
-// the warp's staging tile may be written again (its last store has read it)
+// the oldest of the warp's kTiles staging tiles may be written again (its store has read it)
+template <int kTiles>
 __device__ __forceinline__ void stage_free(int lane) {
-    if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(kTiles - 1) : "memory");
     __syncwarp();
 }
 // the warp's staging tile is complete: send it off
@@ -120,70 +139,130 @@ __device__ __forceinline__ void stage_send(const CUtensorMap* map, uint32_t stag
     __syncwarp();
     if (lane == 0) tma_store_2d(map, stage, x, y);
 }
+__device__ __forceinline__ void scale32(float* z, float by) {
+    const f32x2 b2 = pack2(by, by);
+#pragma unroll
+    for (int i = 0; i < 32; i += 2) unpack2(mul2(pack2(z[i], z[i + 1]), b2), z[i], z[i + 1]);
+}
+// an arrival on a barrier of either CTA of the pair
+__device__ __forceinline__ void mbar_arrive_remote(uint32_t bar_cluster_addr) {
+    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar_cluster_addr) : "memory");
+}
+// keeps what reads z behind this point
+__device__ __forceinline__ void pin32(float* z) {
+#pragma unroll
+    for (int i = 0; i < 32; i += 8)
+        asm volatile("" : "+f"(z[i]), "+f"(z[i + 1]), "+f"(z[i + 2]), "+f"(z[i + 3]), "+f"(z[i + 4]), "+f"(z[i + 5]), "+f"(z[i + 6]), "+f"(z[i + 7]));
+}
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {  // nearest, ties to even; NaN stays NaN
     uint32_t r;
     asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
     return r;
 }
 
-// The allow-mask of 32 columns of one row, fetched ahead of its use. Bytes: eight words, four columns each; bits: one word.
+// The allow-mask of the warp's 32 rows × 128 columns: loads that go out before the accumulators are waited for, and what they become
+// in each lane, a bit per column of its row (columns past the vocabulary: 0). Of a byte mask the warp reads one row at a time, four
+// bytes a lane, one 128-byte line per load (eight bytes a lane of 32 rows at a time touched 32 lines per load, and L1 with them: the
+// product with such a mask ran at 0.66 of its rate without), and four ballots hand row r's bits to lane r: column c is bit c / 4 of
+// word c mod 4. Of a bit mask each lane reads its row's four words: column c is bit c mod 32 of word c / 32.
 template <int MASK>
-struct MaskWords {
-    uint32_t w[MASK == kMaskBytes ? 8 : 1];
-    __device__ __forceinline__ void load(const HeadGemm& p, uint64_t caller_row, uint32_t v, bool live) {
+struct MaskAhead {
+    uint32_t raw[MASK == kMaskBytes ? 32 : 4];
+    uint32_t keep[4];
+    __device__ __forceinline__ void load(const HeadGemm& p, uint32_t caller_row, uint32_t v, bool live, int lane) {
         if constexpr (MASK == kMaskBits) {
-            w[0] = live && v < p.vocab ? __ldg(reinterpret_cast<const uint32_t*>(p.allow) + caller_row * p.allow_stride + (v >> 5)) : 0u;
+            const uint32_t* mp = reinterpret_cast<const uint32_t*>(p.allow) + (uint64_t)caller_row * p.allow_stride + (v >> 5);
+#pragma unroll
+            for (int c = 0; c < 4; c++) raw[c] = live && v + 32 * c < p.vocab ? ldg_stream4(mp + c) : 0u;
         } else if constexpr (MASK == kMaskBytes) {
-            const uint8_t* mp = p.allow + caller_row * p.allow_stride + v;
-            if (live && p.allow_wide && v + 32 <= p.vocab) {
+            const uint32_t here = v + 4 * lane;
+            const uint32_t lives = __ballot_sync(0xffffffffu, live);
+            const uint8_t* mp = p.allow + here;
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const uint2 q = ldg_stream8(mp + 8 * i);
-                    w[2 * i] = q.x;
-                    w[2 * i + 1] = q.y;
+            for (int r = 0; r < 32; r++) {
+                const uint32_t row = __shfl_sync(0xffffffffu, caller_row, r);
+                const uint8_t* q = mp + (uint64_t)row * p.allow_stride;
+                uint32_t x = 0u;
+                if ((lives >> r & 1u) && here < p.vocab) {  // V is a multiple of 8: a lane's four columns exist or do not
+                    if (p.allow_wide) x = ldg_stream4(q);
+                    else x = (uint32_t)q[0] | (uint32_t)q[1] << 8 | (uint32_t)q[2] << 16 | (uint32_t)q[3] << 24;
                 }
-            } else {
-#pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    uint32_t x = 0u;
-#pragma unroll 1
-                    for (int j = 0; j < 4; j++)
-                        if (live && v + 4 * i + j < p.vocab) x |= (uint32_t)mp[4 * i + j] << (8 * j);
-                    w[i] = x;
-                }
+                raw[r] = x;
             }
-            // bit 7 of a byte: the byte is not 0
-#pragma unroll
-            for (int i = 0; i < 8; i++) w[i] |= (w[i] & 0x7f7f7f7fu) + 0x7f7f7f7fu;
         }
     }
-    __device__ __forceinline__ bool allows(int i) const {
-        if constexpr (MASK == kMaskBits) return (w[0] >> i) & 1u;
-        if constexpr (MASK == kMaskBytes) return w[i >> 2] & (0x80u << (8 * (i & 3)));
-        return true;
+    __device__ __forceinline__ void settle(const HeadGemm& p, uint32_t v, int lane) {
+        if constexpr (MASK == kMaskBytes) {
+#pragma unroll
+            for (int r = 0; r < 32; r++) {
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const uint32_t b = __ballot_sync(0xffffffffu, (raw[r] & (0xffu << (8 * j))) != 0u);
+                    if (lane == r) keep[j] = b;
+                }
+            }
+        } else {
+#pragma unroll
+            for (int c = 0; c < 4; c++) {
+                const uint32_t left = v + 32 * c < p.vocab ? p.vocab - v - 32 * c : 0u;
+                const uint32_t k = left >= 32u ? 0xffffffffu : (1u << left) - 1u;
+                keep[c] = MASK == kMaskBits ? k & raw[c] : k;
+            }
+        }
     }
+    // some column of the 32 from 32·c on is kept; all of them are
+    __device__ __forceinline__ bool any(int c) const {
+        if constexpr (MASK == kMaskBytes) return ((keep[0] | keep[1] | keep[2] | keep[3]) >> (8 * c)) & 0xffu;
+        return keep[c] != 0u;
+    }
+    __device__ __forceinline__ bool all(int c) const {
+        if constexpr (MASK == kMaskBytes) return false;
+        return keep[c] == 0xffffffffu;
+    }
+    __device__ __forceinline__ bool column(int c, int i) const {
+        if constexpr (MASK == kMaskBytes) return keep[i & 3] >> (8 * c + (i >> 2)) & 1u;
+        return keep[c] >> i & 1u;
+    }
+};
+
+// What an epilogue thread needs to know of its row, fetched while the tile before is worked on.
+struct RowInfo {
+    uint32_t caller_row;
+    int32_t token;
+    float4 cf;
+    float2 xs;  // scale of an 8-bit row and its inverse
+    bool live;
 };
 
 // ∂/∂z of 32 columns of one row from the accumulators y, as 16 packed bf16 pairs. With the row's coefficients pre-multiplied
 // (a′ = a·xs, …): ln π in units of log2 is one fused multiply-add of y, dz = −π·(a′ + b′·(ln π + H)), and the token's entry gets a′.
 template <int MASK>
-__device__ __forceinline__ void epi_grad(const HeadGemm& p, bool live, uint32_t v, const float y[32], const float4& cf, float ys, int32_t token, const MaskWords<MASK>& mask, uint32_t out[16]) {
-    if (!live || v >= p.vocab) {
+__device__ __forceinline__ void epi_grad(const HeadGemm& p, bool live, uint32_t v, const float y[32], const float4& cf, float ys, int32_t token, const MaskAhead<MASK>& mask, int c, uint32_t out[16]) {
+    if (!live || !mask.any(c)) {
 #pragma unroll
         for (int i = 0; i < 16; i++) out[i] = 0u;
         return;
     }
-    const float na = -cf.x, lse2 = -cf.z, nb2 = -cf.y * 0.69314718055994531f, nab = -cf.w;
+    const f32x2 ys2 = pack2(ys, ys), lse2 = pack2(-cf.z, -cf.z);
     float g[32];
     if (p.entropy_term) {
+        const float nb2 = -cf.y * 0.69314718055994531f;
+        const f32x2 b2 = pack2(nb2, nb2), ab2 = pack2(-cf.w, -cf.w);
 #pragma unroll
-        for (int i = 0; i < 32; i++) {
-            const float l2 = fmaf(y[i], ys, lse2);
-            g[i] = ex2_approx(l2) * fmaf(fmaxf(l2, -1e30f), nb2, nab);  // a −inf logit: π = 0, and 0·inf cannot appear
+        for (int i = 0; i < 32; i += 2) {
+            float l0, l1;
+            unpack2(fma2(pack2(y[i], y[i + 1]), ys2, lse2), l0, l1);
+            // a −inf logit: π = 0, and 0·inf cannot appear
+            unpack2(mul2(pack2(ex2_approx(l0), ex2_approx(l1)), fma2(pack2(fmaxf(l0, -1e30f), fmaxf(l1, -1e30f)), b2, ab2)), g[i], g[i + 1]);
         }
     } else {
+        const f32x2 na2 = pack2(-cf.x, -cf.x);
 #pragma unroll
-        for (int i = 0; i < 32; i++) g[i] = ex2_approx(fmaf(y[i], ys, lse2)) * na;
+        for (int i = 0; i < 32; i += 2) {
+            float l0, l1;
+            unpack2(fma2(pack2(y[i], y[i + 1]), ys2, lse2), l0, l1);
+            unpack2(mul2(pack2(ex2_approx(l0), ex2_approx(l1)), na2), g[i], g[i + 1]);
+        }
     }
     const uint32_t tk = (uint32_t)(token - (int32_t)v);
     if (tk < 32u) {
@@ -191,15 +270,10 @@ __device__ __forceinline__ void epi_grad(const HeadGemm& p, bool live, uint32_t 
         for (int i = 0; i < 32; i++)
             if ((uint32_t)i == tk) g[i] += cf.x;
     }
-    if constexpr (MASK != kMaskNone) {
+    if (!mask.all(c)) {
 #pragma unroll
         for (int i = 0; i < 32; i++)
-            if (!mask.allows(i)) g[i] = 0.f;
-    }
-    if (v + 32 > p.vocab) {
-#pragma unroll
-        for (int i = 0; i < 32; i++)
-            if (v + i >= p.vocab) g[i] = 0.f;
+            if (!mask.column(c, i)) g[i] = 0.f;
     }
 #pragma unroll
     for (int i = 0; i < 16; i++) out[i] = pack_bf16(g[2 * i], g[2 * i + 1]);
@@ -207,16 +281,12 @@ __device__ __forceinline__ void epi_grad(const HeadGemm& p, bool live, uint32_t 
 
 // 32 columns of one row folded into (m, S, W): m in accumulator units, W in units of log2.
 template <int MASK>
-__device__ __forceinline__ void epi_stats(const HeadGemm& p, uint32_t v, float y[32], float c2, int32_t token, const MaskWords<MASK>& mask, float& m, float& S, float& W, float& ytok) {
-    if constexpr (MASK != kMaskNone) {
+__device__ __forceinline__ void epi_stats(const HeadGemm& p, uint32_t v, float y[32], float c2, int32_t token, const MaskAhead<MASK>& mask, int c, float& m, float& S, float& W, float& ytok) {
+    if (!mask.any(c)) return;
+    if (!mask.all(c)) {
 #pragma unroll
         for (int i = 0; i < 32; i++)
-            if (!mask.allows(i)) y[i] = -FLT_MAX;
-    }
-    if (v + 32 > p.vocab) {
-#pragma unroll
-        for (int i = 0; i < 32; i++)
-            if (v + i >= p.vocab) y[i] = -FLT_MAX;
+            if (!mask.column(c, i)) y[i] = -FLT_MAX;
     }
     const uint32_t tk = (uint32_t)(token - (int32_t)v);
     if (tk < 32u) {
@@ -224,10 +294,14 @@ __device__ __forceinline__ void epi_stats(const HeadGemm& p, uint32_t v, float y
         for (int i = 0; i < 32; i++)
             if ((uint32_t)i == tk) ytok = y[i];
     }
-    float cm = fmax3_nan(y[0], y[1], y[2]);
+    float c4[4];
 #pragma unroll
-    for (int i = 3; i < 31; i += 2) cm = fmax3_nan(cm, y[i], y[i + 1]);
-    cm = fmax_nan(cm, y[31]);
+    for (int k = 0; k < 4; k++) {
+        c4[k] = fmax3_nan(y[8 * k], y[8 * k + 1], y[8 * k + 2]);
+        c4[k] = fmax3_nan(c4[k], y[8 * k + 3], y[8 * k + 4]);
+        c4[k] = fmax3_nan(c4[k], y[8 * k + 5], fmax_nan(y[8 * k + 6], y[8 * k + 7]));
+    }
+    const float cm = fmax_nan(fmax3_nan(c4[0], c4[1], c4[2]), c4[3]);
     if (cm <= -FLT_MAX) return;  // every column here is excluded or −inf (a NaN goes on)
     if (!(cm <= m)) {
         if (m > -FLT_MAX) {
@@ -238,24 +312,35 @@ __device__ __forceinline__ void epi_stats(const HeadGemm& p, uint32_t v, float y
         m = cm;
     }
     const float m2 = -m * c2;
-    float s0 = 0.f, s1 = 0.f, w0 = 0.f, w1 = 0.f;
+    const f32x2 c22 = pack2(c2, c2), m22 = pack2(m2, m2);
+    f32x2 s0 = pack2(0.f, 0.f), s1 = s0, w0 = s0, w1 = s0;
     if (p.entropy_term) {
 #pragma unroll
         for (int i = 0; i < 32; i += 2) {
-            const float t0 = fmaxf(fmaf(y[i], c2, m2), -1e30f), t1 = fmaxf(fmaf(y[i + 1], c2, m2), -1e30f);
-            const float e0 = ex2_approx(t0), e1 = ex2_approx(t1);
-            s0 += e0; s1 += e1;
-            w0 = fmaf(e0, t0, w0); w1 = fmaf(e1, t1, w1);
+            float t0, t1;
+            unpack2(fma2(pack2(y[i], y[i + 1]), c22, m22), t0, t1);
+            t0 = fmaxf(t0, -1e30f);
+            t1 = fmaxf(t1, -1e30f);
+            const f32x2 e = pack2(ex2_approx(t0), ex2_approx(t1)), t = pack2(t0, t1);
+            if (i & 2) { s1 = add2(s1, e); w1 = fma2(e, t, w1); }
+            else { s0 = add2(s0, e); w0 = fma2(e, t, w0); }
         }
+        float a0, a1;
+        unpack2(add2(w0, w1), a0, a1);
+        W += a0 + a1;
     } else {
 #pragma unroll
         for (int i = 0; i < 32; i += 2) {
-            s0 += ex2_approx(fmaf(y[i], c2, m2));
-            s1 += ex2_approx(fmaf(y[i + 1], c2, m2));
+            float t0, t1;
+            unpack2(fma2(pack2(y[i], y[i + 1]), c22, m22), t0, t1);
+            const f32x2 e = pack2(ex2_approx(t0), ex2_approx(t1));
+            if (i & 2) s1 = add2(s1, e);
+            else s0 = add2(s0, e);
         }
     }
-    S += s0 + s1;
-    W += w0 + w1;
+    float a0, a1;
+    unpack2(add2(s0, s1), a0, a1);
+    S += a0 + a1;
 }
 
 // 32 consecutive results of one output row to `out` (bf16 or f32), added to what it holds if asked.
@@ -323,7 +408,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kHgThreads, 1)
     constexpr uint32_t kKStep = kI8 ? 128 : 64;  // elements of K per stage (128 bytes)
     const uint32_t smem_base = (smem_addr(smem_raw) + 1023u) & ~1023u;
     const uint32_t b_bytes = (p.bn / 2) * 128, stage_bytes = kHgABytes + b_bytes;
-    const uint32_t bars = smem_base + kHgSmemTiles + kHgEpiWarps * kHgStageOut;
+    const uint32_t bars = smem_base + smem_tiles(EPI) + kHgEpiWarps * stage_tiles(EPI) * kHgStageOut;
     const uint32_t bar_full = bars, bar_empty = bars + 8 * kHgMaxStages, bar_acc_full = bars + 16 * kHgMaxStages, bar_acc_empty = bar_acc_full + 16, bar_done = bar_acc_empty + 16;
     __shared__ uint32_t tmem_slot;
     __shared__ volatile uint32_t abort_flag;
@@ -334,8 +419,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kHgThreads, 1)
     const uint32_t in_use = p.m_count ? *p.m_count : 0u;
     const uint32_t mm = p.m_count ? min(in_use - min(in_use, p.m_first), p.m) : p.m, kk = p.k_count ? min(*p.k_count, p.k) : p.k;
     const uint32_t tiles_m = (mm + 2 * kHgBM - 1) / (2 * kHgBM), tiles_n = (p.n + p.bn - 1) / p.bn;
-    const uint32_t kchunks = (kk + kKStep - 1) / kKStep, kper = (kchunks + p.nsplit - 1) / p.nsplit;
-    const uint32_t tiles = tiles_m * tiles_n * p.nsplit;  // the host keeps this below 2^31
+    const uint32_t kchunks = (kk + kKStep - 1) / kKStep, nsplit = p.split ? hidden_split(tiles_m * tiles_n, p.split) : 1u, kper = (kchunks + nsplit - 1) / nsplit;
+    const bool to_acc = p.acc_out || nsplit > 1;
+    const uint32_t tiles = tiles_m * tiles_n * nsplit;  // the host keeps this below 2^31
     struct Item {
         uint32_t split, tm, tn, k0, k1;
     };
@@ -353,6 +439,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kHgThreads, 1)
     };
 
     if (threadIdx.x == 0) {
+        if (EPI == kEpiStats && blockIdx.x == 0 && p.zero) *p.zero = 0u;
         abort_flag = 0u;
         for (uint32_t s = 0; s < kHgMaxStages; s++) {
             mbar_init(bar_full + 8 * s, 1);
@@ -451,65 +538,94 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kHgThreads, 1)
         // ---- epilogue (both CTAs): thread = row of the output (of the transposed one for kEpiInt8) ---------
         const uint32_t quarter = (uint32_t)warp & 3u, half = ((uint32_t)warp - 2u) >> 2;
         const uint32_t half_cols = p.bn / 2;  // this warp's columns: [half · bn/2, + bn/2), a multiple of 16
-        const uint32_t stage_out = smem_base + kHgSmemTiles + ((uint32_t)warp - 2u) * kHgStageOut;
+        const uint32_t stage_out = smem_base + smem_tiles(EPI) + ((uint32_t)warp - 2u) * stage_tiles(EPI) * kHgStageOut;
+        uint32_t sent = 0;  // staging tiles sent off so far
         float alpha = 1.f;
         if constexpr (EPI == kEpiHidden || EPI == kEpiWeight) alpha = p.alpha ? *p.alpha : 1.f;
+        auto row_info = [&](const Item& w) {
+            RowInfo r;
+            const uint32_t row = w.tm * 2 * kHgBM + rank * kHgBM + quarter * 32u + (uint32_t)lane;
+            r.live = row < mm;
+            r.caller_row = row;
+            r.token = -1;
+            r.cf = make_float4(0.f, 0.f, 0.f, 0.f);
+            r.xs = make_float2(1.f, 1.f);
+            if (r.live) {
+                if constexpr (EPI == kEpiGrad || EPI == kEpiStats || EPI == kEpiHidden)
+                    if (p.rows_at) r.caller_row = __ldg(p.rows_at + row);
+                if constexpr (EPI == kEpiGrad) r.cf = __ldg(p.coef + row);
+                if constexpr (EPI == kEpiGrad || EPI == kEpiHidden) {
+                    const float4 mo = __ldg(p.more + row);
+                    r.xs = make_float2(mo.x, mo.y);
+                    r.token = __float_as_int(mo.z);
+                }
+                if constexpr (EPI == kEpiInt8) r.xs.x = __ldg(p.m_scale + row);
+            }
+            return r;
+        };
         uint32_t n = 0;
         bool ok = true;
+        RowInfo ahead;
+        MaskAhead<MASK> mask;
+        if (pair < tiles) {
+            const Item w = item(pair);
+            ahead = row_info(w);
+            mask.load(p, ahead.caller_row, p.v0 + w.tn * p.bn + half * half_cols, ahead.live, lane);
+        }
         for (uint32_t t = pair; t < tiles; t += pairs) {
             const Item w = item(t);
-            const bool some = w.k0 != w.k1;
+            const bool some = w.k0 != w.k1, more_tiles = t + pairs < tiles;
+            const RowInfo r = ahead;
+            const Item next = more_tiles ? item(t + pairs) : w;
+            if (more_tiles) ahead = row_info(next);
             const uint32_t acc = n & 1u;
-            if (some && ok) {
-                ok = __all_sync(0xffffffffu, mbar_wait(bar_acc_full + 8 * acc, (n >> 1) & 1u, &abort_flag));
-                tc_fence_after();
-            }
+            auto wait = [&] {
+                if (some && ok) {
+                    ok = __all_sync(0xffffffffu, mbar_wait(bar_acc_full + 8 * acc, (n >> 1) & 1u, &abort_flag));
+                    tc_fence_after();
+                }
+            };
+            // the accumulator may be overwritten: this warp has it in registers. Before the results are stored: the arrival waits for
+            // whatever the warp has stored.
+            auto release = [&] {
+                tc_fence_before();
+                __syncwarp();
+                if (ok && lane == 0) mbar_arrive_remote(in_first_cta(bar_acc_empty + 8 * acc));
+            };
             const uint32_t row0 = w.tm * 2 * kHgBM + rank * kHgBM + quarter * 32u, row = row0 + (uint32_t)lane;
-            const bool live = row < mm;
+            const bool live = r.live;
             const uint32_t taddr = tmem + ((quarter * 32u) << 16) + acc * 256 + half * half_cols;
             const uint32_t col0 = w.tn * p.bn + half * half_cols;
             if constexpr (EPI == kEpiGrad || EPI == kEpiStats) {
-                float4 cf = make_float4(0.f, 0.f, 0.f, 0.f);
-                uint64_t caller_row = row;
-                int32_t token = -1;
-                float ys = p.zscale * kLog2e;
-                if (live) {
-                    if (p.rows_at) caller_row = __ldg(p.rows_at + row);
-                    if constexpr (EPI == kEpiGrad) {
-                        cf = __ldg(p.coef + row);
-                        const float4 mo = __ldg(p.more + row);
-                        ys *= mo.x;
-                        token = __float_as_int(mo.z);
-                    } else if (p.tokens) {
-                        token = __ldg(p.tokens + caller_row);
-                    }
-                }
+                const float ys = p.zscale * kLog2e * r.xs.x;
+                int32_t token = r.token;
+                if (EPI == kEpiStats && live && p.tokens) token = __ldg(p.tokens + r.caller_row);
                 float m = -FLT_MAX, S = 0.f, W = 0.f, ytok = __int_as_float(0x7fc00000);
-                MaskWords<MASK> mask;
-                mask.load(p, caller_row, p.v0 + col0, live);
+                wait();
+                mask.settle(p, p.v0 + col0, lane);
 #pragma unroll 1
-                for (uint32_t c = 0; c < half_cols; c += 32) {
+                for (int c = 0; c < 4; c++) {
                     float y[32];
-                    tc_ld32(taddr + c, reinterpret_cast<uint32_t*>(y));
-                    MaskWords<MASK> next;
-                    if (c + 32 < half_cols) next.load(p, caller_row, p.v0 + col0 + c + 32, live);
+                    tc_ld32(taddr + 32 * c, reinterpret_cast<uint32_t*>(y));
                     tc_wait_ld();
+                    pin32(y);
+                    if (c == 3) release();
+                    if (c == 1 && more_tiles) mask.load(p, ahead.caller_row, p.v0 + next.tn * p.bn + half * half_cols, ahead.live, lane);
                     if (!ok) {
 #pragma unroll
                         for (int i = 0; i < 32; i++) y[i] = __int_as_float(0x7fc00000);
                     }
-                    const uint32_t v = p.v0 + col0 + c;
+                    const uint32_t v = p.v0 + col0 + 32 * c;
                     if constexpr (EPI == kEpiGrad) {
                         uint32_t g[16];
-                        epi_grad<MASK>(p, live, v, y, cf, ys, token, mask, g);
-                        if ((c & 32) == 0) stage_free(lane);
+                        epi_grad<MASK>(p, live, v, y, r.cf, ys, token, mask, c, g);
+                        if ((c & 1) == 0) stage_free<1>(lane);
 #pragma unroll
-                        for (int j = 0; j < 4; j++) sts_piece(stage_out, lane, (int)(c & 32) / 8 + j, g[4 * j], g[4 * j + 1], g[4 * j + 2], g[4 * j + 3]);
-                        if (c & 32) stage_send(&map_out, stage_out, lane, (int32_t)(col0 + c - 32), (int32_t)row0);
+                        for (int j = 0; j < 4; j++) sts_piece(stage_out, lane, 4 * (c & 1) + j, g[4 * j], g[4 * j + 1], g[4 * j + 2], g[4 * j + 3]);
+                        if (c & 1) stage_send(&map_out, stage_out, lane, (int32_t)(col0 + 32 * (c - 1)), (int32_t)row0);
                     } else {
-                        if (v < p.vocab) epi_stats<MASK>(p, v, y, ys, token, mask, m, S, W, ytok);
+                        epi_stats<MASK>(p, v, y, ys, token, mask, c, m, S, W, ytok);
                     }
-                    mask = next;
                 }
                 if constexpr (EPI == kEpiStats) {
                     // the maximum and the token's logit in logit units, the entropy sum in natural units; S = −1: this pair gave up
@@ -518,78 +634,88 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kHgThreads, 1)
             } else if constexpr (EPI != kEpiInt8) {
                 uint64_t orow = (uint64_t)p.out_row0 + row;
                 float scale = alpha;
-                if constexpr (EPI == kEpiHidden) {
-                    if (live && !p.acc_out) {
-                        orow = __ldg(p.rows_at + row);
-                        scale = alpha * __ldg(p.more + row).y;
-                    }
+                if (EPI == kEpiHidden && !to_acc) {
+                    orow = r.caller_row;
+                    scale = alpha * r.xs.y;
                 }
+                wait();
+                const bool there = some && ok;
 #pragma unroll 1
-                for (uint32_t c = 0; c < half_cols; c += 32) {
-                    float y[32];
-                    if (some && ok) {
-                        tc_ld32(taddr + c, reinterpret_cast<uint32_t*>(y));
+                for (int c = 0; c < 4; c++) {
+                    float z[32];
+                    if (there) {
+                        tc_ld32(taddr + 32 * c, reinterpret_cast<uint32_t*>(z));
                         tc_wait_ld();
+                        pin32(z);
+                        if (c == 3) release();
                     } else {
 #pragma unroll
-                        for (int i = 0; i < 32; i++) y[i] = ok ? 0.f : __int_as_float(0x7fc00000);
+                        for (int i = 0; i < 32; i++) z[i] = ok ? 0.f : __int_as_float(0x7fc00000);
                     }
-                    const uint32_t col = col0 + c;
+                    const uint32_t col = col0 + 32 * c;
                     if (EPI == kEpiWeight && p.staged) {
-#pragma unroll
-                        for (int i = 0; i < 32; i++) y[i] *= scale;
+                        scale32(z, scale);
+                        const uint32_t tile = stage_out + (sent & 1u) * kHgStageOut;
+                        const bool inside = row0 < mm;
                         if (p.out_f32) {
-                            stage_free(lane);
+                            stage_free<2>(lane);
 #pragma unroll
                             for (int j = 0; j < 8; j++)
-                                sts_piece(stage_out, lane, j, __float_as_uint(y[4 * j]), __float_as_uint(y[4 * j + 1]), __float_as_uint(y[4 * j + 2]), __float_as_uint(y[4 * j + 3]));
-                            if (col < p.n && row0 < mm) stage_send(&map_out, stage_out, lane, (int32_t)(p.out_col0 + col), (int32_t)(p.out_row0 + row0));
+                                sts_piece(tile, lane, j, __float_as_uint(z[4 * j]), __float_as_uint(z[4 * j + 1]), __float_as_uint(z[4 * j + 2]), __float_as_uint(z[4 * j + 3]));
+                            if (inside && col < p.n) {
+                                stage_send(&map_out, tile, lane, (int32_t)(p.out_col0 + col), (int32_t)(p.out_row0 + row0));
+                                sent++;
+                            }
                         } else {
-                            if ((c & 32) == 0) stage_free(lane);
+                            if ((c & 1) == 0) stage_free<2>(lane);
 #pragma unroll
                             for (int j = 0; j < 4; j++)
-                                sts_piece(stage_out, lane, (int)(c & 32) / 8 + j, pack_bf16(y[8 * j], y[8 * j + 1]), pack_bf16(y[8 * j + 2], y[8 * j + 3]), pack_bf16(y[8 * j + 4], y[8 * j + 5]),
-                                          pack_bf16(y[8 * j + 6], y[8 * j + 7]));
-                            if ((c & 32) && col - 32 < p.n && row0 < mm) stage_send(&map_out, stage_out, lane, (int32_t)(p.out_col0 + col - 32), (int32_t)(p.out_row0 + row0));
+                                sts_piece(tile, lane, 4 * (c & 1) + j, pack_bf16(z[8 * j], z[8 * j + 1]), pack_bf16(z[8 * j + 2], z[8 * j + 3]), pack_bf16(z[8 * j + 4], z[8 * j + 5]),
+                                          pack_bf16(z[8 * j + 6], z[8 * j + 7]));
+                            if ((c & 1) && inside && col - 32 < p.n) {
+                                stage_send(&map_out, tile, lane, (int32_t)(p.out_col0 + col - 32), (int32_t)(p.out_row0 + row0));
+                                sent++;
+                            }
                         }
                     } else if (live && col < p.n) {
-                        float* part = p.acc ? p.acc + ((uint64_t)w.split * p.acc_rows + row) * p.n + col : nullptr;
+                        float* part = p.acc + ((uint64_t)w.split * (tiles_m * 2 * kHgBM) + row) * p.n + col;
                         if (p.acc_in) {
 #pragma unroll
                             for (int i = 0; i < 32; i += 4)
                                 if (col + i < p.n) {
                                     const float4 q = *reinterpret_cast<const float4*>(part + i);
-                                    y[i] += q.x; y[i + 1] += q.y; y[i + 2] += q.z; y[i + 3] += q.w;
+                                    z[i] += q.x; z[i + 1] += q.y; z[i + 2] += q.z; z[i + 3] += q.w;
                                 }
                         }
-                        if (p.acc_out) {
-                            store_row32(part, 0, true, false, true, p.n - col, y);
+                        if (to_acc) {
+                            store_row32(part, 0, true, false, true, p.n - col, z);
                         } else {
-#pragma unroll
-                            for (int i = 0; i < 32; i++) y[i] *= scale;
-                            store_row32(p.out, orow * p.out_pitch + p.out_col0 + col, p.out_f32, p.out_add, p.wide, p.n - col, y);
+                            scale32(z, scale);
+                            store_row32(p.out, orow * p.out_pitch + p.out_col0 + col, p.out_f32, p.out_add, p.wide, p.n - col, z);
                         }
                     }
                 }
             } else {
                 // thread = vocabulary entry, registers = tokens: a warp's store covers 32 consecutive entries of a row
-                const float scale = live ? __ldg(p.m_scale + row) : 0.f;
+                const float scale = r.xs.x;
+                wait();
 #pragma unroll 1
                 for (uint32_t c = 0; c < half_cols; c += 16) {
-                    uint32_t r[16];
+                    uint32_t z[16];
                     if (some && ok) {
-                        tc_ld16(taddr + c, r);
+                        tc_ld16(taddr + c, z);
                         tc_wait_ld();
+                        if (c + 16 >= half_cols) release();
                     } else {
 #pragma unroll
-                        for (int i = 0; i < 16; i++) r[i] = 0u;
+                        for (int i = 0; i < 16; i++) z[i] = 0u;
                     }
                     const uint32_t col = col0 + c;
                     if (live) {
 #pragma unroll
                         for (int i = 0; i < 16; i++) {
                             if (col + i < p.n) {
-                                float y = ((float)(int32_t)r[i] * __ldg(p.n_scale + col + i)) * scale;
+                                float y = ((float)(int32_t)z[i] * __ldg(p.n_scale + col + i)) * scale;
                                 if (!ok) y = __int_as_float(0x7fc00000);
                                 const uint64_t at = (uint64_t)(col + i) * p.out_pitch + row;
                                 if (p.out_f32) reinterpret_cast<float*>(p.out)[at] = y;
@@ -599,12 +725,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kHgThreads, 1)
                     }
                 }
             }
-            if (some) {
-                tc_fence_before();
-                __syncwarp();
-                if (ok && lane == 0) mbar_arrive_cluster(in_first_cta(bar_acc_empty + 8 * acc));
-                n++;
-            }
+            if (some) n++;
         }
         if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");  // this warp's last stores are written
     }

@@ -27,7 +27,8 @@ struct HeadRows {
     const float* scales;      // [rows] of int8 rows, or null: bf16
     uint32_t* count;          // out: scored rows
     uint32_t* rows_at;        // out [rows]: the scored rows in order
-    uint16_t* x;              // out bf16 [rows rounded up to 256, d]
+    uint16_t* x;              // out bf16 [rows rounded up to 256, x_pitch]
+    uint32_t x_pitch;         // d rounded up to 128 bytes: TMA reads then cover whole lines
     // rows that are not scored: zeros into d_hidden (backward, unless null) or into the results (forward)
     void* d_hidden;
     uint32_t d_hidden_f32;
@@ -130,7 +131,7 @@ __global__ void __launch_bounds__(kRowsThreads) head_rows_kernel(HeadRows p) {
                 }
                 continue;
             }
-            uint4* o = reinterpret_cast<uint4*>(p.x + (uint64_t)at * p.d);
+            uint4* o = reinterpret_cast<uint4*>(p.x + (uint64_t)at * p.x_pitch);
             if (p.scales && fabsf(p.scales[row]) < 0x1p-100f) {
                 for (uint32_t i = lane; i < pieces; i += 32) o[i] = make_uint4(0u, 0u, 0u, 0u);
             } else if (p.scales) {
@@ -156,12 +157,54 @@ __global__ void __launch_bounds__(kRowsThreads) head_rows_kernel(HeadRows p) {
         __syncthreads();
     }
     for (uint64_t i = total + (uint64_t)blockIdx.x * kW + warp; i < ((total + 255u) & ~255u); i += (uint64_t)gridDim.x * kW) {
-        uint4* o = reinterpret_cast<uint4*>(p.x + i * p.d);
+        uint4* o = reinterpret_cast<uint4*>(p.x + i * p.x_pitch);
         for (uint32_t k = lane; k < pieces; k += 32) o[k] = make_uint4(0u, 0u, 0u, 0u);
     }
 }
 
-// The partial statistics of a row merged: a warp per scored row, lane l taking the partials l, l + 32, …, f64 sums, a butterfly.
+// Per seed: out = Σ keep·(−logp) / max(Σ keep, 1) and its gradient g_logp = upstream·(−keep / max(Σ keep, 1)), by one block: thread t
+// takes the positions t, t + blockDim, …, f64 sums, a butterfly, the warps in order. Positions with keep = 0 are not looked at.
+struct CeMean {
+    uint64_t seeds, n;
+    const float* logp;
+    const float* keep;
+    const float* upstream;
+    float* out;
+    float* g_logp;
+};
+__device__ __forceinline__ void ce_mean_seed(const CeMean& p, uint64_t seed, double (*sh)[2]) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const uint64_t base = seed * p.n;
+    double v = 0.0, c = 0.0;
+#pragma unroll 4
+    for (uint64_t i = threadIdx.x; i < p.n; i += blockDim.x) {
+        const float k = p.keep ? p.keep[base + i] : 1.f;
+        c += (double)k;
+        if (p.out && k != 0.f) v -= (double)(__ldcg(p.logp + base + i) * k);
+    }
+#pragma unroll
+    for (int k = 16; k >= 1; k >>= 1) {
+        v += __shfl_xor_sync(0xffffffffu, v, k);
+        c += __shfl_xor_sync(0xffffffffu, c, k);
+    }
+    __syncthreads();
+    if (lane == 0) { sh[warp][0] = v; sh[warp][1] = c; }
+    __syncthreads();
+    v = c = 0.0;
+    for (uint32_t w = 0; w < blockDim.x >> 5; w++) { v += sh[w][0]; c += sh[w][1]; }
+    const double count = c > 1.0 ? c : 1.0;
+    if (p.out && threadIdx.x == 0) p.out[seed] = (float)(v / count);
+    if (!p.g_logp) return;
+    const float g = (float)((p.upstream ? (double)p.upstream[seed] : 1.0) / count);
+    for (uint64_t i = threadIdx.x; i < p.n; i += blockDim.x) p.g_logp[base + i] = p.keep ? -(p.keep[base + i] * g) : -g;
+}
+__global__ void __launch_bounds__(512) ce_mean_kernel(CeMean p) {
+    __shared__ double sh[16][2];
+    ce_mean_seed(p, blockIdx.x, sh);
+}
+
+// The partial statistics of a row merged by kW warps (one when there are many rows, eight when there are few): thread t takes the
+// partials t, t + 32·kW, …, f64 sums, a butterfly, then the warps in order.
 struct HeadFinish {
     uint32_t rows;              // of this launch
     const uint32_t* count;      // device: scored rows in all, or null
@@ -170,19 +213,25 @@ struct HeadFinish {
     const float* scored;        // with rows_at null: rows that are not scored get zeros
     const float4* parts;
     uint32_t nparts;
-    const int32_t* tokens;
     float* logp;
     float* entropy;
     float4* rowstats;
     uint8_t* status;
+    // the mean cross-entropy per seed, by the last block to finish: which one that is changes no sum
+    CeMean ce;                  // ce.seeds = 0: not wanted
+    uint32_t* done;
 };
-__global__ void __launch_bounds__(256) head_finish_kernel(HeadFinish p) {
-    const uint32_t i = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
-    const int lane = threadIdx.x & 31;
+template <int kW>
+__device__ __forceinline__ void head_finish_row(const HeadFinish& p) {
+    __shared__ float sm[8], st_[8];
+    __shared__ double sz[8], sw[8];
+    __shared__ uint32_t sg[8];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const uint32_t i = kW == 1 ? blockIdx.x * 8 + warp : blockIdx.x, t = kW == 1 ? lane : threadIdx.x;
     if (i >= p.rows || (p.count && p.first + i >= *p.count)) return;
     const uint64_t row = p.rows_at ? p.rows_at[i] : i;
     if (!p.rows_at && p.scored && p.scored[row] == 0.f) {
-        if (lane == 0) {
+        if (t == 0) {
             if (p.logp) p.logp[row] = 0.f;
             if (p.entropy) p.entropy[row] = 0.f;
             if (p.rowstats) p.rowstats[row] = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -194,7 +243,7 @@ __global__ void __launch_bounds__(256) head_finish_kernel(HeadFinish p) {
     float m = -FLT_MAX, ztok = __int_as_float(0x7fc00000);
     uint32_t gave_up = 0u;
 #pragma unroll 4
-    for (uint32_t j = lane; j < p.nparts; j += 32) {
+    for (uint32_t j = t; j < p.nparts; j += 32 * kW) {
         const float4 a = q[j];
         m = fmax_nan(m, a.x);
         gave_up |= a.y < 0.f ? 1u : 0u;
@@ -202,9 +251,21 @@ __global__ void __launch_bounds__(256) head_finish_kernel(HeadFinish p) {
     }
 #pragma unroll
     for (int k = 16; k >= 1; k >>= 1) m = fmax_nan(m, __shfl_xor_sync(0xffffffffu, m, k));
+    const uint32_t has = __ballot_sync(0xffffffffu, ztok == ztok);
+    if (has) ztok = __shfl_sync(0xffffffffu, ztok, __ffs(has) - 1);
+    gave_up = __any_sync(0xffffffffu, gave_up);
+    if (kW > 1) {
+        if (lane == 0) { sm[warp] = m; st_[warp] = ztok; sg[warp] = gave_up; }
+        __syncthreads();
+        for (int w = 0; w < kW; w++) {
+            m = fmax_nan(m, sm[w]);
+            gave_up |= sg[w];
+            if (st_[w] == st_[w]) ztok = st_[w];
+        }
+    }
     double Z = 0.0, W = 0.0;
 #pragma unroll 4
-    for (uint32_t j = lane; j < p.nparts; j += 32) {
+    for (uint32_t j = t; j < p.nparts; j += 32 * kW) {
         const float4 a = q[j];
         if (a.y > 0.f) {
             const float dm = a.x - m;
@@ -218,61 +279,58 @@ __global__ void __launch_bounds__(256) head_finish_kernel(HeadFinish p) {
         Z += __shfl_xor_sync(0xffffffffu, Z, k);
         W += __shfl_xor_sync(0xffffffffu, W, k);
     }
-    const uint32_t has = __ballot_sync(0xffffffffu, ztok == ztok);
-    if (has) ztok = __shfl_sync(0xffffffffu, ztok, __ffs(has) - 1);
-    gave_up = __any_sync(0xffffffffu, gave_up);
-    if (lane) return;
+    if (kW > 1) {
+        if (lane == 0) { sz[warp] = Z; sw[warp] = W; }
+        __syncthreads();
+        Z = W = 0.0;
+        for (int w = 0; w < kW; w++) { Z += sz[w]; W += sw[w]; }
+    }
+    if (t) return;
     uint32_t st = gave_up ? 4u : 0u;
     if (m != m) st |= 2u;
     else if (m <= -FLT_MAX) st |= 1u;
-    const float nan = __int_as_float(0x7fc00000), lnZ = (float)log(Z);
-    if (p.rowstats) p.rowstats[row] = st ? make_float4(nan, nan, nan, nan) : make_float4(m, lnZ, 0.f, 0.f);
-    if (p.entropy) p.entropy[row] = st ? nan : (float)(log(Z) - W / Z);
+    const float nan = __int_as_float(0x7fc00000);
+    const double lnZ = log(Z);
+    if (p.rowstats) p.rowstats[row] = st ? make_float4(nan, nan, nan, nan) : make_float4(m, (float)lnZ, 0.f, 0.f);
+    if (p.entropy) p.entropy[row] = st ? nan : (float)(lnZ - W / Z);
     // a token outside [0, V) has no logit: NaN; an excluded one has log-prob −inf
-    if (p.logp) p.logp[row] = st ? nan : ztok <= -FLT_MAX ? NRL_NEG_INF : (ztok - m) - lnZ;
+    if (p.logp) p.logp[row] = st ? nan : ztok <= -FLT_MAX ? NRL_NEG_INF : (ztok - m) - (float)lnZ;
     if (p.status) p.status[row] = (uint8_t)st;
 }
 
-// A block per seed: value = Σ keep·(−logp) / max(Σ keep, 1) and its gradient upstream·(−keep / max(Σ keep, 1)). Positions with
-// keep = 0 are not looked at.
-__global__ void __launch_bounds__(512) ce_mean_kernel(uint64_t n, const float* logp, const float* keep, const float* upstream, float* out, float* g_logp) {
-    __shared__ double sv[16], sc[16];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const uint64_t base = (uint64_t)blockIdx.x * n;
-    double v = 0.0, c = 0.0;
-#pragma unroll 4
-    for (uint64_t i = threadIdx.x; i < n; i += blockDim.x) {
-        const float k = keep ? keep[base + i] : 1.f;
-        c += (double)k;
-        if (out && k != 0.f) v -= (double)(logp[base + i] * k);
-    }
-#pragma unroll
-    for (int k = 16; k >= 1; k >>= 1) {
-        v += __shfl_xor_sync(0xffffffffu, v, k);
-        c += __shfl_xor_sync(0xffffffffu, c, k);
-    }
-    if (lane == 0) { sv[warp] = v; sc[warp] = c; }
+template <int kW>
+__global__ void __launch_bounds__(256) head_finish_kernel(HeadFinish p) {
+    head_finish_row<kW>(p);
+    if (!p.ce.seeds) return;
+    __shared__ double sh[8][2];
+    __shared__ uint32_t last;
+    __threadfence();
     __syncthreads();
-    v = c = 0.0;
-    for (int w = 0; w < 16; w++) { v += sv[w]; c += sc[w]; }
-    const double count = c > 1.0 ? c : 1.0;
-    if (out && threadIdx.x == 0) out[blockIdx.x] = (float)(v / count);
-    if (!g_logp) return;
-    const float g = (float)((upstream ? (double)upstream[blockIdx.x] : 1.0) / count);
-    for (uint64_t i = threadIdx.x; i < n; i += blockDim.x) g_logp[base + i] = keep ? -(keep[base + i] * g) : -g;
+    if (threadIdx.x == 0) last = atomicAdd(p.done, 1u) == gridDim.x - 1 ? 1u : 0u;
+    __syncthreads();
+    if (!last) return;
+    __threadfence();
+    for (uint64_t s = 0; s < p.ce.seeds; s++) ce_mean_seed(p.ce, s, sh);
 }
 
-// d_hidden of the scored rows from the ranges of a split sum, added in range order.
-__global__ void __launch_bounds__(128) head_fold_kernel(const uint32_t* count, const float* alpha, const float4* more, const uint32_t* rows_at, const float* acc, uint64_t acc_rows, uint32_t nsplit,
-                                                        uint32_t d, void* out, uint32_t out_f32, uint32_t add) {
-    const uint32_t i = blockIdx.x;
-    if (i >= *count) return;
-    const float scale = *alpha * more[i].y;
-    const uint64_t r = rows_at[i];
-    for (uint32_t c = threadIdx.x * 4; c < d; c += blockDim.x * 4) {
+// d_hidden of the scored rows from the ranges of a split sum, added in range order; nothing to do where K was not split. A block
+// takes 512 columns of a row and goes on with the grid's stride (the host does not know the number of rows).
+__global__ void __launch_bounds__(128) head_fold_kernel(const uint32_t* count, const float* alpha, const float4* more, const uint32_t* rows_at, const float* acc, uint32_t chunks, uint32_t d, void* out,
+                                                        uint32_t out_f32, uint32_t add) {
+    const uint32_t n = *count, tiles_m = (n + 255) / 256, nsplit = hidden_split(tiles_m * ((d + 255) / 256), chunks), across = (d + 511) / 512;
+    if (nsplit == 1) return;
+    const float common = *alpha;
+    const uint64_t range = (uint64_t)tiles_m * 256 * d;
+    for (uint32_t b = blockIdx.x; b < n * across; b += gridDim.x) {
+        const uint32_t i = b / across, c = ((b - i * across) * 128 + threadIdx.x) * 4;
+        if (c >= d) continue;
+        const float scale = common * more[i].y;
+        const uint64_t r = rows_at[i];
+        const float* q0 = acc + (uint64_t)i * d + c;
         float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
         for (uint32_t s = 0; s < nsplit; s++) {
-            const float4 q = *reinterpret_cast<const float4*>(acc + ((uint64_t)s * acc_rows + i) * d + c);
+            const float4 q = *reinterpret_cast<const float4*>(q0 + s * range);
             y.x += q.x; y.y += q.y; y.z += q.z; y.w += q.w;
         }
         y.x *= scale; y.y *= scale; y.z *= scale; y.w *= scale;
@@ -299,94 +357,141 @@ __global__ void __launch_bounds__(128) head_fold_kernel(const uint32_t* count, c
 // q = rint(127·x / max|x|) (ties to even) and the scale max|x| / 127 in f32, so x ≈ q·scale. 127·x is exact for bf16 x and the
 // division is correctly rounded, so q is the integer of exact arithmetic: x / (max|x| / 127) would fall on either side of the
 // ties that x = max|x| / 2 produces. A row with an infinity or a NaN gets a non-finite scale and zeros.
-__device__ __forceinline__ int32_t quantise(float x, float big) {
-    const float q = __fdiv_rn(x * 127.f, big);
-    return big > 0.f ? max(-127, min(127, __float2int_rn(q))) : 0;
-}
+// The division is a product with 127 / max|x| wherever that cannot change the integer, which is unless the quotient lies within 1e-4
+// of a tie (the product's error is below 127·2^-22), and the rounding is an addition of 1.5·2^23, whose low byte then is the integer:
+// with the IEEE division and the conversion instructions the kernel was bound by arithmetic (39 us for 8192 × 4096 bf16).
+struct Quantiser {
+    float big, c;
+    __device__ __forceinline__ explicit Quantiser(float b) : big(b) { c = b >= 0x1p-100f && b <= FLT_MAX ? 127.f * __frcp_rn(b) : __int_as_float(0x7fc00000); }
+    // the integer in the low byte, and how far the quotient is from it
+    __device__ __forceinline__ uint32_t near(float x, float& off) const {
+        const float a = x * c, r = a + 12582912.f;
+        off = fabsf(a - (r - 12582912.f));
+        return __float_as_uint(r);
+    }
+    __device__ __forceinline__ uint32_t exact(float x) const { return big > 0.f ? (uint32_t)max(-127, min(127, __float2int_rn(__fdiv_rn(x * 127.f, big)))) : 0u; }
+    __device__ __forceinline__ uint32_t operator()(float x) const {
+        float off;
+        const uint32_t q = near(x, off);
+        return off <= 0.4999f ? q : exact(x);
+    }
+    __device__ __forceinline__ uint2 eight(const float z[8]) const {
+        uint32_t q[8];
+        float worst = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            float off;
+            q[i] = near(z[i], off);
+            worst = fmax_nan(worst, off);
+        }
+        if (!(worst <= 0.4999f)) {
+#pragma unroll
+            for (int i = 0; i < 8; i++) q[i] = exact(z[i]);
+        }
+        return make_uint2(__byte_perm(__byte_perm(q[0], q[1], 0x0040), __byte_perm(q[2], q[3], 0x0040), 0x5410), __byte_perm(__byte_perm(q[4], q[5], 0x0040), __byte_perm(q[6], q[7], 0x0040), 0x5410));
+    }
+};
 template <int DT>
 __device__ __forceinline__ float load_x(const void* x, uint64_t i) {
     if (DT == NRL_BF16) return __uint_as_float((uint32_t)reinterpret_cast<const uint16_t*>(x)[i] << 16);
     return reinterpret_cast<const float*>(x)[i];
 }
+// eight elements as they lie in memory
 template <int DT>
-__device__ __forceinline__ void load_x8(const void* x, uint64_t i, float z[8]) {
-    if (DT == NRL_BF16) {
-        const uint4 q = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(x) + i);
-        z[0] = bf16_lo(q.x); z[1] = bf16_hi(q.x); z[2] = bf16_lo(q.y); z[3] = bf16_hi(q.y);
-        z[4] = bf16_lo(q.z); z[5] = bf16_hi(q.z); z[6] = bf16_lo(q.w); z[7] = bf16_hi(q.w);
-    } else {
-        const float4 a = reinterpret_cast<const float4*>(reinterpret_cast<const float*>(x) + i)[0], b = reinterpret_cast<const float4*>(reinterpret_cast<const float*>(x) + i)[1];
-        z[0] = a.x; z[1] = a.y; z[2] = a.z; z[3] = a.w; z[4] = b.x; z[5] = b.y; z[6] = b.z; z[7] = b.w;
-    }
-}
-// the block's maximum, a NaN winning; `sm` holds 33 floats
-__device__ __forceinline__ float block_max_nan(float m, float* sm) {
+struct RawX {
+    uint4 q[DT == NRL_BF16 ? 1 : 2];
+    __device__ __forceinline__ void load(const void* x, uint64_t i) {
+        const uint4* s = reinterpret_cast<const uint4*>(reinterpret_cast<const uint8_t*>(x) + i * (DT == NRL_BF16 ? 2 : 4));
 #pragma unroll
-    for (int k = 16; k >= 1; k >>= 1) m = fmax_nan(m, __shfl_xor_sync(0xffffffffu, m, k));
-    if ((threadIdx.x & 31) == 0) sm[threadIdx.x >> 5] = m;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        for (uint32_t w = 1; w < blockDim.x >> 5; w++) m = fmax_nan(m, sm[w]);
-        sm[32] = m;
+        for (int k = 0; k < (DT == NRL_BF16 ? 1 : 2); k++) q[k] = s[k];
     }
-    __syncthreads();
-    return sm[32];
-}
+    __device__ __forceinline__ void unpack(float z[8]) const {
+        if constexpr (DT == NRL_BF16) {
+            z[0] = bf16_lo(q[0].x); z[1] = bf16_hi(q[0].x); z[2] = bf16_lo(q[0].y); z[3] = bf16_hi(q[0].y);
+            z[4] = bf16_lo(q[0].z); z[5] = bf16_hi(q[0].z); z[6] = bf16_lo(q[0].w); z[7] = bf16_hi(q[0].w);
+        } else {
+            z[0] = __uint_as_float(q[0].x); z[1] = __uint_as_float(q[0].y); z[2] = __uint_as_float(q[0].z); z[3] = __uint_as_float(q[0].w);
+            z[4] = __uint_as_float(q[1].x); z[5] = __uint_as_float(q[1].y); z[6] = __uint_as_float(q[1].z); z[7] = __uint_as_float(q[1].w);
+        }
+    }
+};
 
-// A block per row; `vec`: the row starts are 16-byte aligned and d is a multiple of 8. Up to 8192 elements stay in registers
-// between the maximum and the rounding; what a longer row has beyond them is read a second time.
-template <int DT>
-__global__ void __launch_bounds__(256) quantise_rows_kernel(const void* x, uint32_t d, uint64_t pitch, int8_t* q, float* scales, bool vec) {
-    __shared__ float sm[33];
-    const uint64_t row = blockIdx.x, at = row * d;
-    constexpr int kHeld = 4;
-    float z[kHeld][8];
+// kW warps per row (eight, or one when there are rows enough to fill the device: no barrier then, and eight rows to a block); `vec`:
+// the row starts are 16-byte aligned and d is a multiple of 8. Up to 4096 elements (one warp) or 8192 (eight) stay in registers between
+// the maximum and the rounding; what a longer row has beyond them is read a second time.
+template <int DT, int kW>
+__global__ void __launch_bounds__(256) quantise_rows_kernel(const void* x, uint64_t rows, uint32_t d, uint64_t pitch, int8_t* q, float* scales, bool vec) {
+    __shared__ float sm[8];
+    constexpr uint32_t kT = 32 * kW;                          // threads per row
+    constexpr int kHeld = kW == 1 ? (DT == NRL_BF16 ? 16 : 8) : 4;  // vectors of 8 a thread holds
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const uint64_t row = kW == 1 ? (uint64_t)blockIdx.x * 8 + warp : blockIdx.x;
+    const uint32_t t = kW == 1 ? (uint32_t)lane : threadIdx.x;
+    if (row >= rows) return;
+    const uint64_t at = row * d;
+    RawX<DT> held[kHeld];
     float big = 0.f;
-    if (vec) {
+    auto most = [&](const float z[8]) {
 #pragma unroll
-        for (int k = 0; k < kHeld; k++) {
-            const uint32_t c = (threadIdx.x + k * 256) * 8;
-            if (c < d) load_x8<DT>(x, at + c, z[k]);
-        }
-#pragma unroll
-        for (int k = 0; k < kHeld; k++)
-            if ((threadIdx.x + k * 256) * 8 < d) {
-#pragma unroll
-                for (int i = 0; i < 8; i++) big = fmax_nan(big, fabsf(z[k][i]));
-            }
-        for (uint32_t c = (threadIdx.x + kHeld * 256) * 8; c < d; c += 256 * 8) {
-            float t[8];
-            load_x8<DT>(x, at + c, t);
-#pragma unroll
-            for (int i = 0; i < 8; i++) big = fmax_nan(big, fabsf(t[i]));
-        }
-    } else {
-        for (uint32_t c = threadIdx.x; c < d; c += blockDim.x) big = fmax_nan(big, fabsf(load_x<DT>(x, at + c)));
-    }
-    big = block_max_nan(big, sm);
-    int8_t* o = q + row * pitch;
-    auto store8 = [&](const float t[8], uint32_t c) {
-        uint32_t w[2] = {0u, 0u};
-#pragma unroll
-        for (int i = 0; i < 8; i++) w[i >> 2] |= ((uint32_t)quantise(t[i], big) & 0xffu) << (8 * (i & 3));
-        *reinterpret_cast<uint2*>(o + c) = make_uint2(w[0], w[1]);
+        for (int i = 0; i < 8; i++) big = fmax_nan(big, fabsf(z[i]));
     };
     if (vec) {
 #pragma unroll
         for (int k = 0; k < kHeld; k++) {
-            const uint32_t c = (threadIdx.x + k * 256) * 8;
-            if (c < d) store8(z[k], c);
+            const uint32_t c = (t + k * kT) * 8;
+            if (c < d) held[k].load(x, at + c);
         }
-        for (uint32_t c = (threadIdx.x + kHeld * 256) * 8; c < d; c += 256 * 8) {
-            float t[8];
-            load_x8<DT>(x, at + c, t);
-            store8(t, c);
+#pragma unroll
+        for (int k = 0; k < kHeld; k++)
+            if ((t + k * kT) * 8 < d) {
+                float z[8];
+                held[k].unpack(z);
+                most(z);
+            }
+        for (uint32_t c = (t + kHeld * kT) * 8; c < d; c += kT * 8) {
+            RawX<DT> r;
+            float z[8];
+            r.load(x, at + c);
+            r.unpack(z);
+            most(z);
         }
     } else {
-        for (uint32_t c = threadIdx.x; c < d; c += blockDim.x) o[c] = (int8_t)quantise(load_x<DT>(x, at + c), big);
+        for (uint32_t c = t; c < d; c += kT) big = fmax_nan(big, fabsf(load_x<DT>(x, at + c)));
     }
-    for (uint64_t c = d + threadIdx.x; c < pitch; c += blockDim.x) o[c] = 0;
-    if (threadIdx.x == 0) scales[row] = __fdiv_rn(big, 127.f);
+#pragma unroll
+    for (int k = 16; k >= 1; k >>= 1) big = fmax_nan(big, __shfl_xor_sync(0xffffffffu, big, k));
+    if (kW > 1) {
+        if (lane == 0) sm[warp] = big;
+        __syncthreads();
+        for (int w = 0; w < kW; w++) big = fmax_nan(big, sm[w]);
+    }
+    const Quantiser quantise(big);
+    int8_t* o = q + row * pitch;
+    auto store8 = [&](const float z[8], uint32_t c) {
+        *reinterpret_cast<uint2*>(o + c) = quantise.eight(z);
+    };
+    if (vec) {
+#pragma unroll
+        for (int k = 0; k < kHeld; k++) {
+            const uint32_t c = (t + k * kT) * 8;
+            if (c < d) {
+                float z[8];
+                held[k].unpack(z);
+                store8(z, c);
+            }
+        }
+        for (uint32_t c = (t + kHeld * kT) * 8; c < d; c += kT * 8) {
+            RawX<DT> r;
+            float z[8];
+            r.load(x, at + c);
+            r.unpack(z);
+            store8(z, c);
+        }
+    } else {
+        for (uint32_t c = t; c < d; c += kT) o[c] = (int8_t)quantise(load_x<DT>(x, at + c));
+    }
+    for (uint64_t c = d + t; c < pitch; c += kT) o[c] = 0;
+    if (t == 0) scales[row] = __fdiv_rn(big, 127.f);
 }
 
 // Columns of a bf16 [d, V] weight as rows [V, pitch] of integers: a block takes 64 columns, finds their maxima over d and then
@@ -408,9 +513,9 @@ __global__ void __launch_bounds__(256) quantise_columns_kernel(const uint16_t* w
         if (v < V) scales[v] = __fdiv_rn(m, 127.f);
     }
     __syncthreads();
-    const float b = big[c];
+    const Quantiser quantise(big[c]);
     for (uint32_t k0 = 0; k0 < pitch; k0 += 64) {
-        for (uint32_t k = part_of; k < 64; k += 4) tile[c][k] = v < V && k0 + k < d ? (int8_t)quantise(load_x<NRL_BF16>(w, (uint64_t)(k0 + k) * V + v), b) : (int8_t)0;
+        for (uint32_t k = part_of; k < 64; k += 4) tile[c][k] = v < V && k0 + k < d ? (int8_t)quantise(load_x<NRL_BF16>(w, (uint64_t)(k0 + k) * V + v)) : (int8_t)0;
         __syncthreads();
         // 64 rows of 64 bytes, four bytes a thread and step
         for (uint32_t i = threadIdx.x; i < 64 * 16; i += 256) {

@@ -23,17 +23,22 @@ static int need_cc10() {
     return cc_major == 10 ? NRL_OK : NRL_E_UNSUPPORTED;  // tcgen05 / tensor memory
 }
 
-constexpr uint32_t kPairs = 74;  // CTA pairs that run side by side (148 SMs)
-
 template <int EPI, int MASK = kMaskNone>
 static int launch_gemm(const CUtensorMap& ma, const CUtensorMap& mb, const CUtensorMap& mo, HeadGemm p, uint64_t tiles, cudaStream_t st) {
-    p.stages = kHgSmemTiles / (kHgABytes + (p.bn / 2) * 128);
+    p.stages = smem_tiles(EPI) / (kHgABytes + (p.bn / 2) * 128);
     if (p.stages > kHgMaxStages) p.stages = kHgMaxStages;
     if (tiles > 0x7fffffffull) return NRL_E_UNSUPPORTED;
-    cudaError_t e = cudaFuncSetAttribute(head_gemm_kernel<EPI, MASK>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kHgSmemBytes);
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return (int)e;
+    static std::atomic<uint64_t> ready{0};  // devices on which this kernel may have its shared memory
+    if (dev >= 64 || !(ready.load(std::memory_order_acquire) >> dev & 1u)) {
+        e = cudaFuncSetAttribute(head_gemm_kernel<EPI, MASK>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem_bytes(EPI));
+        if (e != cudaSuccess) return (int)e;
+        if (dev < 64) ready.fetch_or(1ull << dev, std::memory_order_release);
+    }
     const unsigned grid = 2u * (unsigned)(tiles < kPairs ? (tiles ? tiles : 1) : kPairs);
-    head_gemm_kernel<EPI, MASK><<<grid, kHgThreads, kHgSmemBytes, st>>>(ma, mb, mo, p);
+    head_gemm_kernel<EPI, MASK><<<grid, kHgThreads, smem_bytes(EPI), st>>>(ma, mb, mo, p);
     return after_launch();
 }
 template <int EPI>
@@ -46,9 +51,9 @@ static inline uint64_t up(uint64_t x, uint64_t to) { return (x + to - 1) / to * 
 static inline uint32_t tiles256(uint64_t x) { return (uint32_t)((x + 255) / 256); }
 
 static int launch_rows(HeadRows& hr, cudaStream_t st) {
-    // a block owns 16 rows; more when there would be over 1024 blocks, since each looks at every row's upstream
+    // a block owns 8 rows, one per warp; more when there would be over 1024 blocks, since each looks at every row's upstream
     hr.per_block = (uint32_t)((hr.rows + 1023) / 1024);
-    if (hr.per_block < 16) hr.per_block = 16;
+    if (hr.per_block < 8) hr.per_block = 8;
     head_rows_kernel<<<(unsigned)((hr.rows + hr.per_block - 1) / hr.per_block), kRowsThreads, 0, st>>>(hr);
     return after_launch();
 }
@@ -61,14 +66,15 @@ static bool bad_mask(uint32_t flags, nrl_devptr mask, uint64_t stride, uint32_t 
 static void set_mask(HeadGemm& g, nrl_devptr mask, uint64_t stride) {
     g.allow = (const uint8_t*)mask;
     g.allow_stride = stride;
-    g.allow_wide = (mask | stride) % 8 == 0 ? 1u : 0u;
+    g.allow_wide = (mask | stride) % 4 == 0 ? 1u : 0u;
 }
 
-// How a backward call is cut: pieces of `vc` vocabulary columns (their dz is what exists of [rows, V] at any time) and
-// `nsplit` ranges of a piece's columns in dx = dz·Wᵀ. A function of (rows, V, d) only.
+// How a backward call is cut: pieces of `vc` vocabulary columns; their dz is what exists of [rows, V] at any time. A function of
+// (rows, V, d) only.
 struct BwdPlan {
     uint64_t rows_pad;
-    uint32_t vc, pieces, nsplit;
+    uint32_t vc, pieces, chunks;
+    bool may_split;
     uint64_t off_coef, off_more, off_rows, off_x, off_dz, off_acc, bytes;
 };
 static BwdPlan bwd_plan(uint64_t rows, uint32_t V, uint32_t d) {
@@ -81,26 +87,25 @@ static BwdPlan bwd_plan(uint64_t rows, uint32_t V, uint32_t d) {
     b.pieces = (uint32_t)((V + vc - 1) / vc);
     b.vc = (uint32_t)up((V + b.pieces - 1) / b.pieces, 256);  // pieces of about the same width
     b.pieces = (V + b.vc - 1) / b.vc;
-    // few tiles of dx: the columns of a piece go to several pairs
-    const uint64_t tiles = (uint64_t)tiles256(rows) * tiles256(d);
-    const uint32_t chunks = (b.vc + 63) / 64;
-    double best = 0.0;
-    b.nsplit = 1;
-    for (uint32_t s = 1; s <= 64 && (s == 1 || chunks / s >= 8); s++) {
-        const uint64_t units = tiles * s, waves = (units + kPairs - 1) / kPairs;
-        const double eff = (double)units / (double)(waves * kPairs);
-        if (eff > best + 0.08) { best = eff; b.nsplit = s; }
-        if (waves > 4) break;
+    b.chunks = b.vc / 64;
+    // any number of scored rows up to `rows` may turn up: whether one of them would have dx's K split
+    uint64_t split_units = 0;
+    const uint32_t tn = tiles256(d), tm = tiles256(rows);
+    for (uint32_t m = 1; m <= tm && m * tn <= kPairs; m++) {
+        const uint32_t s = hidden_split(m * tn, b.chunks);
+        if (s > 1 && (uint64_t)m * s > split_units) split_units = (uint64_t)m * s;
     }
+    b.may_split = split_units > 0;
     uint64_t at = 256;
     b.off_coef = at; at += up(rows * 16, 256);
     b.off_more = at; at += up(rows * 16, 256);
     b.off_rows = at; at += up(rows * 4, 256);
-    b.off_x = at; at += b.rows_pad * d * 2;
+    b.off_x = at; at += b.rows_pad * up(d, 64) * 2;
     b.off_dz = at; at += b.rows_pad * b.vc * 2;
     b.off_acc = at;
-    if (b.pieces > 1 || b.nsplit > 1) at += (uint64_t)b.nsplit * b.rows_pad * d * 4;
-    b.bytes = at;
+    uint64_t acc = split_units * 256 * d * 4;
+    if (b.pieces > 1 && acc < b.rows_pad * d * 4) acc = b.rows_pad * d * 4;
+    b.bytes = at + acc;
     return b;
 }
 
@@ -152,6 +157,7 @@ extern "C" int nrl_readout_bwd(const nrl_readout_bwd_args* a, nrl_stream stream)
     hr.more = (float4*)(ws + b.off_more);
     hr.rows_at = (uint32_t*)(ws + b.off_rows);
     hr.x = (uint16_t*)(ws + b.off_x);
+    hr.x_pitch = (uint32_t)up(a->d, 64);
     hr.d_hidden = (a->flags & NRL_READOUT_BWD_ADD_D_HIDDEN) ? nullptr : (void*)a->d_hidden;
     hr.d_hidden_f32 = (a->flags & NRL_READOUT_BWD_D_HIDDEN_F32) ? 1u : 0u;
     rc = launch_rows(hr, st);
@@ -160,7 +166,6 @@ extern "C" int nrl_readout_bwd(const nrl_readout_bwd_args* a, nrl_stream stream)
     HeadGemm g;
     memset(&g, 0, sizeof g);
     g.bn = 256;
-    g.nsplit = 1;
     g.group_m = 16;
     g.coef = hr.coef;
     g.more = hr.more;
@@ -171,18 +176,18 @@ extern "C" int nrl_readout_bwd(const nrl_readout_bwd_args* a, nrl_stream stream)
     const uint32_t allow_bits = a->flags & NRL_READOUT_MASK_BITS;
     g.vocab = a->V;
     g.alpha = hr.alpha;
-    g.acc_rows = b.rows_pad;
 
     const uint64_t x = ws + b.off_x, dz = ws + b.off_dz;
+    // boxes of 64 elements of K × 128 rows, or of 64 columns × 64 elements of K; the weight is read along K by one product and across
+    // it by the other
+    const uint64_t w_in = vd ? a->d : a->V, w_rows = vd ? a->V : a->d;
     CUtensorMap x_k, x_mn, w_k, w_mn, dz_k, dz_mn, dz_out, dw_out;
     const bool dw32 = (a->flags & NRL_READOUT_BWD_D_WEIGHTS_F32) != 0;
     memset(&dw_out, 0, sizeof dw_out);
-    // boxes of 64 elements of K × 128 rows, or of 64 columns × 64 elements of K
-    if ((rc = encode_2d(&x_k, false, x, a->d, b.rows_pad, a->d, 64, 128)) || (rc = encode_2d(&x_mn, false, x, a->d, b.rows_pad, a->d, 64, 64)) ||
+    if ((rc = encode_2d(&x_k, false, x, a->d, b.rows_pad, hr.x_pitch, 64, 128)) || (rc = encode_2d(&x_mn, false, x, a->d, b.rows_pad, hr.x_pitch, 64, 64)) ||
         (rc = encode_2d(&dz_k, false, dz, b.vc, b.rows_pad, b.vc, 64, 128)) || (rc = encode_2d(&dz_mn, false, dz, b.vc, b.rows_pad, b.vc, 64, 64)) ||
-        (rc = encode_2d(&dz_out, false, dz, b.vc, b.rows_pad, b.vc, 64, 32)) ||
-        (rc = encode_2d(&w_k, false, a->weights, vd ? a->d : a->V, vd ? a->V : a->d, vd ? a->d : a->V, 64, 128)) ||
-        (rc = encode_2d(&w_mn, false, a->weights, vd ? a->d : a->V, vd ? a->V : a->d, vd ? a->d : a->V, 64, 64)))
+        (rc = encode_2d(&dz_out, false, dz, b.vc, b.rows_pad, b.vc, 64, 32)) || (rc = encode_2d(&w_k, false, a->weights, w_in, w_rows, w_in, 64, 128)) ||
+        (rc = encode_2d(&w_mn, false, a->weights, w_in, w_rows, w_in, 64, 64)))
         return rc;
     if (a->d_weights) {
         rc = dw32 ? encode_2d_f32(&dw_out, a->d_weights, vd ? a->d : a->V, vd ? a->V : a->d, 32, 32) : encode_2d(&dw_out, false, a->d_weights, vd ? a->d : a->V, vd ? a->V : a->d, vd ? a->d : a->V, 64, 32);
@@ -211,19 +216,20 @@ extern "C" int nrl_readout_bwd(const nrl_readout_bwd_args* a, nrl_stream stream)
             p.k = cols;
             p.b_mn = vd ? 1u : 0u;
             p.b_k0 = v0;
-            p.nsplit = b.nsplit;
-            p.acc = b.pieces > 1 || b.nsplit > 1 ? (float*)(ws + b.off_acc) : nullptr;
+            p.split = b.may_split ? b.chunks : 0u;
+            p.acc = (float*)(ws + b.off_acc);
             p.acc_in = piece > 0 ? 1u : 0u;
-            p.acc_out = b.nsplit > 1 || piece + 1 < b.pieces ? 1u : 0u;
+            p.acc_out = piece + 1 < b.pieces ? 1u : 0u;
             p.out = (void*)a->d_hidden;
             p.out_pitch = a->d;
             p.out_f32 = hr.d_hidden_f32;
             p.out_add = (a->flags & NRL_READOUT_BWD_ADD_D_HIDDEN) ? 1u : 0u;
             p.wide = (a->d_hidden % 32 == 0 && (p.out_f32 || a->d % 16 == 0)) ? 1u : 0u;
-            rc = launch_gemm<kEpiHidden>(dz_k, vd ? w_mn : w_k, dz_out, p, (uint64_t)tiles256(a->rows) * tiles256(a->d) * b.nsplit, st);
+            rc = launch_gemm<kEpiHidden>(dz_k, vd ? w_mn : w_k, dz_out, p, b.may_split ? kPairs : (uint64_t)tiles256(a->rows) * tiles256(a->d), st);
             if (rc) return rc;
-            if (b.nsplit > 1 && piece + 1 == b.pieces) {
-                head_fold_kernel<<<(unsigned)a->rows, 128, 0, st>>>(hr.count, hr.alpha, hr.more, hr.rows_at, p.acc, b.rows_pad, b.nsplit, a->d, (void*)a->d_hidden, p.out_f32, p.out_add);
+            if (b.may_split && piece + 1 == b.pieces) {
+                const uint64_t most = (a->rows < (uint64_t)kPairs * 256 ? a->rows : (uint64_t)kPairs * 256) * ((a->d + 511) / 512);  // more rows are never split
+                head_fold_kernel<<<(unsigned)(most < 8 * 148 ? most : 8 * 148), 128, 0, st>>>(hr.count, hr.alpha, hr.more, hr.rows_at, p.acc, b.chunks, a->d, (void*)a->d_hidden, p.out_f32, p.out_add);
                 rc = after_launch();
                 if (rc) return rc;
             }
@@ -264,7 +270,7 @@ static ScoredPlan scored_plan(uint64_t rows, uint32_t V, uint32_t d, bool scored
     s.rows_pad = up(rows, 256);
     uint64_t at = 256;
     s.off_rows = at; at += s.gather ? up(rows * 4, 256) : 0;
-    s.off_x = at; at += s.gather ? s.rows_pad * d * 2 : 0;
+    s.off_x = at; at += s.gather ? s.rows_pad * up(d, 64) * 2 : 0;
     s.off_parts = at; at += (s.rows_pad < kScoredChunk ? s.rows_pad : kScoredChunk) * tiles256(V) * 2 * 16;
     s.bytes = at;
     return s;
@@ -283,6 +289,7 @@ extern "C" int nrl_readout_scored_fwd(const nrl_readout_scored_args* a, nrl_stre
     if (a->V > 0x40000000u || a->d > 0x40000000u || a->rows > 0x40000000ull) return NRL_E_UNSUPPORTED;  // TMA coordinates are 32-bit
     if (((a->tokens | a->scored | a->logp | a->entropy) & 3u) || (a->rowstats & 15u) || (a->workspace & 255u)) return NRL_E_BAD_ARG;
     if (a->logp && !a->tokens) return NRL_E_BAD_ARG;
+    if (a->seeds ? (!a->logp || a->rows % a->seeds != 0 || (!a->ce_loss && !a->ce_g_logp) || ((a->ce_loss | a->ce_g_logp) & 3u)) : (a->ce_loss || a->ce_g_logp)) return NRL_E_BAD_ARG;
     if (a->reserved != 0 || !(a->temperature >= 0.f) || !isfinite(a->temperature)) return NRL_E_BAD_ARG;
     if (bad_mask(a->flags, a->allow_mask, a->allow_row_stride, a->V)) return NRL_E_BAD_ARG;
     int rc = need_cc10();
@@ -303,6 +310,7 @@ extern "C" int nrl_readout_scored_fwd(const nrl_readout_scored_args* a, nrl_stre
         hr.count = (uint32_t*)ws;
         hr.rows_at = (uint32_t*)(ws + s.off_rows);
         hr.x = (uint16_t*)(ws + s.off_x);
+        hr.x_pitch = (uint32_t)up(a->d, 64);
         hr.logp = (float*)a->logp;
         hr.out_entropy = (float*)a->entropy;
         hr.out_rowstats = (float4*)a->rowstats;
@@ -311,7 +319,7 @@ extern "C" int nrl_readout_scored_fwd(const nrl_readout_scored_args* a, nrl_stre
         if (rc) return rc;
     }
     CUtensorMap mx, mw;
-    rc = encode_2d(&mx, false, s.gather ? ws + s.off_x : a->hidden, a->d, s.gather ? s.rows_pad : a->rows, a->d, 64, 128);
+    rc = encode_2d(&mx, false, s.gather ? ws + s.off_x : a->hidden, a->d, s.gather ? s.rows_pad : a->rows, s.gather ? up(a->d, 64) : a->d, 64, 128);
     if (rc) return rc;
     rc = vd ? encode_2d(&mw, false, a->weights, a->d, a->V, a->d, 64, 128) : encode_2d(&mw, false, a->weights, a->V, a->d, a->V, 64, 64);
     if (rc) return rc;
@@ -320,7 +328,6 @@ extern "C" int nrl_readout_scored_fwd(const nrl_readout_scored_args* a, nrl_stre
         HeadGemm p;
         memset(&p, 0, sizeof p);
         p.bn = 256;
-        p.nsplit = 1;
         p.group_m = 16;
         p.m = (uint32_t)n;
         p.m_count = s.gather ? (const uint32_t*)ws : nullptr;
@@ -336,6 +343,7 @@ extern "C" int nrl_readout_scored_fwd(const nrl_readout_scored_args* a, nrl_stre
         set_mask(p, a->allow_mask, a->allow_row_stride);
         if (!s.gather && a->allow_mask) p.allow += r0 * a->allow_row_stride * ((a->flags & NRL_READOUT_MASK_BITS) ? 4u : 1u);
         p.vocab = a->V;
+        p.zero = (uint32_t*)(ws + 8);
         p.parts = (float4*)(ws + s.off_parts);
         p.parts_pitch = tiles256(a->V) * 2;
         rc = launch_masked<kEpiStats>(mx, mw, mx, p, a->flags & NRL_READOUT_MASK_BITS, (uint64_t)tiles256(n) * tiles256(a->V), st);
@@ -350,12 +358,16 @@ extern "C" int nrl_readout_scored_fwd(const nrl_readout_scored_args* a, nrl_stre
         f.scored = a->scored ? (const float*)a->scored + at : nullptr;
         f.parts = p.parts;
         f.nparts = p.parts_pitch;
-        f.tokens = p.tokens;
         f.logp = a->logp ? (float*)a->logp + at : nullptr;
         f.entropy = a->entropy ? (float*)a->entropy + at : nullptr;
         f.rowstats = (float4*)a->rowstats + at;
         f.status = a->status ? (uint8_t*)a->status + at : nullptr;
-        head_finish_kernel<<<(unsigned)((n + 7) / 8), 256, 0, st>>>(f);
+        if (a->seeds && r0 + n == a->rows) {  // the last launch: every row's log-prob is there when its last block is done
+            f.ce = {a->seeds, a->rows / a->seeds, (const float*)a->logp, (const float*)a->scored, nullptr, (float*)a->ce_loss, (float*)a->ce_g_logp};
+            f.done = (uint32_t*)(ws + 8);
+        }
+        if (n <= 8 * 148) head_finish_kernel<8><<<(unsigned)n, 256, 0, st>>>(f);
+        else head_finish_kernel<1><<<(unsigned)((n + 7) / 8), 256, 0, st>>>(f);
         rc = after_launch();
         if (rc) return rc;
     }
@@ -366,7 +378,7 @@ extern "C" int nrl_ce_mean(uint64_t s, uint64_t n, nrl_devptr logp, nrl_devptr k
     if (s == 0 || n == 0 || (!out && !g_logp) || (out && !logp)) return NRL_E_BAD_ARG;
     if ((logp | keep | upstream | out | g_logp) & 3u) return NRL_E_BAD_ARG;
     if (s > 0x7fffffffull) return NRL_E_UNSUPPORTED;
-    ce_mean_kernel<<<(unsigned)s, 512, 0, (cudaStream_t)stream>>>(n, (const float*)logp, (const float*)keep, (const float*)upstream, (float*)out, (float*)g_logp);
+    ce_mean_kernel<<<(unsigned)s, 512, 0, (cudaStream_t)stream>>>(CeMean{s, n, (const float*)logp, (const float*)keep, (const float*)upstream, (float*)out, (float*)g_logp});
     return after_launch();
 }
 
@@ -379,8 +391,18 @@ extern "C" int nrl_i8_quantize_rows(uint32_t dtype, uint64_t rows, uint32_t d, n
     if (rows > 0x7fffffffull) return NRL_E_UNSUPPORTED;
     const bool vec = d % 8 == 0 && (x & 15u) == 0;
     const cudaStream_t st = (cudaStream_t)stream;
-    if (dtype == NRL_BF16) quantise_rows_kernel<NRL_BF16><<<(unsigned)rows, 256, 0, st>>>((const void*)x, d, pitch, (int8_t*)values, (float*)scales, vec);
-    else quantise_rows_kernel<NRL_F32><<<(unsigned)rows, 256, 0, st>>>((const void*)x, d, pitch, (int8_t*)values, (float*)scales, vec);
+    const void* xp = (const void*)x;
+    int8_t* q = (int8_t*)values;
+    float* sp = (float*)scales;
+    const bool many = rows >= 8 * 148;  // a warp per row fills the device
+    const unsigned grid = (unsigned)(many ? (rows + 7) / 8 : rows);
+    if (dtype == NRL_BF16) {
+        if (many) quantise_rows_kernel<NRL_BF16, 1><<<grid, 256, 0, st>>>(xp, rows, d, pitch, q, sp, vec);
+        else quantise_rows_kernel<NRL_BF16, 8><<<grid, 256, 0, st>>>(xp, rows, d, pitch, q, sp, vec);
+    } else {
+        if (many) quantise_rows_kernel<NRL_F32, 1><<<grid, 256, 0, st>>>(xp, rows, d, pitch, q, sp, vec);
+        else quantise_rows_kernel<NRL_F32, 8><<<grid, 256, 0, st>>>(xp, rows, d, pitch, q, sp, vec);
+    }
     return after_launch();
 }
 
@@ -400,7 +422,7 @@ extern "C" int nrl_i8_dequantize_rows(uint32_t dtype, uint64_t rows, uint32_t d,
     return after_launch();
 }
 
-extern "C" int nrl_i8_matmul(const nrl_i8_matmul_args* a, nrl_stream stream) {
+static int i8_check(const nrl_i8_matmul_args* a) {
     if (!a || a->struct_size != sizeof(nrl_i8_matmul_args)) return NRL_E_BAD_ARG;
     if (a->rows == 0 || a->n == 0 || a->k == 0 || !a->x || !a->x_scales || !a->w || !a->w_scales || !a->out) return NRL_E_BAD_ARG;
     if (a->dtype != NRL_F32 && a->dtype != NRL_BF16) return NRL_E_UNSUPPORTED;
@@ -409,7 +431,27 @@ extern "C" int nrl_i8_matmul(const nrl_i8_matmul_args* a, nrl_stream stream) {
         return NRL_E_BAD_ARG;
     if (a->rows > 0x40000000ull || a->n > 0x40000000u) return NRL_E_UNSUPPORTED;  // TMA coordinates are 32-bit
     if (a->k > 131072u) return NRL_E_UNSUPPORTED;                                  // 127·127·k must fit 31 bits
-    int rc = need_cc10();
+    return need_cc10();
+}
+
+extern "C" uint64_t nrl_i8_linear_workspace_bytes(uint64_t rows, uint32_t k) { return up(rows * 4, 256) + rows * up(k, 16); }
+
+extern "C" int nrl_i8_linear(uint32_t x_dtype, const nrl_i8_matmul_args* a, nrl_devptr workspace, uint64_t workspace_bytes, nrl_stream stream) {
+    if (!a || a->struct_size != sizeof(nrl_i8_matmul_args) || a->x_scales || a->x_pitch) return NRL_E_BAD_ARG;
+    if (a->rows == 0 || a->k == 0 || (workspace & 255u)) return NRL_E_BAD_ARG;
+    if (!workspace || workspace_bytes < nrl_i8_linear_workspace_bytes(a->rows, a->k)) return NRL_E_WORKSPACE;
+    nrl_i8_matmul_args q = *a;
+    q.x_scales = workspace;
+    q.x = workspace + up(a->rows * 4, 256);
+    q.x_pitch = up(a->k, 16);
+    int rc = i8_check(&q);  // nothing is launched for a product that is refused
+    if (rc) return rc;
+    rc = nrl_i8_quantize_rows(x_dtype, a->rows, a->k, a->x, q.x, q.x_pitch, q.x_scales, stream);
+    return rc ? rc : nrl_i8_matmul(&q, stream);
+}
+
+extern "C" int nrl_i8_matmul(const nrl_i8_matmul_args* a, nrl_stream stream) {
+    int rc = i8_check(a);
     if (rc) return rc;
     // M = the weight's rows, N = the tokens: few tokens make a narrow tile, and the weight streams through it
     HeadGemm p;
@@ -419,7 +461,6 @@ extern "C" int nrl_i8_matmul(const nrl_i8_matmul_args* a, nrl_stream stream) {
     p.m = a->n;
     p.n = (uint32_t)a->rows;
     p.k = a->k;
-    p.nsplit = 1;
     p.group_m = 16;
     p.m_scale = (const float*)a->w_scales;
     p.n_scale = (const float*)a->x_scales;

@@ -12,7 +12,7 @@ the vocabulary makes the loss NaN instead of raising.
 import torch
 
 from . import capi, ops
-from .rl import Head, Loss
+from .rl import Head, Loss, _as
 
 
 class CeOptions:
@@ -81,12 +81,11 @@ def _ce(logits, targets, keep, smoothing, reduce):
 def _head_ce(head, S, N, tok, keep, smoothing, reduce):
     if smoothing > 0.0:
         raise ValueError("label smoothing needs the sum of a row's logits: a Head has none")
-    run = head.run(tok, keep)
-    logp, keep = run.fwd.logp.reshape(S, N), None if keep is None else keep.reshape(S, N)
+    run = head.run(tok, keep, ce_seeds=S if reduce else 0)
+    logp = run.fwd.logp
     if not reduce:
-        return Loss(-logp, lambda up: run.backward(g_logp=-up))
-    value, unit = ops.ce_mean(logp, keep)
-    return Loss(value, lambda up: run.backward(g_logp=ops.ce_mean(logp, keep, up.reshape(S), want_loss=False)[1]), lambda: run.backward(g_logp=unit))
+        return Loss(-logp.reshape(S, N), lambda up: run.backward(g_logp=-up))
+    return Loss(run.fwd.ce_loss, lambda up: run.backward(g_logp=ops.ce_mean(logp, S, keep, up, want_loss=False)[1]), lambda: run.backward(g_logp=run.fwd.ce_g_logp))
 
 
 def nll(logits, targets):
@@ -104,8 +103,10 @@ def cross_entropy(logits, targets):
 def masked_cross_entropy(logits, targets, mask):
     """`sum(nll · mask) / max(count, 1)` per seed (src/nn/loss.rs:27-34)."""
     S, N, V, _ = _rows(logits)
+    if isinstance(logits, Head):
+        return _head_ce(logits, S, N, targets, _as(mask, torch.float32), 0.0, True)
     keep = mask.reshape(S * N).to(torch.float32).contiguous()
-    return _ce(logits, _targets(targets, S, N, V, check=not isinstance(logits, Head)), keep, 0.0, reduce=True)
+    return _ce(logits, _targets(targets, S, N, V), keep, 0.0, reduce=True)
 
 
 def cross_entropy_with(logits, targets, mask=None, opts=None):

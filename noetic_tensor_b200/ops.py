@@ -24,12 +24,31 @@ def _p(t):
 
 
 def _stream(dev):
-    return C.c_void_p(torch.cuda.current_stream(dev).cuda_stream)
+    return torch._C._cuda_getCurrentRawStream(dev.index)  # the handle of torch.cuda.current_stream(dev)
+
+
+def _launch(dev, name, *args):
+    """The library's function `name` on `dev` and torch's current stream there."""
+    if torch.cuda.current_device() != dev.index:
+        with torch.cuda.device(dev):
+            return _launch(dev, name, *args)
+    rc = getattr(capi.lib(), name)(*args, _stream(dev))
+    if rc != 0:
+        capi.check(rc, name)
 
 
 def _need(t, dtype, shape, what, dev):
-    if t.device != dev or t.dtype != dtype or tuple(t.shape) != tuple(shape) or not t.is_contiguous():
+    if t.dtype is not dtype or t.shape != tuple(shape) or not t.is_contiguous() or t.device != dev:
         raise ValueError(f"{what}: expected contiguous {dtype} {tuple(shape)} on {dev}, got {t.dtype} {tuple(t.shape)} on {t.device}")
+
+
+def _need_flat(t, dtype, n, what, dev):
+    """The address of a contiguous tensor of `n` elements, whatever its shape; None is 0."""
+    if t is None:
+        return 0
+    if t.dtype is not dtype or t.numel() != n or not t.is_contiguous() or t.device != dev:
+        raise ValueError(f"{what}: expected {n} contiguous {dtype} on {dev}, got {t.dtype} {tuple(t.shape)} on {t.device}")
+    return t.data_ptr()
 
 
 def _masks(V, rows, allow, add, dev):
@@ -490,61 +509,73 @@ def readout_forward(hidden, weights, *, tokens=None, weights_are_vd=False, round
     return out
 
 
-def readout_scored_forward(hidden, weights, *, tokens=None, scored=None, want_entropy=False, weights_are_vd=False, allow=None, allow_bits=None, temperature=1.0, workspace=None):
+def _readout_shape(hidden_shape, d, weights, weights_are_vd, dev):
+    """(rows, d, V) of a readout call, hidden [..., d]."""
+    if weights.dim() != 2 or weights.shape[1 if weights_are_vd else 0] != d:
+        raise ValueError(f"weights: expected {'[V, d]' if weights_are_vd else '[d, V]'} with d = {d}, got {tuple(weights.shape)}")
+    V = weights.shape[0 if weights_are_vd else 1]
+    _need_flat(weights, torch.bfloat16, d * V, "weights", dev)
+    return hidden_shape.numel() // d, d, V
+
+
+class ScoredReadout:
+    """Outputs of nrl_readout_scored_fwd (fields are None when not requested)."""
+
+    __slots__ = ("logp", "entropy", "rowstats", "status", "ce_loss", "ce_g_logp")
+
+    def __init__(self):
+        self.logp = self.entropy = self.ce_loss = self.ce_g_logp = None
+
+
+def readout_scored_forward(hidden, weights, *, tokens=None, scored=None, want_entropy=False, weights_are_vd=False, allow=None, allow_bits=None, temperature=1.0, workspace=None, ce_seeds=0):
     """`readout_forward` of given tokens over the positions of a training batch that `scored` (float32
-    [rows], 0: not scored; None: all) lets into the loss (nrl_readout_scored_fwd): a Readout with `logp`
+    [rows], 0: not scored; None: all) lets into the loss (nrl_readout_scored_fwd): a ScoredReadout with `logp`
     (with `tokens`), `entropy` (with `want_entropy`), `rowstats` and `status`, all 0 at the other positions,
-    which are not read. A token outside the vocabulary has log-prob NaN. `readout_backward` is its backward."""
+    which are not read. A token outside the vocabulary has log-prob NaN. `hidden` may have any leading shape,
+    `tokens` and `scored` the same. With `ce_seeds` = S the result also has what `ce_mean` of S seeds with
+    keep = scored gives, `ce_loss` [S] and `ce_g_logp` [rows]. `readout_backward` is its backward."""
     dev = hidden.device
     if dev.type != "cuda":
         raise ValueError("readout_scored_forward needs CUDA tensors: this library has no CPU path")
-    rows, d = hidden.shape
-    V = weights.shape[0] if weights_are_vd else weights.shape[1]
-    _need(hidden, torch.bfloat16, (rows, d), "hidden", dev)
-    _need(weights, torch.bfloat16, (V, d) if weights_are_vd else (d, V), "weights", dev)
-    a = capi.ReadoutScoredArgs()
-    a.struct_size = C.sizeof(a)
-    a.flags = capi.READOUT_W_VD if weights_are_vd else 0
-    a.V, a.d, a.rows, a.temperature = V, d, rows, float(temperature)
-    a.hidden, a.weights = _p(hidden), _p(weights)
-    out = Readout()
-    out.logits = out.tokens = out.logp = out.entropy = None
+    rows, d, V = _readout_shape(hidden.shape, hidden.shape[-1], weights, weights_are_vd, dev)
+    a = capi.ReadoutScoredArgs(C.sizeof(capi.ReadoutScoredArgs), capi.READOUT_W_VD if weights_are_vd else 0, V, d, rows, _need_flat(hidden, torch.bfloat16, rows * d, "hidden", dev), weights.data_ptr(),
+                               _need_flat(tokens, torch.int32, rows, "tokens", dev), _need_flat(scored, torch.float32, rows, "scored", dev))
+    a.temperature = temperature
+    out = ScoredReadout()
     if tokens is not None:
-        _need(tokens, torch.int32, (rows,), "tokens", dev)
         out.logp = torch.empty(rows, dtype=torch.float32, device=dev)
-        a.tokens, a.logp = _p(tokens), _p(out.logp)
-    if scored is not None:
-        _need(scored, torch.float32, (rows,), "scored", dev)
-        a.scored = _p(scored)
-    allow = _readout_masks(a, V, rows, allow, allow_bits, dev)
+        a.logp = out.logp.data_ptr()
+    if ce_seeds:
+        out.ce_loss, out.ce_g_logp = torch.empty(ce_seeds, dtype=torch.float32, device=dev), torch.empty(rows, dtype=torch.float32, device=dev)
+        a.seeds, a.ce_loss, a.ce_g_logp = ce_seeds, out.ce_loss.data_ptr(), out.ce_g_logp.data_ptr()
+    if allow is not None or allow_bits is not None:
+        allow = _readout_masks(a, V, rows, allow, allow_bits, dev)
     if want_entropy:
         out.entropy = torch.empty(rows, dtype=torch.float32, device=dev)
-        a.entropy = _p(out.entropy)
+        a.entropy = out.entropy.data_ptr()
     out.rowstats = torch.empty(rows, 4, dtype=torch.float32, device=dev)
     out.status = torch.empty(rows, dtype=torch.uint8, device=dev)
-    a.rowstats, a.status = _p(out.rowstats), _p(out.status)
+    a.rowstats, a.status = out.rowstats.data_ptr(), out.status.data_ptr()
     if workspace is None:
         workspace = torch.empty(capi.lib().nrl_readout_scored_workspace_bytes(rows, V, d, scored is not None), dtype=torch.uint8, device=dev)
-    a.workspace, a.workspace_bytes = _p(workspace), workspace.numel() * workspace.element_size()
-    with torch.cuda.device(dev):
-        capi.check(capi.lib().nrl_readout_scored_fwd(C.byref(a), _stream(dev)), "nrl_readout_scored_fwd")
+    a.workspace, a.workspace_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+    _launch(dev, "nrl_readout_scored_fwd", C.byref(a))
     return out
 
 
-def ce_mean(logp, keep=None, upstream=None, want_loss=True):
-    """masked_cross_entropy of given log-probs [S, N]: (value [S] or None, d(Σ value · upstream) / d(logp)
-    [S, N]) in one launch (nrl_ce_mean); `upstream` None: ones."""
+def ce_mean(logp, S, keep=None, upstream=None, want_loss=True):
+    """masked_cross_entropy of given log-probs, S seeds of logp.numel() / S positions: (value [S] or None,
+    d(Σ value · upstream) / d(logp) in logp's shape) in one launch (nrl_ce_mean); `upstream` None: ones."""
     dev = logp.device
-    S, N = logp.shape
-    _need(logp, torch.float32, (S, N), "logp", dev)
-    if keep is not None:
-        _need(keep, torch.float32, (S, N), "keep", dev)
-    if upstream is not None:
-        _need(upstream, torch.float32, (S,), "upstream", dev)
+    if dev.type != "cuda":
+        raise ValueError("ce_mean needs CUDA tensors: this library has no CPU path")
+    n = logp.numel()
+    if S < 1 or n % S:
+        raise ValueError(f"ce_mean: {n} positions of {S} seeds")
+    lp, kp, up = _need_flat(logp, torch.float32, n, "logp", dev), _need_flat(keep, torch.float32, n, "keep", dev), _need_flat(upstream, torch.float32, S, "upstream", dev)
     value = torch.empty(S, dtype=torch.float32, device=dev) if want_loss else None
     g = torch.empty_like(logp)
-    with torch.cuda.device(dev):
-        capi.check(capi.lib().nrl_ce_mean(S, N, _p(logp), _p(keep), _p(upstream), _p(value), _p(g), _stream(dev)), "nrl_ce_mean")
+    _launch(dev, "nrl_ce_mean", S, n // S, lp, kp, up, _p(value), g.data_ptr())
     return value, g
 
 
@@ -555,26 +586,30 @@ class Int8Rows:
     __slots__ = ("values", "scales", "d")
 
     def __init__(self, values, scales, d):
-        dev = values.device
         if values.dim() != 2 or not 0 < d <= values.shape[1] or values.shape[1] % 16:
             raise ValueError("values: int8 [rows, pitch], pitch >= d and a multiple of 16")
-        _need(values, torch.int8, tuple(values.shape), "values", dev)
-        _need(scales, torch.float32, (values.shape[0],), "scales", dev)
+        _need_flat(values, torch.int8, values.numel(), "values", values.device)
+        _need(scales, torch.float32, values.shape[:1], "scales", values.device)
         self.values, self.scales, self.d = values, scales, d
 
 
+def _int8_rows(rows, d, dev):
+    q = Int8Rows.__new__(Int8Rows)
+    q.values, q.scales, q.d = torch.empty(rows, (d + 15) // 16 * 16, dtype=torch.int8, device=dev), torch.empty(rows, dtype=torch.float32, device=dev), d
+    return q
+
+
 def quantize_rows(x):
-    """`x` [rows, d] (float32 or bfloat16) as Int8Rows: q = rint(127 x / max|x|), scale max|x| / 127
-    (nrl_i8_quantize_rows). A row with an infinity or a NaN gets a non-finite scale."""
+    """`x` [..., d] (float32 or bfloat16) as Int8Rows, a row per leading position: q = rint(127 x / max|x|),
+    scale max|x| / 127 (nrl_i8_quantize_rows). A row with an infinity or a NaN gets a non-finite scale."""
     dev = x.device
     if dev.type != "cuda":
         raise ValueError("quantize_rows needs CUDA tensors: this library has no CPU path")
-    rows, d = x.shape
+    d = x.shape[-1]
     if not x.is_contiguous():
         raise ValueError("x must be contiguous")
-    q = Int8Rows(torch.empty(rows, (d + 15) // 16 * 16, dtype=torch.int8, device=dev), torch.empty(rows, dtype=torch.float32, device=dev), d)
-    with torch.cuda.device(dev):
-        capi.check(capi.lib().nrl_i8_quantize_rows(_dt(x), rows, d, _p(x), _p(q.values), q.values.shape[1], _p(q.scales), _stream(dev)), "nrl_i8_quantize_rows")
+    q = _int8_rows(x.numel() // d, d, dev)
+    _launch(dev, "nrl_i8_quantize_rows", _dt(x), q.values.shape[0], d, x.data_ptr(), q.values.data_ptr(), q.values.shape[1], q.scales.data_ptr())
     return q
 
 
@@ -588,9 +623,8 @@ def quantize_weight(weights, weights_are_vd=False):
         raise ValueError("quantize_weight needs CUDA tensors: this library has no CPU path")
     d, V = weights.shape
     _need(weights, torch.bfloat16, (d, V), "weights", dev)
-    q = Int8Rows(torch.empty(V, (d + 15) // 16 * 16, dtype=torch.int8, device=dev), torch.empty(V, dtype=torch.float32, device=dev), d)
-    with torch.cuda.device(dev):
-        capi.check(capi.lib().nrl_i8_quantize_columns(d, V, _p(weights), _p(q.values), q.values.shape[1], _p(q.scales), _stream(dev)), "nrl_i8_quantize_columns")
+    q = _int8_rows(V, d, dev)
+    _launch(dev, "nrl_i8_quantize_columns", d, V, weights.data_ptr(), q.values.data_ptr(), q.values.shape[1], q.scales.data_ptr())
     return q
 
 
@@ -600,8 +634,7 @@ def dequantize_rows(q, dtype=torch.bfloat16):
     if dev.type != "cuda":
         raise ValueError("dequantize_rows needs CUDA tensors: this library has no CPU path")
     out = torch.empty(q.values.shape[0], q.d, dtype=dtype, device=dev)
-    with torch.cuda.device(dev):
-        capi.check(capi.lib().nrl_i8_dequantize_rows(_dt(out), out.shape[0], q.d, _p(q.values), q.values.shape[1], _p(q.scales), _p(out), _stream(dev)), "nrl_i8_dequantize_rows")
+    _launch(dev, "nrl_i8_dequantize_rows", _dt(out), out.shape[0], q.d, q.values.data_ptr(), q.values.shape[1], q.scales.data_ptr(), out.data_ptr())
     return out
 
 
@@ -613,23 +646,36 @@ def int8_matmul(x, w, dtype=torch.float32):
         raise ValueError("int8_matmul needs CUDA tensors: this library has no CPU path")
     if x.d != w.d or w.values.device != dev:
         raise ValueError(f"int8_matmul: rows of {x.d} and of {w.d} integers on {dev} and {w.values.device}")
-    out = torch.empty(x.values.shape[0], w.values.shape[0], dtype=dtype, device=dev)
-    a = capi.I8MatmulArgs()
-    a.struct_size = C.sizeof(a)
-    a.dtype, a.rows, a.n, a.k = _dt(out), out.shape[0], out.shape[1], x.d
-    a.x, a.x_pitch, a.x_scales = _p(x.values), x.values.shape[1], _p(x.scales)
-    a.w, a.w_pitch, a.w_scales = _p(w.values), w.values.shape[1], _p(w.scales)
-    a.out = _p(out)
-    with torch.cuda.device(dev):
-        capi.check(capi.lib().nrl_i8_matmul(C.byref(a), _stream(dev)), "nrl_i8_matmul")
+    (rows, x_pitch), (n, w_pitch) = x.values.shape, w.values.shape
+    out = torch.empty(rows, n, dtype=dtype, device=dev)
+    a = capi.I8MatmulArgs(C.sizeof(capi.I8MatmulArgs), _dt(out), rows, n, x.d, x.values.data_ptr(), x_pitch, x.scales.data_ptr(), w.values.data_ptr(), w_pitch, w.scales.data_ptr(), out.data_ptr())
+    _launch(dev, "nrl_i8_matmul", C.byref(a))
+    return out
+
+
+def int8_linear(x, w, dtype=torch.float32):
+    """`int8_matmul(quantize_rows(x), w, dtype)` in one call (nrl_i8_linear): `x` [..., d] float32 or bfloat16,
+    `w` Int8Rows [V, d], result [..., V]."""
+    dev = x.device
+    if dev.type != "cuda":
+        raise ValueError("int8_linear needs CUDA tensors: this library has no CPU path")
+    d = x.shape[-1]
+    (n, w_pitch), rows = w.values.shape, x.numel() // d
+    if d != w.d or w.values.device != dev or not x.is_contiguous():
+        raise ValueError(f"int8_linear: contiguous rows of {w.d} values on {w.values.device}, got {tuple(x.shape)} on {dev}")
+    out = torch.empty(x.shape[:-1] + (n,), dtype=dtype, device=dev)
+    a = capi.I8MatmulArgs(C.sizeof(capi.I8MatmulArgs), _dt(out), rows, n, d, x.data_ptr(), 0, 0, w.values.data_ptr(), w_pitch, w.scales.data_ptr(), out.data_ptr())
+    workspace = torch.empty(capi.lib().nrl_i8_linear_workspace_bytes(rows, d), dtype=torch.uint8, device=dev)
+    _launch(dev, "nrl_i8_linear", _dt(x), C.byref(a), workspace.data_ptr(), workspace.numel())
     return out
 
 
 def readout_backward(hidden, weights, fwd, *, tokens=None, g_logp=None, g_ent=None, weights_are_vd=False, allow=None, allow_bits=None, temperature=1.0, want_hidden=True,
-                     want_weights=True, grad_dtype=torch.bfloat16, add_hidden=None, add_weights=None, workspace=None):
+                     want_weights=True, grad_dtype=torch.bfloat16, add_hidden=None, add_weights=None, workspace=None, hidden_shape=None):
     """(d_hidden, d_weights) of Σ g_logp·logp + Σ g_ent·entropy of the results `fwd` of
-    `readout_scored_forward` or `readout_forward` (their `rowstats` and, with `g_ent`, `entropy`), the logits computed again in pieces (nrl_readout_bwd).
-    `hidden`: the bf16 [rows, d] of the forward call, or an Int8Rows checkpoint of it. Gradients are
+    `readout_scored_forward` or `readout_forward` (their `rowstats` and, with `g_ent`, `entropy`), the
+    logits computed again in pieces (nrl_readout_bwd). `hidden`: the bf16 [..., d] of the forward call, or
+    an Int8Rows checkpoint of it (d_hidden then has `hidden_shape`, default [rows, d]). Gradients are
     `grad_dtype` (bfloat16 or float32); `add_hidden` / `add_weights` are tensors they are added to in place
     (their own dtype counts). Rows whose upstreams are 0 are not read."""
     quant = hidden if isinstance(hidden, Int8Rows) else None
@@ -637,58 +683,48 @@ def readout_backward(hidden, weights, fwd, *, tokens=None, g_logp=None, g_ent=No
     dev = x.device
     if dev.type != "cuda":
         raise ValueError("readout_backward needs CUDA tensors: this library has no CPU path")
-    rows, d = x.shape[0], (quant.d if quant else x.shape[1])
-    V = weights.shape[0] if weights_are_vd else weights.shape[1]
-    wshape = (V, d) if weights_are_vd else (d, V)
-    _need(weights, torch.bfloat16, wshape, "weights", dev)
-    if grad_dtype not in (torch.bfloat16, torch.float32):
+    if hidden_shape is None:
+        hidden_shape = torch.Size((x.shape[0], quant.d)) if quant else x.shape
+    rows, d, V = _readout_shape(hidden_shape, quant.d if quant else x.shape[-1], weights, weights_are_vd, dev)
+    if grad_dtype is not torch.bfloat16 and grad_dtype is not torch.float32:
         raise TypeError(f"gradients must be bfloat16 or float32, got {grad_dtype}")
     if g_logp is None and g_ent is None:
         raise ValueError("give `g_logp`, `g_ent` or both")
-    a = capi.ReadoutBwdArgs()
-    a.struct_size = C.sizeof(a)
-    a.flags = capi.READOUT_W_VD if weights_are_vd else 0
-    a.V, a.d, a.rows, a.temperature = V, d, rows, float(temperature)
+    flags = capi.READOUT_W_VD if weights_are_vd else 0
     if quant:
-        a.flags |= capi.READOUT_BWD_HIDDEN_I8
-        a.hidden_scales, a.hidden_pitch = _p(quant.scales), x.shape[1]
+        if x.shape[0] != rows:
+            raise ValueError(f"hidden: {x.shape[0]} rows of integers for {rows} positions")
+        flags |= capi.READOUT_BWD_HIDDEN_I8
+        xp, sp, pitch = x.data_ptr(), quant.scales.data_ptr(), x.shape[1]
     else:
-        _need(x, torch.bfloat16, (rows, d), "hidden", dev)
-    a.hidden, a.weights = _p(x), _p(weights)
-    _need(fwd.rowstats, torch.float32, (rows, 4), "rowstats", dev)
-    a.rowstats = _p(fwd.rowstats)
-    if g_logp is not None:
-        _need(g_logp, torch.float32, (rows,), "g_logp", dev)
-        if tokens is None:
-            raise ValueError("`g_logp` needs the tokens")
-        _need(tokens, torch.int32, (rows,), "tokens", dev)
-        a.g_logp, a.tokens = _p(g_logp), _p(tokens)
-    if g_ent is not None:
-        _need(g_ent, torch.float32, (rows,), "g_ent", dev)
-        _need(fwd.entropy, torch.float32, (rows,), "entropy", dev)
-        a.g_ent, a.entropy = _p(g_ent), _p(fwd.entropy)
-    allow = _readout_masks(a, V, rows, allow, allow_bits, dev)
+        xp, sp, pitch = _need_flat(x, torch.bfloat16, rows * d, "hidden", dev), 0, 0
+    if g_logp is not None and tokens is None:
+        raise ValueError("`g_logp` needs the tokens")
 
     def out(add, want, shape, f32_flag, add_flag, what):
+        nonlocal flags
         if add is not None:
             if add.dtype not in (torch.bfloat16, torch.float32):
                 raise TypeError(f"{what}: bfloat16 or float32, got {add.dtype}")
             _need(add, add.dtype, shape, what, dev)
-            a.flags |= add_flag
+            flags |= add_flag
         elif want:
             add = torch.empty(shape, dtype=grad_dtype, device=dev)
-        if add is not None and add.dtype == torch.float32:
-            a.flags |= f32_flag
+        if add is not None and add.dtype is torch.float32:
+            flags |= f32_flag
         return add
 
-    d_hidden = out(add_hidden, want_hidden, (rows, d), capi.READOUT_BWD_D_HIDDEN_F32, capi.READOUT_BWD_ADD_D_HIDDEN, "add_hidden")
-    d_weights = out(add_weights, want_weights, wshape, capi.READOUT_BWD_D_WEIGHTS_F32, capi.READOUT_BWD_ADD_D_WEIGHTS, "add_weights")
-    a.d_hidden, a.d_weights = _p(d_hidden), _p(d_weights)
+    d_hidden = out(add_hidden, want_hidden, hidden_shape, capi.READOUT_BWD_D_HIDDEN_F32, capi.READOUT_BWD_ADD_D_HIDDEN, "add_hidden")
+    d_weights = out(add_weights, want_weights, weights.shape, capi.READOUT_BWD_D_WEIGHTS_F32, capi.READOUT_BWD_ADD_D_WEIGHTS, "add_weights")
     if workspace is None:
         workspace = torch.empty(capi.lib().nrl_readout_bwd_workspace_bytes(rows, V, d), dtype=torch.uint8, device=dev)
-    a.workspace, a.workspace_bytes = _p(workspace), workspace.numel() * workspace.element_size()
-    with torch.cuda.device(dev):
-        capi.check(capi.lib().nrl_readout_bwd(C.byref(a), _stream(dev)), "nrl_readout_bwd")
+    a = capi.ReadoutBwdArgs(C.sizeof(capi.ReadoutBwdArgs), flags, V, d, rows, xp, sp, pitch, weights.data_ptr(),
+                            0 if g_logp is None else _need_flat(tokens, torch.int32, rows, "tokens", dev), _need_flat(fwd.rowstats, torch.float32, rows * 4, "rowstats", dev),
+                            0 if g_ent is None else _need_flat(fwd.entropy, torch.float32, rows, "entropy", dev), _need_flat(g_logp, torch.float32, rows, "g_logp", dev),
+                            _need_flat(g_ent, torch.float32, rows, "g_ent", dev), _p(d_hidden), _p(d_weights), 0, 0, workspace.data_ptr(), workspace.numel() * workspace.element_size(), temperature)
+    if allow is not None or allow_bits is not None:
+        allow = _readout_masks(a, V, rows, allow, allow_bits, dev)
+    _launch(dev, "nrl_readout_bwd", C.byref(a))
     return d_hidden, d_weights
 
 

@@ -105,36 +105,35 @@ class Head:
     def __init__(self, hidden, weight, temperature=1.0, vocab_mask=None, weight_is_vd=False, checkpoint=False, grad_dtype=torch.bfloat16):
         if not (0.0 < temperature < float("inf")):
             raise ValueError(f"tempered_logits: temperature {temperature} (must be positive)")
-        self.d, self.V = hidden.shape[-1], weight.shape[0 if weight_is_vd else 1]
-        self.shape = tuple(hidden.shape[:-1]) + (self.V,)
-        self.flat = hidden.reshape(-1, self.d).contiguous()
         if vocab_mask is not None and vocab_mask.dtype not in (torch.uint8, torch.bool, torch.int32):
             raise ValueError("Head: vocab_mask is a uint8/bool allow-mask or int32 words of bits")
-        self.allow, self.bits = _vocab_mask_args(vocab_mask, self.V)
-        self.weight, self.weight_is_vd, self.temperature, self.checkpoint, self.grad_dtype = weight, weight_is_vd, float(temperature), checkpoint, grad_dtype
+        self.V = weight.shape[0 if weight_is_vd else 1]
+        self.shape = hidden.shape[:-1] + (self.V,)
+        self.hidden, self.weight = hidden.contiguous(), weight
+        allow, bits = _vocab_mask_args(vocab_mask, self.V)
+        self.kw = dict(weights_are_vd=weight_is_vd, allow=allow, allow_bits=bits, temperature=float(temperature))
+        self.checkpoint, self.grad_dtype = checkpoint, grad_dtype
 
-    def run(self, tokens=None, scored=None, want_entropy=False):
-        return _HeadRun(self, tokens, scored, want_entropy)
+    def run(self, tokens=None, scored=None, want_entropy=False, ce_seeds=0):
+        return _HeadRun(self, tokens, scored, want_entropy, ce_seeds)
 
 
-def _flat(t, dtype):
-    return None if t is None else t.reshape(-1).to(dtype).contiguous()
+def _as(t, dtype):
+    """`t` as a contiguous tensor of `dtype`: itself where it is one."""
+    return t if t is None or (t.dtype is dtype and t.is_contiguous()) else t.to(dtype).contiguous()
 
 
 class _HeadRun:
     """A forward of a Head and what its backward needs (not the hidden states when they are checkpointed)."""
 
-    def __init__(self, head, tokens, scored, want_entropy):
-        self.tokens = _flat(tokens, torch.int32)
-        self.kw = dict(weights_are_vd=head.weight_is_vd, allow=head.allow, allow_bits=head.bits, temperature=head.temperature)
-        self.weight, self.grad_dtype, self.shape = head.weight, head.grad_dtype, head.shape[:-1] + (head.d,)
-        self.fwd = ops.readout_scored_forward(head.flat, head.weight, tokens=self.tokens, scored=_flat(scored, torch.float32), want_entropy=want_entropy, **self.kw)
-        self.saved = ops.quantize_rows(head.flat) if head.checkpoint else head.flat
+    def __init__(self, head, tokens, scored, want_entropy, ce_seeds):
+        self.tokens, self.weight, self.kw, self.grad_dtype, self.shape = _as(tokens, torch.int32), head.weight, head.kw, head.grad_dtype, head.hidden.shape
+        self.fwd = ops.readout_scored_forward(head.hidden, head.weight, tokens=self.tokens, scored=_as(scored, torch.float32), want_entropy=want_entropy, ce_seeds=ce_seeds, **head.kw)
+        self.saved = ops.quantize_rows(head.hidden) if head.checkpoint else head.hidden
 
     def backward(self, g_logp=None, g_ent=None):
-        d_hidden, d_weight = ops.readout_backward(self.saved, self.weight, self.fwd, tokens=self.tokens, g_logp=_flat(g_logp, torch.float32), g_ent=_flat(g_ent, torch.float32),
-                                                  grad_dtype=self.grad_dtype, **self.kw)
-        return d_hidden.reshape(self.shape), d_weight
+        return ops.readout_backward(self.saved, self.weight, self.fwd, tokens=self.tokens, g_logp=_as(g_logp, torch.float32), g_ent=_as(g_ent, torch.float32), grad_dtype=self.grad_dtype,
+                                    hidden_shape=self.shape, **self.kw)
 
 
 class Int8Weight(ops.Int8Rows):
@@ -154,9 +153,7 @@ def head_logits(hidden, weight, dtype=torch.float32):
     """`head(x)` (src/nn/decoder.rs:270-279) in 8-bit integers: `hidden` [..., d] (bf16 or f32) is
     quantised with a scale per position, `weight` is an Int8Weight; logits [..., V] of `dtype` (float32 or
     bfloat16), ready for `sample_categorical` and the other functions here that take logits."""
-    lead = hidden.shape[:-1]
-    q = ops.quantize_rows(hidden.reshape(-1, hidden.shape[-1]).contiguous())
-    return ops.int8_matmul(q, weight, dtype).reshape(*lead, weight.values.shape[0])
+    return ops.int8_linear(hidden.contiguous(), weight, dtype)
 
 
 def _tempered(x):
