@@ -210,18 +210,28 @@ struct MaskAhead {
             }
         }
     }
-    // some column of the 32 from 32·c on is kept; all of them are
-    __device__ __forceinline__ bool any(int c) const {
-        if constexpr (MASK == kMaskBytes) return ((keep[0] | keep[1] | keep[2] | keep[3]) >> (8 * c)) & 0xffu;
-        return keep[c] != 0u;
-    }
-    __device__ __forceinline__ bool all(int c) const {
-        if constexpr (MASK == kMaskBytes) return false;
-        return keep[c] == 0xffffffffu;
-    }
-    __device__ __forceinline__ bool column(int c, int i) const {
-        if constexpr (MASK == kMaskBytes) return keep[i & 3] >> (8 * c + (i >> 2)) & 1u;
-        return keep[c] >> i & 1u;
+    // the 32 columns from 32·c on: one word, or (bytes) eight columns in each of four
+    struct Chunk {
+        uint32_t w[MASK == kMaskBytes ? 4 : 1];
+        __device__ __forceinline__ bool any() const {
+            if constexpr (MASK == kMaskBytes) return (w[0] | w[1] | w[2] | w[3]) & 0xffu;
+            return w[0] != 0u;
+        }
+        __device__ __forceinline__ bool all() const { return MASK != kMaskBytes && w[0] == 0xffffffffu; }
+        __device__ __forceinline__ bool column(int i) const {
+            if constexpr (MASK == kMaskBytes) return w[i & 3] & (1u << (i >> 2));
+            return w[0] & (1u << i);
+        }
+    };
+    __device__ __forceinline__ Chunk chunk(int c) const {
+        Chunk k;
+        if constexpr (MASK == kMaskBytes) {
+#pragma unroll
+            for (int j = 0; j < 4; j++) k.w[j] = keep[j] >> (8 * c);
+        } else {
+            k.w[0] = c < 2 ? (c == 0 ? keep[0] : keep[1]) : (c == 2 ? keep[2] : keep[3]);
+        }
+        return k;
     }
 };
 
@@ -237,8 +247,8 @@ struct RowInfo {
 // ∂/∂z of 32 columns of one row from the accumulators y, as 16 packed bf16 pairs. With the row's coefficients pre-multiplied
 // (a′ = a·xs, …): ln π in units of log2 is one fused multiply-add of y, dz = −π·(a′ + b′·(ln π + H)), and the token's entry gets a′.
 template <int MASK>
-__device__ __forceinline__ void epi_grad(const HeadGemm& p, bool live, uint32_t v, const float y[32], const float4& cf, float ys, int32_t token, const MaskAhead<MASK>& mask, int c, uint32_t out[16]) {
-    if (!live || !mask.any(c)) {
+__device__ __forceinline__ void epi_grad(const HeadGemm& p, bool live, uint32_t v, const float y[32], const float4& cf, float ys, int32_t token, const typename MaskAhead<MASK>::Chunk& mask, uint32_t out[16]) {
+    if (!live || !mask.any()) {
 #pragma unroll
         for (int i = 0; i < 16; i++) out[i] = 0u;
         return;
@@ -270,10 +280,10 @@ __device__ __forceinline__ void epi_grad(const HeadGemm& p, bool live, uint32_t 
         for (int i = 0; i < 32; i++)
             if ((uint32_t)i == tk) g[i] += cf.x;
     }
-    if (!mask.all(c)) {
+    if (!mask.all()) {
 #pragma unroll
         for (int i = 0; i < 32; i++)
-            if (!mask.column(c, i)) g[i] = 0.f;
+            if (!mask.column(i)) g[i] = 0.f;
     }
 #pragma unroll
     for (int i = 0; i < 16; i++) out[i] = pack_bf16(g[2 * i], g[2 * i + 1]);
@@ -281,12 +291,12 @@ __device__ __forceinline__ void epi_grad(const HeadGemm& p, bool live, uint32_t 
 
 // 32 columns of one row folded into (m, S, W): m in accumulator units, W in units of log2.
 template <int MASK>
-__device__ __forceinline__ void epi_stats(const HeadGemm& p, uint32_t v, float y[32], float c2, int32_t token, const MaskAhead<MASK>& mask, int c, float& m, float& S, float& W, float& ytok) {
-    if (!mask.any(c)) return;
-    if (!mask.all(c)) {
+__device__ __forceinline__ void epi_stats(const HeadGemm& p, uint32_t v, float y[32], float c2, int32_t token, const typename MaskAhead<MASK>::Chunk& mask, float& m, float& S, float& W, float& ytok) {
+    if (!mask.any()) return;
+    if (!mask.all()) {
 #pragma unroll
         for (int i = 0; i < 32; i++)
-            if (!mask.column(c, i)) y[i] = -FLT_MAX;
+            if (!mask.column(i)) y[i] = -FLT_MAX;
     }
     const uint32_t tk = (uint32_t)(token - (int32_t)v);
     if (tk < 32u) {
@@ -416,6 +426,36 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kHgThreads, 1)
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = cluster_cta_rank();
     const uint32_t pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+    if (threadIdx.x == 0) {
+        abort_flag = 0u;
+        for (uint32_t s = 0; s < kHgMaxStages; s++) {
+            mbar_init(bar_full + 8 * s, 1);
+            mbar_init(bar_empty + 8 * s, 1);
+        }
+        for (int a = 0; a < 2; a++) {
+            mbar_init(bar_acc_full + 8 * a, 1);
+            mbar_init(bar_acc_empty + 8 * a, 2 * kHgEpiWarps);
+        }
+        mbar_init(bar_done, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_addr(&tmem_slot)) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+        tc_fence_before();
+    }
+    if (threadIdx.x == 64) {
+        prefetch_map(&map_a);
+        prefetch_map(&map_b);
+        if (EPI == kEpiGrad || EPI == kEpiWeight) prefetch_map(&map_out);
+    }
+    __syncthreads();
+    cluster_sync_all();  // both CTAs' barriers exist before anything crosses between them
+    tc_fence_after();
+    const uint32_t tmem = tmem_slot;
+    after_previous_kernel();  // what came before is done; nothing above reads or writes global memory
+    if (EPI == kEpiStats && blockIdx.x == 0 && threadIdx.x == 0 && p.zero) *p.zero = 0u;
     const uint32_t in_use = p.m_count ? *p.m_count : 0u;
     const uint32_t mm = p.m_count ? min(in_use - min(in_use, p.m_first), p.m) : p.m, kk = p.k_count ? min(*p.k_count, p.k) : p.k;
     const uint32_t tiles_m = (mm + 2 * kHgBM - 1) / (2 * kHgBM), tiles_n = (p.n + p.bn - 1) / p.bn;
@@ -438,59 +478,36 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kHgThreads, 1)
         return it;
     };
 
-    if (threadIdx.x == 0) {
-        if (EPI == kEpiStats && blockIdx.x == 0 && p.zero) *p.zero = 0u;
-        abort_flag = 0u;
-        for (uint32_t s = 0; s < kHgMaxStages; s++) {
-            mbar_init(bar_full + 8 * s, 1);
-            mbar_init(bar_empty + 8 * s, 1);
-        }
-        for (int a = 0; a < 2; a++) {
-            mbar_init(bar_acc_full + 8 * a, 1);
-            mbar_init(bar_acc_empty + 8 * a, 2 * kHgEpiWarps);
-        }
-        mbar_init(bar_done, 1);
-        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-    }
-    if (warp == 1) {
-        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_addr(&tmem_slot)) : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
-        tc_fence_before();
-    }
-    __syncthreads();
-    cluster_sync_all();  // both CTAs' barriers exist before anything crosses between them
-    tc_fence_after();
-    const uint32_t tmem = tmem_slot;
-
+    if (warp < 2) next_kernel_may_start();
     if (warp == 0) {
         // ---- loader (both CTAs) -------------------------------------------------------------------
         if (lane == 0) {
-            uint32_t s = 0, phase = 1u, issued = 0;
+            const uint32_t full_first = in_first_cta(bar_full);
+            uint32_t s = 0, phase = 1u, issued = 0, a_at = smem_base;
             bool ok = true;
             for (uint32_t t = pair; t < tiles && ok; t += pairs) {
                 const Item w = item(t);
                 const int32_t m0 = (int32_t)(p.a_m0 + w.tm * 2 * kHgBM + rank * kHgBM), n0 = (int32_t)(p.b_n0 + w.tn * p.bn + rank * (p.bn / 2));
                 for (uint32_t kc = w.k0; kc < w.k1; kc++) {
                     if (!mbar_wait(bar_empty + 8 * s, phase, &abort_flag)) { ok = false; break; }
-                    const uint32_t full_first = in_first_cta(bar_full + 8 * s);
-                    if (rank == 0) mbar_expect_tx(bar_full + 8 * s, 2 * stage_bytes);  // both CTAs' copies land on this barrier
-                    const uint32_t a_at = smem_base + s * stage_bytes, b_at = a_at + kHgABytes;
-                    const int32_t k0 = (int32_t)(kc * kKStep);
+                    if (rank == 0) mbar_expect_tx(bar_full + 8 * s, 2 * stage_bytes);  // both CTAs' copies land on the first CTA's barrier
+                    const uint32_t bar = full_first + 8 * s, b_at = a_at + kHgABytes;
+                    const int32_t k0 = (int32_t)(kc * kKStep), kb = (int32_t)p.b_k0 + k0;
                     if (p.a_mn) {  // two boxes of 64 m × 64 k
-                        tma_load_2d_pair(a_at, &map_a, m0, k0, full_first);
-                        tma_load_2d_pair(a_at + 8192, &map_a, m0 + 64, k0, full_first);
+                        tma_load_2d_pair(a_at, &map_a, m0, k0, bar);
+                        tma_load_2d_pair(a_at + 8192, &map_a, m0 + 64, k0, bar);
                     } else {
-                        tma_load_2d_pair(a_at, &map_a, k0, m0, full_first);
+                        tma_load_2d_pair(a_at, &map_a, k0, m0, bar);
                     }
-                    const int32_t kb = (int32_t)p.b_k0 + k0;
                     if (p.b_mn) {
-                        for (uint32_t j = 0; j < p.bn / 128; j++) tma_load_2d_pair(b_at + j * 8192, &map_b, n0 + (int32_t)(64 * j), kb, full_first);
+                        tma_load_2d_pair(b_at, &map_b, n0, kb, bar);
+                        tma_load_2d_pair(b_at + 8192, &map_b, n0 + 64, kb, bar);
                     } else {
-                        tma_load_2d_pair(b_at, &map_b, kb, n0, full_first);
+                        tma_load_2d_pair(b_at, &map_b, kb, n0, bar);
                     }
                     issued++;
-                    if (++s == p.stages) { s = 0; phase ^= 1u; }
+                    a_at += stage_bytes;
+                    if (++s == p.stages) { s = 0; phase ^= 1u; a_at = smem_base; }
                 }
             }
             if ((!ok || abort_flag) && issued) {  // copies in flight get time to land before the pair may end
@@ -504,7 +521,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kHgThreads, 1)
             const uint32_t shape = ((p.bn >> 3) << 17) | ((uint32_t)((2 * kHgBM) >> 4) << 24);
             // f32 accumulators of bf16 products, or s32 accumulators of s8 products
             const uint32_t idesc = kI8 ? ((2u << 4) | (1u << 7) | (1u << 10) | shape) : ((1u << 4) | (1u << 7) | (1u << 10) | (p.a_mn << 15) | (p.b_mn << 16) | shape);
+            // contiguous along K: rows of 128 bytes, groups of 8 rows 1024 bytes apart, 32 bytes of K per product; contiguous along M / N:
+            // 64-wide blocks 8 KB apart, groups of 8 k-rows 1024 bytes apart, 16 k-rows per product. One descriptor per operand, the
+            // rest are additions to its address field (this thread's instructions between two products are what the tensor pipe waits for)
+            const uint64_t da0 = p.a_mn ? smem_desc_sw128(smem_base, 8192, 1024) : smem_desc_sw128(smem_base, 16, 1024);
+            const uint64_t db0 = p.b_mn ? smem_desc_sw128(smem_base + kHgABytes, 8192, 1024) : smem_desc_sw128(smem_base + kHgABytes, 16, 1024);
+            const uint32_t a_step = (p.a_mn ? 2048u : 32u) >> 4, b_step = (p.b_mn ? 2048u : 32u) >> 4, s_step = stage_bytes >> 4;
             uint32_t s = 0, phase = 0u, n = 0;
+            uint64_t da = da0, db = db0;
             bool ok = true;
             for (uint32_t t = pair; t < tiles && ok; t += pairs) {
                 const Item w = item(t);
@@ -516,18 +540,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kHgThreads, 1)
                 for (uint32_t kc = w.k0; kc < w.k1; kc++) {
                     if (!mbar_wait(bar_full + 8 * s, phase, &abort_flag)) { ok = false; break; }
                     tc_fence_after();
-                    const uint32_t a_addr = smem_base + s * stage_bytes, b_addr = a_addr + kHgABytes;
 #pragma unroll
                     for (int k = 0; k < 4; k++) {
-                        // contiguous along K: rows of 128 bytes, groups of 8 rows 1024 bytes apart, 32 bytes of K per product;
-                        // contiguous along M / N: 64-wide blocks 8 KB apart, groups of 8 k-rows 1024 bytes apart, 16 k-rows per product
-                        const uint64_t da = p.a_mn ? smem_desc_sw128(a_addr + k * 2048, 8192, 1024) : smem_desc_sw128(a_addr + k * 32, 16, 1024);
-                        const uint64_t db = p.b_mn ? smem_desc_sw128(b_addr + k * 2048, 8192, 1024) : smem_desc_sw128(b_addr + k * 32, 16, 1024);
-                        if constexpr (kI8) tc_mma_i8_pair(d_tmem, da, db, idesc, (kc != w.k0) | (uint32_t)(k != 0));
-                        else tc_mma_bf16_pair(d_tmem, da, db, idesc, (kc != w.k0) | (uint32_t)(k != 0));
+                        const uint32_t add = k ? 1u : kc != w.k0;
+                        if constexpr (kI8) tc_mma_i8_pair(d_tmem, da + k * a_step, db + k * b_step, idesc, add);
+                        else tc_mma_bf16_pair(d_tmem, da + k * a_step, db + k * b_step, idesc, add);
                     }
                     tc_commit_pair(bar_empty + 8 * s);
-                    if (++s == p.stages) { s = 0; phase ^= 1u; }
+                    da += s_step;
+                    db += s_step;
+                    if (++s == p.stages) { s = 0; phase ^= 1u; da = da0; db = db0; }
                 }
                 if (ok) tc_commit_pair(bar_acc_full + 8 * acc);
                 n++;
@@ -584,6 +606,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kHgThreads, 1)
                     ok = __all_sync(0xffffffffu, mbar_wait(bar_acc_full + 8 * acc, (n >> 1) & 1u, &abort_flag));
                     tc_fence_after();
                 }
+                if (!more_tiles) next_kernel_may_start();
             };
             // the accumulator may be overwritten: this warp has it in registers. Before the results are stored: the arrival waits for
             // whatever the warp has stored.
@@ -618,13 +641,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kHgThreads, 1)
                     const uint32_t v = p.v0 + col0 + 32 * c;
                     if constexpr (EPI == kEpiGrad) {
                         uint32_t g[16];
-                        epi_grad<MASK>(p, live, v, y, r.cf, ys, token, mask, c, g);
+                        epi_grad<MASK>(p, live, v, y, r.cf, ys, token, mask.chunk(c), g);
                         if ((c & 1) == 0) stage_free<1>(lane);
 #pragma unroll
                         for (int j = 0; j < 4; j++) sts_piece(stage_out, lane, 4 * (c & 1) + j, g[4 * j], g[4 * j + 1], g[4 * j + 2], g[4 * j + 3]);
                         if (c & 1) stage_send(&map_out, stage_out, lane, (int32_t)(col0 + 32 * (c - 1)), (int32_t)row0);
                     } else {
-                        epi_stats<MASK>(p, v, y, ys, token, mask, c, m, S, W, ytok);
+                        epi_stats<MASK>(p, v, y, ys, token, mask.chunk(c), m, S, W, ytok);
                     }
                 }
                 if constexpr (EPI == kEpiStats) {

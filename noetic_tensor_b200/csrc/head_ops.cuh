@@ -59,6 +59,8 @@ __global__ void __launch_bounds__(kRowsThreads) head_rows_kernel(HeadRows p) {
     __shared__ uint32_t sum_before[kW], sum_all[kW], wcount[kW];
     __shared__ float wmax[kW];
     __shared__ uint32_t place_of[kRowsThreads];
+    next_kernel_may_start();
+    after_previous_kernel();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const uint64_t first = (uint64_t)blockIdx.x * p.per_block, last = min(first + p.per_block, p.rows);
     uint32_t before = 0, total = 0;
@@ -200,6 +202,8 @@ __device__ __forceinline__ void ce_mean_seed(const CeMean& p, uint64_t seed, dou
 }
 __global__ void __launch_bounds__(512) ce_mean_kernel(CeMean p) {
     __shared__ double sh[16][2];
+    next_kernel_may_start();
+    after_previous_kernel();
     ce_mean_seed(p, blockIdx.x, sh);
 }
 
@@ -300,6 +304,8 @@ __device__ __forceinline__ void head_finish_row(const HeadFinish& p) {
 
 template <int kW>
 __global__ void __launch_bounds__(256) head_finish_kernel(HeadFinish p) {
+    next_kernel_may_start();
+    after_previous_kernel();
     head_finish_row<kW>(p);
     if (!p.ce.seeds) return;
     __shared__ double sh[8][2];
@@ -317,6 +323,8 @@ __global__ void __launch_bounds__(256) head_finish_kernel(HeadFinish p) {
 // takes 512 columns of a row and goes on with the grid's stride (the host does not know the number of rows).
 __global__ void __launch_bounds__(128) head_fold_kernel(const uint32_t* count, const float* alpha, const float4* more, const uint32_t* rows_at, const float* acc, uint32_t chunks, uint32_t d, void* out,
                                                         uint32_t out_f32, uint32_t add) {
+    next_kernel_may_start();
+    after_previous_kernel();
     const uint32_t n = *count, tiles_m = (n + 255) / 256, nsplit = hidden_split(tiles_m * ((d + 255) / 256), chunks), across = (d + 511) / 512;
     if (nsplit == 1) return;
     const float common = *alpha;
@@ -422,6 +430,8 @@ struct RawX {
 template <int DT, int kW>
 __global__ void __launch_bounds__(256) quantise_rows_kernel(const void* x, uint64_t rows, uint32_t d, uint64_t pitch, int8_t* q, float* scales, bool vec) {
     __shared__ float sm[8];
+    next_kernel_may_start();
+    after_previous_kernel();
     constexpr uint32_t kT = 32 * kW;                          // threads per row
     constexpr int kHeld = kW == 1 ? (DT == NRL_BF16 ? 16 : 8) : 4;  // vectors of 8 a thread holds
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -500,6 +510,8 @@ __global__ void __launch_bounds__(256) quantise_columns_kernel(const uint16_t* w
     __shared__ float part[4][64];
     __shared__ float big[64];
     __shared__ int8_t tile[64][68];
+    next_kernel_may_start();
+    after_previous_kernel();
     const uint32_t c = threadIdx.x & 63, part_of = threadIdx.x >> 6;
     const uint32_t v = blockIdx.x * 64 + c;
     float m = 0.f;
@@ -527,6 +539,8 @@ __global__ void __launch_bounds__(256) quantise_columns_kernel(const uint16_t* w
 }
 
 __global__ void __launch_bounds__(256) dequantise_rows_kernel(const int8_t* q, const float* scales, uint32_t d, uint64_t pitch, void* out, uint32_t out_f32) {
+    next_kernel_may_start();
+    after_previous_kernel();
     const uint64_t row = blockIdx.x;
     const float s = scales[row];
     for (uint32_t c = threadIdx.x; c < d; c += blockDim.x) {

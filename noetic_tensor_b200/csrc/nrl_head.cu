@@ -9,9 +9,13 @@ using namespace nrl;
 
 extern std::atomic<uint64_t> nrl_g_launches;
 
-static inline int after_launch(int n = 1) {
-    nrl_g_launches.fetch_add((uint64_t)n, std::memory_order_relaxed);
-    cudaError_t e = cudaGetLastError();
+// One launch in stream order, counted. The products start early (launch_next), and small grids; a larger grid of small blocks that
+// waits beside a product's last tiles delayed the pass by 7 us (the statistics of 2048 rows at V = 32 000, d = 1024: 121 against 114 us).
+template <typename... Params, typename... Args>
+static int launch(void (*kernel)(Params...), dim3 grid, unsigned block, size_t smem, cudaStream_t stream, const Args&... args) {
+    nrl_g_launches.fetch_add(1, std::memory_order_relaxed);
+    const cudaError_t e = launch_next(smem != 0 || grid.x <= 2 * kPairs, kernel, grid, dim3(block), smem, stream, args...);
+    if (e != cudaSuccess) (void)cudaGetLastError();
     return e == cudaSuccess ? NRL_OK : (int)e;
 }
 
@@ -38,8 +42,7 @@ static int launch_gemm(const CUtensorMap& ma, const CUtensorMap& mb, const CUten
         if (dev < 64) ready.fetch_or(1ull << dev, std::memory_order_release);
     }
     const unsigned grid = 2u * (unsigned)(tiles < kPairs ? (tiles ? tiles : 1) : kPairs);
-    head_gemm_kernel<EPI, MASK><<<grid, kHgThreads, smem_bytes(EPI), st>>>(ma, mb, mo, p);
-    return after_launch();
+    return launch(head_gemm_kernel<EPI, MASK>, dim3(grid), kHgThreads, smem_bytes(EPI), st, ma, mb, mo, p);
 }
 template <int EPI>
 static int launch_masked(const CUtensorMap& ma, const CUtensorMap& mb, const CUtensorMap& mo, const HeadGemm& p, uint32_t allow_bits, uint64_t tiles, cudaStream_t st) {
@@ -54,8 +57,7 @@ static int launch_rows(HeadRows& hr, cudaStream_t st) {
     // a block owns 8 rows, one per warp; more when there would be over 1024 blocks, since each looks at every row's upstream
     hr.per_block = (uint32_t)((hr.rows + 1023) / 1024);
     if (hr.per_block < 8) hr.per_block = 8;
-    head_rows_kernel<<<(unsigned)((hr.rows + hr.per_block - 1) / hr.per_block), kRowsThreads, 0, st>>>(hr);
-    return after_launch();
+    return launch(head_rows_kernel, dim3((unsigned)((hr.rows + hr.per_block - 1) / hr.per_block)), kRowsThreads, 0, st, hr);
 }
 
 // the mask fields that the forward and the backward share: what a call may give
@@ -229,8 +231,7 @@ extern "C" int nrl_readout_bwd(const nrl_readout_bwd_args* a, nrl_stream stream)
             if (rc) return rc;
             if (b.may_split && piece + 1 == b.pieces) {
                 const uint64_t most = (a->rows < (uint64_t)kPairs * 256 ? a->rows : (uint64_t)kPairs * 256) * ((a->d + 511) / 512);  // more rows are never split
-                head_fold_kernel<<<(unsigned)(most < 8 * 148 ? most : 8 * 148), 128, 0, st>>>(hr.count, hr.alpha, hr.more, hr.rows_at, p.acc, b.chunks, a->d, (void*)a->d_hidden, p.out_f32, p.out_add);
-                rc = after_launch();
+                rc = launch(head_fold_kernel, dim3((unsigned)(most < 8 * 148 ? most : 8 * 148)), 128, 0, st, hr.count, hr.alpha, hr.more, hr.rows_at, p.acc, b.chunks, a->d, (void*)a->d_hidden, p.out_f32, p.out_add);
                 if (rc) return rc;
             }
         }
@@ -366,9 +367,7 @@ extern "C" int nrl_readout_scored_fwd(const nrl_readout_scored_args* a, nrl_stre
             f.ce = {a->seeds, a->rows / a->seeds, (const float*)a->logp, (const float*)a->scored, nullptr, (float*)a->ce_loss, (float*)a->ce_g_logp};
             f.done = (uint32_t*)(ws + 8);
         }
-        if (n <= 8 * 148) head_finish_kernel<8><<<(unsigned)n, 256, 0, st>>>(f);
-        else head_finish_kernel<1><<<(unsigned)((n + 7) / 8), 256, 0, st>>>(f);
-        rc = after_launch();
+        rc = n <= 8 * 148 ? launch(head_finish_kernel<8>, dim3((unsigned)n), 256, 0, st, f) : launch(head_finish_kernel<1>, dim3((unsigned)((n + 7) / 8)), 256, 0, st, f);
         if (rc) return rc;
     }
     return NRL_OK;
@@ -378,8 +377,7 @@ extern "C" int nrl_ce_mean(uint64_t s, uint64_t n, nrl_devptr logp, nrl_devptr k
     if (s == 0 || n == 0 || (!out && !g_logp) || (out && !logp)) return NRL_E_BAD_ARG;
     if ((logp | keep | upstream | out | g_logp) & 3u) return NRL_E_BAD_ARG;
     if (s > 0x7fffffffull) return NRL_E_UNSUPPORTED;
-    ce_mean_kernel<<<(unsigned)s, 512, 0, (cudaStream_t)stream>>>(CeMean{s, n, (const float*)logp, (const float*)keep, (const float*)upstream, (float*)out, (float*)g_logp});
-    return after_launch();
+    return launch(ce_mean_kernel, dim3((unsigned)s), 512, 0, (cudaStream_t)stream, CeMean{s, n, (const float*)logp, (const float*)keep, (const float*)upstream, (float*)out, (float*)g_logp});
 }
 
 // ---- 8-bit integers -----------------------------------------------------------------------------------
@@ -396,21 +394,15 @@ extern "C" int nrl_i8_quantize_rows(uint32_t dtype, uint64_t rows, uint32_t d, n
     float* sp = (float*)scales;
     const bool many = rows >= 8 * 148;  // a warp per row fills the device
     const unsigned grid = (unsigned)(many ? (rows + 7) / 8 : rows);
-    if (dtype == NRL_BF16) {
-        if (many) quantise_rows_kernel<NRL_BF16, 1><<<grid, 256, 0, st>>>(xp, rows, d, pitch, q, sp, vec);
-        else quantise_rows_kernel<NRL_BF16, 8><<<grid, 256, 0, st>>>(xp, rows, d, pitch, q, sp, vec);
-    } else {
-        if (many) quantise_rows_kernel<NRL_F32, 1><<<grid, 256, 0, st>>>(xp, rows, d, pitch, q, sp, vec);
-        else quantise_rows_kernel<NRL_F32, 8><<<grid, 256, 0, st>>>(xp, rows, d, pitch, q, sp, vec);
-    }
-    return after_launch();
+    const dim3 g(grid);
+    if (dtype == NRL_BF16) return many ? launch(quantise_rows_kernel<NRL_BF16, 1>, g, 256, 0, st, xp, rows, d, pitch, q, sp, vec) : launch(quantise_rows_kernel<NRL_BF16, 8>, g, 256, 0, st, xp, rows, d, pitch, q, sp, vec);
+    return many ? launch(quantise_rows_kernel<NRL_F32, 1>, g, 256, 0, st, xp, rows, d, pitch, q, sp, vec) : launch(quantise_rows_kernel<NRL_F32, 8>, g, 256, 0, st, xp, rows, d, pitch, q, sp, vec);
 }
 
 extern "C" int nrl_i8_quantize_columns(uint32_t d, uint32_t V, nrl_devptr weights, nrl_devptr values, uint64_t pitch, nrl_devptr scales, nrl_stream stream) {
     if (d == 0 || V == 0 || !weights || !values || !scales || (scales & 3u) || (weights & 1u)) return NRL_E_BAD_ARG;
     if (pitch < d || pitch % 16 != 0 || (values & 15u)) return NRL_E_BAD_ARG;
-    quantise_columns_kernel<<<(V + 63) / 64, 256, 0, (cudaStream_t)stream>>>((const uint16_t*)weights, d, V, pitch, (int8_t*)values, (float*)scales);
-    return after_launch();
+    return launch(quantise_columns_kernel, dim3((V + 63) / 64), 256, 0, (cudaStream_t)stream, (const uint16_t*)weights, d, V, pitch, (int8_t*)values, (float*)scales);
 }
 
 extern "C" int nrl_i8_dequantize_rows(uint32_t dtype, uint64_t rows, uint32_t d, nrl_devptr values, uint64_t pitch, nrl_devptr scales, nrl_devptr out, nrl_stream stream) {
@@ -418,8 +410,7 @@ extern "C" int nrl_i8_dequantize_rows(uint32_t dtype, uint64_t rows, uint32_t d,
     if (dtype != NRL_F32 && dtype != NRL_BF16) return NRL_E_UNSUPPORTED;
     if (pitch < d || (out & (dtype == NRL_F32 ? 3u : 1u))) return NRL_E_BAD_ARG;
     if (rows > 0x7fffffffull) return NRL_E_UNSUPPORTED;
-    dequantise_rows_kernel<<<(unsigned)rows, 256, 0, (cudaStream_t)stream>>>((const int8_t*)values, (const float*)scales, d, pitch, (void*)out, dtype == NRL_F32 ? 1u : 0u);
-    return after_launch();
+    return launch(dequantise_rows_kernel, dim3((unsigned)rows), 256, 0, (cudaStream_t)stream, (const int8_t*)values, (const float*)scales, d, pitch, (void*)out, dtype == NRL_F32 ? 1u : 0u);
 }
 
 static int i8_check(const nrl_i8_matmul_args* a) {

@@ -32,6 +32,7 @@ __device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map
     asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(bar)
                  : "memory");
 }
+__device__ __forceinline__ void prefetch_map(const CUtensorMap* map) { asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory"); }
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_commit(uint32_t bar) { asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory"); }
@@ -100,6 +101,29 @@ __device__ __forceinline__ float round_through_bf16(float x) {
     if ((u & 0x7fffffffu) > 0x7f800000u) return x;  // NaN stays NaN
     u = (u + 0x7fffu + ((u >> 16) & 1u)) & 0xffff0000u;  // nearest, ties to even (src/tensor/half.rs:16-27)
     return __uint_as_float(u);
+}
+
+// ---- kernels in a row -------------------------------------------------------------------------------
+// A kernel launched with launch_next() may start while the one before it in the stream still runs: what it does before
+// after_previous_kernel() (barriers, tensor memory) costs no time of its own. Every such kernel waits there, with every thread and
+// before its first access to global memory, until the kernel before it has completed, so the order of all memory accesses is the
+// stream's. next_kernel_may_start() lets the next one begin, once every thread of the grid has said so or ended: short kernels say it
+// at once, the products when a warp comes to its last tile.
+__device__ __forceinline__ void after_previous_kernel() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void next_kernel_may_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+template <typename... Params, typename... Args>
+inline cudaError_t launch_next(bool early, void (*kernel)(Params...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, const Args&... args) {
+    cudaLaunchAttribute at;
+    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t c = {};
+    c.gridDim = grid;
+    c.blockDim = block;
+    c.dynamicSmemBytes = smem;
+    c.stream = stream;
+    c.attrs = &at;
+    c.numAttrs = early ? 1 : 0;
+    return cudaLaunchKernelEx(&c, kernel, static_cast<Params>(args)...);
 }
 
 // ---- host: tensor maps ------------------------------------------------------------------------------

@@ -509,22 +509,45 @@ def readout_forward(hidden, weights, *, tokens=None, weights_are_vd=False, round
     return out
 
 
-def _readout_shape(hidden_shape, d, weights, weights_are_vd, dev):
-    """(rows, d, V) of a readout call, hidden [..., d]."""
-    if weights.dim() != 2 or weights.shape[1 if weights_are_vd else 0] != d:
-        raise ValueError(f"weights: expected {'[V, d]' if weights_are_vd else '[d, V]'} with d = {d}, got {tuple(weights.shape)}")
-    V = weights.shape[0 if weights_are_vd else 1]
+def _readout_weight(weights, d, weights_are_vd, dev):
+    """The vocabulary size of a readout weight for `d`-wide hidden states, checked."""
+    shape = weights.shape
+    if len(shape) != 2 or shape[1 if weights_are_vd else 0] != d:
+        raise ValueError(f"weights: expected {'[V, d]' if weights_are_vd else '[d, V]'} with d = {d}, got {tuple(shape)}")
+    V = shape[0 if weights_are_vd else 1]
     _need_flat(weights, torch.bfloat16, d * V, "weights", dev)
-    return hidden_shape.numel() // d, d, V
+    return V
 
 
 class ScoredReadout:
-    """Outputs of nrl_readout_scored_fwd (fields are None when not requested)."""
+    """Outputs of nrl_readout_scored_fwd, in one buffer: `rowstats` [rows, 4], `status` uint8 [rows] and,
+    when requested (else None), `logp`, `entropy`, `ce_g_logp` [rows] and `ce_loss` [seeds]."""
 
-    __slots__ = ("logp", "entropy", "rowstats", "status", "ce_loss", "ce_g_logp")
+    __slots__ = ("rows", "seeds", "_buf", "_logp", "_entropy", "_g", "_loss", "_status")
 
-    def __init__(self):
-        self.logp = self.entropy = self.ce_loss = self.ce_g_logp = None
+    def __init__(self, rows, want_logp, want_entropy, seeds, dev):
+        # offsets in floats; 0 is the row statistics, so 0 elsewhere means "not requested"
+        self.rows, self.seeds = rows, seeds
+        self._status = at = 4 * rows
+        at += (rows + 3) // 4
+        self._logp = self._entropy = self._g = self._loss = 0
+        if want_logp:
+            self._logp, at = at, at + rows
+        if want_entropy:
+            self._entropy, at = at, at + rows
+        if seeds:
+            self._g, self._loss, at = at, at + rows, at + rows + seeds
+        self._buf = torch.empty(at, dtype=torch.float32, device=dev)
+
+    def _vector(self, at, n):
+        return self._buf[at : at + n] if at else None
+
+    rowstats = property(lambda self: self._buf[: 4 * self.rows].reshape(self.rows, 4))
+    status = property(lambda self: self._buf[self._status :].view(torch.uint8)[: self.rows])
+    logp = property(lambda self: self._vector(self._logp, self.rows))
+    entropy = property(lambda self: self._vector(self._entropy, self.rows))
+    ce_g_logp = property(lambda self: self._vector(self._g, self.rows))
+    ce_loss = property(lambda self: self._vector(self._loss, self.seeds))
 
 
 def readout_scored_forward(hidden, weights, *, tokens=None, scored=None, want_entropy=False, weights_are_vd=False, allow=None, allow_bits=None, temperature=1.0, workspace=None, ce_seeds=0):
@@ -537,28 +560,19 @@ def readout_scored_forward(hidden, weights, *, tokens=None, scored=None, want_en
     dev = hidden.device
     if dev.type != "cuda":
         raise ValueError("readout_scored_forward needs CUDA tensors: this library has no CPU path")
-    rows, d, V = _readout_shape(hidden.shape, hidden.shape[-1], weights, weights_are_vd, dev)
-    a = capi.ReadoutScoredArgs(C.sizeof(capi.ReadoutScoredArgs), capi.READOUT_W_VD if weights_are_vd else 0, V, d, rows, _need_flat(hidden, torch.bfloat16, rows * d, "hidden", dev), weights.data_ptr(),
-                               _need_flat(tokens, torch.int32, rows, "tokens", dev), _need_flat(scored, torch.float32, rows, "scored", dev))
-    a.temperature = temperature
-    out = ScoredReadout()
-    if tokens is not None:
-        out.logp = torch.empty(rows, dtype=torch.float32, device=dev)
-        a.logp = out.logp.data_ptr()
-    if ce_seeds:
-        out.ce_loss, out.ce_g_logp = torch.empty(ce_seeds, dtype=torch.float32, device=dev), torch.empty(rows, dtype=torch.float32, device=dev)
-        a.seeds, a.ce_loss, a.ce_g_logp = ce_seeds, out.ce_loss.data_ptr(), out.ce_g_logp.data_ptr()
-    if allow is not None or allow_bits is not None:
-        allow = _readout_masks(a, V, rows, allow, allow_bits, dev)
-    if want_entropy:
-        out.entropy = torch.empty(rows, dtype=torch.float32, device=dev)
-        a.entropy = out.entropy.data_ptr()
-    out.rowstats = torch.empty(rows, 4, dtype=torch.float32, device=dev)
-    out.status = torch.empty(rows, dtype=torch.uint8, device=dev)
-    a.rowstats, a.status = out.rowstats.data_ptr(), out.status.data_ptr()
+    d, n = hidden.shape[-1], hidden.numel()
+    rows = n // d
+    V = _readout_weight(weights, d, weights_are_vd, dev)
+    xp, tp, sp = _need_flat(hidden, torch.bfloat16, n, "hidden", dev), _need_flat(tokens, torch.int32, rows, "tokens", dev), _need_flat(scored, torch.float32, rows, "scored", dev)
+    out = ScoredReadout(rows, tokens is not None, want_entropy, ce_seeds, dev)
+    buf = out._buf.data_ptr()
+    at = lambda offset: buf + 4 * offset if offset else 0  # noqa: E731
     if workspace is None:
         workspace = torch.empty(capi.lib().nrl_readout_scored_workspace_bytes(rows, V, d, scored is not None), dtype=torch.uint8, device=dev)
-    a.workspace, a.workspace_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+    a = capi.ReadoutScoredArgs(C.sizeof(capi.ReadoutScoredArgs), 1 if weights_are_vd else 0, V, d, rows, xp, weights.data_ptr(), tp, sp, at(out._logp), at(out._entropy), buf, at(out._status), 0, 0,
+                               workspace.data_ptr(), workspace.numel() * workspace.element_size(), temperature, 0, ce_seeds, at(out._loss), at(out._g))
+    if allow is not None or allow_bits is not None:
+        allow = _readout_masks(a, V, rows, allow, allow_bits, dev)
     _launch(dev, "nrl_readout_scored_fwd", C.byref(a))
     return out
 
@@ -683,9 +697,11 @@ def readout_backward(hidden, weights, fwd, *, tokens=None, g_logp=None, g_ent=No
     dev = x.device
     if dev.type != "cuda":
         raise ValueError("readout_backward needs CUDA tensors: this library has no CPU path")
+    d = quant.d if quant else x.shape[-1]
     if hidden_shape is None:
-        hidden_shape = torch.Size((x.shape[0], quant.d)) if quant else x.shape
-    rows, d, V = _readout_shape(hidden_shape, quant.d if quant else x.shape[-1], weights, weights_are_vd, dev)
+        hidden_shape = torch.Size((x.shape[0], d)) if quant else x.shape
+    rows = hidden_shape.numel() // d
+    V = _readout_weight(weights, d, weights_are_vd, dev)
     if grad_dtype is not torch.bfloat16 and grad_dtype is not torch.float32:
         raise TypeError(f"gradients must be bfloat16 or float32, got {grad_dtype}")
     if g_logp is None and g_ent is None:
@@ -718,10 +734,15 @@ def readout_backward(hidden, weights, fwd, *, tokens=None, g_logp=None, g_ent=No
     d_weights = out(add_weights, want_weights, weights.shape, capi.READOUT_BWD_D_WEIGHTS_F32, capi.READOUT_BWD_ADD_D_WEIGHTS, "add_weights")
     if workspace is None:
         workspace = torch.empty(capi.lib().nrl_readout_bwd_workspace_bytes(rows, V, d), dtype=torch.uint8, device=dev)
-    a = capi.ReadoutBwdArgs(C.sizeof(capi.ReadoutBwdArgs), flags, V, d, rows, xp, sp, pitch, weights.data_ptr(),
-                            0 if g_logp is None else _need_flat(tokens, torch.int32, rows, "tokens", dev), _need_flat(fwd.rowstats, torch.float32, rows * 4, "rowstats", dev),
-                            0 if g_ent is None else _need_flat(fwd.entropy, torch.float32, rows, "entropy", dev), _need_flat(g_logp, torch.float32, rows, "g_logp", dev),
-                            _need_flat(g_ent, torch.float32, rows, "g_ent", dev), _p(d_hidden), _p(d_weights), 0, 0, workspace.data_ptr(), workspace.numel() * workspace.element_size(), temperature)
+    if type(fwd) is ScoredReadout and fwd.rows == rows and fwd._buf.device == dev:
+        stats = fwd._buf.data_ptr()
+        ent = stats + 4 * fwd._entropy if fwd._entropy else 0
+    else:
+        stats, ent = _need_flat(fwd.rowstats, torch.float32, rows * 4, "rowstats", dev), _need_flat(fwd.entropy, torch.float32, rows, "entropy", dev)
+    if g_ent is not None and not ent:
+        raise ValueError("`g_ent` needs a forward with entropies")
+    a = capi.ReadoutBwdArgs(C.sizeof(capi.ReadoutBwdArgs), flags, V, d, rows, xp, sp, pitch, weights.data_ptr(), 0 if g_logp is None else _need_flat(tokens, torch.int32, rows, "tokens", dev),
+                            stats, ent if g_ent is not None else 0, _need_flat(g_logp, torch.float32, rows, "g_logp", dev), _need_flat(g_ent, torch.float32, rows, "g_ent", dev), _p(d_hidden), _p(d_weights), 0, 0, workspace.data_ptr(), workspace.numel() * workspace.element_size(), temperature)
     if allow is not None or allow_bits is not None:
         allow = _readout_masks(a, V, rows, allow, allow_bits, dev)
     _launch(dev, "nrl_readout_bwd", C.byref(a))
