@@ -98,7 +98,7 @@ struct HeadGemm {
     uint32_t out_f32, out_add; // type of `out`; add to what it holds
     uint32_t out_col0;         // kEpiWeight: first column (or first row, with out_row0) of this piece
     uint32_t out_row0;
-    uint32_t wide;             // rows of out are 32-byte aligned
+    uint32_t wide;             // rows of out are 32-byte aligned (kEpiInt8: n_scale is 16-byte aligned)
     uint32_t staged;           // results leave through shared memory and TMA stores (map_out)
     // kEpiInt8
     const float* m_scale;      // [m]
@@ -153,6 +153,11 @@ __device__ __forceinline__ void pin32(float* z) {
 #pragma unroll
     for (int i = 0; i < 32; i += 8)
         asm volatile("" : "+f"(z[i]), "+f"(z[i + 1]), "+f"(z[i + 2]), "+f"(z[i + 3]), "+f"(z[i + 4]), "+f"(z[i + 5]), "+f"(z[i + 6]), "+f"(z[i + 7]));
+}
+__device__ __forceinline__ void pin16(uint32_t* z) {
+#pragma unroll
+    for (int i = 0; i < 16; i += 8)
+        asm volatile("" : "+r"(z[i]), "+r"(z[i + 1]), "+r"(z[i + 2]), "+r"(z[i + 3]), "+r"(z[i + 4]), "+r"(z[i + 5]), "+r"(z[i + 6]), "+r"(z[i + 7]));
 }
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {  // nearest, ties to even; NaN stays NaN
     uint32_t r;
@@ -722,29 +727,45 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kHgThreads, 1)
                 // thread = vocabulary entry, registers = tokens: a warp's store covers 32 consecutive entries of a row
                 const float scale = r.xs.x;
                 wait();
+                const uint64_t pitch = p.out_pitch * (p.out_f32 ? 4u : 2u);
+                uint8_t* o = reinterpret_cast<uint8_t*>(p.out) + (uint64_t)col0 * pitch + (uint64_t)row * (p.out_f32 ? 4u : 2u);
 #pragma unroll 1
-                for (uint32_t c = 0; c < half_cols; c += 16) {
+                for (uint32_t c = 0; c < half_cols; c += 16, o += 16 * pitch) {
+                    const uint32_t col = col0 + c, left = col < p.n ? min(16u, p.n - col) : 0u;  // tokens here
+                    float ns[16];
+                    if (left == 16u && p.wide) {
+#pragma unroll
+                        for (int i = 0; i < 4; i++) {
+                            const float4 q = __ldg(reinterpret_cast<const float4*>(p.n_scale + col) + i);
+                            ns[4 * i] = q.x; ns[4 * i + 1] = q.y; ns[4 * i + 2] = q.z; ns[4 * i + 3] = q.w;
+                        }
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 16; i++) ns[i] = (uint32_t)i < left ? __ldg(p.n_scale + col + i) : 0.f;
+                    }
                     uint32_t z[16];
                     if (some && ok) {
                         tc_ld16(taddr + c, z);
                         tc_wait_ld();
+                        pin16(z);
                         if (c + 16 >= half_cols) release();
                     } else {
 #pragma unroll
                         for (int i = 0; i < 16; i++) z[i] = 0u;
                     }
-                    const uint32_t col = col0 + c;
-                    if (live) {
+                    if (!live) continue;
+                    if (!ok) {
 #pragma unroll
-                        for (int i = 0; i < 16; i++) {
-                            if (col + i < p.n) {
-                                float y = ((float)(int32_t)z[i] * __ldg(p.n_scale + col + i)) * scale;
-                                if (!ok) y = __int_as_float(0x7fc00000);
-                                const uint64_t at = (uint64_t)(col + i) * p.out_pitch + row;
-                                if (p.out_f32) reinterpret_cast<float*>(p.out)[at] = y;
-                                else reinterpret_cast<uint16_t*>(p.out)[at] = (uint16_t)pack_bf16(y, 0.f);
-                            }
-                        }
+                        for (int i = 0; i < 16; i++) ns[i] = __int_as_float(0x7fc00000);
+                    }
+                    if (p.out_f32) {
+#pragma unroll
+                        for (int i = 0; i < 16; i++)
+                            if ((uint32_t)i < left) *reinterpret_cast<float*>(o + i * pitch) = ((float)(int32_t)z[i] * ns[i]) * scale;
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 16; i++)
+                            if ((uint32_t)i < left) *reinterpret_cast<uint16_t*>(o + i * pitch) = (uint16_t)pack_bf16(((float)(int32_t)z[i] * ns[i]) * scale, 0.f);
                     }
                 }
             }

@@ -392,7 +392,9 @@ extern "C" int nrl_i8_quantize_rows(uint32_t dtype, uint64_t rows, uint32_t d, n
     const void* xp = (const void*)x;
     int8_t* q = (int8_t*)values;
     float* sp = (float*)scales;
-    const bool many = rows >= 8 * 148;  // a warp per row fills the device
+    // a warp per row where that fills the device and the rows in flight stay in L2 for their second look (8192 rows: 30 against 35 us
+    // for 8 KB of bf16, 53 against 35 for 16 KB of f32)
+    const bool many = rows >= 8 * 148 && (uint64_t)d * (dtype == NRL_F32 ? 4 : 2) <= 8192;
     const unsigned grid = (unsigned)(many ? (rows + 7) / 8 : rows);
     const dim3 g(grid);
     if (dtype == NRL_BF16) return many ? launch(quantise_rows_kernel<NRL_BF16, 1>, g, 256, 0, st, xp, rows, d, pitch, q, sp, vec) : launch(quantise_rows_kernel<NRL_BF16, 8>, g, 256, 0, st, xp, rows, d, pitch, q, sp, vec);
@@ -458,6 +460,7 @@ extern "C" int nrl_i8_matmul(const nrl_i8_matmul_args* a, nrl_stream stream) {
     p.out = (void*)a->out;
     p.out_pitch = a->n;
     p.out_f32 = a->dtype == NRL_F32 ? 1u : 0u;
+    p.wide = a->x_scales % 16 == 0 ? 1u : 0u;
     CUtensorMap mw, mx;
     // the extent along K is k, not the pitch: what lies behind a row's k integers is read as zeros
     rc = encode_2d(&mw, true, a->w, a->k, a->n, a->w_pitch, 128, 128);

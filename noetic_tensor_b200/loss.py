@@ -82,10 +82,9 @@ def _head_ce(head, S, N, tok, keep, smoothing, reduce):
     if smoothing > 0.0:
         raise ValueError("label smoothing needs the sum of a row's logits: a Head has none")
     run = head.run(tok, keep, ce_seeds=S if reduce else 0)
-    logp = run.fwd.logp
     if not reduce:
-        return Loss(-logp.reshape(S, N), lambda up: run.backward(g_logp=-up))
-    return Loss(run.fwd.ce_loss, lambda up: run.backward(g_logp=ops.ce_mean(logp, S, keep, up, want_loss=False)[1]), lambda: run.backward(g_logp=run.fwd.ce_g_logp))
+        return Loss(-run.fwd.logp.reshape(S, N), lambda up: run.backward(g_logp=-up))
+    return Loss(run.fwd.ce_loss, lambda up: run.backward(g_logp=ops.ce_mean(run.fwd.logp, S, keep, up, want_loss=False)[1]), lambda: run.backward(g_logp=run.fwd.ce_g_logp))
 
 
 def nll(logits, targets):
