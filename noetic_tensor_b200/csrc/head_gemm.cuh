@@ -1,7 +1,7 @@
 // The matrix products of the readout's backward pass and of its 8-bit form: one kernel on CTA pairs
 // (tcgen05.mma.cta_group::2, f32 or 32-bit integer accumulators in tensor memory), five epilogues.
 //
-//   kEpiStats   z = x · W for the scored rows x; the epilogue keeps, per row and 128 columns, the maximum,
+//   kEpiStats   z = x · W for the scored rows x; the epilogue keeps, per row and half tile, the maximum,
 //               Σ exp(z − max), Σ exp(z − max)·(z − max) and the given token's logit
 //   kEpiGrad    z = x · W for the scored rows x and a piece of the vocabulary; the epilogue turns the
 //               accumulators into dz = ∂/∂z of the per-row terms and writes them as bf16:
@@ -48,18 +48,15 @@ constexpr float kAccumulatorLoss = 1.6e-8f;
 inline float logit_scale(uint32_t d, float tau) { return (1.f + kAccumulatorLoss * (float)((d + 15) / 16)) / tau; }
 
 // Ranges of K in dx = dz·Wᵀ for `tiles` tiles of dx and `chunks` steps of K: with few tiles the steps of a tile go to several
-// pairs, whose sums are added afterwards. The count that takes the fewest waves' worth of steps, ceil(tiles·s / 74) / s, with at most
-// two waves and at least 24 steps a range (10 us of products: adding up is a launch of 3 us); a split has to gain 5 %. Decided where the number
-// of scored rows is known, on the device, and the same there and in the kernel that adds up.
+// pairs, whose sums are added afterwards. As many ranges as fill one wave of pairs, or two where that takes 5 % fewer steps, each of
+// at least 24 steps (10 us of products: adding up is a launch of 3 us). Decided where the number of scored rows is known, on
+// the device, and the same there and in the kernel that adds up.
 constexpr uint32_t kPairs = 74;  // CTA pairs that run side by side (148 SMs)
 __host__ __device__ inline uint32_t hidden_split(uint32_t tiles, uint32_t chunks) {
-    uint32_t best = 1;
-    float least = (float)((tiles + kPairs - 1) / kPairs);
-    for (uint32_t s = 2; tiles * s <= 2 * kPairs && chunks >= 24 * s; s++) {
-        const float t = (float)((tiles * s + kPairs - 1) / kPairs) / (float)s;
-        if (t < 0.95f * least) { least = t; best = s; }
-    }
-    return best;
+    if (tiles == 0 || tiles > kPairs) return 1u;
+    const uint32_t most = chunks / 24u, a = kPairs / tiles, b = 2 * kPairs / tiles;
+    const uint32_t one = most < a ? (most ? most : 1u) : a, two = most < b ? (most ? most : 1u) : b;  // steps of a tile: 1 / one, or 2 / two
+    return 200u * one < 95u * two ? two : one;
 }
 
 struct HeadGemm {
@@ -67,7 +64,7 @@ struct HeadGemm {
     const uint32_t* m_count;   // device: the rows in use along M, of which this launch takes m from m_first on; or null: all m
     uint32_t m_first;
     const uint32_t* k_count;   // device: the extent along K (≤ k), or null
-    uint32_t bn;               // columns per tile (a multiple of 32, ≤ 256)
+    uint32_t bn;               // columns per tile: 256 or 128, kEpiInt8 a multiple of 32 up to 256
     uint32_t stages;
     uint32_t a_mn, b_mn;       // A / B contiguous along M / N instead of K
     uint32_t b_n0, b_k0;       // where this piece of the vocabulary begins in B, along N / along K
@@ -87,7 +84,7 @@ struct HeadGemm {
     uint32_t allow_wide;       // every row of the byte mask is 4-byte aligned
     uint32_t vocab;            // V
     uint32_t v0;               // first column of this piece
-    float4* parts;             // kEpiStats [rows, parts_pitch]: (max, sum, entropy sum, token's logit) per 128 columns
+    float4* parts;             // kEpiStats [rows, parts_pitch]: (max, sum, entropy sum, token's logit) per half tile
     uint32_t parts_pitch;
     // kEpiHidden, kEpiWeight
     const float* alpha;        // device scalar
@@ -506,7 +503,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kHgThreads, 1)
                     }
                     if (p.b_mn) {
                         tma_load_2d_pair(b_at, &map_b, n0, kb, bar);
-                        tma_load_2d_pair(b_at + 8192, &map_b, n0 + 64, kb, bar);
+                        if (p.bn == 256) tma_load_2d_pair(b_at + 8192, &map_b, n0 + 64, kb, bar);
                     } else {
                         tma_load_2d_pair(b_at, &map_b, kb, n0, bar);
                     }
@@ -565,6 +562,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kHgThreads, 1)
         // ---- epilogue (both CTAs): thread = row of the output (of the transposed one for kEpiInt8) ---------
         const uint32_t quarter = (uint32_t)warp & 3u, half = ((uint32_t)warp - 2u) >> 2;
         const uint32_t half_cols = p.bn / 2;  // this warp's columns: [half · bn/2, + bn/2), a multiple of 16
+        const int chunks = (int)half_cols / 32;  // four or two of 32 columns in the bf16 products
         const uint32_t stage_out = smem_base + smem_tiles(EPI) + ((uint32_t)warp - 2u) * stage_tiles(EPI) * kHgStageOut;
         uint32_t sent = 0;  // staging tiles sent off so far
         float alpha = 1.f;
@@ -632,13 +630,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kHgThreads, 1)
                 wait();
                 mask.settle(p, p.v0 + col0, lane);
 #pragma unroll 1
-                for (int c = 0; c < 4; c++) {
+                for (int c = 0; c < chunks; c++) {
                     float y[32];
                     tc_ld32(taddr + 32 * c, reinterpret_cast<uint32_t*>(y));
                     tc_wait_ld();
                     pin32(y);
-                    if (c == 3) release();
-                    if (c == 1 && more_tiles) mask.load(p, ahead.caller_row, p.v0 + next.tn * p.bn + half * half_cols, ahead.live, lane);
+                    if (c == chunks - 1) release();
+                    if (c == 0 && more_tiles) mask.load(p, ahead.caller_row, p.v0 + next.tn * p.bn + half * half_cols, ahead.live, lane);
                     if (!ok) {
 #pragma unroll
                         for (int i = 0; i < 32; i++) y[i] = __int_as_float(0x7fc00000);
@@ -669,13 +667,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kHgThreads, 1)
                 wait();
                 const bool there = some && ok;
 #pragma unroll 1
-                for (int c = 0; c < 4; c++) {
+                for (int c = 0; c < chunks; c++) {
                     float z[32];
                     if (there) {
                         tc_ld32(taddr + 32 * c, reinterpret_cast<uint32_t*>(z));
                         tc_wait_ld();
                         pin32(z);
-                        if (c == 3) release();
+                        if (c == chunks - 1) release();
                     } else {
 #pragma unroll
                         for (int i = 0; i < 32; i++) z[i] = ok ? 0.f : __int_as_float(0x7fc00000);

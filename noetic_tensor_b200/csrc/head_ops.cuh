@@ -319,44 +319,55 @@ __global__ void __launch_bounds__(256) head_finish_kernel(HeadFinish p) {
     for (uint64_t s = 0; s < p.ce.seeds; s++) ce_mean_seed(p.ce, s, sh);
 }
 
-// d_hidden of the scored rows from the ranges of a split sum, added in range order; nothing to do where K was not split. A block
-// takes 512 columns of a row and goes on with the grid's stride (the host does not know the number of rows).
-__global__ void __launch_bounds__(128) head_fold_kernel(const uint32_t* count, const float* alpha, const float4* more, const uint32_t* rows_at, const float* acc, uint32_t chunks, uint32_t d, void* out,
+// d_hidden of the scored rows from the ranges of a split sum; nothing to do where K was not split. A block takes 128 columns of a row,
+// 32 threads × 4 columns, with eight groups of threads: group g adds the ranges g, g + 8, … in order, then the groups are added in
+// order. It goes on with the grid's stride (the host does not know the number of rows).
+__global__ void __launch_bounds__(256) head_fold_kernel(const uint32_t* count, const float* alpha, const float4* more, const uint32_t* rows_at, const float* acc, uint32_t chunks, uint32_t d, void* out,
                                                         uint32_t out_f32, uint32_t add) {
+    __shared__ float4 part[8][32];
     next_kernel_may_start();
     after_previous_kernel();
-    const uint32_t n = *count, tiles_m = (n + 255) / 256, nsplit = hidden_split(tiles_m * ((d + 255) / 256), chunks), across = (d + 511) / 512;
+    const uint32_t n = *count, tiles_m = (n + 255) / 256, nsplit = hidden_split(tiles_m * ((d + 255) / 256), chunks), across = (d + 127) / 128;
     if (nsplit == 1) return;
     const float common = *alpha;
     const uint64_t range = (uint64_t)tiles_m * 256 * d;
+    const uint32_t t = threadIdx.x & 31, g = threadIdx.x >> 5;
     for (uint32_t b = blockIdx.x; b < n * across; b += gridDim.x) {
-        const uint32_t i = b / across, c = ((b - i * across) * 128 + threadIdx.x) * 4;
-        if (c >= d) continue;
-        const float scale = common * more[i].y;
-        const uint64_t r = rows_at[i];
+        const uint32_t i = b / across, c = ((b - i * across) * 32 + t) * 4;
         const float* q0 = acc + (uint64_t)i * d + c;
         float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-        for (uint32_t s = 0; s < nsplit; s++) {
-            const float4 q = *reinterpret_cast<const float4*>(q0 + s * range);
-            y.x += q.x; y.y += q.y; y.z += q.z; y.w += q.w;
-        }
-        y.x *= scale; y.y *= scale; y.z *= scale; y.w *= scale;
-        if (out_f32) {
-            float4* o = reinterpret_cast<float4*>(reinterpret_cast<float*>(out) + r * d + c);
-            if (add) {
-                const float4 q = *o;
+        if (c < d) {
+#pragma unroll 8
+            for (uint32_t s = g; s < nsplit; s += 8) {
+                const float4 q = *reinterpret_cast<const float4*>(q0 + s * range);
                 y.x += q.x; y.y += q.y; y.z += q.z; y.w += q.w;
             }
-            *o = y;
-        } else {
-            uint2* o = reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(out) + r * d + c);
-            if (add) {
-                const uint2 q = *o;
-                y.x += bf16_lo(q.x); y.y += bf16_hi(q.x); y.z += bf16_lo(q.y); y.w += bf16_hi(q.y);
-            }
-            *o = make_uint2(pack_bf16(y.x, y.y), pack_bf16(y.z, y.w));
         }
+        part[g][t] = y;
+        __syncthreads();
+        if (g == 0 && c < d) {
+#pragma unroll
+            for (int k = 1; k < 8; k++) { y.x += part[k][t].x; y.y += part[k][t].y; y.z += part[k][t].z; y.w += part[k][t].w; }
+            const float scale = common * more[i].y;
+            const uint64_t r = rows_at[i];
+            y.x *= scale; y.y *= scale; y.z *= scale; y.w *= scale;
+            if (out_f32) {
+                float4* o = reinterpret_cast<float4*>(reinterpret_cast<float*>(out) + r * d + c);
+                if (add) {
+                    const float4 q = *o;
+                    y.x += q.x; y.y += q.y; y.z += q.z; y.w += q.w;
+                }
+                *o = y;
+            } else {
+                uint2* o = reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(out) + r * d + c);
+                if (add) {
+                    const uint2 q = *o;
+                    y.x += bf16_lo(q.x); y.y += bf16_hi(q.x); y.z += bf16_lo(q.y); y.w += bf16_hi(q.y);
+                }
+                *o = make_uint2(pack_bf16(y.x, y.y), pack_bf16(y.z, y.w));
+            }
+        }
+        __syncthreads();
     }
 }
 

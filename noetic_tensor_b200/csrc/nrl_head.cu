@@ -53,6 +53,11 @@ static int launch_masked(const CUtensorMap& ma, const CUtensorMap& mb, const CUt
 static inline uint64_t up(uint64_t x, uint64_t to) { return (x + to - 1) / to * to; }
 static inline uint32_t tiles256(uint64_t x) { return (uint32_t)((x + 255) / 256); }
 
+// Columns per tile of a bf16 product over `rows` × `cols`: half the width where that puts twice the pairs to work (140 rows at
+// V = 1120, d = 1808: five pairs took 20 us).
+static uint32_t tile_width(uint64_t rows, uint64_t cols) { return (uint64_t)tiles256(rows) * tiles256(cols) <= kPairs / 2 ? 128u : 256u; }
+static uint64_t tiles_of(uint64_t rows, uint64_t cols, uint32_t bn) { return (uint64_t)tiles256(rows) * ((cols + bn - 1) / bn); }
+
 static int launch_rows(HeadRows& hr, cudaStream_t st) {
     // a block owns 8 rows, one per warp; more when there would be over 1024 blocks, since each looks at every row's upstream
     hr.per_block = (uint32_t)((hr.rows + 1023) / 1024);
@@ -75,7 +80,7 @@ static void set_mask(HeadGemm& g, nrl_devptr mask, uint64_t stride) {
 // (rows, V, d) only.
 struct BwdPlan {
     uint64_t rows_pad;
-    uint32_t vc, pieces, chunks;
+    uint32_t vc, pieces, chunks, grad_bn;
     bool may_split;
     uint64_t off_coef, off_more, off_rows, off_x, off_dz, off_acc, bytes;
 };
@@ -90,6 +95,7 @@ static BwdPlan bwd_plan(uint64_t rows, uint32_t V, uint32_t d) {
     b.vc = (uint32_t)up((V + b.pieces - 1) / b.pieces, 256);  // pieces of about the same width
     b.pieces = (V + b.vc - 1) / b.vc;
     b.chunks = b.vc / 64;
+    b.grad_bn = tile_width(rows, b.vc);
     // any number of scored rows up to `rows` may turn up: whether one of them would have dx's K split
     uint64_t split_units = 0;
     const uint32_t tn = tiles256(d), tm = tiles256(rows);
@@ -183,12 +189,12 @@ extern "C" int nrl_readout_bwd(const nrl_readout_bwd_args* a, nrl_stream stream)
     // boxes of 64 elements of K × 128 rows, or of 64 columns × 64 elements of K; the weight is read along K by one product and across
     // it by the other
     const uint64_t w_in = vd ? a->d : a->V, w_rows = vd ? a->V : a->d;
-    CUtensorMap x_k, x_mn, w_k, w_mn, dz_k, dz_mn, dz_out, dw_out;
+    CUtensorMap x_k, x_mn, w_rows_k, w_k, w_mn, dz_k, dz_mn, dz_out, dw_out;
     const bool dw32 = (a->flags & NRL_READOUT_BWD_D_WEIGHTS_F32) != 0;
     memset(&dw_out, 0, sizeof dw_out);
     if ((rc = encode_2d(&x_k, false, x, a->d, b.rows_pad, hr.x_pitch, 64, 128)) || (rc = encode_2d(&x_mn, false, x, a->d, b.rows_pad, hr.x_pitch, 64, 64)) ||
         (rc = encode_2d(&dz_k, false, dz, b.vc, b.rows_pad, b.vc, 64, 128)) || (rc = encode_2d(&dz_mn, false, dz, b.vc, b.rows_pad, b.vc, 64, 64)) ||
-        (rc = encode_2d(&dz_out, false, dz, b.vc, b.rows_pad, b.vc, 64, 32)) || (rc = encode_2d(&w_k, false, a->weights, w_in, w_rows, w_in, 64, 128)) ||
+        (rc = encode_2d(&dz_out, false, dz, b.vc, b.rows_pad, b.vc, 64, 32)) || (rc = vd ? encode_2d(&w_rows_k, false, a->weights, w_in, w_rows, w_in, 64, b.grad_bn / 2) : encode_2d(&w_k, false, a->weights, w_in, w_rows, w_in, 64, 128)) ||
         (rc = encode_2d(&w_mn, false, a->weights, w_in, w_rows, w_in, 64, 64)))
         return rc;
     if (a->d_weights) {
@@ -207,7 +213,8 @@ extern "C" int nrl_readout_bwd(const nrl_readout_bwd_args* a, nrl_stream stream)
             p.b_mn = vd ? 0u : 1u;
             p.b_n0 = v0;
             p.v0 = v0;
-            rc = launch_masked<kEpiGrad>(x_k, vd ? w_k : w_mn, dz_out, p, allow_bits, (uint64_t)tiles256(a->rows) * tiles256(cols), st);
+            p.bn = b.grad_bn;
+            rc = launch_masked<kEpiGrad>(x_k, vd ? w_rows_k : w_mn, dz_out, p, allow_bits, tiles_of(a->rows, cols, p.bn), st);
             if (rc) return rc;
         }
         if (a->d_hidden) {  // dx += dz · Wᵀ
@@ -230,8 +237,8 @@ extern "C" int nrl_readout_bwd(const nrl_readout_bwd_args* a, nrl_stream stream)
             rc = launch_gemm<kEpiHidden>(dz_k, vd ? w_mn : w_k, dz_out, p, b.may_split ? kPairs : (uint64_t)tiles256(a->rows) * tiles256(a->d), st);
             if (rc) return rc;
             if (b.may_split && piece + 1 == b.pieces) {
-                const uint64_t most = (a->rows < (uint64_t)kPairs * 256 ? a->rows : (uint64_t)kPairs * 256) * ((a->d + 511) / 512);  // more rows are never split
-                rc = launch(head_fold_kernel, dim3((unsigned)(most < 8 * 148 ? most : 8 * 148)), 128, 0, st, hr.count, hr.alpha, hr.more, hr.rows_at, p.acc, b.chunks, a->d, (void*)a->d_hidden, p.out_f32, p.out_add);
+                const uint64_t most = (a->rows < (uint64_t)kPairs * 256 ? a->rows : (uint64_t)kPairs * 256) * ((a->d + 127) / 128);  // more rows are never split
+                rc = launch(head_fold_kernel, dim3((unsigned)(most < 8 * 148 ? most : 8 * 148)), 256, 0, st, hr.count, hr.alpha, hr.more, hr.rows_at, p.acc, b.chunks, a->d, (void*)a->d_hidden, p.out_f32, p.out_add);
                 if (rc) return rc;
             }
         }
@@ -250,7 +257,8 @@ extern "C" int nrl_readout_bwd(const nrl_readout_bwd_args* a, nrl_stream stream)
             p.out_add = (a->flags & NRL_READOUT_BWD_ADD_D_WEIGHTS) ? 1u : 0u;
             p.wide = (a->d_weights % 32 == 0 && (p.out_f32 || p.out_pitch % 16 == 0)) ? 1u : 0u;
             p.staged = p.out_add ? 0u : 1u;  // sums into what is there go through registers
-            rc = launch_gemm<kEpiWeight>(vd ? dz_mn : x_mn, vd ? x_mn : dz_mn, dw_out, p, (uint64_t)tiles256(p.m) * tiles256(p.n), st);
+            p.bn = tile_width(p.m, p.n);
+            rc = launch_gemm<kEpiWeight>(vd ? dz_mn : x_mn, vd ? x_mn : dz_mn, dw_out, p, tiles_of(p.m, p.n, p.bn), st);
             if (rc) return rc;
         }
     }
@@ -263,16 +271,19 @@ constexpr uint64_t kScoredChunk = 16384;  // rows per launch: what bounds the pa
 
 struct ScoredPlan {
     bool gather;  // the scored rows are brought together first
+    uint32_t bn, parts_pitch;
     uint64_t rows_pad, off_rows, off_x, off_parts, bytes;
 };
 static ScoredPlan scored_plan(uint64_t rows, uint32_t V, uint32_t d, bool scored) {
     ScoredPlan s;
     s.gather = scored && rows > 256;  // up to one row block nothing is saved by leaving rows out
     s.rows_pad = up(rows, 256);
+    s.bn = tile_width(rows, V);
+    s.parts_pitch = 2 * ((V + s.bn - 1) / s.bn);
     uint64_t at = 256;
     s.off_rows = at; at += s.gather ? up(rows * 4, 256) : 0;
     s.off_x = at; at += s.gather ? s.rows_pad * up(d, 64) * 2 : 0;
-    s.off_parts = at; at += (s.rows_pad < kScoredChunk ? s.rows_pad : kScoredChunk) * tiles256(V) * 2 * 16;
+    s.off_parts = at; at += (s.rows_pad < kScoredChunk ? s.rows_pad : kScoredChunk) * s.parts_pitch * 16;
     s.bytes = at;
     return s;
 }
@@ -322,13 +333,13 @@ extern "C" int nrl_readout_scored_fwd(const nrl_readout_scored_args* a, nrl_stre
     CUtensorMap mx, mw;
     rc = encode_2d(&mx, false, s.gather ? ws + s.off_x : a->hidden, a->d, s.gather ? s.rows_pad : a->rows, s.gather ? up(a->d, 64) : a->d, 64, 128);
     if (rc) return rc;
-    rc = vd ? encode_2d(&mw, false, a->weights, a->d, a->V, a->d, 64, 128) : encode_2d(&mw, false, a->weights, a->V, a->d, a->V, 64, 64);
+    rc = vd ? encode_2d(&mw, false, a->weights, a->d, a->V, a->d, 64, s.bn / 2) : encode_2d(&mw, false, a->weights, a->V, a->d, a->V, 64, 64);
     if (rc) return rc;
     for (uint64_t r0 = 0; r0 < a->rows; r0 += kScoredChunk) {
         const uint64_t n = a->rows - r0 < kScoredChunk ? a->rows - r0 : kScoredChunk;
         HeadGemm p;
         memset(&p, 0, sizeof p);
-        p.bn = 256;
+        p.bn = s.bn;
         p.group_m = 16;
         p.m = (uint32_t)n;
         p.m_count = s.gather ? (const uint32_t*)ws : nullptr;
@@ -346,8 +357,8 @@ extern "C" int nrl_readout_scored_fwd(const nrl_readout_scored_args* a, nrl_stre
         p.vocab = a->V;
         p.zero = (uint32_t*)(ws + 8);
         p.parts = (float4*)(ws + s.off_parts);
-        p.parts_pitch = tiles256(a->V) * 2;
-        rc = launch_masked<kEpiStats>(mx, mw, mx, p, a->flags & NRL_READOUT_MASK_BITS, (uint64_t)tiles256(n) * tiles256(a->V), st);
+        p.parts_pitch = s.parts_pitch;
+        rc = launch_masked<kEpiStats>(mx, mw, mx, p, a->flags & NRL_READOUT_MASK_BITS, tiles_of(n, a->V, s.bn), st);
         if (rc) return rc;
         HeadFinish f;
         memset(&f, 0, sizeof f);

@@ -210,32 +210,19 @@ def row_backward(logits, fwd, *, ref_logits=None, allow=None, add_mask=None, tem
 
 
 def _tok_args(kind, logp, other, weights, mask, clip_low=0.0, clip_high=0.0, dual=None, clamp=None):
-    S, B, T = logp.shape
-    dev = logp.device
-    a = capi.TokenLossArgs()
-    a.struct_size = C.sizeof(a)
-    a.kind, a.S, a.B, a.T = kind, S, B, T
-    _need(logp, torch.float32, (S, B, T), "logp", dev)
-    a.logp = _p(logp)
+    shape, dev = logp.shape, logp.device
+    S, B, T = shape
+    _need(logp, torch.float32, shape, "logp", dev)
+    w_per_seq = 0
     if other is not None:
-        _need(other, torch.float32, (S, B, T), "old/ref log-probs", dev)
-        a.other = _p(other)
+        _need(other, torch.float32, shape, "old/ref log-probs", dev)
     if weights is not None:
-        if weights.dim() == 2:
-            _need(weights, torch.float32, (S, B), "weights", dev)
-            a.weights_per_sequence = 1
-        else:
-            _need(weights, torch.float32, (S, B, T), "weights", dev)
-        a.weights = _p(weights)
+        w_per_seq = 1 if weights.dim() == 2 else 0
+        _need(weights, torch.float32, (S, B) if w_per_seq else shape, "weights", dev)
     if mask is not None:
-        _need(mask, torch.float32, (S, B, T), "mask", dev)
-        a.mask = _p(mask)
-    a.clip_low, a.clip_high = clip_low, clip_high
-    if dual is not None:
-        a.has_dual, a.dual = 1, dual
-    if clamp is not None:
-        a.has_clamp, a.clamp = 1, clamp
-    return a
+        _need(mask, torch.float32, shape, "mask", dev)
+    return capi.TokenLossArgs(C.sizeof(capi.TokenLossArgs), kind, S, B, T, logp.data_ptr(), _p(other), _p(weights), w_per_seq, dual is not None, _p(mask), clip_low, clip_high,
+                              0.0 if dual is None else dual, 0.0 if clamp is None else clamp, clamp is not None)
 
 
 def token_loss(kind, logp, *, other=None, weights=None, mask=None, clip_low=0.0, clip_high=0.0, dual=None, clamp=None, want_grad=True, upstream=None, accumulate_into=None):
@@ -268,32 +255,25 @@ def token_objective(kind, logp, reduction, *, other=None, weights=None, mask=Non
     """A token loss of `logp` plus the per-token KL and entropy, all reduced per seed with one
     TokenReduction, and the per-token upstream gradients of the row backward, in one launch
     (nrl_token_objective). `up_*` are the upstream gradients [S] of the three reduced values (None = ones)."""
-    dev = logp.device
-    S, B, T = logp.shape
-    a = capi.TokenObjectiveArgs()
-    a.struct_size = C.sizeof(a)
-    a.reduction = reduction
-    a.policy = _tok_args(kind, logp, other, weights, mask, clip_low, clip_high, dual, clamp)
-    out = TokenObjective()
-    f32 = dict(dtype=torch.float32, device=dev)
+    shape, dev = logp.shape, logp.device
+    S = shape[0]
+    policy = _tok_args(kind, logp, other, weights, mask, clip_low, clip_high, dual, clamp)
     for name, t in (("kl", kl), ("entropy", entropy)):
         if t is not None:
-            _need(t, torch.float32, (S, B, T), name, dev)
+            _need(t, torch.float32, shape, name, dev)
     for name, t in (("up_policy", up_policy), ("up_kl", up_kl), ("up_entropy", up_entropy)):
         if t is not None:
             _need(t, torch.float32, (S,), name, dev)
-    a.kl, a.entropy = _p(kl), _p(entropy)
-    a.up_policy, a.up_kl, a.up_entropy = _p(up_policy), _p(up_kl), _p(up_entropy)
-    out.policy = torch.empty(S, **f32)
-    out.kl = torch.empty(S, **f32) if kl is not None else None
-    out.entropy = torch.empty(S, **f32) if entropy is not None else None
-    out.g_logp = torch.empty(S, B, T, **f32) if want_grads else None
-    out.g_kl = torch.empty(S, B, T, **f32) if (want_grads and kl is not None) else None
-    out.g_ent = torch.empty(S, B, T, **f32) if (want_grads and entropy is not None) else None
-    a.out_policy, a.out_kl, a.out_entropy = _p(out.policy), _p(out.kl), _p(out.entropy)
-    a.g_logp, a.g_kl, a.g_ent = _p(out.g_logp), _p(out.g_kl), _p(out.g_ent)
-    with torch.cuda.device(dev):
-        capi.check(capi.lib().nrl_token_objective(C.byref(a), _stream(dev)), "nrl_token_objective")
+    out = TokenObjective()
+
+    def new(size, want):
+        return torch.empty(size, dtype=torch.float32, device=dev) if want else None
+
+    out.policy, out.kl, out.entropy = new(S, True), new(S, kl is not None), new(S, entropy is not None)
+    out.g_logp, out.g_kl, out.g_ent = new(shape, want_grads), new(shape, want_grads and kl is not None), new(shape, want_grads and entropy is not None)
+    a = capi.TokenObjectiveArgs(C.sizeof(capi.TokenObjectiveArgs), reduction, policy, _p(kl), _p(entropy), _p(up_policy), _p(up_kl), _p(up_entropy), out.policy.data_ptr(), _p(out.kl), _p(out.entropy),
+                                _p(out.g_logp), _p(out.g_kl), _p(out.g_ent))
+    _launch(dev, "nrl_token_objective", C.byref(a))
     return out
 
 
