@@ -11,12 +11,14 @@
 //   kEpiWeight  dW = xᵀ · dz for a piece of the vocabulary
 //   kEpiInt8    z[r, v] = s_r·w_v·Σ_k q[r, k]·p[v, k] in 8-bit integers (sums exact in 32 bits)
 //
-// A pair of CTAs owns 256 rows × `bn` columns of the output; each CTA loads its 128 rows of A and half
+// A pair of CTAs (tcgen05 cta_group::2) owns 256 rows × `bn` columns of the output; each CTA loads its 128 rows of A and half
 // of B per stage (TMA, 128-byte swizzle, no multicast), one thread of the first CTA issues the products
 // for both, and the 256-column accumulators are double-buffered so that a tile's epilogue runs under the
 // next tile's products. The grid is persistent: 74 pairs walk the tiles in a fixed order, so every sum
 // has a fixed order and results are bitwise reproducible. A and B may each be contiguous along K or along
-// their other axis (the descriptors' major bits), so dz, x and W are read as they lie in memory.
+// their other axis (the descriptors' major bits), so dz, x and W are read as they lie in memory. With at most 128 rows every CTA
+// works by itself (cta_group::1, PAIR = false): a pair would multiply 128 rows of zeros, and the pass is then bound by the weight's
+// bytes instead of the tensor pipe.
 //
 // Bound: the tensor pipe for the large products, HBM for the few-row forms (the weight is read once per
 // call). Waits are bounded as in the readout forward; a role that gives up raises the pair's abort flag
@@ -48,16 +50,27 @@ constexpr float kAccumulatorLoss = 1.6e-8f;
 inline float logit_scale(uint32_t d, float tau) { return (1.f + kAccumulatorLoss * (float)((d + 15) / 16)) / tau; }
 
 // Ranges of K in dx = dz·Wᵀ for `tiles` tiles of dx and `chunks` steps of K: with few tiles the steps of a tile go to several
-// pairs, whose sums are added afterwards. As many ranges as fill one wave of pairs, or two where that takes 5 % fewer steps, each of
+// pairs (or single CTAs), whose sums are added afterwards. As many ranges as fill one wave of those, or two where that takes 5 % fewer steps, each of
 // at least 24 steps (10 us of products: adding up is a launch of 3 us). Decided where the number of scored rows is known, on
 // the device, and the same there and in the kernel that adds up.
 constexpr uint32_t kPairs = 74;  // CTA pairs that run side by side (148 SMs)
-__host__ __device__ inline uint32_t hidden_split(uint32_t tiles, uint32_t chunks) {
-    if (tiles == 0 || tiles > kPairs) return 1u;
-    const uint32_t most = chunks / 24u, a = kPairs / tiles, b = 2 * kPairs / tiles;
+__host__ __device__ inline uint32_t hidden_split(uint32_t tiles, uint32_t chunks, uint32_t side_by_side) {
+    if (tiles == 0 || tiles > side_by_side) return 1u;
+    const uint32_t most = chunks / 24u, a = side_by_side / tiles, b = 2 * side_by_side / tiles;
     const uint32_t one = most < a ? (most ? most : 1u) : a, two = most < b ? (most ? most : 1u) : b;  // steps of a tile: 1 / one, or 2 / two
     return 200u * one < 95u * two ? two : one;
 }
+
+// n / d for n < 2^32 without a division: m = floor((2^32 − 1) / d) gives the quotient or one less.
+struct FastDiv {
+    uint32_t d, m;
+    __device__ __forceinline__ explicit FastDiv(uint32_t by) : d(by), m(by > 1u ? 0xffffffffu / by : 0u) {}
+    __device__ __forceinline__ uint32_t operator()(uint32_t n) const {
+        if (d <= 1u) return n;
+        const uint32_t q = __umulhi(n, m);
+        return n - q * d >= d ? q + 1u : q;
+    }
+};
 
 struct HeadGemm {
     uint32_t m, n, k;          // extents of the product
@@ -97,6 +110,7 @@ struct HeadGemm {
     uint32_t out_row0;
     uint32_t wide;             // rows of out are 32-byte aligned (kEpiInt8: n_scale is 16-byte aligned)
     uint32_t staged;           // results leave through shared memory and TMA stores (map_out)
+    __host__ __device__ static uint32_t acc_rows(uint32_t rows_in_use) { return (rows_in_use + 255u) & ~255u; }
     // kEpiInt8
     const float* m_scale;      // [m]
     const float* n_scale;      // [n]
@@ -412,22 +426,24 @@ __device__ __forceinline__ void store_row32(void* out, uint64_t at, bool f32, bo
     }
 }
 
-template <int EPI, int MASK>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kHgThreads, 1)
+// launched in clusters of two with PAIR, of one without
+template <int EPI, int MASK, bool PAIR>
+__global__ void __launch_bounds__(kHgThreads, 1)
     head_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap map_out, const __grid_constant__ HeadGemm p) {
     extern __shared__ uint8_t smem_raw[];
     constexpr bool kI8 = EPI == kEpiInt8;
     constexpr uint32_t kKStep = kI8 ? 128 : 64;  // elements of K per stage (128 bytes)
     const uint32_t smem_base = (smem_addr(smem_raw) + 1023u) & ~1023u;
-    const uint32_t b_bytes = (p.bn / 2) * 128, stage_bytes = kHgABytes + b_bytes;
+    constexpr uint32_t kCtas = PAIR ? 2 : 1, kRows = kCtas * kHgBM;  // CTAs that share a tile, and its rows
+    const uint32_t b_bytes = (p.bn / kCtas) * 128, stage_bytes = kHgABytes + b_bytes;
     const uint32_t bars = smem_base + smem_tiles(EPI) + kHgEpiWarps * stage_tiles(EPI) * kHgStageOut;
     const uint32_t bar_full = bars, bar_empty = bars + 8 * kHgMaxStages, bar_acc_full = bars + 16 * kHgMaxStages, bar_acc_empty = bar_acc_full + 16, bar_done = bar_acc_empty + 16;
     __shared__ uint32_t tmem_slot;
     __shared__ volatile uint32_t abort_flag;
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const uint32_t rank = cluster_cta_rank();
-    const uint32_t pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+    const uint32_t rank = PAIR ? cluster_cta_rank() : 0u;
+    const uint32_t pair = blockIdx.x / kCtas, pairs = gridDim.x / kCtas;
     if (threadIdx.x == 0) {
         abort_flag = 0u;
         for (uint32_t s = 0; s < kHgMaxStages; s++) {
@@ -436,15 +452,20 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kHgThreads, 1)
         }
         for (int a = 0; a < 2; a++) {
             mbar_init(bar_acc_full + 8 * a, 1);
-            mbar_init(bar_acc_empty + 8 * a, 2 * kHgEpiWarps);
+            mbar_init(bar_acc_empty + 8 * a, kCtas * kHgEpiWarps);
         }
         mbar_init(bar_done, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
     if (warp == 1) {
-        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_addr(&tmem_slot)) : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+        if constexpr (PAIR) {
+            asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_addr(&tmem_slot)) : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+        } else {
+            asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_addr(&tmem_slot)) : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        }
         tc_fence_before();
     }
     if (threadIdx.x == 64) {
@@ -453,28 +474,30 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kHgThreads, 1)
         if (EPI == kEpiGrad || EPI == kEpiWeight) prefetch_map(&map_out);
     }
     __syncthreads();
-    cluster_sync_all();  // both CTAs' barriers exist before anything crosses between them
+    if constexpr (PAIR) cluster_sync_all();  // both CTAs' barriers exist before anything crosses between them
     tc_fence_after();
     const uint32_t tmem = tmem_slot;
     after_previous_kernel();  // what came before is done; nothing above reads or writes global memory
     if (EPI == kEpiStats && blockIdx.x == 0 && threadIdx.x == 0 && p.zero) *p.zero = 0u;
     const uint32_t in_use = p.m_count ? *p.m_count : 0u;
     const uint32_t mm = p.m_count ? min(in_use - min(in_use, p.m_first), p.m) : p.m, kk = p.k_count ? min(*p.k_count, p.k) : p.k;
-    const uint32_t tiles_m = (mm + 2 * kHgBM - 1) / (2 * kHgBM), tiles_n = (p.n + p.bn - 1) / p.bn;
-    const uint32_t kchunks = (kk + kKStep - 1) / kKStep, nsplit = p.split ? hidden_split(tiles_m * tiles_n, p.split) : 1u, kper = (kchunks + nsplit - 1) / nsplit;
+    const uint32_t tiles_m = (mm + kRows - 1) / kRows, tiles_n = (p.n + p.bn - 1) / p.bn;
+    const uint32_t kchunks = (kk + kKStep - 1) / kKStep, nsplit = p.split ? hidden_split(tiles_m * tiles_n, p.split, PAIR ? kPairs : 2 * kPairs) : 1u, kper = (kchunks + nsplit - 1) / nsplit;
     const bool to_acc = p.acc_out || nsplit > 1;
     const uint32_t tiles = tiles_m * tiles_n * nsplit;  // the host keeps this below 2^31
     struct Item {
         uint32_t split, tm, tn, k0, k1;
     };
+    const FastDiv by_tiles(tiles_m * tiles_n), by_group(p.group_m * tiles_n), by_full(p.group_m), by_last(tiles_m > 0 ? tiles_m - (tiles_m - 1) / p.group_m * p.group_m : 1u);
     auto item = [&](uint32_t t) {
         Item it;
-        it.split = t / (tiles_m * tiles_n);
-        t -= it.split * (tiles_m * tiles_n);
-        const uint32_t per = p.group_m * tiles_n, g = t / per, first = g * p.group_m, here = min(p.group_m, tiles_m - first);
-        t -= g * per;
-        it.tm = first + t % here;
-        it.tn = t / here;
+        it.split = by_tiles(t);
+        t -= it.split * by_tiles.d;
+        const uint32_t g = by_group(t), first = g * p.group_m;
+        t -= g * by_group.d;
+        const bool full = first + p.group_m <= tiles_m;
+        it.tn = full ? by_full(t) : by_last(t);
+        it.tm = first + t - it.tn * (full ? by_full.d : by_last.d);
         it.k0 = min(it.split * kper, kchunks);
         it.k1 = min(it.k0 + kper, kchunks);
         return it;
@@ -484,28 +507,37 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kHgThreads, 1)
     if (warp == 0) {
         // ---- loader (both CTAs) -------------------------------------------------------------------
         if (lane == 0) {
-            const uint32_t full_first = in_first_cta(bar_full);
+            const uint32_t full_first = PAIR ? in_first_cta(bar_full) : bar_full;
             uint32_t s = 0, phase = 1u, issued = 0, a_at = smem_base;
             bool ok = true;
             for (uint32_t t = pair; t < tiles && ok; t += pairs) {
                 const Item w = item(t);
-                const int32_t m0 = (int32_t)(p.a_m0 + w.tm * 2 * kHgBM + rank * kHgBM), n0 = (int32_t)(p.b_n0 + w.tn * p.bn + rank * (p.bn / 2));
+                const int32_t m0 = (int32_t)(p.a_m0 + w.tm * kRows + rank * kHgBM), n0 = (int32_t)(p.b_n0 + w.tn * p.bn + rank * (p.bn / kCtas));
                 for (uint32_t kc = w.k0; kc < w.k1; kc++) {
                     if (!mbar_wait(bar_empty + 8 * s, phase, &abort_flag)) { ok = false; break; }
-                    if (rank == 0) mbar_expect_tx(bar_full + 8 * s, 2 * stage_bytes);  // both CTAs' copies land on the first CTA's barrier
+                    if (rank == 0) mbar_expect_tx(bar_full + 8 * s, kCtas * stage_bytes);  // both CTAs' copies land on the first CTA's barrier
                     const uint32_t bar = full_first + 8 * s, b_at = a_at + kHgABytes;
                     const int32_t k0 = (int32_t)(kc * kKStep), kb = (int32_t)p.b_k0 + k0;
-                    if (p.a_mn) {  // two boxes of 64 m × 64 k
-                        tma_load_2d_pair(a_at, &map_a, m0, k0, bar);
-                        tma_load_2d_pair(a_at + 8192, &map_a, m0 + 64, k0, bar);
-                    } else {
-                        tma_load_2d_pair(a_at, &map_a, k0, m0, bar);
-                    }
-                    if (p.b_mn) {
-                        tma_load_2d_pair(b_at, &map_b, n0, kb, bar);
-                        if (p.bn == 256) tma_load_2d_pair(b_at + 8192, &map_b, n0 + 64, kb, bar);
-                    } else {
-                        tma_load_2d_pair(b_at, &map_b, kb, n0, bar);
+                    if constexpr (PAIR) {
+                        if (p.a_mn) {  // two boxes of 64 m × 64 k
+                            tma_load_2d_pair(a_at, &map_a, m0, k0, bar);
+                            tma_load_2d_pair(a_at + 8192, &map_a, m0 + 64, k0, bar);
+                        } else {
+                            tma_load_2d_pair(a_at, &map_a, k0, m0, bar);
+                        }
+                        if (p.b_mn) {
+                            tma_load_2d_pair(b_at, &map_b, n0, kb, bar);
+                            if (p.bn == 256) tma_load_2d_pair(b_at + 8192, &map_b, n0 + 64, kb, bar);
+                        } else {
+                            tma_load_2d_pair(b_at, &map_b, kb, n0, bar);
+                        }
+                    } else {  // A is contiguous along K in the products that run on single CTAs
+                        tma_load_2d(a_at, &map_a, k0, m0, bar);
+                        if (p.b_mn) {
+                            for (uint32_t j = 0; j < p.bn / 64; j++) tma_load_2d(b_at + 8192 * j, &map_b, n0 + (int32_t)(64 * j), kb, bar);
+                        } else {
+                            tma_load_2d(b_at, &map_b, kb, n0, bar);
+                        }
                     }
                     issued++;
                     a_at += stage_bytes;
@@ -520,7 +552,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kHgThreads, 1)
     } else if (warp == 1) {
         // ---- tensor-core issue (first CTA only) -------------------------------------------------------
         if (rank == 0 && lane == 0) {
-            const uint32_t shape = ((p.bn >> 3) << 17) | ((uint32_t)((2 * kHgBM) >> 4) << 24);
+            const uint32_t shape = ((p.bn >> 3) << 17) | ((kRows >> 4) << 24);
             // f32 accumulators of bf16 products, or s32 accumulators of s8 products
             const uint32_t idesc = kI8 ? ((2u << 4) | (1u << 7) | (1u << 10) | shape) : ((1u << 4) | (1u << 7) | (1u << 10) | (p.a_mn << 15) | (p.b_mn << 16) | shape);
             // contiguous along K: rows of 128 bytes, groups of 8 rows 1024 bytes apart, 32 bytes of K per product; contiguous along M / N:
@@ -529,6 +561,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kHgThreads, 1)
             const uint64_t da0 = p.a_mn ? smem_desc_sw128(smem_base, 8192, 1024) : smem_desc_sw128(smem_base, 16, 1024);
             const uint64_t db0 = p.b_mn ? smem_desc_sw128(smem_base + kHgABytes, 8192, 1024) : smem_desc_sw128(smem_base + kHgABytes, 16, 1024);
             const uint32_t a_step = (p.a_mn ? 2048u : 32u) >> 4, b_step = (p.b_mn ? 2048u : 32u) >> 4, s_step = stage_bytes >> 4;
+            auto commit = [](uint32_t bar) {
+                if constexpr (PAIR) tc_commit_pair(bar);
+                else tc_commit(bar);
+            };
             uint32_t s = 0, phase = 0u, n = 0;
             uint64_t da = da0, db = db0;
             bool ok = true;
@@ -546,17 +582,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kHgThreads, 1)
                     for (int k = 0; k < 4; k++) {
                         const uint32_t add = k ? 1u : kc != w.k0;
                         if constexpr (kI8) tc_mma_i8_pair(d_tmem, da + k * a_step, db + k * b_step, idesc, add);
-                        else tc_mma_bf16_pair(d_tmem, da + k * a_step, db + k * b_step, idesc, add);
+                        else if constexpr (PAIR) tc_mma_bf16_pair(d_tmem, da + k * a_step, db + k * b_step, idesc, add);
+                        else tc_mma_bf16(d_tmem, da + k * a_step, db + k * b_step, idesc, add);
                     }
-                    tc_commit_pair(bar_empty + 8 * s);
+                    commit(bar_empty + 8 * s);
                     da += s_step;
                     db += s_step;
                     if (++s == p.stages) { s = 0; phase ^= 1u; da = da0; db = db0; }
                 }
-                if (ok) tc_commit_pair(bar_acc_full + 8 * acc);
+                if (ok) commit(bar_acc_full + 8 * acc);
                 n++;
             }
-            tc_commit_pair(bar_done);
+            commit(bar_done);
         }
     } else {
         // ---- epilogue (both CTAs): thread = row of the output (of the transposed one for kEpiInt8) ---------
@@ -569,7 +606,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kHgThreads, 1)
         if constexpr (EPI == kEpiHidden || EPI == kEpiWeight) alpha = p.alpha ? *p.alpha : 1.f;
         auto row_info = [&](const Item& w) {
             RowInfo r;
-            const uint32_t row = w.tm * 2 * kHgBM + rank * kHgBM + quarter * 32u + (uint32_t)lane;
+            const uint32_t row = w.tm * kRows + rank * kHgBM + quarter * 32u + (uint32_t)lane;
             r.live = row < mm;
             r.caller_row = row;
             r.token = -1;
@@ -601,8 +638,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kHgThreads, 1)
             const Item w = item(t);
             const bool some = w.k0 != w.k1, more_tiles = t + pairs < tiles;
             const RowInfo r = ahead;
-            const Item next = more_tiles ? item(t + pairs) : w;
-            if (more_tiles) ahead = row_info(next);
+            Item next = w;
+            if (more_tiles) {
+                next = item(t + pairs);
+                ahead = row_info(next);
+            }
             const uint32_t acc = n & 1u;
             auto wait = [&] {
                 if (some && ok) {
@@ -616,9 +656,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kHgThreads, 1)
             auto release = [&] {
                 tc_fence_before();
                 __syncwarp();
-                if (ok && lane == 0) mbar_arrive_remote(in_first_cta(bar_acc_empty + 8 * acc));
+                if (ok && lane == 0) {
+                    if constexpr (PAIR) mbar_arrive_remote(in_first_cta(bar_acc_empty + 8 * acc));
+                    else mbar_arrive(bar_acc_empty + 8 * acc);
+                }
             };
-            const uint32_t row0 = w.tm * 2 * kHgBM + rank * kHgBM + quarter * 32u, row = row0 + (uint32_t)lane;
+            const uint32_t row0 = w.tm * kRows + rank * kHgBM + quarter * 32u, row = row0 + (uint32_t)lane;
             const bool live = r.live;
             const uint32_t taddr = tmem + ((quarter * 32u) << 16) + acc * 256 + half * half_cols;
             const uint32_t col0 = w.tn * p.bn + half * half_cols;
@@ -704,7 +747,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kHgThreads, 1)
                             }
                         }
                     } else if (live && col < p.n) {
-                        float* part = p.acc + ((uint64_t)w.split * (tiles_m * 2 * kHgBM) + row) * p.n + col;
+                        float* part = p.acc + ((uint64_t)w.split * p.acc_rows(mm) + row) * p.n + col;
                         if (p.acc_in) {
 #pragma unroll
                             for (int i = 0; i < 32; i += 4)
@@ -782,10 +825,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kHgThreads, 1)
         }
         __syncwarp();
     }
-    cluster_sync_all();  // neither CTA leaves while the other may still reach into its shared or tensor memory
+    if constexpr (PAIR) cluster_sync_all();  // neither CTA leaves while the other may still reach into its shared or tensor memory
     if (warp == 1) {
         tc_fence_after();
-        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+        if constexpr (PAIR) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+        else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
     }
 }
 

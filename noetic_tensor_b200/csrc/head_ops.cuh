@@ -322,15 +322,15 @@ __global__ void __launch_bounds__(256) head_finish_kernel(HeadFinish p) {
 // d_hidden of the scored rows from the ranges of a split sum; nothing to do where K was not split. A block takes 128 columns of a row,
 // 32 threads × 4 columns, with eight groups of threads: group g adds the ranges g, g + 8, … in order, then the groups are added in
 // order. It goes on with the grid's stride (the host does not know the number of rows).
-__global__ void __launch_bounds__(256) head_fold_kernel(const uint32_t* count, const float* alpha, const float4* more, const uint32_t* rows_at, const float* acc, uint32_t chunks, uint32_t d, void* out,
+__global__ void __launch_bounds__(256) head_fold_kernel(const uint32_t* count, const float* alpha, const float4* more, const uint32_t* rows_at, const float* acc, uint32_t chunks, uint32_t side_by_side, uint32_t bn, uint32_t d, void* out,
                                                         uint32_t out_f32, uint32_t add) {
     __shared__ float4 part[8][32];
     next_kernel_may_start();
     after_previous_kernel();
-    const uint32_t n = *count, tiles_m = (n + 255) / 256, nsplit = hidden_split(tiles_m * ((d + 255) / 256), chunks), across = (d + 127) / 128;
+    const uint32_t n = *count, tiles_m = (n + 255) / 256, nsplit = hidden_split(tiles_m * ((d + bn - 1) / bn), chunks, side_by_side), across = (d + 127) / 128;
     if (nsplit == 1) return;
     const float common = *alpha;
-    const uint64_t range = (uint64_t)tiles_m * 256 * d;
+    const uint64_t range = (uint64_t)HeadGemm::acc_rows(n) * d;
     const uint32_t t = threadIdx.x & 31, g = threadIdx.x >> 5;
     for (uint32_t b = blockIdx.x; b < n * across; b += gridDim.x) {
         const uint32_t i = b / across, c = ((b - i * across) * 32 + t) * 4;

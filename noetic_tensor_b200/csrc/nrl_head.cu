@@ -12,11 +12,15 @@ extern std::atomic<uint64_t> nrl_g_launches;
 // One launch in stream order, counted. The products start early (launch_next), and small grids; a larger grid of small blocks that
 // waits beside a product's last tiles delayed the pass by 7 us (the statistics of 2048 rows at V = 32 000, d = 1024: 121 against 114 us).
 template <typename... Params, typename... Args>
-static int launch(void (*kernel)(Params...), dim3 grid, unsigned block, size_t smem, cudaStream_t stream, const Args&... args) {
+static int launch_as(unsigned cluster, void (*kernel)(Params...), dim3 grid, unsigned block, size_t smem, cudaStream_t stream, const Args&... args) {
     nrl_g_launches.fetch_add(1, std::memory_order_relaxed);
-    const cudaError_t e = launch_next(smem != 0 || grid.x <= 2 * kPairs, kernel, grid, dim3(block), smem, stream, args...);
+    const cudaError_t e = launch_next(smem != 0 || grid.x <= 2 * kPairs, cluster, kernel, grid, dim3(block), smem, stream, args...);
     if (e != cudaSuccess) (void)cudaGetLastError();
     return e == cudaSuccess ? NRL_OK : (int)e;
+}
+template <typename... Params, typename... Args>
+static int launch(void (*kernel)(Params...), dim3 grid, unsigned block, size_t smem, cudaStream_t stream, const Args&... args) {
+    return launch_as(1, kernel, grid, block, smem, stream, args...);
 }
 
 static int need_cc10() {
@@ -27,9 +31,10 @@ static int need_cc10() {
     return cc_major == 10 ? NRL_OK : NRL_E_UNSUPPORTED;  // tcgen05 / tensor memory
 }
 
-template <int EPI, int MASK = kMaskNone>
-static int launch_gemm(const CUtensorMap& ma, const CUtensorMap& mb, const CUtensorMap& mo, HeadGemm p, uint64_t tiles, cudaStream_t st) {
-    p.stages = smem_tiles(EPI) / (kHgABytes + (p.bn / 2) * 128);
+template <int EPI, int MASK, bool PAIR>
+static int launch_tiles(const CUtensorMap& ma, const CUtensorMap& mb, const CUtensorMap& mo, HeadGemm p, uint64_t tiles, cudaStream_t st) {
+    constexpr unsigned ctas = PAIR ? 2 : 1;
+    p.stages = smem_tiles(EPI) / (kHgABytes + (p.bn / ctas) * 128);
     if (p.stages > kHgMaxStages) p.stages = kHgMaxStages;
     if (tiles > 0x7fffffffull) return NRL_E_UNSUPPORTED;
     int dev = 0;
@@ -37,17 +42,22 @@ static int launch_gemm(const CUtensorMap& ma, const CUtensorMap& mb, const CUten
     if (e != cudaSuccess) return (int)e;
     static std::atomic<uint64_t> ready{0};  // devices on which this kernel may have its shared memory
     if (dev >= 64 || !(ready.load(std::memory_order_acquire) >> dev & 1u)) {
-        e = cudaFuncSetAttribute(head_gemm_kernel<EPI, MASK>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem_bytes(EPI));
+        e = cudaFuncSetAttribute(head_gemm_kernel<EPI, MASK, PAIR>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem_bytes(EPI));
         if (e != cudaSuccess) return (int)e;
         if (dev < 64) ready.fetch_or(1ull << dev, std::memory_order_release);
     }
-    const unsigned grid = 2u * (unsigned)(tiles < kPairs ? (tiles ? tiles : 1) : kPairs);
-    return launch(head_gemm_kernel<EPI, MASK>, dim3(grid), kHgThreads, smem_bytes(EPI), st, ma, mb, mo, p);
+    const uint64_t most = 2 * kPairs / ctas;
+    return launch_as(ctas, head_gemm_kernel<EPI, MASK, PAIR>, dim3(ctas * (unsigned)(tiles < most ? (tiles ? tiles : 1) : most)), kHgThreads, smem_bytes(EPI), st, ma, mb, mo, p);
+}
+// on pairs of CTAs or, `single`, on CTAs by themselves
+template <int EPI, int MASK = kMaskNone>
+static int launch_gemm(bool single, const CUtensorMap& ma, const CUtensorMap& mb, const CUtensorMap& mo, const HeadGemm& p, uint64_t tiles, cudaStream_t st) {
+    return single ? launch_tiles<EPI, MASK, false>(ma, mb, mo, p, tiles, st) : launch_tiles<EPI, MASK, true>(ma, mb, mo, p, tiles, st);
 }
 template <int EPI>
-static int launch_masked(const CUtensorMap& ma, const CUtensorMap& mb, const CUtensorMap& mo, const HeadGemm& p, uint32_t allow_bits, uint64_t tiles, cudaStream_t st) {
-    if (!p.allow) return launch_gemm<EPI, kMaskNone>(ma, mb, mo, p, tiles, st);
-    return allow_bits ? launch_gemm<EPI, kMaskBits>(ma, mb, mo, p, tiles, st) : launch_gemm<EPI, kMaskBytes>(ma, mb, mo, p, tiles, st);
+static int launch_masked(bool single, const CUtensorMap& ma, const CUtensorMap& mb, const CUtensorMap& mo, const HeadGemm& p, uint32_t allow_bits, uint64_t tiles, cudaStream_t st) {
+    if (!p.allow) return launch_gemm<EPI, kMaskNone>(single, ma, mb, mo, p, tiles, st);
+    return allow_bits ? launch_gemm<EPI, kMaskBits>(single, ma, mb, mo, p, tiles, st) : launch_gemm<EPI, kMaskBytes>(single, ma, mb, mo, p, tiles, st);
 }
 
 static inline uint64_t up(uint64_t x, uint64_t to) { return (x + to - 1) / to * to; }
@@ -55,7 +65,10 @@ static inline uint32_t tiles256(uint64_t x) { return (uint32_t)((x + 255) / 256)
 
 // Columns per tile of a bf16 product over `rows` × `cols`: half the width where that puts twice the pairs to work (140 rows at
 // V = 1120, d = 1808: five pairs took 20 us).
-static uint32_t tile_width(uint64_t rows, uint64_t cols) { return (uint64_t)tiles256(rows) * tiles256(cols) <= kPairs / 2 ? 128u : 256u; }
+// With `single` CTAs there are twice as many workers.
+static uint32_t tile_width(uint64_t rows, uint64_t cols, bool single) { return (uint64_t)tiles256(rows) * tiles256(cols) <= (single ? kPairs : kPairs / 2) ? 128u : 256u; }
+// At most one CTA's rows: single CTAs instead of pairs.
+static bool runs_single(uint64_t rows) { return rows <= kHgBM; }
 static uint64_t tiles_of(uint64_t rows, uint64_t cols, uint32_t bn) { return (uint64_t)tiles256(rows) * ((cols + bn - 1) / bn); }
 
 static int launch_rows(HeadRows& hr, cudaStream_t st) {
@@ -80,13 +93,14 @@ static void set_mask(HeadGemm& g, nrl_devptr mask, uint64_t stride) {
 // (rows, V, d) only.
 struct BwdPlan {
     uint64_t rows_pad;
-    uint32_t vc, pieces, chunks, grad_bn;
-    bool may_split;
+    uint32_t vc, pieces, chunks, grad_bn, hidden_bn, side_by_side;
+    bool may_split, single;
     uint64_t off_coef, off_more, off_rows, off_x, off_dz, off_acc, bytes;
 };
 static BwdPlan bwd_plan(uint64_t rows, uint32_t V, uint32_t d) {
     BwdPlan b;
     b.rows_pad = up(rows, 256);
+    b.single = runs_single(rows);
     // dz of a piece is at most 512 MB, but not narrower than 4096 columns: dx's f32 sums are read and written once per piece
     uint64_t vc = (512ull << 20) / (b.rows_pad * 2) / 256 * 256;
     if (vc < 4096) vc = 4096;
@@ -95,12 +109,15 @@ static BwdPlan bwd_plan(uint64_t rows, uint32_t V, uint32_t d) {
     b.vc = (uint32_t)up((V + b.pieces - 1) / b.pieces, 256);  // pieces of about the same width
     b.pieces = (V + b.vc - 1) / b.vc;
     b.chunks = b.vc / 64;
-    b.grad_bn = tile_width(rows, b.vc);
+    b.grad_bn = tile_width(rows, b.vc, b.single);
     // any number of scored rows up to `rows` may turn up: whether one of them would have dx's K split
+    b.side_by_side = b.single ? 2 * kPairs : kPairs;
+    // half-width tiles of dx where even its ranges leave pairs idle
+    b.hidden_bn = (uint64_t)tiles256(rows) * tiles256(d) * (b.chunks >= 48 ? b.chunks / 24 : 1) < b.side_by_side ? 128u : 256u;
     uint64_t split_units = 0;
-    const uint32_t tn = tiles256(d), tm = tiles256(rows);
-    for (uint32_t m = 1; m <= tm && m * tn <= kPairs; m++) {
-        const uint32_t s = hidden_split(m * tn, b.chunks);
+    const uint32_t tn = (d + b.hidden_bn - 1) / b.hidden_bn, tm = tiles256(rows);
+    for (uint32_t m = 1; m <= tm && m * tn <= b.side_by_side; m++) {
+        const uint32_t s = hidden_split(m * tn, b.chunks, b.side_by_side);
         if (s > 1 && (uint64_t)m * s > split_units) split_units = (uint64_t)m * s;
     }
     b.may_split = split_units > 0;
@@ -194,7 +211,7 @@ extern "C" int nrl_readout_bwd(const nrl_readout_bwd_args* a, nrl_stream stream)
     memset(&dw_out, 0, sizeof dw_out);
     if ((rc = encode_2d(&x_k, false, x, a->d, b.rows_pad, hr.x_pitch, 64, 128)) || (rc = encode_2d(&x_mn, false, x, a->d, b.rows_pad, hr.x_pitch, 64, 64)) ||
         (rc = encode_2d(&dz_k, false, dz, b.vc, b.rows_pad, b.vc, 64, 128)) || (rc = encode_2d(&dz_mn, false, dz, b.vc, b.rows_pad, b.vc, 64, 64)) ||
-        (rc = encode_2d(&dz_out, false, dz, b.vc, b.rows_pad, b.vc, 64, 32)) || (rc = vd ? encode_2d(&w_rows_k, false, a->weights, w_in, w_rows, w_in, 64, b.grad_bn / 2) : encode_2d(&w_k, false, a->weights, w_in, w_rows, w_in, 64, 128)) ||
+        (rc = encode_2d(&dz_out, false, dz, b.vc, b.rows_pad, b.vc, 64, 32)) || (rc = vd ? encode_2d(&w_rows_k, false, a->weights, w_in, w_rows, w_in, 64, b.single ? b.grad_bn : b.grad_bn / 2) : encode_2d(&w_k, false, a->weights, w_in, w_rows, w_in, 64, b.single ? b.hidden_bn : b.hidden_bn / 2)) ||
         (rc = encode_2d(&w_mn, false, a->weights, w_in, w_rows, w_in, 64, 64)))
         return rc;
     if (a->d_weights) {
@@ -214,7 +231,7 @@ extern "C" int nrl_readout_bwd(const nrl_readout_bwd_args* a, nrl_stream stream)
             p.b_n0 = v0;
             p.v0 = v0;
             p.bn = b.grad_bn;
-            rc = launch_masked<kEpiGrad>(x_k, vd ? w_rows_k : w_mn, dz_out, p, allow_bits, tiles_of(a->rows, cols, p.bn), st);
+            rc = launch_masked<kEpiGrad>(b.single, x_k, vd ? w_rows_k : w_mn, dz_out, p, allow_bits, tiles_of(a->rows, cols, p.bn), st);
             if (rc) return rc;
         }
         if (a->d_hidden) {  // dx += dz · Wᵀ
@@ -225,6 +242,7 @@ extern "C" int nrl_readout_bwd(const nrl_readout_bwd_args* a, nrl_stream stream)
             p.k = cols;
             p.b_mn = vd ? 1u : 0u;
             p.b_k0 = v0;
+            p.bn = b.hidden_bn;
             p.split = b.may_split ? b.chunks : 0u;
             p.acc = (float*)(ws + b.off_acc);
             p.acc_in = piece > 0 ? 1u : 0u;
@@ -234,11 +252,11 @@ extern "C" int nrl_readout_bwd(const nrl_readout_bwd_args* a, nrl_stream stream)
             p.out_f32 = hr.d_hidden_f32;
             p.out_add = (a->flags & NRL_READOUT_BWD_ADD_D_HIDDEN) ? 1u : 0u;
             p.wide = (a->d_hidden % 32 == 0 && (p.out_f32 || a->d % 16 == 0)) ? 1u : 0u;
-            rc = launch_gemm<kEpiHidden>(dz_k, vd ? w_mn : w_k, dz_out, p, b.may_split ? kPairs : (uint64_t)tiles256(a->rows) * tiles256(a->d), st);
+            rc = launch_gemm<kEpiHidden>(b.single, dz_k, vd ? w_mn : w_k, dz_out, p, b.may_split ? 2 * kPairs : tiles_of(a->rows, a->d, p.bn), st);
             if (rc) return rc;
             if (b.may_split && piece + 1 == b.pieces) {
                 const uint64_t most = (a->rows < (uint64_t)kPairs * 256 ? a->rows : (uint64_t)kPairs * 256) * ((a->d + 127) / 128);  // more rows are never split
-                rc = launch(head_fold_kernel, dim3((unsigned)(most < 8 * 148 ? most : 8 * 148)), 256, 0, st, hr.count, hr.alpha, hr.more, hr.rows_at, p.acc, b.chunks, a->d, (void*)a->d_hidden, p.out_f32, p.out_add);
+                rc = launch(head_fold_kernel, dim3((unsigned)(most < 8 * 148 ? most : 8 * 148)), 256, 0, st, hr.count, hr.alpha, hr.more, hr.rows_at, p.acc, b.chunks, b.side_by_side, b.hidden_bn, a->d, (void*)a->d_hidden, p.out_f32, p.out_add);
                 if (rc) return rc;
             }
         }
@@ -257,8 +275,8 @@ extern "C" int nrl_readout_bwd(const nrl_readout_bwd_args* a, nrl_stream stream)
             p.out_add = (a->flags & NRL_READOUT_BWD_ADD_D_WEIGHTS) ? 1u : 0u;
             p.wide = (a->d_weights % 32 == 0 && (p.out_f32 || p.out_pitch % 16 == 0)) ? 1u : 0u;
             p.staged = p.out_add ? 0u : 1u;  // sums into what is there go through registers
-            p.bn = tile_width(p.m, p.n);
-            rc = launch_gemm<kEpiWeight>(vd ? dz_mn : x_mn, vd ? x_mn : dz_mn, dw_out, p, tiles_of(p.m, p.n, p.bn), st);
+            p.bn = tile_width(p.m, p.n, false);
+            rc = launch_tiles<kEpiWeight, kMaskNone, true>(vd ? dz_mn : x_mn, vd ? x_mn : dz_mn, dw_out, p, tiles_of(p.m, p.n, p.bn), st);
             if (rc) return rc;
         }
     }
@@ -271,6 +289,7 @@ constexpr uint64_t kScoredChunk = 16384;  // rows per launch: what bounds the pa
 
 struct ScoredPlan {
     bool gather;  // the scored rows are brought together first
+    bool single;
     uint32_t bn, parts_pitch;
     uint64_t rows_pad, off_rows, off_x, off_parts, bytes;
 };
@@ -278,7 +297,8 @@ static ScoredPlan scored_plan(uint64_t rows, uint32_t V, uint32_t d, bool scored
     ScoredPlan s;
     s.gather = scored && rows > 256;  // up to one row block nothing is saved by leaving rows out
     s.rows_pad = up(rows, 256);
-    s.bn = tile_width(rows, V);
+    s.single = runs_single(rows);
+    s.bn = tile_width(rows, V, s.single);
     s.parts_pitch = 2 * ((V + s.bn - 1) / s.bn);
     uint64_t at = 256;
     s.off_rows = at; at += s.gather ? up(rows * 4, 256) : 0;
@@ -333,7 +353,7 @@ extern "C" int nrl_readout_scored_fwd(const nrl_readout_scored_args* a, nrl_stre
     CUtensorMap mx, mw;
     rc = encode_2d(&mx, false, s.gather ? ws + s.off_x : a->hidden, a->d, s.gather ? s.rows_pad : a->rows, s.gather ? up(a->d, 64) : a->d, 64, 128);
     if (rc) return rc;
-    rc = vd ? encode_2d(&mw, false, a->weights, a->d, a->V, a->d, 64, s.bn / 2) : encode_2d(&mw, false, a->weights, a->V, a->d, a->V, 64, 64);
+    rc = vd ? encode_2d(&mw, false, a->weights, a->d, a->V, a->d, 64, s.single ? s.bn : s.bn / 2) : encode_2d(&mw, false, a->weights, a->V, a->d, a->V, 64, 64);
     if (rc) return rc;
     for (uint64_t r0 = 0; r0 < a->rows; r0 += kScoredChunk) {
         const uint64_t n = a->rows - r0 < kScoredChunk ? a->rows - r0 : kScoredChunk;
@@ -358,7 +378,7 @@ extern "C" int nrl_readout_scored_fwd(const nrl_readout_scored_args* a, nrl_stre
         p.zero = (uint32_t*)(ws + 8);
         p.parts = (float4*)(ws + s.off_parts);
         p.parts_pitch = s.parts_pitch;
-        rc = launch_masked<kEpiStats>(mx, mw, mx, p, a->flags & NRL_READOUT_MASK_BITS, tiles_of(n, a->V, s.bn), st);
+        rc = launch_masked<kEpiStats>(s.single, mx, mw, mx, p, a->flags & NRL_READOUT_MASK_BITS, tiles_of(n, a->V, s.bn), st);
         if (rc) return rc;
         HeadFinish f;
         memset(&f, 0, sizeof f);
@@ -478,5 +498,5 @@ extern "C" int nrl_i8_matmul(const nrl_i8_matmul_args* a, nrl_stream stream) {
     if (rc) return rc;
     rc = encode_2d(&mx, true, a->x, a->k, a->rows, a->x_pitch, 128, p.bn / 2);
     if (rc) return rc;
-    return launch_gemm<kEpiInt8>(mw, mx, mw, p, (uint64_t)tiles256(a->n) * ((a->rows + p.bn - 1) / p.bn), (cudaStream_t)stream);
+    return launch_tiles<kEpiInt8, kMaskNone, true>(mw, mx, mw, p, (uint64_t)tiles256(a->n) * ((a->rows + p.bn - 1) / p.bn), (cudaStream_t)stream);
 }

@@ -112,17 +112,26 @@ __device__ __forceinline__ float round_through_bf16(float x) {
 __device__ __forceinline__ void after_previous_kernel() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void next_kernel_may_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 template <typename... Params, typename... Args>
-inline cudaError_t launch_next(bool early, void (*kernel)(Params...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, const Args&... args) {
-    cudaLaunchAttribute at;
-    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at.val.programmaticStreamSerializationAllowed = 1;
+inline cudaError_t launch_next(bool early, unsigned cluster, void (*kernel)(Params...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, const Args&... args) {
+    cudaLaunchAttribute at[2];
+    unsigned n = 0;
+    if (early) {
+        at[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        at[n++].val.programmaticStreamSerializationAllowed = 1;
+    }
+    if (cluster > 1) {
+        at[n].id = cudaLaunchAttributeClusterDimension;
+        at[n].val.clusterDim.x = cluster;
+        at[n].val.clusterDim.y = at[n].val.clusterDim.z = 1;
+        n++;
+    }
     cudaLaunchConfig_t c = {};
     c.gridDim = grid;
     c.blockDim = block;
     c.dynamicSmemBytes = smem;
     c.stream = stream;
-    c.attrs = &at;
-    c.numAttrs = early ? 1 : 0;
+    c.attrs = at;
+    c.numAttrs = n;
     return cudaLaunchKernelEx(&c, kernel, static_cast<Params>(args)...);
 }
 
