@@ -709,6 +709,35 @@ __global__ void __launch_bounds__(kHgThreads, 1)
                 }
                 wait();
                 const bool there = some && ok;
+                if (EPI == kEpiWeight && p.staged && !p.out_f32) {
+                    // 64 columns at a time: one wait for tensor memory and one store of whole lines per 64
+#pragma unroll 1
+                    for (int c = 0; c < chunks; c += 2) {
+                        float z[64];
+                        if (there) {
+                            tc_ld32(taddr + 32 * c, reinterpret_cast<uint32_t*>(z));
+                            tc_ld32(taddr + 32 * c + 32, reinterpret_cast<uint32_t*>(z + 32));
+                            tc_wait_ld();
+                            pin32(z);
+                            pin32(z + 32);
+                            if (c + 2 >= chunks) release();
+                        } else {
+#pragma unroll
+                            for (int i = 0; i < 64; i++) z[i] = ok ? 0.f : __int_as_float(0x7fc00000);
+                        }
+                        scale32(z, scale);
+                        scale32(z + 32, scale);
+                        const uint32_t tile = stage_out + (sent & 1u) * kHgStageOut, col = col0 + 32 * c;
+                        stage_free<2>(lane);
+#pragma unroll
+                        for (int j = 0; j < 8; j++)
+                            sts_piece(tile, lane, j, pack_bf16(z[8 * j], z[8 * j + 1]), pack_bf16(z[8 * j + 2], z[8 * j + 3]), pack_bf16(z[8 * j + 4], z[8 * j + 5]), pack_bf16(z[8 * j + 6], z[8 * j + 7]));
+                        if (row0 < mm && col < p.n) {
+                            stage_send(&map_out, tile, lane, (int32_t)(p.out_col0 + col), (int32_t)(p.out_row0 + row0));
+                            sent++;
+                        }
+                    }
+                } else {
 #pragma unroll 1
                 for (int c = 0; c < chunks; c++) {
                     float z[32];
@@ -725,26 +754,12 @@ __global__ void __launch_bounds__(kHgThreads, 1)
                     if (EPI == kEpiWeight && p.staged) {
                         scale32(z, scale);
                         const uint32_t tile = stage_out + (sent & 1u) * kHgStageOut;
-                        const bool inside = row0 < mm;
-                        if (p.out_f32) {
-                            stage_free<2>(lane);
+                        stage_free<2>(lane);
 #pragma unroll
-                            for (int j = 0; j < 8; j++)
-                                sts_piece(tile, lane, j, __float_as_uint(z[4 * j]), __float_as_uint(z[4 * j + 1]), __float_as_uint(z[4 * j + 2]), __float_as_uint(z[4 * j + 3]));
-                            if (inside && col < p.n) {
-                                stage_send(&map_out, tile, lane, (int32_t)(p.out_col0 + col), (int32_t)(p.out_row0 + row0));
-                                sent++;
-                            }
-                        } else {
-                            if ((c & 1) == 0) stage_free<2>(lane);
-#pragma unroll
-                            for (int j = 0; j < 4; j++)
-                                sts_piece(tile, lane, 4 * (c & 1) + j, pack_bf16(z[8 * j], z[8 * j + 1]), pack_bf16(z[8 * j + 2], z[8 * j + 3]), pack_bf16(z[8 * j + 4], z[8 * j + 5]),
-                                          pack_bf16(z[8 * j + 6], z[8 * j + 7]));
-                            if ((c & 1) && inside && col - 32 < p.n) {
-                                stage_send(&map_out, tile, lane, (int32_t)(p.out_col0 + col - 32), (int32_t)(p.out_row0 + row0));
-                                sent++;
-                            }
+                        for (int j = 0; j < 8; j++) sts_piece(tile, lane, j, __float_as_uint(z[4 * j]), __float_as_uint(z[4 * j + 1]), __float_as_uint(z[4 * j + 2]), __float_as_uint(z[4 * j + 3]));
+                        if (row0 < mm && col < p.n) {
+                            stage_send(&map_out, tile, lane, (int32_t)(p.out_col0 + col), (int32_t)(p.out_row0 + row0));
+                            sent++;
                         }
                     } else if (live && col < p.n) {
                         float* part = p.acc + ((uint64_t)w.split * p.acc_rows(mm) + row) * p.n + col;
@@ -763,6 +778,7 @@ __global__ void __launch_bounds__(kHgThreads, 1)
                             store_row32(p.out, orow * p.out_pitch + p.out_col0 + col, p.out_f32, p.out_add, p.wide, p.n - col, z);
                         }
                     }
+                }
                 }
             } else {
                 // thread = vocabulary entry, registers = tokens: a warp's store covers 32 consecutive entries of a row
