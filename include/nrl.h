@@ -615,9 +615,10 @@ int nrl_ce_mean(uint64_t s, uint64_t n, nrl_devptr logp, nrl_devptr keep, nrl_de
  * divided by the call's largest |upstream| before it is rounded to bf16 (2^-8 relative per entry at most, as the
  * operands of every bf16 product) and the factor is put back in f32; all sums are f32 in a fixed order, so
  * results are bitwise reproducible. A row whose upstreams are all 0 is not scored: nothing of it is
- * read, it costs no products and its d_hidden is 0 (left as it is with ADD). A row the forward refused
- * (NaN statistics) with a non-zero upstream makes its d_hidden and d_weights NaN. An upstream whose token
- * lies outside [0, V) has no one-hot term.
+ * read, it costs no products and its d_hidden is 0 (left as it is with ADD). A row with NaN statistics and a
+ * non-zero upstream makes its d_hidden and d_weights NaN, except that a row whose mask allows nothing
+ * contributes 0, as its gradient is 0 at every excluded token. An upstream whose token lies outside
+ * [0, V) has no one-hot term.
  *
  * `hidden` may be an 8-bit checkpoint of the hidden states (NRL_READOUT_BWD_HIDDEN_I8): integers and one
  * scale per row as nrl_i8_quantize_rows writes them. The logits are then those of values·scale (products of

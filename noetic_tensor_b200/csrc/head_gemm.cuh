@@ -308,13 +308,16 @@ __device__ __forceinline__ void epi_grad(const HeadGemm& p, bool live, uint32_t 
 // 32 columns of one row folded into (m, S, W): m in accumulator units, W in units of log2.
 template <int MASK>
 __device__ __forceinline__ void epi_stats(const HeadGemm& p, uint32_t v, float y[32], float c2, int32_t token, const typename MaskAhead<MASK>::Chunk& mask, float& m, float& S, float& W, float& ytok) {
-    if (!mask.any()) return;
+    const uint32_t tk = (uint32_t)(token - (int32_t)v);
+    if (!mask.any()) {
+        if (tk < 32u) ytok = -FLT_MAX;  // the token itself is excluded
+        return;
+    }
     if (!mask.all()) {
 #pragma unroll
         for (int i = 0; i < 32; i++)
             if (!mask.column(i)) y[i] = -FLT_MAX;
     }
-    const uint32_t tk = (uint32_t)(token - (int32_t)v);
     if (tk < 32u) {
 #pragma unroll
         for (int i = 0; i < 32; i++)
@@ -668,7 +671,10 @@ __global__ void __launch_bounds__(kHgThreads, 1)
             if constexpr (EPI == kEpiGrad || EPI == kEpiStats) {
                 const float ys = p.zscale * kLog2e * r.xs.x;
                 int32_t token = r.token;
-                if (EPI == kEpiStats && live && p.tokens) token = __ldg(p.tokens + r.caller_row);
+                if (EPI == kEpiStats && live && p.tokens) {
+                    token = __ldg(p.tokens + r.caller_row);
+                    if ((uint32_t)token >= p.vocab) token = -1;  // no such column, not even past the vocabulary's end in its last tile
+                }
                 float m = -FLT_MAX, S = 0.f, W = 0.f, ytok = __int_as_float(0x7fc00000);
                 wait();
                 mask.settle(p, p.v0 + col0, lane);

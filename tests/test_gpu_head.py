@@ -205,3 +205,431 @@ def test_int8_extreme_integers_and_nonfinite_scales():
     w = ops.Int8Rows(torch.full((40, k), -127, dtype=torch.int8, device=dev()), torch.ones(40, device=dev()), k)
     got = ops.int8_matmul(x, w)
     assert (got[0] == float(-127 * 127 * k)).all() and torch.isnan(got[1]).all() and torch.isinf(got[2]).all()
+
+
+# ---- the forward over the scored rows ---------------------------------------------------------------
+
+
+def forward_truth(x, w_vd, tok, allow, tau):
+    z = x.double() @ w_vd.double().t() / tau
+    if allow is not None:
+        z = torch.where(allow.expand(z.shape) != 0, z, torch.full_like(z, -math.inf))
+    lse = torch.logsumexp(z, 1)
+    lp = z - lse[:, None]
+    H = -torch.where(lp > -math.inf, lp.exp() * lp, torch.zeros_like(lp)).sum(1)
+    # |δz| of an f32 sum of d products, twice (the logit and ln Z), against the largest Σ|x·w| of the row
+    e = 4.0 * (x.shape[1] + 16) * U32 * (x.double().abs() @ w_vd.double().abs().t()).amax(1) / tau
+    return lp[torch.arange(len(tok), device=x.device), tok.long()], H, lse, e
+
+
+@pytest.mark.parametrize("rows,d,V", [(1, 8, 8), (16, 64, 1000), (129, 256, 1024), (300, 136, 4104), (700, 1032, 2056), (17000, 64, 264), (40, 2048, 32000)])
+@pytest.mark.parametrize("layout", ["dV", "Vd"])
+@pytest.mark.parametrize("form", [None, "bytes", "row", "bits"])
+def test_scored_forward_against_64_bits(rows, d, V, layout, form):
+    from noetic_tensor_b200 import ops
+
+    x, w, tok, g = make(rows, d, V, rows + V, layout)
+    w_vd, vd = (w, True) if layout == "Vd" else (w.t(), False)
+    allow = None if form is None else (torch.rand(1 if form == "row" else rows, V, generator=g, device=dev()) < 0.5).to(torch.uint8)
+    if allow is not None:
+        allow[:, 1] = 1
+    kw = {} if form is None else dict(allow_bits=bits_of(allow)) if form == "bits" else dict(allow=allow)
+    scored = (torch.rand(rows, generator=g, device=dev()) < 0.7).float()
+    scored[0] = 1.0
+    x[scored == 0] = math.nan  # what an unscored position holds is not looked at
+    tau = 1.0 if form is None else 0.7
+    o = ops.readout_scored_forward(x, w, tokens=tok, scored=scored, want_entropy=True, weights_are_vd=vd, temperature=tau, ce_seeds=1, **kw)
+    on = scored != 0
+    lp, H, lse, e = forward_truth(x[on], w_vd, tok[on], allow if allow is None or allow.shape[0] == 1 else allow[on], tau)
+    assert (o.status == 0).all()
+    got = o.logp[on].double()
+    assert torch.equal(got == -math.inf, lp == -math.inf)
+    fin = lp > -math.inf
+    assert ((got - lp).abs()[fin] <= (e + 8 * U32 * lp.abs())[fin]).all()
+    assert ((o.entropy[on].double() - H).abs() <= e * (1 + lse.abs()) + 64 * U32 * (1 + H)).all()
+    assert ((o.rowstats[on, 0].double() + o.rowstats[on, 1].double() - lse).abs() <= e + 8 * U32 * (1 + lse.abs())).all()
+    assert (o.logp[~on] == 0).all() and (o.entropy[~on] == 0).all() and (o.rowstats[~on] == 0).all()
+    # the mean cross-entropy of the same call, and the call of its own
+    nll = -o.logp[on].double()
+    want = nll.sum() / max(1, int(on.sum()))
+    assert (torch.isinf(want) and torch.isinf(o.ce_loss[0])) or abs(o.ce_loss[0].item() - want.item()) <= 4 * U32 * abs(want.item())
+    value, grad = ops.ce_mean(o.logp, 1, scored)
+    assert torch.equal(value, o.ce_loss) and torch.equal(grad, o.ce_g_logp)
+    assert (grad[~on] == 0).all() and ((grad[on].double() + 1.0 / int(on.sum())).abs() <= 2 * U32 / int(on.sum())).all()
+    again = ops.readout_scored_forward(x, w, tokens=tok, scored=scored, want_entropy=True, weights_are_vd=vd, temperature=tau, ce_seeds=1, **kw)
+    assert torch.equal(o._buf[: 4 * rows].view(torch.int32), again._buf[: 4 * rows].view(torch.int32)) and torch.equal(o.logp, again.logp) and torch.equal(o.entropy, again.entropy)
+
+
+def test_scored_forward_agrees_with_the_sampling_forward():
+    from noetic_tensor_b200 import ops
+
+    x, w, tok, _ = make(300, 512, 8200, 4)
+    a, b = ops.readout_scored_forward(x, w, tokens=tok, want_entropy=True), ops.readout_forward(x, w, tokens=tok)
+    e = forward_truth(x, w.t(), tok, None, 1.0)[3]
+    assert ((a.logp.double() - b.logp.double()).abs() <= 2 * e + 16 * U32 * b.logp.double().abs()).all()
+    ga = ops.readout_backward(x, w, a, tokens=tok, g_logp=torch.ones(300, device=dev()))
+    gb = ops.readout_backward(x, w, b, tokens=tok, g_logp=torch.ones(300, device=dev()))
+    for p, q in zip(ga, gb):
+        assert ((p.double() - q.double()).norm() <= 1e-2 * q.double().norm()).item()
+
+
+def test_tokens_and_rows_that_have_no_log_prob():
+    from noetic_tensor_b200 import ops
+
+    rows, d, V = 140, 64, 1000
+    x, w, tok, g = make(rows, d, V, 9)
+    allow = torch.ones(rows, V, dtype=torch.uint8, device=dev())
+    allow[3] = 0  # nothing allowed
+    allow[4, tok[4].long()] = 0  # the token itself is excluded
+    allow[5] = 0
+    allow[5, 999 if tok[5] < 500 else 0] = 1  # the token's whole neighbourhood is excluded
+    tok[6], tok[7], tok[8] = V, -1, V + 20
+    x[9, 3] = math.nan
+    o = ops.readout_scored_forward(x, w, tokens=tok, want_entropy=True, allow=allow)
+    st = o.status.cpu().numpy()
+    assert st[3] == 1 and st[9] == 2 and (np.delete(st, [3, 9]) == 0).all()
+    lp = o.logp
+    assert torch.isnan(lp[[3, 6, 7, 8, 9]]).all() and (lp[[4, 5]] == -math.inf).all() and torch.isfinite(lp[10:]).all() and torch.isfinite(o.entropy[[4, 5, 6, 7, 8]]).all()
+    up = torch.zeros(rows, device=dev())
+    up[10:] = 1.0
+    dh, dw = ops.readout_backward(x, w, o, tokens=tok, g_logp=up, allow=allow)  # the refused rows are not scored: nothing of them arrives
+    assert torch.isfinite(dh).all() and torch.isfinite(dw).all() and (dh[:10] == 0).all()
+    up[3] = 1.0  # nothing allowed: the gradient is 0 at every excluded token, here at all of them
+    dh3, dw3 = ops.readout_backward(x, w, o, tokens=tok, g_logp=up, allow=allow)
+    # d_weights sums the same terms, moved by one place: two f32 sums of up to 131 terms x·∂/∂z, |∂/∂z| ≤ 1, differ by at most
+    # 2·131·2^-24·Σ|x| and may be rounded to neighbouring bf16 numbers
+    spread = 2 * 131 * U32 * x[10:].double().abs().sum(0)[:, None]
+    assert torch.equal(dh3, dh) and ((dw3.double() - dw.double()).abs() <= 2 * U16 * dw.double().abs() + spread).all()
+    up[9] = 1.0  # a NaN among the hidden states
+    dh, dw = ops.readout_backward(x, w, o, tokens=tok, g_logp=up, allow=allow)
+    assert torch.isnan(dh[9]).all() and torch.isnan(dw).any() and torch.isfinite(dh[10:]).all()
+
+
+def test_nothing_scored():
+    from noetic_tensor_b200 import loss, ops, rl
+
+    for rows in (5, 300):
+        x, w, tok, _ = make(rows, 64, 264, 2)
+        zero = torch.zeros(rows, device=dev())
+        o = ops.readout_scored_forward(x, w, tokens=tok, scored=zero, ce_seeds=1)
+        assert (o.logp == 0).all() and (o.ce_loss == 0).all()
+        dh, dw = ops.readout_backward(x, w, o, tokens=tok, g_logp=zero)
+        assert (dh == 0).all() and (dw == 0).all()
+        l = loss.masked_cross_entropy(rl.Head(x.reshape(1, 1, rows, 64), w), tok.reshape(1, 1, rows), zero.reshape(1, 1, rows))
+        dh, dw = l.backward()
+        assert (l.value == 0).all() and (dh == 0).all() and (dw == 0).all()
+
+
+def test_masked_positions_may_hold_anything():
+    from noetic_tensor_b200 import loss, rl
+
+    for checkpoint in (False, True):
+        x, w, tok, g = make(300, 136, 1000, 11)
+        mask = (torch.rand(300, generator=g, device=dev()) < 0.5).float()
+        y = x.clone()
+        y[mask == 0] = math.nan
+        y[(mask == 0).nonzero()[0]] = math.inf
+        shape = (2, 3, 50)
+        a = loss.masked_cross_entropy(rl.Head(x.reshape(*shape, 136), w, checkpoint=checkpoint), tok.reshape(shape), mask.reshape(shape))
+        b = loss.masked_cross_entropy(rl.Head(y.reshape(*shape, 136), w, checkpoint=checkpoint), tok.reshape(shape), mask.reshape(shape))
+        assert torch.equal(a.value, b.value)
+        for p, q in zip(a.backward(), b.backward()):
+            assert torch.equal(p, q)
+
+
+# ---- more of the backward ----------------------------------------------------------------------------
+
+
+def test_several_pieces_of_the_vocabulary():
+    """Enough rows that dz of the whole vocabulary would be over 512 MB: the sums of d_hidden are carried from piece to piece."""
+    from noetic_tensor_b200 import ops
+
+    rows, d, V = 16500, 64, 20008
+    x, w, tok, g = make(rows, d, V, 5)
+    up = torch.randn(rows, generator=g, device=dev())
+    f = ops.readout_scored_forward(x, w, tokens=tok)
+    dh, dw = ops.readout_backward(x, w, f, tokens=tok, g_logp=up, grad_dtype=torch.float32)
+    pick = torch.arange(0, rows, 97, device=dev())
+    th, _, eh, _ = truth(x[pick], w.t(), tok[pick], up[pick], None, None, 1.0)
+    held(dh[pick], th, eh, "d_hidden")
+    tw, ew = torch.zeros(V, d, dtype=torch.float64, device=dev()), torch.zeros(V, d, dtype=torch.float64, device=dev())
+    for r in range(0, rows, 4125):
+        p = slice(r, r + 4125)
+        _, a, _, b = truth(x[p], w.t(), tok[p], up[p], None, None, 1.0)
+        tw += a
+        ew += b
+    held(dw.t(), tw, ew + rows * U32 * ew / U16, "d_weights")
+
+
+@pytest.mark.parametrize("rows,d,V", [(40, 136, 1000), (300, 264, 4104), (64, 512, 40008)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_adding_to_gradients(rows, d, V, dtype):
+    from noetic_tensor_b200 import ops
+
+    x, w, tok, g = make(rows, d, V, rows + d)
+    up = torch.randn(rows, generator=g, device=dev())
+    up[::5] = 0
+    f = ops.readout_scored_forward(x, w, tokens=tok)
+    dh, dw = ops.readout_backward(x, w, f, tokens=tok, g_logp=up, grad_dtype=torch.float32)
+    h0, w0 = torch.randn(rows, d, generator=g, device=dev()).to(dtype), torch.randn(d, V, generator=g, device=dev()).to(dtype)
+    ha, wa = h0.clone(), w0.clone()
+    ops.readout_backward(x, w, f, tokens=tok, g_logp=up, add_hidden=ha, add_weights=wa)
+    u = U16 if dtype == torch.bfloat16 else 2 * U32
+    for got, old, new in ((ha, h0, dh), (wa, w0, dw)):
+        want = old.double() + new.double()
+        assert ((got.double() - want).abs() <= u * want.abs() + 4 * U32 * (old.double().abs() + new.double().abs())).all()
+    assert torch.equal(ha[::5], h0[::5])  # rows without an upstream stay as they are
+    only_h = ops.readout_backward(x, w, f, tokens=tok, g_logp=up, want_weights=False)
+    only_w = ops.readout_backward(x, w, f, tokens=tok, g_logp=up, want_hidden=False)
+    both = ops.readout_backward(x, w, f, tokens=tok, g_logp=up)
+    assert only_h[1] is None and only_w[0] is None and torch.equal(only_h[0], both[0]) and torch.equal(only_w[1], both[1])
+
+
+def test_gradients_against_differences():
+    """Directional derivatives of the loss in 64 bits by central differences against the kernels' gradients."""
+    from noetic_tensor_b200 import ops
+
+    rows, d, V = 60, 72, 264
+    x, w, tok, g = make(rows, d, V, 21)
+    up, ent = torch.randn(rows, generator=g, device=dev()), 0.3 * torch.randn(rows, generator=g, device=dev())
+    f = ops.readout_scored_forward(x, w, tokens=tok, want_entropy=True)
+    dh, dw = ops.readout_backward(x, w, f, tokens=tok, g_logp=up, g_ent=ent, grad_dtype=torch.float32)
+    _, _, eh, ew = truth(x, w.t(), tok, up, ent, None, 1.0)
+
+    def value(x, w):
+        lp = torch.log_softmax(x @ w, 1)
+        return (up.double() * lp[torch.arange(rows), tok.long()]).sum() + (ent.double() * -(lp.exp() * lp).sum(1)).sum()
+
+    X, W, h = x.double(), w.double(), 1e-4
+    for _ in range(4):
+        vx, vw = torch.randn(rows, d, generator=g, device=dev()).double(), torch.randn(d, V, generator=g, device=dev()).double()
+        diff = (value(X + h * vx, W + h * vw) - value(X - h * vx, W - h * vw)) / (2 * h)
+        got = (dh.double() * vx).sum() + (dw.double() * vw).sum()
+        bound = (eh * vx.abs()).sum() + (ew.t() * vw.abs()).sum()
+        assert (got - diff).abs() <= bound + 1e-5 * diff.abs()
+
+
+# ---- rl.Head through the losses --------------------------------------------------------------------------
+
+
+def head_case(S, B, T, d, V, seed, layout="dV"):
+    x, w, tok, g = make(S * B * T, d, V, seed, layout)
+    mask = (torch.rand(S, B, T, generator=g, device=dev()) < 0.8).float()
+    return x.reshape(S, B, T, d), w, tok.reshape(S, B, T), mask, g
+
+
+@pytest.mark.parametrize("S,B,T,d,V", [(1, 1, 1, 8, 8), (2, 3, 50, 136, 1000), (3, 2, 61, 512, 4104)])
+@pytest.mark.parametrize("what", ["pg", "ppo", "k1", "k3", "token_log_probs", "entropy", "nll", "ce", "masked_ce", "ignore"])
+def test_losses_on_a_head_against_the_losses_on_its_logits(S, B, T, d, V, what):
+    """The same functions on f32 logits of the same operands: values within the f32 sums' spread of the logits, gradients
+    within what the bf16 rounding of ∂/∂z allows (2-norms: at most u of the majorant, which these draws keep below 4 u of the gradient)."""
+    from noetic_tensor_b200 import loss, rl
+
+    x, w, tok, mask, g = head_case(S, B, T, d, V, S + T + V)
+    logits = (x.double() @ w.double()).float()
+    adv, old = torch.randn(S, B, T, generator=g, device=dev()), -2 * torch.rand(S, B, T, generator=g, device=dev()) - 3
+
+    def run(z):
+        if what == "pg":
+            return rl.policy_gradient_loss(z, tok, adv, mask)
+        if what == "ppo":
+            return rl.clipped_policy_loss(z, tok, old, adv, mask)
+        if what == "k1":
+            return rl.kl_estimate(z, tok, old, rl.K1, mask=mask, reduction=rl.SEQUENCE_MEAN)
+        if what == "k3":
+            return rl.kl_estimate(z, tok, old, rl.K3, delta_clamp=20.0, mask=mask, reduction=rl.PER_SEQUENCE)
+        if what == "token_log_probs":
+            return rl.token_log_probs(z, tok, mask)
+        if what == "entropy":
+            return rl.categorical_entropy(z, mask, rl.SUM)
+        if what == "nll":
+            return loss.nll(z, tok)
+        if what == "ce":
+            return loss.cross_entropy(z, tok)
+        if what == "masked_ce":
+            return loss.masked_cross_entropy(z, tok, mask)
+        return loss.cross_entropy_with(z, tok, mask, loss.CeOptions(ignore_index=int(tok[0, 0, 0])))
+
+    a, b = run(rl.Head(x, w, grad_dtype=torch.float32)), run(logits)
+    assert a.value.shape == b.value.shape
+    assert ((a.value - b.value).abs() <= 1e-4 * (1 + b.value.abs())).all()
+    for up in (None, torch.randn(b.value.shape, generator=g, device=dev())):
+        dh, dw = a.backward(up)
+        dz = b.backward(up).reshape(-1, V).double()
+        th, tw = dz @ w.double().t(), x.reshape(-1, d).double().t() @ dz
+        assert dh.shape == x.shape and dw.shape == w.shape
+        for got, want in ((dh.reshape(-1, d), th), (dw, tw)):
+            assert (got.double() - want).norm() <= 4 * U16 * want.norm() + 1e-12
+
+
+def test_a_run_of_them_together():
+    """Decode with the 8-bit head, score the drawn tokens and train on them from an 8-bit checkpoint, on another stream."""
+    from noetic_tensor_b200 import ops, rl
+
+    S, B, T, d, V = 2, 3, 17, 264, 4104
+    x, w, _, mask, g = head_case(S, B, T, d, V, 3)
+    adv = torch.randn(S, B, T, generator=g, device=dev())
+    w8 = rl.Int8Weight.of(w)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        logits = rl.head_logits(x, w8)
+        tokens, lp8 = rl.sample_categorical(logits, 1.0, uniforms=torch.rand(S, B, T, generator=g, device=dev()))
+        l = rl.policy_gradient_loss(rl.Head(x, w, checkpoint=True), tokens, adv, mask)
+        dh, dw = l.backward()
+    s.synchronize()
+    exact = x.double() @ w.double()
+    # the 8-bit logits: half a step of each row's and each entry's integers
+    step_x, step_w = x.double().abs().amax(-1, keepdim=True) / 254, (w.double().abs().amax(0) / 254)
+    tol = step_x * w.double().abs().sum(0) + step_w * x.double().abs().sum(-1, keepdim=True) + d * step_x * step_w
+    assert ((logits.double() - exact).abs() <= tol * (1 + 1e-5) + 1e-4).all()
+    lp = torch.log_softmax(exact, -1).gather(-1, tokens.long()[..., None])[..., 0]
+    want = (-(lp * adv) * mask.double()).sum((1, 2)) / mask.double().sum((1, 2))
+    assert ((l.value.double() - want).abs() <= 1e-4 * (1 + want.abs())).all()
+    q = ops.quantize_rows(x.reshape(-1, d))
+    xq = q.values[:, :d].double() * q.scales.double()[:, None]
+    up = (-adv * mask / mask.sum((1, 2), keepdim=True)).reshape(-1)
+    lse = torch.logsumexp(exact, -1).reshape(-1)
+    th, tw, eh, ew = truth(xq, w.t(), tokens.reshape(-1), up, None, None, 1.0, stats=(lse, torch.zeros_like(lse)))
+    held(dh.reshape(-1, d), th, eh, "d_hidden")
+    held(dw.t(), tw, ew, "d_weights")
+
+
+def test_the_checkpoint_does_not_keep_the_hidden_states():
+    import gc
+    import weakref
+
+    from noetic_tensor_b200 import loss, rl
+
+    x, w, tok, mask, _ = head_case(1, 2, 100, 136, 1000, 8)
+    held_by = weakref.ref(x)
+    l = loss.masked_cross_entropy(rl.Head(x, w, checkpoint=True), tok, mask)
+    del x
+    gc.collect()
+    assert held_by() is None
+    dh, dw = l.backward()
+    assert dh.shape == (1, 2, 100, 136) and torch.isfinite(dh).all()
+
+
+def test_captured_and_replayed():
+    """Two graphs of whole steps with new inputs copied in, replayed in turn, give the eager results bit for bit."""
+    from noetic_tensor_b200 import loss, rl
+
+    cases = [head_case(1, 2, 100, 136, 1000, s) for s in (1, 2, 3)]
+    w = cases[0][1]
+    eager = []
+    for x, _, tok, mask, _ in cases:
+        l = loss.masked_cross_entropy(rl.Head(x, w), tok, mask)
+        eager.append((l.value.clone(),) + tuple(t.clone() for t in l.backward()))
+    x, tok, mask = (t.clone() for t in (cases[0][0], cases[0][2], cases[0][3]))
+    w8 = rl.Int8Weight.of(w)
+    graphs = []
+    for _ in range(2):
+        s = torch.cuda.Stream()
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            loss.masked_cross_entropy(rl.Head(x, w), tok, mask).backward()
+            rl.head_logits(x, w8)
+        torch.cuda.current_stream().wait_stream(s)
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            l = loss.masked_cross_entropy(rl.Head(x, w), tok, mask)
+            out = (l.value,) + tuple(l.backward())
+            z = rl.head_logits(x, w8)
+        graphs.append((g, out, z))
+    for k in (1, 0, 2, 1):
+        for dst, src in ((x, cases[k][0]), (tok, cases[k][2]), (mask, cases[k][3])):
+            dst.copy_(src)
+        for g, _, _ in graphs:
+            g.replay()
+        torch.cuda.synchronize()
+        want_z = rl.head_logits(cases[k][0], w8)
+        for _, out, z in graphs:
+            assert all(torch.equal(p, q) for p, q in zip(out, eager[k])) and torch.equal(z, want_z)
+
+
+def test_two_streams_at_once():
+    from noetic_tensor_b200 import loss, rl
+
+    cases = [head_case(1, 2, 200, 264, 4104, s) for s in (1, 2)]
+    want = []
+    for x, w, tok, mask, _ in cases:
+        l = loss.masked_cross_entropy(rl.Head(x, w), tok, mask)
+        want.append((l.value,) + l.backward())
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in cases]
+    got = [[], []]
+    for _ in range(5):
+        for k, (x, w, tok, mask, _) in enumerate(cases):
+            with torch.cuda.stream(streams[k]):
+                l = loss.masked_cross_entropy(rl.Head(x, w), tok, mask)
+                got[k].append((l.value,) + l.backward())
+    torch.cuda.synchronize()
+    for k in range(2):
+        for r in got[k]:
+            assert all(torch.equal(p, q) for p, q in zip(r, want[k]))
+
+
+# ---- masks and tensors at odd addresses, refusals ----------------------------------------------------------
+
+
+def test_masks_at_odd_addresses():
+    from noetic_tensor_b200 import ops
+
+    rows, d, V = 140, 64, 1000
+    x, w, tok, g = make(rows, d, V, 17)
+    allow = (torch.rand(rows, V, generator=g, device=dev()) < 0.5).to(torch.uint8)
+    allow[:, 0] = 1
+    big = torch.zeros(rows * V + 8, dtype=torch.uint8, device=dev())
+    up = torch.randn(rows, generator=g, device=dev())
+    base = None
+    for off in (0, 1, 4):
+        m = big[off : off + rows * V].view(rows, V)
+        m.copy_(allow * 3)  # any byte that is not 0 allows
+        f = ops.readout_scored_forward(x, w, tokens=tok, allow=m)
+        r = (f.logp,) + ops.readout_backward(x, w, f, tokens=tok, g_logp=up, allow=m)
+        if base is None:
+            base = r
+        assert all(torch.equal(p, q) for p, q in zip(r, base))
+    f = ops.readout_scored_forward(x, w, tokens=tok, allow=allow.bool())
+    assert torch.equal(f.logp, base[0])
+
+
+def test_refusals():
+    from noetic_tensor_b200 import capi, loss, ops, rl
+
+    x, w, tok, mask, _ = head_case(1, 2, 10, 64, 512, 1)
+    f = ops.readout_scored_forward(x, w, tokens=tok)
+    up = torch.ones(20, device=dev())
+    bad = [
+        (ValueError, lambda: rl.Head(x, w, temperature=0.0)),
+        (ValueError, lambda: rl.Head(x, w, vocab_mask=torch.zeros(1, 512, device=dev()))),
+        (ValueError, lambda: ops.readout_scored_forward(x.float(), w, tokens=tok)),
+        (ValueError, lambda: ops.readout_scored_forward(x, w.t().contiguous(), tokens=tok)),
+        (ValueError, lambda: ops.readout_scored_forward(x, w.t(), tokens=tok, weights_are_vd=True)),
+        (ValueError, lambda: ops.readout_scored_forward(x, w, tokens=tok[:, :1])),
+        (ValueError, lambda: ops.readout_scored_forward(x.cpu(), w, tokens=tok)),
+        (capi.NrlError, lambda: ops.readout_scored_forward(x[..., :60].contiguous(), w[:60], tokens=tok)),
+        (capi.NrlError, lambda: ops.readout_scored_forward(x, w, tokens=tok, temperature=-1.0)),
+        (capi.NrlError, lambda: ops.readout_scored_forward(x, w, tokens=tok, ce_seeds=3)),
+        (capi.NrlError, lambda: ops.readout_scored_forward(x, w, ce_seeds=1)),
+        (capi.NrlError, lambda: ops.readout_scored_forward(x, w, tokens=tok, workspace=torch.empty(256, dtype=torch.uint8, device=dev()))),
+        (ValueError, lambda: ops.readout_backward(x, w, f, tokens=tok)),
+        (ValueError, lambda: ops.readout_backward(x, w, f, g_logp=up)),
+        (ValueError, lambda: ops.readout_backward(x, w, f, g_ent=up)),
+        (ValueError, lambda: ops.readout_backward(x, w, f, tokens=tok, g_logp=up[:5])),
+        (TypeError, lambda: ops.readout_backward(x, w, f, tokens=tok, g_logp=up, grad_dtype=torch.float16)),
+        (ValueError, lambda: ops.readout_backward(x, w, f, tokens=tok, g_logp=up, add_weights=w.t())),
+        (ValueError, lambda: ops.readout_backward(ops.quantize_rows(x[:, :1].contiguous()), w, f, tokens=tok, g_logp=up, hidden_shape=x.shape)),
+        (capi.NrlError, lambda: ops.readout_backward(x, w, f, tokens=tok, g_logp=up, workspace=torch.empty(256, dtype=torch.uint8, device=dev()))),
+        (ValueError, lambda: rl.categorical_kl(rl.Head(x, w), torch.zeros(1, 2, 10, 512, device=dev()))),
+        (ValueError, lambda: loss.cross_entropy_with(rl.Head(x, w), tok, mask, loss.CeOptions(smoothing=0.1))),
+        (ValueError, lambda: ops.Int8Rows(torch.zeros(3, 20, dtype=torch.int8, device=dev()), torch.zeros(3, device=dev()), 20)),
+        (ValueError, lambda: ops.int8_matmul(ops.quantize_rows(x[0, 0]), ops.quantize_rows(x[0, 0, :, :32].contiguous()))),
+        (TypeError, lambda: ops.quantize_rows(x.half())),
+        (ValueError, lambda: ops.quantize_rows(x[..., ::2])),
+    ]
+    for error, call in bad:
+        with pytest.raises(error):
+            call()
+    assert torch.isfinite(ops.readout_backward(x, w, f, tokens=tok, g_logp=up)[1]).all()  # a refused call leaves nothing behind
