@@ -544,11 +544,14 @@ inline Tensor token_log_probs(const Tensor& logits, const IntTensor& tokens) {
 // [.., V] logits in between (src/nn/decoder.rs:270-279 followed by src/nn/rl.rs:134-141, 405-414):
 // `hidden` BF16 [.., d], `weight` BF16 [d, V] (the Linear's [in, out] layout, src/nn/linear.rs:1-3),
 // tokens [..]. Returns the log-probabilities [..] and, if asked, the per-position entropies.
-// Untracked: the backward of the fused form (d hidden, d weight) is not built; needs a
-// compute-capability-10 device (tcgen05). `round_bf16`: statistics of the logits rounded to bf16.
+// With `hidden` or `weight` tracked the results are too: their backward computes the logits again in
+// pieces of the vocabulary (nrl_readout_bwd) and gives F32 gradients of both; with `checkpoint` the hidden
+// states live until then as 8-bit integers with a scale per position. Needs a compute-capability-10
+// device (tcgen05). `round_bf16` (untracked only): statistics of the logits rounded to bf16.
 namespace detail {
 // the allow-mask of a fused head call: U8 [.., V] or [1, V], or I32 words of one bit per token [.., W] or [1, W]
-inline void head_mask(nrl_readout_args& a, const Tensor* vocab_mask, uint64_t rows, uint64_t V) {
+template <class Args>
+inline void head_mask(Args& a, const Tensor* vocab_mask, uint64_t rows, uint64_t V) {
     if (!vocab_mask) return;
     if (vocab_mask->dtype() == DType::I32) {
         const uint64_t words = vocab_mask->shape().back(), n = numel(vocab_mask->shape());
@@ -564,12 +567,159 @@ inline void head_mask(nrl_readout_args& a, const Tensor* vocab_mask, uint64_t ro
     a.allow_mask = vocab_mask->dev();
     a.allow_row_stride = n == V ? 0 : V;
 }
+
+// rows as 8-bit integers with a scale each (nrl_i8_quantize_rows / nrl_i8_quantize_columns)
+struct Int8Rows {
+    Tensor values, scales;  // U8 storage of int8 [rows, pitch], F32 [rows]
+    uint64_t rows = 0, d = 0, pitch = 0;
+    static Int8Rows empty(uint64_t rows, uint64_t d, Device dev) {
+        Int8Rows q;
+        q.rows = rows;
+        q.d = d;
+        q.pitch = (d + 15) / 16 * 16;
+        q.values = Tensor::empty(Shape{(size_t)rows, (size_t)q.pitch}, DType::U8, dev);
+        q.scales = Tensor::empty(Shape{(size_t)rows}, DType::F32, dev);
+        return q;
+    }
+    static Int8Rows of(const Tensor& x) {  // [.., d], a row per leading position
+        const uint64_t d = x.shape().back();
+        Int8Rows q = empty(numel(x.shape()) / d, d, x.device());
+        nrl(nrl_i8_quantize_rows(dt(x), q.rows, (uint32_t)d, x.dev(), q.values.dev(), q.pitch, q.scales.dev(), stream()), "i8_quantize_rows");
+        return q;
+    }
+};
+
+// what a tracked head forward leaves for its backward
+struct HeadSaved {
+    Tensor hidden, weight, tokens, rowstats, entropy, mask;
+    Int8Rows checkpoint;  // in place of `hidden` when its d > 0
+    Shape hidden_shape;
+    std::shared_ptr<Node> hidden_leaf, weight_leaf;
+    bool has_mask = false;
+    uint64_t rows = 0, V = 0, d = 0;
+    float temperature = 1.f;
+    Device device{0};
+
+    void backward(const Tensor* g_logp, const Tensor* g_ent, std::map<uint64_t, Tensor>& grads) const {
+        nrl_readout_bwd_args b;
+        std::memset(&b, 0, sizeof b);
+        b.struct_size = sizeof b;
+        b.V = (uint32_t)V; b.d = (uint32_t)d; b.rows = rows; b.temperature = temperature;
+        b.flags = NRL_READOUT_BWD_D_HIDDEN_F32 | NRL_READOUT_BWD_D_WEIGHTS_F32;
+        if (checkpoint.d) {
+            b.flags |= NRL_READOUT_BWD_HIDDEN_I8;
+            b.hidden = checkpoint.values.dev(); b.hidden_scales = checkpoint.scales.dev(); b.hidden_pitch = checkpoint.pitch;
+        } else {
+            b.hidden = hidden.dev();
+        }
+        b.weights = weight.dev(); b.tokens = tokens.dev(); b.rowstats = rowstats.dev();
+        b.entropy = g_ent ? entropy.dev() : 0;
+        b.g_logp = g_logp ? g_logp->dev() : 0;
+        b.g_ent = g_ent ? g_ent->dev() : 0;
+        if (has_mask) head_mask(b, &mask, rows, V);
+        auto slot = [&](const std::shared_ptr<Node>& leaf, const Shape& shape, uint32_t add) -> nrl_devptr {
+            if (!leaf) return 0;
+            auto it = grads.find(leaf->id);
+            if (it == grads.end()) it = grads.emplace(leaf->id, Tensor::empty(shape, DType::F32, device)).first;
+            else b.flags |= add;  // the tape's `new + old`
+            return it->second.dev();
+        };
+        b.d_hidden = slot(hidden_leaf, hidden_shape, NRL_READOUT_BWD_ADD_D_HIDDEN);
+        b.d_weights = slot(weight_leaf, weight.shape(), NRL_READOUT_BWD_ADD_D_WEIGHTS);
+        const uint64_t need = nrl_readout_bwd_workspace_bytes(rows, (uint32_t)V, (uint32_t)d);
+        Tensor ws = Tensor::empty(Shape{(size_t)need}, DType::U8, device);
+        b.workspace = ws.dev(); b.workspace_bytes = need;
+        nrl(nrl_readout_bwd(&b, stream()), "readout_bwd");
+        cu(cudaStreamSynchronize(stream()), "sync");  // the workspace goes out of scope here
+    }
+};
+// the tracked form of head_token_log_probs below: its arguments are checked, `tok` is on the device
+inline Tensor head_tracked(const Tensor& hidden, const Tensor& weight, const Tensor& tok, Tensor* entropy, const Tensor* vocab_mask, double temperature, bool checkpoint) {
+    auto s = std::make_shared<HeadSaved>();
+    const Shape lead(hidden.shape().begin(), hidden.shape().end() - 1);
+    s->d = weight.shape()[0]; s->V = weight.shape()[1]; s->rows = numel(lead);
+    s->hidden_shape = hidden.shape();
+    s->hidden_leaf = hidden.node_;
+    s->weight_leaf = weight.node_;
+    s->weight = weight.detach();
+    s->tokens = tok;
+    s->temperature = (float)temperature;
+    s->device = hidden.device();
+    if (vocab_mask) { s->has_mask = true; s->mask = *vocab_mask; }
+    Tensor logp = Tensor::empty(lead, DType::F32, hidden.device());
+    s->rowstats = Tensor::empty(Shape{(size_t)s->rows, 4}, DType::F32, hidden.device());
+    const uint64_t need = nrl_readout_scored_workspace_bytes(s->rows, (uint32_t)s->V, (uint32_t)s->d, 0);
+    Tensor ws = Tensor::empty(Shape{(size_t)need}, DType::U8, hidden.device());
+    nrl_readout_scored_args a;
+    std::memset(&a, 0, sizeof a);
+    a.struct_size = sizeof a;
+    a.V = (uint32_t)s->V; a.d = (uint32_t)s->d; a.rows = s->rows; a.temperature = (float)temperature;
+    head_mask(a, vocab_mask, s->rows, s->V);
+    a.hidden = hidden.dev(); a.weights = weight.dev(); a.tokens = tok.dev();
+    a.logp = logp.dev(); a.rowstats = s->rowstats.dev();
+    if (entropy) {
+        *entropy = Tensor::empty(lead, DType::F32, hidden.device());
+        s->entropy = *entropy;
+        a.entropy = entropy->dev();
+    }
+    a.workspace = ws.dev(); a.workspace_bytes = need;
+    nrl(nrl_readout_scored_fwd(&a, stream()), "readout_scored_fwd");
+    if (checkpoint) s->checkpoint = Int8Rows::of(hidden);
+    else s->hidden = hidden.detach();
+    cu(cudaStreamSynchronize(stream()), "sync");  // the workspace goes out of scope here
+    auto node = [&](Tensor& value, bool is_entropy) {
+        value.node_ = std::make_shared<Node>();
+        value.node_->id = Tensor::next_id();
+        if (hidden.node_) value.node_->parents.push_back(hidden.node_);
+        if (weight.node_) value.node_->parents.push_back(weight.node_);
+        value.node_->backward = [s, is_entropy](const Tensor& g, std::map<uint64_t, Tensor>& grads) {
+            const Tensor flat = g.reshape(Shape{numel(g.shape())});
+            s->backward(is_entropy ? nullptr : &flat, is_entropy ? &flat : nullptr, grads);
+        };
+    };
+    node(logp, false);
+    if (entropy) node(*entropy, true);
+    return logp;
+}
 }  // namespace detail
+
+// A readout weight laid out once as 8-bit integers [V, pitch] with a scale per vocabulary entry.
+struct Int8Weight {
+    detail::Int8Rows rows;
+    static Int8Weight of(const Tensor& weight) {  // BF16 [d, V], the Linear's [in, out] layout
+        if (weight.dtype() != DType::BF16 || weight.rank() != 2) throw std::runtime_error("Int8Weight: BF16 weight [d, V]");
+        Int8Weight w;
+        w.rows = detail::Int8Rows::empty(weight.shape()[1], weight.shape()[0], weight.device());
+        nrl(nrl_i8_quantize_columns((uint32_t)w.rows.d, (uint32_t)w.rows.rows, weight.dev(), w.rows.values.dev(), w.rows.pitch, w.rows.scales.dev(), detail::stream()), "i8_quantize_columns");
+        return w;
+    }
+};
+// `Decoder::head(x)` (src/nn/decoder.rs:270-279) in 8-bit integers: `hidden` [.., d] (BF16 or F32) is quantised with a scale per
+// position; logits [.., V] in F32 (or BF16), ready for sample_categorical and the other functions here. Untracked.
+inline Tensor head_logits(const Tensor& hidden, const Int8Weight& weight, DType out = DType::F32) {
+    if (out != DType::F32 && out != DType::BF16) throw std::runtime_error("head_logits: F32 or BF16 logits");
+    if (hidden.rank() < 1 || hidden.shape().back() != weight.rows.d) throw std::runtime_error("head_logits: hidden [.., d] of the weight's d");
+    Shape shape(hidden.shape().begin(), hidden.shape().end() - 1);
+    const uint64_t n = numel(shape);
+    shape.push_back((size_t)weight.rows.rows);
+    Tensor z = Tensor::empty(shape, out, hidden.device());
+    const uint64_t need = nrl_i8_linear_workspace_bytes(n, (uint32_t)weight.rows.d);
+    Tensor ws = Tensor::empty(Shape{(size_t)need}, DType::U8, hidden.device());
+    nrl_i8_matmul_args a;
+    std::memset(&a, 0, sizeof a);
+    a.struct_size = sizeof a;
+    a.dtype = out == DType::F32 ? NRL_F32 : NRL_BF16;
+    a.rows = n; a.n = (uint32_t)weight.rows.rows; a.k = (uint32_t)weight.rows.d;
+    a.x = hidden.dev(); a.w = weight.rows.values.dev(); a.w_pitch = weight.rows.pitch; a.w_scales = weight.rows.scales.dev(); a.out = z.dev();
+    nrl(nrl_i8_linear(detail::dt(hidden), &a, ws.dev(), need, detail::stream()), "i8_linear");
+    cu(cudaStreamSynchronize(detail::stream()), "sync");  // the workspace goes out of scope here
+    return z;
+}
 
 // `vocab_mask` / `temperature`: the logits are the tempered ones (src/nn/rl.rs:475-486), what a rollout drawn by
 // head_sample_categorical under the same mask and temperature is scored with.
 inline Tensor head_token_log_probs(const Tensor& hidden, const Tensor& weight, const IntTensor& tokens, Tensor* entropy = nullptr, bool round_bf16 = false, const Tensor* vocab_mask = nullptr,
-                                   double temperature = 1.0) {
+                                   double temperature = 1.0, bool checkpoint = false) {
     if (!(temperature > 0.0 && std::isfinite(temperature))) throw std::runtime_error("tempered_logits: temperature must be > 0");
     if (hidden.dtype() != DType::BF16 || weight.dtype() != DType::BF16) throw std::runtime_error("head_token_log_probs: BF16 hidden states and weight");
     if (hidden.rank() < 1 || weight.rank() != 2 || weight.shape()[0] != hidden.shape().back()) throw std::runtime_error("head_token_log_probs: hidden [.., d], weight [d, V]");
@@ -581,6 +731,10 @@ inline Tensor head_token_log_probs(const Tensor& hidden, const Tensor& weight, c
         if (t < 0 || (uint64_t)t >= V) throw std::runtime_error("gather index out of range");
     Tensor tok = Tensor::empty(Shape{(size_t)rows}, DType::I32, hidden.device());
     cu(cudaMemcpy(tok.ptr(), h.data(), h.size() * 4, cudaMemcpyHostToDevice), "upload tokens");
+    if (hidden.tracked() || weight.tracked()) {
+        if (round_bf16) throw std::runtime_error("head_token_log_probs: round_bf16 has no backward");
+        return detail::head_tracked(hidden, weight, tok, entropy, vocab_mask, temperature, checkpoint);
+    }
     Tensor logp = Tensor::empty(lead, DType::F32, hidden.device());
     Tensor status = Tensor::empty(Shape{(size_t)rows}, DType::U8, hidden.device());
     const uint64_t need = nrl_readout_workspace_bytes(rows, (uint32_t)V, (uint32_t)d, 0u);
