@@ -591,6 +591,8 @@ typedef struct nrl_readout_scored_args {
     uint64_t seeds;          /* > 0: also nrl_ce_mean of the log-probs as [seeds, rows / seeds] with keep = scored and upstreams of 1, or 0 */
     nrl_devptr ce_loss;      /* out f32 [seeds], or 0 */
     nrl_devptr ce_g_logp;    /* out f32 [rows], or 0 */
+    nrl_devptr ce_weights;   /* f32 [rows], or 0: the loss is then policy_gradient_loss (src/nn/rl.rs:228-235) with these signed weights and
+                                the token mean, sum over scored of -logp * weight / max(sum(scored), 1), and its gradient */
 } nrl_readout_scored_args;
 uint64_t nrl_readout_scored_workspace_bytes(uint64_t rows, uint32_t V, uint32_t d, uint32_t has_scored);
 int nrl_readout_scored_fwd(const nrl_readout_scored_args* args, nrl_stream stream);

@@ -116,7 +116,7 @@ class ReadoutScoredArgs(C.Structure):
         ("struct_size", u32), ("flags", u32), ("V", u32), ("d", u32), ("rows", u64),
         ("hidden", ptr), ("weights", ptr), ("tokens", ptr), ("scored", ptr), ("logp", ptr), ("entropy", ptr), ("rowstats", ptr), ("status", ptr),
         ("allow_mask", ptr), ("allow_row_stride", u64), ("workspace", ptr), ("workspace_bytes", u64), ("temperature", f32), ("reserved", u32),
-        ("seeds", u64), ("ce_loss", ptr), ("ce_g_logp", ptr),
+        ("seeds", u64), ("ce_loss", ptr), ("ce_g_logp", ptr), ("ce_weights", ptr),
     ]
 
 

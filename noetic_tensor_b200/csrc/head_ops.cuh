@@ -165,11 +165,13 @@ __global__ void __launch_bounds__(kRowsThreads) head_rows_kernel(HeadRows p) {
 }
 
 // Per seed: out = Σ keep·(−logp) / max(Σ keep, 1) and its gradient g_logp = upstream·(−keep / max(Σ keep, 1)), by one block: thread t
-// takes the positions t, t + blockDim, …, f64 sums, a butterfly, the warps in order. Positions with keep = 0 are not looked at.
+// takes the positions t, t + blockDim, …, f64 sums, a butterfly, the warps in order. Positions with keep = 0 are not looked at. With
+// `weights` it is the policy-gradient loss: the kept positions' −logp·weight over the same count, keep itself not a factor.
 struct CeMean {
     uint64_t seeds, n;
     const float* logp;
     const float* keep;
+    const float* weights;
     const float* upstream;
     float* out;
     float* g_logp;
@@ -182,7 +184,7 @@ __device__ __forceinline__ void ce_mean_seed(const CeMean& p, uint64_t seed, dou
     for (uint64_t i = threadIdx.x; i < p.n; i += blockDim.x) {
         const float k = p.keep ? p.keep[base + i] : 1.f;
         c += (double)k;
-        if (p.out && k != 0.f) v -= (double)(__ldcg(p.logp + base + i) * k);
+        if (p.out && k != 0.f) v -= (double)(__ldcg(p.logp + base + i) * (p.weights ? p.weights[base + i] : k));
     }
 #pragma unroll
     for (int k = 16; k >= 1; k >>= 1) {
@@ -198,7 +200,10 @@ __device__ __forceinline__ void ce_mean_seed(const CeMean& p, uint64_t seed, dou
     if (p.out && threadIdx.x == 0) p.out[seed] = (float)(v / count);
     if (!p.g_logp) return;
     const float g = (float)((p.upstream ? (double)p.upstream[seed] : 1.0) / count);
-    for (uint64_t i = threadIdx.x; i < p.n; i += blockDim.x) p.g_logp[base + i] = p.keep ? -(p.keep[base + i] * g) : -g;
+    for (uint64_t i = threadIdx.x; i < p.n; i += blockDim.x) {
+        const float k = p.keep ? p.keep[base + i] : 1.f;
+        p.g_logp[base + i] = p.weights ? (k != 0.f ? -(p.weights[base + i] * g) : 0.f) : -(k * g);
+    }
 }
 __global__ void __launch_bounds__(512) ce_mean_kernel(CeMean p) {
     __shared__ double sh[16][2];

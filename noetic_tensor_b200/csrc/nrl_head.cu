@@ -321,7 +321,7 @@ extern "C" int nrl_readout_scored_fwd(const nrl_readout_scored_args* a, nrl_stre
     if (a->V > 0x40000000u || a->d > 0x40000000u || a->rows > 0x40000000ull) return NRL_E_UNSUPPORTED;  // TMA coordinates are 32-bit
     if (((a->tokens | a->scored | a->logp | a->entropy) & 3u) || (a->rowstats & 15u) || (a->workspace & 255u)) return NRL_E_BAD_ARG;
     if (a->logp && !a->tokens) return NRL_E_BAD_ARG;
-    if (a->seeds ? (!a->logp || a->rows % a->seeds != 0 || (!a->ce_loss && !a->ce_g_logp) || ((a->ce_loss | a->ce_g_logp) & 3u)) : (a->ce_loss || a->ce_g_logp)) return NRL_E_BAD_ARG;
+    if (a->seeds ? (!a->logp || a->rows % a->seeds != 0 || (!a->ce_loss && !a->ce_g_logp) || ((a->ce_loss | a->ce_g_logp | a->ce_weights) & 3u)) : (a->ce_loss || a->ce_g_logp || a->ce_weights)) return NRL_E_BAD_ARG;
     if (a->reserved != 0 || !(a->temperature >= 0.f) || !isfinite(a->temperature)) return NRL_E_BAD_ARG;
     if (bad_mask(a->flags, a->allow_mask, a->allow_row_stride, a->V)) return NRL_E_BAD_ARG;
     int rc = need_cc10();
@@ -395,7 +395,7 @@ extern "C" int nrl_readout_scored_fwd(const nrl_readout_scored_args* a, nrl_stre
         f.rowstats = (float4*)a->rowstats + at;
         f.status = a->status ? (uint8_t*)a->status + at : nullptr;
         if (a->seeds && r0 + n == a->rows) {  // the last launch: every row's log-prob is there when its last block is done
-            f.ce = {a->seeds, a->rows / a->seeds, (const float*)a->logp, (const float*)a->scored, nullptr, (float*)a->ce_loss, (float*)a->ce_g_logp};
+            f.ce = {a->seeds, a->rows / a->seeds, (const float*)a->logp, (const float*)a->scored, (const float*)a->ce_weights, nullptr, (float*)a->ce_loss, (float*)a->ce_g_logp};
             f.done = (uint32_t*)(ws + 8);
         }
         rc = n <= 8 * 148 ? launch(head_finish_kernel<8>, dim3((unsigned)n), 256, 0, st, f) : launch(head_finish_kernel<1>, dim3((unsigned)((n + 7) / 8)), 256, 0, st, f);
@@ -408,7 +408,7 @@ extern "C" int nrl_ce_mean(uint64_t s, uint64_t n, nrl_devptr logp, nrl_devptr k
     if (s == 0 || n == 0 || (!out && !g_logp) || (out && !logp)) return NRL_E_BAD_ARG;
     if ((logp | keep | upstream | out | g_logp) & 3u) return NRL_E_BAD_ARG;
     if (s > 0x7fffffffull) return NRL_E_UNSUPPORTED;
-    return launch(ce_mean_kernel, dim3((unsigned)s), 512, 0, (cudaStream_t)stream, CeMean{s, n, (const float*)logp, (const float*)keep, (const float*)upstream, (float*)out, (float*)g_logp});
+    return launch(ce_mean_kernel, dim3((unsigned)s), 512, 0, (cudaStream_t)stream, CeMean{s, n, (const float*)logp, (const float*)keep, nullptr, (const float*)upstream, (float*)out, (float*)g_logp});
 }
 
 // ---- 8-bit integers -----------------------------------------------------------------------------------

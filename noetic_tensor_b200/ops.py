@@ -530,13 +530,14 @@ class ScoredReadout:
     ce_loss = property(lambda self: self._vector(self._loss, self.seeds))
 
 
-def readout_scored_forward(hidden, weights, *, tokens=None, scored=None, want_entropy=False, weights_are_vd=False, allow=None, allow_bits=None, temperature=1.0, workspace=None, ce_seeds=0):
+def readout_scored_forward(hidden, weights, *, tokens=None, scored=None, want_entropy=False, weights_are_vd=False, allow=None, allow_bits=None, temperature=1.0, workspace=None, ce_seeds=0, ce_weights=None):
     """`readout_forward` of given tokens over the positions of a training batch that `scored` (float32
     [rows], 0: not scored; None: all) lets into the loss (nrl_readout_scored_fwd): a ScoredReadout with `logp`
     (with `tokens`), `entropy` (with `want_entropy`), `rowstats` and `status`, all 0 at the other positions,
     which are not read. A token outside the vocabulary has log-prob NaN. `hidden` may have any leading shape,
     `tokens` and `scored` the same. With `ce_seeds` = S the result also has what `ce_mean` of S seeds with
-    keep = scored gives, `ce_loss` [S] and `ce_g_logp` [rows]. `readout_backward` is its backward."""
+    keep = scored gives, `ce_loss` [S] and `ce_g_logp` [rows]; with `ce_weights` (float32 [rows]) besides, the
+    token-mean policy-gradient loss of these signed weights in its place. `readout_backward` is its backward."""
     dev = hidden.device
     if dev.type != "cuda":
         raise ValueError("readout_scored_forward needs CUDA tensors: this library has no CPU path")
@@ -550,7 +551,7 @@ def readout_scored_forward(hidden, weights, *, tokens=None, scored=None, want_en
     if workspace is None:
         workspace = torch.empty(capi.lib().nrl_readout_scored_workspace_bytes(rows, V, d, scored is not None), dtype=torch.uint8, device=dev)
     a = capi.ReadoutScoredArgs(C.sizeof(capi.ReadoutScoredArgs), 1 if weights_are_vd else 0, V, d, rows, xp, weights.data_ptr(), tp, sp, at(out._logp), at(out._entropy), buf, at(out._status), 0, 0,
-                               workspace.data_ptr(), workspace.numel() * workspace.element_size(), temperature, 0, ce_seeds, at(out._loss), at(out._g))
+                               workspace.data_ptr(), workspace.numel() * workspace.element_size(), temperature, 0, ce_seeds, at(out._loss), at(out._g), _need_flat(ce_weights, torch.float32, rows, "weights", dev))
     if allow is not None or allow_bits is not None:
         allow = _readout_masks(a, V, rows, allow, allow_bits, dev)
     _launch(dev, "nrl_readout_scored_fwd", C.byref(a))

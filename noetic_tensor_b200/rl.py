@@ -114,8 +114,8 @@ class Head:
         self.kw = dict(weights_are_vd=weight_is_vd, allow=allow, allow_bits=bits, temperature=float(temperature))
         self.checkpoint, self.grad_dtype = checkpoint, grad_dtype
 
-    def run(self, tokens=None, scored=None, want_entropy=False, ce_seeds=0):
-        return _HeadRun(self, tokens, scored, want_entropy, ce_seeds)
+    def run(self, tokens=None, scored=None, want_entropy=False, ce_seeds=0, ce_weights=None):
+        return _HeadRun(self, tokens, scored, want_entropy, ce_seeds, ce_weights)
 
 
 def _as(t, dtype):
@@ -126,9 +126,10 @@ def _as(t, dtype):
 class _HeadRun:
     """A forward of a Head and what its backward needs (not the hidden states when they are checkpointed)."""
 
-    def __init__(self, head, tokens, scored, want_entropy, ce_seeds):
+    def __init__(self, head, tokens, scored, want_entropy, ce_seeds, ce_weights):
         self.tokens, self.weight, self.kw, self.grad_dtype, self.shape = _as(tokens, torch.int32), head.weight, head.kw, head.grad_dtype, head.hidden.shape
-        self.fwd = ops.readout_scored_forward(head.hidden, head.weight, tokens=self.tokens, scored=_as(scored, torch.float32), want_entropy=want_entropy, ce_seeds=ce_seeds, **head.kw)
+        self.fwd = ops.readout_scored_forward(head.hidden, head.weight, tokens=self.tokens, scored=_as(scored, torch.float32), want_entropy=want_entropy, ce_seeds=ce_seeds, ce_weights=ce_weights,
+                                              **head.kw)
         self.saved = ops.quantize_rows(head.hidden) if head.checkpoint else head.hidden
 
     def backward(self, g_logp=None, g_ent=None):
@@ -224,11 +225,11 @@ def sample_categorical_reference(logits, temperature, vocab_mask, rng):
 class _TokenLogProbs:
     """token_log_probs (src/nn/rl.rs:134-141) and its backward to the logits."""
 
-    def __init__(self, logits, tokens, mask=None):
+    def __init__(self, logits, tokens, mask=None, **head):
         self.z = _tempered(logits)
         self.lead = self.z.shape[:-1]
         if isinstance(self.z, Head):
-            self.run, self.z = self.z.run(tokens, mask), None
+            self.run, self.z = self.z.run(tokens, mask, **head), None
             self.logp = self.run.fwd.logp.reshape(self.lead)
             return
         self.fwd = ops.row_forward(self.z.flat, tokens=tokens.reshape(-1).to(torch.int32).contiguous(), want_entropy=False, **self.z.kw())
@@ -263,15 +264,23 @@ _CHECK_NAMES = {
 
 
 def _token_level(kind, logits, tokens, mask, reduction, **kw):
-    t = _TokenLogProbs(logits, tokens, mask)
-    lp = t.logp.reshape(t.lead) if len(t.lead) == 3 else None
-    if lp is None:
+    lead = logits.shape[:-1]
+    if len(lead) != 3:
         raise ValueError("logp must be [S, B, T]")
+    # a Head's token-mean policy gradient comes out of the forward call itself, value and gradient
+    fused = isinstance(logits, Head) and kind == capi.LOSS_PG and reduction == TOKEN_MEAN and kw["weights"].shape == lead and (mask is None or mask.shape == lead)
+    if fused:
+        mask = _as(mask, torch.float32)
+    t = _TokenLogProbs(logits, tokens, mask, **(dict(ce_seeds=lead[0], ce_weights=kw["weights"]) if fused else {}))
+    lp = t.logp
     # the checks of src/nn/rl.rs:230, 268-269, 386-387
     what, what_other = _CHECK_NAMES[kind]
     debug_check(what, lp, mask)
     if what_other is not None:
         debug_check(what_other, kw["other"], mask)
+    if fused:
+        return Loss(t.run.fwd.ce_loss, lambda up: t.grad_logits(ops.token_objective(kind, lp, reduction, mask=mask, up_policy=up, **kw).g_logp),
+                    lambda: t.grad_logits(t.run.fwd.ce_g_logp))
     if t.z is None and reduction in (SUM, TOKEN_MEAN, SEQUENCE_MEAN):
         o = ops.token_objective(kind, lp, reduction, mask=mask, **kw)  # the value and its gradient in one launch
         return Loss(o.policy, lambda up: t.grad_logits(ops.token_objective(kind, lp, reduction, mask=mask, up_policy=up, **kw).g_logp), lambda: t.grad_logits(o.g_logp))

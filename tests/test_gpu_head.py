@@ -462,6 +462,43 @@ def test_losses_on_a_head_against_the_losses_on_its_logits(S, B, T, d, V, what):
             assert (got.double() - want).norm() <= 4 * U16 * want.norm() + 1e-12
 
 
+@pytest.mark.parametrize("form", ["ones", "parts of one", "none kept", "no mask", "per sequence", "bool"])
+def test_policy_gradient_of_a_head_and_of_its_log_probs(form):
+    """The loss that the forward leaves is the reduction of its own log-probs: f64 sums of f32 terms, rounded once (and once
+    more for the gradient's product); where nothing is kept both are 0, whatever the weights hold."""
+    from noetic_tensor_b200 import ops, rl
+
+    S, B, T, d, V = 3, 2, 37, 72, 1000
+    x, w, tok, mask, g = head_case(S, B, T, d, V, 8)
+    adv = torch.randn(S, B, T, generator=g, device=dev())
+    if form == "parts of one":
+        mask = mask * torch.rand(S, B, T, generator=g, device=dev())
+    elif form == "none kept":
+        mask[1] = 0
+        adv[1] = math.nan
+    elif form == "no mask":
+        mask = None
+    elif form == "per sequence":
+        adv = adv[:, :, 0].contiguous()
+    l = rl.policy_gradient_loss(rl.Head(x, w), tok, adv, mask.bool() if form == "bool" else mask)
+    lp = ops.readout_scored_forward(x, w, tokens=tok, scored=mask).logp.reshape(S, B, T).double()
+    k = torch.ones_like(lp) if mask is None else mask.double()
+    a = (adv[:, :, None].expand(S, B, T) if adv.dim() == 2 else adv).double()
+    n = k.sum((1, 2)).clamp(min=1.0)
+    terms = torch.where(k != 0, -lp * a, torch.zeros_like(lp))
+    want = terms.sum((1, 2)) / n
+    # a term is rounded once, their sum at most once per term where it is kept in f32 (the separate reduction)
+    assert ((l.value.double() - want).abs() <= (B * T + 4) * U32 * terms.abs().sum((1, 2)) / n).all()
+    r = ops.readout_scored_forward(x, w, tokens=tok, scored=mask)
+    g_logp = (torch.where(k != 0, -a, torch.zeros_like(a)) / n[:, None, None]).float().reshape(-1)
+    for got, again in zip(l.backward(), l.backward(torch.ones_like(l.value))):
+        assert torch.isfinite(got).all()
+        # two roundings of the same gradient of the log-probs: at most bf16's step apart after the products
+        assert (got.double() - again.double()).norm() <= 4 * U16 * got.double().norm()
+    for got, ref in zip(l.backward(), ops.readout_backward(x, w, r, tokens=tok, g_logp=g_logp)):
+        assert (got.double() - ref.double()).norm() <= 4 * U16 * ref.double().norm()
+
+
 def test_a_run_of_them_together():
     """Decode with the 8-bit head, score the drawn tokens and train on them from an 8-bit checkpoint, on another stream."""
     from noetic_tensor_b200 import ops, rl
@@ -613,6 +650,9 @@ def test_refusals():
         (capi.NrlError, lambda: ops.readout_scored_forward(x, w, tokens=tok, temperature=-1.0)),
         (capi.NrlError, lambda: ops.readout_scored_forward(x, w, tokens=tok, ce_seeds=3)),
         (capi.NrlError, lambda: ops.readout_scored_forward(x, w, ce_seeds=1)),
+        (capi.NrlError, lambda: ops.readout_scored_forward(x, w, tokens=tok, ce_weights=up)),
+        (ValueError, lambda: ops.readout_scored_forward(x, w, tokens=tok, ce_seeds=1, ce_weights=up[:5])),
+        (ValueError, lambda: rl.policy_gradient_loss(rl.Head(x, w), tok, up.reshape(1, 2, 10).double(), mask)),
         (capi.NrlError, lambda: ops.readout_scored_forward(x, w, tokens=tok, workspace=torch.empty(256, dtype=torch.uint8, device=dev()))),
         (ValueError, lambda: ops.readout_backward(x, w, f, tokens=tok)),
         (ValueError, lambda: ops.readout_backward(x, w, f, g_logp=up)),

@@ -6,7 +6,7 @@ from noetic_tensor_b200 import capi
 
 
 def test_struct_layouts():
-    assert C.sizeof(capi.ReadoutScoredArgs) == 4 * 4 + 8 + 8 * 8 + 2 * 8 + 2 * 8 + 4 + 4 + 3 * 8
+    assert C.sizeof(capi.ReadoutScoredArgs) == 4 * 4 + 8 + 8 * 8 + 2 * 8 + 2 * 8 + 4 + 4 + 4 * 8
     assert C.sizeof(capi.ReadoutBwdArgs) == 4 * 4 + 8 + 15 * 8 + 4 + 4
     assert C.sizeof(capi.I8MatmulArgs) == 2 * 4 + 8 + 2 * 4 + 7 * 8
 
@@ -49,7 +49,7 @@ def test_scored_forward_refuses():
         (U, dict(V=510)), (U, dict(d=60)), (U, dict(hidden=4104)), (U, dict(rows=1 << 31)), (B, dict(rowstats=4100)), (B, dict(workspace=4112)), (B, dict(logp=4096)), (B, dict(tokens=2)),
         (B, dict(temperature=-1.0)), (B, dict(temperature=float("nan"))), (B, dict(reserved=1)), (B, dict(allow_mask=4096, allow_row_stride=100)),
         (B, dict(flags=capi.READOUT_MASK_BITS)), (B, dict(flags=capi.READOUT_MASK_BITS, allow_mask=4096, allow_row_stride=3)),
-        (B, dict(seeds=1)), (B, dict(seeds=3, tokens=4096, logp=4096, ce_loss=4096)), (B, dict(seeds=2, tokens=4096, logp=4096)), (B, dict(ce_loss=4096)),
+        (B, dict(seeds=1)), (B, dict(seeds=3, tokens=4096, logp=4096, ce_loss=4096)), (B, dict(seeds=2, tokens=4096, logp=4096)), (B, dict(ce_loss=4096)), (B, dict(ce_weights=4096)),
     ])
     assert l.nrl_readout_scored_fwd(None, None) == B
 
