@@ -607,6 +607,7 @@ __global__ void __launch_bounds__(kHgThreads, 1)
         uint32_t sent = 0;  // staging tiles sent off so far
         float alpha = 1.f;
         if constexpr (EPI == kEpiHidden || EPI == kEpiWeight) alpha = p.alpha ? *p.alpha : 1.f;
+        // plain loads: the kernel before this one may have written these while this one was starting, so they are not read-only data
         auto row_info = [&](const Item& w) {
             RowInfo r;
             const uint32_t row = w.tm * kRows + rank * kHgBM + quarter * 32u + (uint32_t)lane;
@@ -617,14 +618,14 @@ __global__ void __launch_bounds__(kHgThreads, 1)
             r.xs = make_float2(1.f, 1.f);
             if (r.live) {
                 if constexpr (EPI == kEpiGrad || EPI == kEpiStats || EPI == kEpiHidden)
-                    if (p.rows_at) r.caller_row = __ldg(p.rows_at + row);
-                if constexpr (EPI == kEpiGrad) r.cf = __ldg(p.coef + row);
+                    if (p.rows_at) r.caller_row = p.rows_at[row];
+                if constexpr (EPI == kEpiGrad) r.cf = p.coef[row];
                 if constexpr (EPI == kEpiGrad || EPI == kEpiHidden) {
-                    const float4 mo = __ldg(p.more + row);
+                    const float4 mo = p.more[row];
                     r.xs = make_float2(mo.x, mo.y);
                     r.token = __float_as_int(mo.z);
                 }
-                if constexpr (EPI == kEpiInt8) r.xs.x = __ldg(p.m_scale + row);
+                if constexpr (EPI == kEpiInt8) r.xs.x = p.m_scale[row];
             }
             return r;
         };
@@ -799,12 +800,12 @@ __global__ void __launch_bounds__(kHgThreads, 1)
                     if (left == 16u && p.wide) {
 #pragma unroll
                         for (int i = 0; i < 4; i++) {
-                            const float4 q = __ldg(reinterpret_cast<const float4*>(p.n_scale + col) + i);
+                            const float4 q = reinterpret_cast<const float4*>(p.n_scale + col)[i];
                             ns[4 * i] = q.x; ns[4 * i + 1] = q.y; ns[4 * i + 2] = q.z; ns[4 * i + 3] = q.w;
                         }
                     } else {
 #pragma unroll
-                        for (int i = 0; i < 16; i++) ns[i] = (uint32_t)i < left ? __ldg(p.n_scale + col + i) : 0.f;
+                        for (int i = 0; i < 16; i++) ns[i] = (uint32_t)i < left ? p.n_scale[col + i] : 0.f;
                     }
                     uint32_t z[16];
                     if (some && ok) {

@@ -176,15 +176,17 @@ struct CeMean {
     float* out;
     float* g_logp;
 };
+constexpr int kMeanThreads = 1024;
+// one seed, by all threads of the block; sh: a pair per warp
 __device__ __forceinline__ void ce_mean_seed(const CeMean& p, uint64_t seed, double (*sh)[2]) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const uint64_t base = seed * p.n;
     double v = 0.0, c = 0.0;
-#pragma unroll 4
+#pragma unroll 8
     for (uint64_t i = threadIdx.x; i < p.n; i += blockDim.x) {
-        const float k = p.keep ? p.keep[base + i] : 1.f;
+        const float k = p.keep ? p.keep[base + i] : 1.f, lp = p.out ? __ldcg(p.logp + base + i) : 0.f, w = p.weights ? p.weights[base + i] : k;
         c += (double)k;
-        if (p.out && k != 0.f) v -= (double)(__ldcg(p.logp + base + i) * (p.weights ? p.weights[base + i] : k));
+        if (k != 0.f) v -= (double)(lp * w);
     }
 #pragma unroll
     for (int k = 16; k >= 1; k >>= 1) {
@@ -195,18 +197,20 @@ __device__ __forceinline__ void ce_mean_seed(const CeMean& p, uint64_t seed, dou
     if (lane == 0) { sh[warp][0] = v; sh[warp][1] = c; }
     __syncthreads();
     v = c = 0.0;
-    for (uint32_t w = 0; w < blockDim.x >> 5; w++) { v += sh[w][0]; c += sh[w][1]; }
+#pragma unroll 8
+    for (int w = 0; w < (int)(blockDim.x >> 5); w++) { v += sh[w][0]; c += sh[w][1]; }
     const double count = c > 1.0 ? c : 1.0;
     if (p.out && threadIdx.x == 0) p.out[seed] = (float)(v / count);
     if (!p.g_logp) return;
     const float g = (float)((p.upstream ? (double)p.upstream[seed] : 1.0) / count);
+#pragma unroll 8
     for (uint64_t i = threadIdx.x; i < p.n; i += blockDim.x) {
-        const float k = p.keep ? p.keep[base + i] : 1.f;
-        p.g_logp[base + i] = p.weights ? (k != 0.f ? -(p.weights[base + i] * g) : 0.f) : -(k * g);
+        const float k = p.keep ? p.keep[base + i] : 1.f, w = p.weights ? p.weights[base + i] : k;
+        p.g_logp[base + i] = k != 0.f ? -(w * g) : 0.f;
     }
 }
-__global__ void __launch_bounds__(512) ce_mean_kernel(CeMean p) {
-    __shared__ double sh[16][2];
+__global__ void __launch_bounds__(kMeanThreads) ce_mean_kernel(CeMean p) {
+    __shared__ double sh[kMeanThreads / 32][2];
     next_kernel_may_start();
     after_previous_kernel();
     ce_mean_seed(p, blockIdx.x, sh);
@@ -226,8 +230,8 @@ struct HeadFinish {
     float* entropy;
     float4* rowstats;
     uint8_t* status;
-    // the mean cross-entropy per seed, by the last block to finish: which one that is changes no sum
-    CeMean ce;                  // ce.seeds = 0: not wanted
+    // the means of a few seeds of a small call, by the last block to finish: which one that is changes no sum
+    CeMean ce;                  // ce.seeds = 0: not here
     uint32_t* done;
 };
 template <int kW>
@@ -393,7 +397,10 @@ struct Quantiser {
         off = fabsf(a - (r - 12582912.f));
         return __float_as_uint(r);
     }
-    __device__ __forceinline__ uint32_t exact(float x) const { return big > 0.f ? (uint32_t)max(-127, min(127, __float2int_rn(__fdiv_rn(x * 127.f, big)))) : 0u; }
+    __device__ __forceinline__ uint32_t exact(float x) const {
+        const float k = big > 0x1p100f ? 0x1p-32f : 1.f;  // 127·x stays finite (what becomes subnormal here rounds to 0 either way)
+        return big > 0.f ? (uint32_t)max(-127, min(127, __float2int_rn(__fdiv_rn(x * k * 127.f, big * k)))) : 0u;
+    }
     __device__ __forceinline__ uint32_t operator()(float x) const {
         float off;
         const uint32_t q = near(x, off);

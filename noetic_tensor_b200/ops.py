@@ -542,7 +542,7 @@ def readout_scored_forward(hidden, weights, *, tokens=None, scored=None, want_en
     if dev.type != "cuda":
         raise ValueError("readout_scored_forward needs CUDA tensors: this library has no CPU path")
     d, n = hidden.shape[-1], hidden.numel()
-    rows = n // d
+    rows = n // d if d else 0
     V = _readout_weight(weights, d, weights_are_vd, dev)
     xp, tp, sp = _need_flat(hidden, torch.bfloat16, n, "hidden", dev), _need_flat(tokens, torch.int32, rows, "tokens", dev), _need_flat(scored, torch.float32, rows, "scored", dev)
     out = ScoredReadout(rows, tokens is not None, want_entropy, ce_seeds, dev)
@@ -603,7 +603,7 @@ def quantize_rows(x):
     d = x.shape[-1]
     if not x.is_contiguous():
         raise ValueError("x must be contiguous")
-    q = _int8_rows(x.numel() // d, d, dev)
+    q = _int8_rows(x.numel() // d if d else 0, d, dev)
     _launch(dev, "nrl_i8_quantize_rows", _dt(x), q.values.shape[0], d, x.data_ptr(), q.values.data_ptr(), q.values.shape[1], q.scales.data_ptr())
     return q
 
@@ -655,7 +655,7 @@ def int8_linear(x, w, dtype=torch.float32):
     if dev.type != "cuda":
         raise ValueError("int8_linear needs CUDA tensors: this library has no CPU path")
     d = x.shape[-1]
-    (n, w_pitch), rows = w.values.shape, x.numel() // d
+    (n, w_pitch), rows = w.values.shape, x.numel() // d if d else 0
     if d != w.d or w.values.device != dev or not x.is_contiguous():
         raise ValueError(f"int8_linear: contiguous rows of {w.d} values on {w.values.device}, got {tuple(x.shape)} on {dev}")
     out = torch.empty(x.shape[:-1] + (n,), dtype=dtype, device=dev)
@@ -681,7 +681,7 @@ def readout_backward(hidden, weights, fwd, *, tokens=None, g_logp=None, g_ent=No
     d = quant.d if quant else x.shape[-1]
     if hidden_shape is None:
         hidden_shape = torch.Size((x.shape[0], d)) if quant else x.shape
-    rows = hidden_shape.numel() // d
+    rows = hidden_shape.numel() // d if d else 0
     V = _readout_weight(weights, d, weights_are_vd, dev)
     if grad_dtype is not torch.bfloat16 and grad_dtype is not torch.float32:
         raise TypeError(f"gradients must be bfloat16 or float32, got {grad_dtype}")

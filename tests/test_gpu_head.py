@@ -168,6 +168,20 @@ def test_quantised_rows(rows, d, dtype):
     assert torch.equal(back, q.values[:, :d].float() * q.scales[:, None])
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("top", [2.0**127, 2.0**122, 2.0**-100, 2.0**-120])
+def test_quantised_rows_of_extreme_magnitude(dtype, top):
+    """Powers of two times small integers: exact in both types, so the integers are those of exact arithmetic, ties included."""
+    from noetic_tensor_b200 import ops
+
+    part = torch.tensor([1.0, -1.0, 0.5, -0.5, 0.25, 0.75, 2.0**-6, 2.0**-7, 2.0**-8, 0.0], device=dev(), dtype=torch.float64)
+    x = (top * part).to(dtype)[None]
+    assert torch.equal(x.double()[0], top * part)
+    q = ops.quantize_rows(x)
+    assert torch.equal(q.values[0, :10].double(), torch.round(127.0 * part))
+    assert torch.equal(q.scales.double(), torch.tensor([top / 127.0], device=dev(), dtype=torch.float64).float().double())
+
+
 @pytest.mark.parametrize("d,V", [(8, 8), (72, 136), (1000, 504), (264, 4104)])
 def test_quantised_weight_layouts(d, V):
     from noetic_tensor_b200 import ops
@@ -195,6 +209,22 @@ def test_int8_product_is_exact(rows, k, n):
         got = ops.int8_matmul(x, w, dt)
         assert got.shape == (rows, n) and got.dtype == dt
         assert ((got.double() - want).abs() <= tol * want.abs() * (1 + 1e-6)).all(), (got.double() - want).abs().max()
+
+
+def test_int8_results_past_32_bits():
+    """Offsets of the result past 2^32 elements, checked where they pass it and at both ends."""
+    from noetic_tensor_b200 import ops
+
+    rows, n, k = 33600, 128256, 32
+    g = torch.Generator(device=dev())
+    g.manual_seed(1)
+    x = torch.randint(-127, 128, (rows, k), generator=g, device=dev(), dtype=torch.int8)
+    w = torch.randint(-127, 128, (n, k), generator=g, device=dev(), dtype=torch.int8)
+    out = ops.int8_matmul(ops.Int8Rows(x, torch.ones(rows, device=dev()), k), ops.Int8Rows(w, torch.ones(n, device=dev()), k), torch.bfloat16)
+    assert out.numel() > 2**32
+    for at in (0, 2**31 // n, 2**32 // n, rows - 4):
+        want = x[at : at + 4].double() @ w.double().t()
+        assert torch.equal(out[at : at + 4], want.float().bfloat16())  # an integer below 2^24, rounded once
 
 
 def test_int8_extreme_integers_and_nonfinite_scales():
@@ -499,6 +529,22 @@ def test_policy_gradient_of_a_head_and_of_its_log_probs(form):
         assert (got.double() - ref.double()).norm() <= 4 * U16 * ref.double().norm()
 
 
+@pytest.mark.parametrize("S,n", [(1, 16), (2, 256), (2, 257), (1, 5000), (9, 130), (5000, 1)])
+def test_means_of_many_seeds(S, n):
+    from noetic_tensor_b200 import ops
+
+    x, w, tok, g = make(S * n, 16, 64, S, "dV")
+    keep = (torch.rand(S * n, generator=g, device=dev()) < 0.5).float()
+    f = ops.readout_scored_forward(x, w, tokens=tok, scored=keep, ce_seeds=S)
+    lp, k = f.logp.double().reshape(S, n), keep.double().reshape(S, n)
+    count = k.sum(1).clamp(min=1.0)
+    want = (-lp * k).sum(1) / count
+    assert ((f.ce_loss.double() - want).abs() <= 2 * U32 * want.abs()).all()  # f32 products summed in f64, one rounding
+    assert ((f.ce_g_logp.double().reshape(S, n) + k / count[:, None]).abs() <= 2 * U32 * k).all()
+    value, g_logp = ops.ce_mean(f.logp, S, keep)
+    assert torch.equal(value, f.ce_loss) and torch.equal(g_logp, f.ce_g_logp)
+
+
 def test_a_run_of_them_together():
     """Decode with the 8-bit head, score the drawn tokens and train on them from an 8-bit checkpoint, on another stream."""
     from noetic_tensor_b200 import ops, rl
@@ -664,6 +710,10 @@ def test_refusals():
         (capi.NrlError, lambda: ops.readout_backward(x, w, f, tokens=tok, g_logp=up, workspace=torch.empty(256, dtype=torch.uint8, device=dev()))),
         (ValueError, lambda: rl.categorical_kl(rl.Head(x, w), torch.zeros(1, 2, 10, 512, device=dev()))),
         (ValueError, lambda: loss.cross_entropy_with(rl.Head(x, w), tok, mask, loss.CeOptions(smoothing=0.1))),
+        (capi.NrlError, lambda: ops.readout_scored_forward(x[:, :0].contiguous(), w, tokens=tok[:, :0].contiguous())),
+        (capi.NrlError, lambda: ops.readout_scored_forward(x[..., :0].contiguous(), w[:0], tokens=tok[:, :0].contiguous())),
+        (capi.NrlError, lambda: ops.quantize_rows(x[..., :0].contiguous())),
+        (capi.NrlError, lambda: ops.int8_linear(x[:, :0].contiguous(), ops.quantize_weight(w))),
         (ValueError, lambda: ops.Int8Rows(torch.zeros(3, 20, dtype=torch.int8, device=dev()), torch.zeros(3, device=dev()), 20)),
         (ValueError, lambda: ops.int8_matmul(ops.quantize_rows(x[0, 0]), ops.quantize_rows(x[0, 0, :, :32].contiguous()))),
         (TypeError, lambda: ops.quantize_rows(x.half())),
