@@ -51,12 +51,13 @@ inline float logit_scale(uint32_t d, float tau) { return (1.f + kAccumulatorLoss
 
 // Ranges of K in dx = dz·Wᵀ for `tiles` tiles of dx and `chunks` steps of K: with few tiles the steps of a tile go to several
 // pairs (or single CTAs), whose sums are added afterwards. As many ranges as fill one wave of those, or two where that takes 5 % fewer steps, each of
-// at least 24 steps (10 us of products: adding up is a launch of 3 us). Decided where the number of scored rows is known, on
+// at least 12 steps (201 rows at V = 4104, d = 512: dz, dx and the adding-up 33 us with at least 24, 27 with 12; with 8, 140 rows at
+// V = 1120 took 10 % longer). Decided where the number of scored rows is known, on
 // the device, and the same there and in the kernel that adds up.
 constexpr uint32_t kPairs = 74;  // CTA pairs that run side by side (148 SMs)
 __host__ __device__ inline uint32_t hidden_split(uint32_t tiles, uint32_t chunks, uint32_t side_by_side) {
     if (tiles == 0 || tiles > side_by_side) return 1u;
-    const uint32_t most = chunks / 24u, a = side_by_side / tiles, b = 2 * side_by_side / tiles;
+    const uint32_t most = chunks / 12u, a = side_by_side / tiles, b = 2 * side_by_side / tiles;
     const uint32_t one = most < a ? (most ? most : 1u) : a, two = most < b ? (most ? most : 1u) : b;  // steps of a tile: 1 / one, or 2 / two
     return 200u * one < 95u * two ? two : one;
 }

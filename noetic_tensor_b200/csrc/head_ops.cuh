@@ -328,9 +328,11 @@ __global__ void __launch_bounds__(256) head_finish_kernel(HeadFinish p) {
     for (uint64_t s = 0; s < p.ce.seeds; s++) ce_mean_seed(p.ce, s, sh);
 }
 
-// d_hidden of the scored rows from the ranges of a split sum; nothing to do where K was not split. A block takes 128 columns of a row,
-// 32 threads × 4 columns, with eight groups of threads: group g adds the ranges g, g + 8, … in order, then the groups are added in
-// order. It goes on with the grid's stride (the host does not know the number of rows).
+// d_hidden of the scored rows from the ranges of a split sum; nothing to do where K was not split. 32 threads take 128 columns of a row,
+// four each, with up to eight groups of them where there are many ranges: group g of G adds the ranges g, g + G, … in order, then the
+// groups are added in order. With few ranges (many rows) the block's eight groups take eight rows instead (three ranges of 1536 × 2048:
+// 29 us cold with eight groups to a row, bound by its barriers; 30 us less in a backward call). The grid goes on with its stride (the
+// host does not know the number of rows).
 __global__ void __launch_bounds__(256) head_fold_kernel(const uint32_t* count, const float* alpha, const float4* more, const uint32_t* rows_at, const float* acc, uint32_t chunks, uint32_t side_by_side, uint32_t bn, uint32_t d, void* out,
                                                         uint32_t out_f32, uint32_t add) {
     __shared__ float4 part[8][32];
@@ -340,23 +342,26 @@ __global__ void __launch_bounds__(256) head_fold_kernel(const uint32_t* count, c
     if (nsplit == 1) return;
     const float common = *alpha;
     const uint64_t range = (uint64_t)HeadGemm::acc_rows(n) * d;
-    const uint32_t t = threadIdx.x & 31, g = threadIdx.x >> 5;
-    for (uint32_t b = blockIdx.x; b < n * across; b += gridDim.x) {
-        const uint32_t i = b / across, c = ((b - i * across) * 32 + t) * 4;
-        const float* q0 = acc + (uint64_t)i * d + c;
+    const uint32_t t = threadIdx.x & 31, warp = threadIdx.x >> 5, G = nsplit >= 16 ? 8u : nsplit >= 8 ? 4u : 1u, g = warp & (G - 1), rows = 8 / G;
+    for (uint32_t b = blockIdx.x; b < (n + rows - 1) / rows * across; b += gridDim.x) {
+        const uint32_t i = b / across * rows + warp / G, c = (b % across * 32 + t) * 4;
+        const bool mine = i < n && c < d;
         float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (c < d) {
+        if (mine) {
+            const float* q0 = acc + (uint64_t)i * d + c;
 #pragma unroll 8
-            for (uint32_t s = g; s < nsplit; s += 8) {
+            for (uint32_t s = g; s < nsplit; s += G) {
                 const float4 q = *reinterpret_cast<const float4*>(q0 + s * range);
                 y.x += q.x; y.y += q.y; y.z += q.z; y.w += q.w;
             }
         }
-        part[g][t] = y;
-        __syncthreads();
-        if (g == 0 && c < d) {
-#pragma unroll
-            for (int k = 1; k < 8; k++) { y.x += part[k][t].x; y.y += part[k][t].y; y.z += part[k][t].z; y.w += part[k][t].w; }
+        if (G > 1) {
+            part[warp][t] = y;
+            __syncthreads();
+            if (g == 0)
+                for (uint32_t k = 1; k < G; k++) { y.x += part[warp + k][t].x; y.y += part[warp + k][t].y; y.z += part[warp + k][t].z; y.w += part[warp + k][t].w; }
+        }
+        if (g == 0 && mine) {
             const float scale = common * more[i].y;
             const uint64_t r = rows_at[i];
             y.x *= scale; y.y *= scale; y.z *= scale; y.w *= scale;
@@ -376,7 +381,7 @@ __global__ void __launch_bounds__(256) head_fold_kernel(const uint32_t* count, c
                 *o = make_uint2(pack_bf16(y.x, y.y), pack_bf16(y.z, y.w));
             }
         }
-        __syncthreads();
+        if (G > 1) __syncthreads();
     }
 }
 

@@ -113,7 +113,7 @@ static BwdPlan bwd_plan(uint64_t rows, uint32_t V, uint32_t d) {
     // any number of scored rows up to `rows` may turn up: whether one of them would have dx's K split
     b.side_by_side = b.single ? 2 * kPairs : kPairs;
     // half-width tiles of dx where even its ranges leave pairs idle
-    b.hidden_bn = (uint64_t)tiles256(rows) * tiles256(d) * (b.chunks >= 48 ? b.chunks / 24 : 1) < b.side_by_side ? 128u : 256u;
+    b.hidden_bn = (uint64_t)tiles256(rows) * tiles256(d) * (b.chunks >= 24 ? b.chunks / 12 : 1) < b.side_by_side ? 128u : 256u;
     uint64_t split_units = 0;
     const uint32_t tn = (d + b.hidden_bn - 1) / b.hidden_bn, tm = tiles256(rows);
     for (uint32_t m = 1; m <= tm && m * tn <= b.side_by_side; m++) {
