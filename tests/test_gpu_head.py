@@ -391,6 +391,25 @@ def test_several_pieces_of_the_vocabulary():
     held(dw.t(), tw, ew + rows * U32 * ew / U16, "d_weights")
 
 
+@pytest.mark.parametrize("rows", [40, 200])
+@pytest.mark.parametrize("layout", ["dV", "Vd"])
+def test_pieces_whose_sums_are_split(rows, layout):
+    """So many columns that few rows have two pieces too: every range of a split sum is carried from piece to piece."""
+    from noetic_tensor_b200 import ops
+
+    d, V = 64, 1060008
+    x, w, tok, g = make(rows, d, V, rows, layout)
+    vd = layout == "Vd"
+    up = torch.randn(rows, generator=g, device=dev())
+    f = ops.readout_scored_forward(x, w, tokens=tok, weights_are_vd=vd)
+    w_vd = w if vd else w.t()
+    th, tw, eh, ew = truth(x, w_vd, tok, up, None, None, 1.0)
+    for dtype in (torch.bfloat16, torch.float32):
+        dh, dw = ops.readout_backward(x, w, f, tokens=tok, g_logp=up, weights_are_vd=vd, grad_dtype=dtype)
+        held(dh, th, eh, "d_hidden")
+        held(dw if vd else dw.t(), tw, ew, "d_weights")
+
+
 @pytest.mark.parametrize("rows,d,V", [(40, 136, 1000), (300, 264, 4104), (64, 512, 40008)])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_adding_to_gradients(rows, d, V, dtype):
