@@ -466,7 +466,7 @@ static int i8_check(const nrl_i8_matmul_args* a) {
     return need_cc10();
 }
 
-extern "C" uint64_t nrl_i8_linear_workspace_bytes(uint64_t rows, uint32_t k) { return up(rows * 4, 256) + rows * up(k, 16); }
+extern "C" uint64_t nrl_i8_linear_workspace_bytes(uint64_t rows, uint32_t k) { return up(rows * 4, 256) + rows * up(k, 128); }
 
 extern "C" int nrl_i8_linear(uint32_t x_dtype, const nrl_i8_matmul_args* a, nrl_devptr workspace, uint64_t workspace_bytes, nrl_stream stream) {
     if (!a || a->struct_size != sizeof(nrl_i8_matmul_args) || a->x_scales || a->x_pitch) return NRL_E_BAD_ARG;
@@ -475,7 +475,7 @@ extern "C" int nrl_i8_linear(uint32_t x_dtype, const nrl_i8_matmul_args* a, nrl_
     nrl_i8_matmul_args q = *a;
     q.x_scales = workspace;
     q.x = workspace + up(a->rows * 4, 256);
-    q.x_pitch = up(a->k, 16);
+    q.x_pitch = up(a->k, 128);  // TMA reads then cover whole lines
     int rc = i8_check(&q);  // nothing is launched for a product that is refused
     if (rc) return rc;
     rc = nrl_i8_quantize_rows(x_dtype, a->rows, a->k, a->x, q.x, q.x_pitch, q.x_scales, stream);
