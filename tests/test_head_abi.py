@@ -92,4 +92,4 @@ def test_scratch_sizes():
     assert l.nrl_readout_bwd_workspace_bytes(0, 512, 64) == 0
     assert l.nrl_readout_scored_workspace_bytes(262144, 128256, 4096, 0) < 16384 * 128256 // 128 * 2 * 16 + 2**20
     assert l.nrl_readout_scored_workspace_bytes(262144, 128256, 4096, 1) > 262144 * 4096 * 2
-    assert l.nrl_i8_linear_workspace_bytes(3, 100) == 256 + 3 * 112
+    assert l.nrl_i8_linear_workspace_bytes(3, 100) == 256 + 3 * 128
