@@ -5,6 +5,7 @@ libnrl.so. The functions here are thin: they check devices/dtypes, allocate the 
 wants the caller to own, fill the argument struct and launch on torch's current stream.
 """
 import ctypes as C
+import functools
 
 import torch
 
@@ -499,6 +500,16 @@ def _readout_weight(weights, d, weights_are_vd, dev):
     return V
 
 
+@functools.lru_cache(maxsize=1024)
+def _scored_workspace_bytes(rows, V, d, has_scored):
+    return capi.lib().nrl_readout_scored_workspace_bytes(rows, V, d, has_scored)
+
+
+@functools.lru_cache(maxsize=1024)
+def _bwd_workspace_bytes(rows, V, d):
+    return capi.lib().nrl_readout_bwd_workspace_bytes(rows, V, d)
+
+
 class ScoredReadout:
     """Outputs of nrl_readout_scored_fwd, in one buffer: `rowstats` [rows, 4], `status` uint8 [rows] and,
     when requested (else None), `logp`, `entropy`, `ce_g_logp` [rows] and `ce_loss` [seeds]."""
@@ -549,7 +560,7 @@ def readout_scored_forward(hidden, weights, *, tokens=None, scored=None, want_en
     buf = out._buf.data_ptr()
     at = lambda offset: buf + 4 * offset if offset else 0  # noqa: E731
     if workspace is None:
-        workspace = torch.empty(capi.lib().nrl_readout_scored_workspace_bytes(rows, V, d, scored is not None), dtype=torch.uint8, device=dev)
+        workspace = torch.empty(_scored_workspace_bytes(rows, V, d, scored is not None), dtype=torch.uint8, device=dev)
     a = capi.ReadoutScoredArgs(C.sizeof(capi.ReadoutScoredArgs), 1 if weights_are_vd else 0, V, d, rows, xp, weights.data_ptr(), tp, sp, at(out._logp), at(out._entropy), buf, at(out._status), 0, 0,
                                workspace.data_ptr(), workspace.numel() * workspace.element_size(), temperature, 0, ce_seeds, at(out._loss), at(out._g), _need_flat(ce_weights, torch.float32, rows, "weights", dev))
     if allow is not None or allow_bits is not None:
@@ -672,7 +683,8 @@ def readout_backward(hidden, weights, fwd, *, tokens=None, g_logp=None, g_ent=No
     logits computed again in pieces (nrl_readout_bwd). `hidden`: the bf16 [..., d] of the forward call, or
     an Int8Rows checkpoint of it (d_hidden then has `hidden_shape`, default [rows, d]). Gradients are
     `grad_dtype` (bfloat16 or float32); `add_hidden` / `add_weights` are tensors they are added to in place
-    (their own dtype counts). Rows whose upstreams are 0 are not read."""
+    (their own dtype counts). Rows whose upstreams are 0 are not read. With neither upstream given, it is the
+    gradient of the loss that `fwd` holds (`ce_g_logp`)."""
     quant = hidden if isinstance(hidden, Int8Rows) else None
     x = quant.values if quant else hidden
     dev = x.device
@@ -685,8 +697,10 @@ def readout_backward(hidden, weights, fwd, *, tokens=None, g_logp=None, g_ent=No
     V = _readout_weight(weights, d, weights_are_vd, dev)
     if grad_dtype is not torch.bfloat16 and grad_dtype is not torch.float32:
         raise TypeError(f"gradients must be bfloat16 or float32, got {grad_dtype}")
-    if g_logp is None and g_ent is None:
-        raise ValueError("give `g_logp`, `g_ent` or both")
+    own = type(fwd) is ScoredReadout and fwd.rows == rows and fwd._buf.device == dev
+    from_loss = 4 * fwd._g if own and g_logp is None and g_ent is None else 0  # where fwd's gradient of the log-probs lies, 0: not used
+    if g_logp is None and g_ent is None and not from_loss:
+        raise ValueError("give `g_logp`, `g_ent` or both, or a forward with a loss")
     flags = capi.READOUT_W_VD if weights_are_vd else 0
     if quant:
         if x.shape[0] != rows:
@@ -695,7 +709,7 @@ def readout_backward(hidden, weights, fwd, *, tokens=None, g_logp=None, g_ent=No
         xp, sp, pitch = x.data_ptr(), quant.scales.data_ptr(), x.shape[1]
     else:
         xp, sp, pitch = _need_flat(x, torch.bfloat16, rows * d, "hidden", dev), 0, 0
-    if g_logp is not None and tokens is None:
+    if (g_logp is not None or from_loss) and tokens is None:
         raise ValueError("`g_logp` needs the tokens")
 
     def out(add, want, shape, f32_flag, add_flag, what):
@@ -714,16 +728,16 @@ def readout_backward(hidden, weights, fwd, *, tokens=None, g_logp=None, g_ent=No
     d_hidden = out(add_hidden, want_hidden, hidden_shape, capi.READOUT_BWD_D_HIDDEN_F32, capi.READOUT_BWD_ADD_D_HIDDEN, "add_hidden")
     d_weights = out(add_weights, want_weights, weights.shape, capi.READOUT_BWD_D_WEIGHTS_F32, capi.READOUT_BWD_ADD_D_WEIGHTS, "add_weights")
     if workspace is None:
-        workspace = torch.empty(capi.lib().nrl_readout_bwd_workspace_bytes(rows, V, d), dtype=torch.uint8, device=dev)
-    if type(fwd) is ScoredReadout and fwd.rows == rows and fwd._buf.device == dev:
+        workspace = torch.empty(_bwd_workspace_bytes(rows, V, d), dtype=torch.uint8, device=dev)
+    if own:
         stats = fwd._buf.data_ptr()
         ent = stats + 4 * fwd._entropy if fwd._entropy else 0
     else:
         stats, ent = _need_flat(fwd.rowstats, torch.float32, rows * 4, "rowstats", dev), _need_flat(fwd.entropy, torch.float32, rows, "entropy", dev)
     if g_ent is not None and not ent:
         raise ValueError("`g_ent` needs a forward with entropies")
-    a = capi.ReadoutBwdArgs(C.sizeof(capi.ReadoutBwdArgs), flags, V, d, rows, xp, sp, pitch, weights.data_ptr(), 0 if g_logp is None else _need_flat(tokens, torch.int32, rows, "tokens", dev),
-                            stats, ent if g_ent is not None else 0, _need_flat(g_logp, torch.float32, rows, "g_logp", dev), _need_flat(g_ent, torch.float32, rows, "g_ent", dev), _p(d_hidden), _p(d_weights), 0, 0, workspace.data_ptr(), workspace.numel() * workspace.element_size(), temperature)
+    a = capi.ReadoutBwdArgs(C.sizeof(capi.ReadoutBwdArgs), flags, V, d, rows, xp, sp, pitch, weights.data_ptr(), 0 if g_logp is None and not from_loss else _need_flat(tokens, torch.int32, rows, "tokens", dev),
+                            stats, ent if g_ent is not None else 0, stats + from_loss if from_loss else _need_flat(g_logp, torch.float32, rows, "g_logp", dev), _need_flat(g_ent, torch.float32, rows, "g_ent", dev), _p(d_hidden), _p(d_weights), 0, 0, workspace.data_ptr(), workspace.numel() * workspace.element_size(), temperature)
     if allow is not None or allow_bits is not None:
         allow = _readout_masks(a, V, rows, allow, allow_bits, dev)
     _launch(dev, "nrl_readout_bwd", C.byref(a))

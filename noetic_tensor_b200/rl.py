@@ -225,11 +225,11 @@ def sample_categorical_reference(logits, temperature, vocab_mask, rng):
 class _TokenLogProbs:
     """token_log_probs (src/nn/rl.rs:134-141) and its backward to the logits."""
 
-    def __init__(self, logits, tokens, mask=None, **head):
+    def __init__(self, logits, tokens, mask=None):
         self.z = _tempered(logits)
         self.lead = self.z.shape[:-1]
         if isinstance(self.z, Head):
-            self.run, self.z = self.z.run(tokens, mask, **head), None
+            self.run, self.z = self.z.run(tokens, mask), None
             self.logp = self.run.fwd.logp.reshape(self.lead)
             return
         self.fwd = ops.row_forward(self.z.flat, tokens=tokens.reshape(-1).to(torch.int32).contiguous(), want_entropy=False, **self.z.kw())
@@ -267,20 +267,15 @@ def _token_level(kind, logits, tokens, mask, reduction, **kw):
     lead = logits.shape[:-1]
     if len(lead) != 3:
         raise ValueError("logp must be [S, B, T]")
-    # a Head's token-mean policy gradient comes out of the forward call itself, value and gradient
-    fused = isinstance(logits, Head) and kind == capi.LOSS_PG and reduction == TOKEN_MEAN and kw["weights"].shape == lead and (mask is None or mask.shape == lead)
-    if fused:
-        mask = _as(mask, torch.float32)
-    t = _TokenLogProbs(logits, tokens, mask, **(dict(ce_seeds=lead[0], ce_weights=kw["weights"]) if fused else {}))
+    if isinstance(logits, Head) and kind == capi.LOSS_PG and reduction == TOKEN_MEAN and kw["weights"].shape == lead and (mask is None or mask.shape == lead):
+        return _head_policy_gradient(logits, tokens, mask, kw["weights"])
+    t = _TokenLogProbs(logits, tokens, mask)
     lp = t.logp
     # the checks of src/nn/rl.rs:230, 268-269, 386-387
     what, what_other = _CHECK_NAMES[kind]
     debug_check(what, lp, mask)
     if what_other is not None:
         debug_check(what_other, kw["other"], mask)
-    if fused:
-        return Loss(t.run.fwd.ce_loss, lambda up: t.grad_logits(ops.token_objective(kind, lp, reduction, mask=mask, up_policy=up, **kw).g_logp),
-                    lambda: t.grad_logits(t.run.fwd.ce_g_logp))
     if t.z is None and reduction in (SUM, TOKEN_MEAN, SEQUENCE_MEAN):
         o = ops.token_objective(kind, lp, reduction, mask=mask, **kw)  # the value and its gradient in one launch
         return Loss(o.policy, lambda up: t.grad_logits(ops.token_objective(kind, lp, reduction, mask=mask, up_policy=up, **kw).g_logp), lambda: t.grad_logits(o.g_logp))
@@ -293,6 +288,20 @@ def _token_level(kind, logits, tokens, mask, reduction, **kw):
         return t.grad_logits(g_logp)
 
     return Loss(value, backward)
+
+
+def _head_policy_gradient(head, tokens, mask, weights):
+    """A Head's token-mean policy gradient comes out of the forward call itself, value and gradient."""
+    lead, mask = head.shape[:-1], _as(mask, torch.float32)
+    run = head.run(tokens, mask, ce_seeds=lead[0], ce_weights=weights)
+    if DEBUG_CHECKS:
+        debug_check("policy_gradient_loss", run.fwd.logp.reshape(lead), mask)
+
+    def backward(up):
+        o = ops.token_objective(capi.LOSS_PG, run.fwd.logp.reshape(lead), TOKEN_MEAN, mask=mask, up_policy=up, weights=weights)
+        return run.backward(g_logp=o.g_logp)
+
+    return Loss(run.fwd.ce_loss, backward, run.backward)
 
 
 def policy_gradient_loss(logits, tokens, weights, mask=None, reduction=TOKEN_MEAN):

@@ -562,6 +562,8 @@ def test_means_of_many_seeds(S, n):
     assert ((f.ce_g_logp.double().reshape(S, n) + k / count[:, None]).abs() <= 2 * U32 * k).all()
     value, g_logp = ops.ce_mean(f.logp, S, keep)
     assert torch.equal(value, f.ce_loss) and torch.equal(g_logp, f.ce_g_logp)
+    for got, want in zip(ops.readout_backward(x, w, f, tokens=tok), ops.readout_backward(x, w, f, tokens=tok, g_logp=g_logp)):
+        assert torch.equal(got, want)  # without an upstream: of the loss in `f`
 
 
 def test_a_run_of_them_together():
@@ -722,6 +724,7 @@ def test_refusals():
         (ValueError, lambda: ops.readout_backward(x, w, f, tokens=tok)),
         (ValueError, lambda: ops.readout_backward(x, w, f, g_logp=up)),
         (ValueError, lambda: ops.readout_backward(x, w, f, g_ent=up)),
+        (ValueError, lambda: ops.readout_backward(x, w, ops.readout_scored_forward(x, w, tokens=tok, ce_seeds=1))),
         (ValueError, lambda: ops.readout_backward(x, w, f, tokens=tok, g_logp=up[:5])),
         (TypeError, lambda: ops.readout_backward(x, w, f, tokens=tok, g_logp=up, grad_dtype=torch.float16)),
         (ValueError, lambda: ops.readout_backward(x, w, f, tokens=tok, g_logp=up, add_weights=w.t())),
