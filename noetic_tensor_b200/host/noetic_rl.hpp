@@ -544,10 +544,10 @@ inline Tensor token_log_probs(const Tensor& logits, const IntTensor& tokens) {
 // [.., V] logits in between (src/nn/decoder.rs:270-279 followed by src/nn/rl.rs:134-141, 405-414):
 // `hidden` BF16 [.., d], `weight` BF16 [d, V] (the Linear's [in, out] layout, src/nn/linear.rs:1-3),
 // tokens [..]. Returns the log-probabilities [..] and, if asked, the per-position entropies.
-// With `hidden` or `weight` tracked the results are too: their backward computes the logits again in
+// With `hidden` or `weight` tracked the results (the values are the same) are too: their backward computes the logits again in
 // pieces of the vocabulary (nrl_readout_bwd) and gives F32 gradients of both; with `checkpoint` the hidden
 // states live until then as 8-bit integers with a scale per position. Needs a compute-capability-10
-// device (tcgen05). `round_bf16` (untracked only): statistics of the logits rounded to bf16.
+// device (tcgen05). `round_bf16`: statistics of the logits rounded to bf16, always untracked.
 namespace detail {
 // the allow-mask of a fused head call: U8 [.., V] or [1, V], or I32 words of one bit per token [.., W] or [1, W]
 template <class Args>
@@ -633,40 +633,22 @@ struct HeadSaved {
         cu(cudaStreamSynchronize(stream()), "sync");  // the workspace goes out of scope here
     }
 };
-// the tracked form of head_token_log_probs below: its arguments are checked, `tok` is on the device
-inline Tensor head_tracked(const Tensor& hidden, const Tensor& weight, const Tensor& tok, Tensor* entropy, const Tensor* vocab_mask, double temperature, bool checkpoint) {
+// makes the results of a head forward tracked: `tok` and `rowstats` are on the device, `logp` and `entropy` as the forward left them
+inline void head_track(const Tensor& hidden, const Tensor& weight, const Tensor& tok, const Tensor& rowstats, Tensor& logp, Tensor* entropy, const Tensor* vocab_mask, double temperature, bool checkpoint) {
     auto s = std::make_shared<HeadSaved>();
-    const Shape lead(hidden.shape().begin(), hidden.shape().end() - 1);
-    s->d = weight.shape()[0]; s->V = weight.shape()[1]; s->rows = numel(lead);
+    s->d = weight.shape()[0]; s->V = weight.shape()[1]; s->rows = numel(logp.shape());
     s->hidden_shape = hidden.shape();
     s->hidden_leaf = hidden.node_;
     s->weight_leaf = weight.node_;
     s->weight = weight.detach();
     s->tokens = tok;
+    s->rowstats = rowstats;
     s->temperature = (float)temperature;
     s->device = hidden.device();
     if (vocab_mask) { s->has_mask = true; s->mask = *vocab_mask; }
-    Tensor logp = Tensor::empty(lead, DType::F32, hidden.device());
-    s->rowstats = Tensor::empty(Shape{(size_t)s->rows, 4}, DType::F32, hidden.device());
-    const uint64_t need = nrl_readout_scored_workspace_bytes(s->rows, (uint32_t)s->V, (uint32_t)s->d, 0);
-    Tensor ws = Tensor::empty(Shape{(size_t)need}, DType::U8, hidden.device());
-    nrl_readout_scored_args a;
-    std::memset(&a, 0, sizeof a);
-    a.struct_size = sizeof a;
-    a.V = (uint32_t)s->V; a.d = (uint32_t)s->d; a.rows = s->rows; a.temperature = (float)temperature;
-    head_mask(a, vocab_mask, s->rows, s->V);
-    a.hidden = hidden.dev(); a.weights = weight.dev(); a.tokens = tok.dev();
-    a.logp = logp.dev(); a.rowstats = s->rowstats.dev();
-    if (entropy) {
-        *entropy = Tensor::empty(lead, DType::F32, hidden.device());
-        s->entropy = *entropy;
-        a.entropy = entropy->dev();
-    }
-    a.workspace = ws.dev(); a.workspace_bytes = need;
-    nrl(nrl_readout_scored_fwd(&a, stream()), "readout_scored_fwd");
+    if (entropy) s->entropy = *entropy;
     if (checkpoint) s->checkpoint = Int8Rows::of(hidden);
     else s->hidden = hidden.detach();
-    cu(cudaStreamSynchronize(stream()), "sync");  // the workspace goes out of scope here
     auto node = [&](Tensor& value, bool is_entropy) {
         value.node_ = std::make_shared<Node>();
         value.node_->id = Tensor::next_id();
@@ -679,7 +661,6 @@ inline Tensor head_tracked(const Tensor& hidden, const Tensor& weight, const Ten
     };
     node(logp, false);
     if (entropy) node(*entropy, true);
-    return logp;
 }
 }  // namespace detail
 
@@ -731,10 +712,9 @@ inline Tensor head_token_log_probs(const Tensor& hidden, const Tensor& weight, c
         if (t < 0 || (uint64_t)t >= V) throw std::runtime_error("gather index out of range");
     Tensor tok = Tensor::empty(Shape{(size_t)rows}, DType::I32, hidden.device());
     cu(cudaMemcpy(tok.ptr(), h.data(), h.size() * 4, cudaMemcpyHostToDevice), "upload tokens");
-    if (hidden.tracked() || weight.tracked()) {
-        if (round_bf16) throw std::runtime_error("head_token_log_probs: round_bf16 has no backward");
-        return detail::head_tracked(hidden, weight, tok, entropy, vocab_mask, temperature, checkpoint);
-    }
+    const bool track = (hidden.tracked() || weight.tracked()) && !round_bf16;
+    Tensor rowstats;
+    if (track) rowstats = Tensor::empty(Shape{(size_t)rows, 4}, DType::F32, hidden.device());
     Tensor logp = Tensor::empty(lead, DType::F32, hidden.device());
     Tensor status = Tensor::empty(Shape{(size_t)rows}, DType::U8, hidden.device());
     const uint64_t need = nrl_readout_workspace_bytes(rows, (uint32_t)V, (uint32_t)d, 0u);
@@ -752,8 +732,10 @@ inline Tensor head_token_log_probs(const Tensor& hidden, const Tensor& weight, c
         *entropy = Tensor::empty(lead, DType::F32, hidden.device());
         a.entropy = entropy->dev();
     }
+    if (track) a.rowstats = rowstats.dev();
     a.workspace = ws.dev(); a.workspace_bytes = need;
     nrl(nrl_readout_fwd(&a, detail::stream()), "readout_fwd");
+    if (track) detail::head_track(hidden, weight, tok, rowstats, logp, entropy, vocab_mask, temperature, checkpoint);
     cu(cudaStreamSynchronize(detail::stream()), "sync");  // the workspace goes out of scope here
     return logp;
 }

@@ -147,7 +147,10 @@ static void test_gradients(bool checkpoint) {
     const Tensor lw = rl::head_token_log_probs(hx.detach(), hw, IntTensor::from_data(tok, {S, B, T}));
     const Gradients gw = backward(rl::policy_gradient_loss(lw, ha, &hm, TokenReduction::TokenMean));
     CHECK(!gw.grad(hx) && gw.grad(hw), "the hidden states are not tracked");
-    CHECK(throws([&] { rl::head_token_log_probs(hx, hw, IntTensor::from_data(tok, {S, B, T}), nullptr, true); }, "round_bf16"), "rounded logits have no backward");
+    // tracking changes no value; of rounded logits the results are untracked
+    CHECK(rl::head_token_log_probs(hx.detach(), hw.detach(), IntTensor::from_data(tok, {S, B, T})).to_vec() == glp, "the tracked values are the untracked ones");
+    const Tensor lr = rl::head_token_log_probs(hx, hw, IntTensor::from_data(tok, {S, B, T}), nullptr, true);
+    CHECK(!lr.tracked() && lr.to_vec() == rl::head_token_log_probs(hx.detach(), hw.detach(), IntTensor::from_data(tok, {S, B, T}), nullptr, true).to_vec(), "rounded logits are untracked");
 }
 
 static void test_int8() {
