@@ -84,7 +84,7 @@ def _head_ce(head, S, N, tok, keep, smoothing, reduce):
     run = head.run(tok, keep, ce_seeds=S if reduce else 0)
     if not reduce:
         return Loss(-run.fwd.logp.reshape(S, N), lambda up: run.backward(g_logp=-up))
-    return Loss(run.fwd.ce_loss, lambda up: run.backward(g_logp=ops.ce_mean(run.fwd.logp, S, keep, up, want_loss=False)[1]), run.backward)
+    return Loss(run.fwd.ce_loss, lambda up: run.backward(g_logp=ops.ce_mean(run.fwd.logp, S, keep, up, want_loss=False)[1]), run.backward_of_loss)
 
 
 def nll(logits, targets):

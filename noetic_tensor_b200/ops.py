@@ -561,6 +561,8 @@ def readout_scored_forward(hidden, weights, *, tokens=None, scored=None, want_en
     at = lambda offset: buf + 4 * offset if offset else 0  # noqa: E731
     if workspace is None:
         workspace = torch.empty(_scored_workspace_bytes(rows, V, d, scored is not None), dtype=torch.uint8, device=dev)
+    elif workspace.device != dev or not workspace.is_contiguous():
+        raise ValueError(f"workspace: contiguous, on {dev}")
     a = capi.ReadoutScoredArgs(C.sizeof(capi.ReadoutScoredArgs), 1 if weights_are_vd else 0, V, d, rows, xp, weights.data_ptr(), tp, sp, at(out._logp), at(out._entropy), buf, at(out._status), 0, 0,
                                workspace.data_ptr(), workspace.numel() * workspace.element_size(), temperature, 0, ce_seeds, at(out._loss), at(out._g), _need_flat(ce_weights, torch.float32, rows, "weights", dev))
     if allow is not None or allow_bits is not None:
@@ -727,8 +729,8 @@ def readout_backward(hidden, weights, fwd, *, tokens=None, g_logp=None, g_ent=No
 
     d_hidden = out(add_hidden, want_hidden, hidden_shape, capi.READOUT_BWD_D_HIDDEN_F32, capi.READOUT_BWD_ADD_D_HIDDEN, "add_hidden")
     d_weights = out(add_weights, want_weights, weights.shape, capi.READOUT_BWD_D_WEIGHTS_F32, capi.READOUT_BWD_ADD_D_WEIGHTS, "add_weights")
-    if workspace is None:
-        workspace = torch.empty(_bwd_workspace_bytes(rows, V, d), dtype=torch.uint8, device=dev)
+    if workspace is not None and (workspace.device != dev or not workspace.is_contiguous()):
+        raise ValueError(f"workspace: contiguous, on {dev}")
     if own:
         stats = fwd._buf.data_ptr()
         ent = stats + 4 * fwd._entropy if fwd._entropy else 0
@@ -736,11 +738,39 @@ def readout_backward(hidden, weights, fwd, *, tokens=None, g_logp=None, g_ent=No
         stats, ent = _need_flat(fwd.rowstats, torch.float32, rows * 4, "rowstats", dev), _need_flat(fwd.entropy, torch.float32, rows, "entropy", dev)
     if g_ent is not None and not ent:
         raise ValueError("`g_ent` needs a forward with entropies")
-    a = capi.ReadoutBwdArgs(C.sizeof(capi.ReadoutBwdArgs), flags, V, d, rows, xp, sp, pitch, weights.data_ptr(), 0 if g_logp is None and not from_loss else _need_flat(tokens, torch.int32, rows, "tokens", dev),
-                            stats, ent if g_ent is not None else 0, stats + from_loss if from_loss else _need_flat(g_logp, torch.float32, rows, "g_logp", dev), _need_flat(g_ent, torch.float32, rows, "g_ent", dev), _p(d_hidden), _p(d_weights), 0, 0, workspace.data_ptr(), workspace.numel() * workspace.element_size(), temperature)
+    tp = 0 if g_logp is None and not from_loss else _need_flat(tokens, torch.int32, rows, "tokens", dev)
+    gp, ep = stats + from_loss if from_loss else _need_flat(g_logp, torch.float32, rows, "g_logp", dev), _need_flat(g_ent, torch.float32, rows, "g_ent", dev)
+    _launch_backward(dev, flags, V, d, rows, xp, sp, pitch, weights.data_ptr(), tp, stats, ent if ep else 0, gp, ep, _p(d_hidden), _p(d_weights), workspace, temperature, allow, allow_bits)
+    return d_hidden, d_weights
+
+
+def _launch_backward(dev, flags, V, d, rows, x, scales, pitch, weights, tokens, stats, ent, g_logp, g_ent, d_hidden, d_weights, workspace, temperature, allow, allow_bits):
+    """nrl_readout_bwd of checked addresses."""
+    if workspace is None:
+        workspace = torch.empty(_bwd_workspace_bytes(rows, V, d), dtype=torch.uint8, device=dev)
+    a = capi.ReadoutBwdArgs(C.sizeof(capi.ReadoutBwdArgs), flags, V, d, rows, x, scales, pitch, weights, tokens, stats, ent, g_logp, g_ent, d_hidden, d_weights, 0, 0,
+                            workspace.data_ptr(), workspace.numel() * workspace.element_size(), temperature)
     if allow is not None or allow_bits is not None:
         allow = _readout_masks(a, V, rows, allow, allow_bits, dev)
     _launch(dev, "nrl_readout_bwd", C.byref(a))
+
+
+def readout_backward_of_loss(fwd, hidden, weights, tokens, *, weights_are_vd=False, allow=None, allow_bits=None, temperature=1.0, grad_dtype=torch.bfloat16, hidden_shape=None):
+    """`readout_backward` of the loss that `fwd` holds, for the arguments that the forward call has checked
+    already: `hidden` as it was there or its Int8Rows, the other arguments as they were."""
+    flags, x, scales, pitch = (capi.READOUT_W_VD if weights_are_vd else 0), hidden, 0, 0
+    if type(hidden) is Int8Rows:
+        flags, x, scales, pitch = flags | capi.READOUT_BWD_HIDDEN_I8, hidden.values, hidden.scales.data_ptr(), hidden.values.shape[1]
+    else:
+        hidden_shape = hidden.shape
+    if grad_dtype is torch.float32:
+        flags |= capi.READOUT_BWD_D_HIDDEN_F32 | capi.READOUT_BWD_D_WEIGHTS_F32
+    elif grad_dtype is not torch.bfloat16:
+        raise TypeError(f"gradients must be bfloat16 or float32, got {grad_dtype}")
+    dev, stats = x.device, fwd._buf.data_ptr()
+    d_hidden, d_weights = torch.empty(hidden_shape, dtype=grad_dtype, device=dev), torch.empty_like(weights, dtype=grad_dtype)
+    _launch_backward(dev, flags, weights.shape[0 if weights_are_vd else 1], hidden_shape[-1], fwd.rows, x.data_ptr(), scales, pitch, weights.data_ptr(), tokens.data_ptr(), stats, 0, stats + 4 * fwd._g, 0,
+                     d_hidden.data_ptr(), d_weights.data_ptr(), None, temperature, allow, allow_bits)
     return d_hidden, d_weights
 
 

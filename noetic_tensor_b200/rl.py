@@ -132,6 +132,9 @@ class _HeadRun:
                                               **head.kw)
         self.saved = ops.quantize_rows(head.hidden) if head.checkpoint else head.hidden
 
+    def backward_of_loss(self):
+        return ops.readout_backward_of_loss(self.fwd, self.saved, self.weight, self.tokens, grad_dtype=self.grad_dtype, hidden_shape=self.shape, **self.kw)
+
     def backward(self, g_logp=None, g_ent=None):
         return ops.readout_backward(self.saved, self.weight, self.fwd, tokens=self.tokens, g_logp=_as(g_logp, torch.float32), g_ent=_as(g_ent, torch.float32), grad_dtype=self.grad_dtype,
                                     hidden_shape=self.shape, **self.kw)
@@ -301,7 +304,7 @@ def _head_policy_gradient(head, tokens, mask, weights):
         o = ops.token_objective(capi.LOSS_PG, run.fwd.logp.reshape(lead), TOKEN_MEAN, mask=mask, up_policy=up, weights=weights)
         return run.backward(g_logp=o.g_logp)
 
-    return Loss(run.fwd.ce_loss, backward, run.backward)
+    return Loss(run.fwd.ce_loss, backward, run.backward_of_loss)
 
 
 def policy_gradient_loss(logits, tokens, weights, mask=None, reduction=TOKEN_MEAN):

@@ -722,6 +722,8 @@ def test_refusals():
         (ValueError, lambda: rl.policy_gradient_loss(rl.Head(x, w), tok, up.reshape(1, 2, 10).double(), mask)),
         (capi.NrlError, lambda: ops.readout_scored_forward(x, w, tokens=tok, workspace=torch.empty(256, dtype=torch.uint8, device=dev()))),
         (ValueError, lambda: ops.readout_backward(x, w, f, tokens=tok)),
+        (ValueError, lambda: ops.readout_scored_forward(x, w, tokens=tok, workspace=torch.empty(1 << 20, dtype=torch.uint8))),
+        (ValueError, lambda: ops.readout_backward(x, w, f, tokens=tok, g_logp=up, workspace=torch.empty(1 << 22, dtype=torch.uint8))),
         (ValueError, lambda: ops.readout_backward(x, w, f, g_logp=up)),
         (ValueError, lambda: ops.readout_backward(x, w, f, g_ent=up)),
         (ValueError, lambda: ops.readout_backward(x, w, ops.readout_scored_forward(x, w, tokens=tok, ce_seeds=1))),
