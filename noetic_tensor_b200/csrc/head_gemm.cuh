@@ -570,7 +570,10 @@ __global__ void __launch_bounds__(kHgThreads, 1)
                 else tc_commit(bar);
             };
             uint32_t s = 0, phase = 0u, n = 0;
-            uint64_t da = da0, db = db0;
+            // the halves apart: no address carries into the upper one, so it stays where the instruction reads it
+            const uint32_t a_hi = (uint32_t)(da0 >> 32), b_hi = (uint32_t)(db0 >> 32);
+            uint32_t a_lo = (uint32_t)da0, b_lo = (uint32_t)db0;
+            auto desc = [](uint32_t hi, uint32_t lo) { return (uint64_t)hi << 32 | lo; };
             bool ok = true;
             for (uint32_t t = pair; t < tiles && ok; t += pairs) {
                 const Item w = item(t);
@@ -585,14 +588,15 @@ __global__ void __launch_bounds__(kHgThreads, 1)
 #pragma unroll
                     for (int k = 0; k < 4; k++) {
                         const uint32_t add = k ? 1u : kc != w.k0;
-                        if constexpr (kI8) tc_mma_i8_pair(d_tmem, da + k * a_step, db + k * b_step, idesc, add);
-                        else if constexpr (PAIR) tc_mma_bf16_pair(d_tmem, da + k * a_step, db + k * b_step, idesc, add);
-                        else tc_mma_bf16(d_tmem, da + k * a_step, db + k * b_step, idesc, add);
+                        const uint64_t da = desc(a_hi, a_lo + k * a_step), db = desc(b_hi, b_lo + k * b_step);
+                        if constexpr (kI8) tc_mma_i8_pair(d_tmem, da, db, idesc, add);
+                        else if constexpr (PAIR) tc_mma_bf16_pair(d_tmem, da, db, idesc, add);
+                        else tc_mma_bf16(d_tmem, da, db, idesc, add);
                     }
                     commit(bar_empty + 8 * s);
-                    da += s_step;
-                    db += s_step;
-                    if (++s == p.stages) { s = 0; phase ^= 1u; da = da0; db = db0; }
+                    a_lo += s_step;
+                    b_lo += s_step;
+                    if (++s == p.stages) { s = 0; phase ^= 1u; a_lo = (uint32_t)da0; b_lo = (uint32_t)db0; }
                 }
                 if (ok) commit(bar_acc_full + 8 * acc);
                 n++;
