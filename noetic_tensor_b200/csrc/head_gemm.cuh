@@ -34,12 +34,15 @@ constexpr int kHgThreads = 64 + 32 * kHgEpiWarps;
 constexpr uint32_t kHgABytes = kHgBM * 128;      // one stage of A: 128 rows × 128 bytes of K
 constexpr uint32_t kHgMaxStages = 10;
 constexpr uint32_t kHgStageOut = 4096;           // 32 rows × 128 bytes of an epilogue warp's results on their way out
-// staging tiles per epilogue warp and bytes of input stages: 192 KB (six stages of 32 KB at bn = 256, more when B is narrower), one
-// stage less where two staging tiles let a warp fill one while the other leaves
-__host__ __device__ constexpr uint32_t stage_tiles(int epi) { return epi == 2 ? 2u : 1u; }
-__host__ __device__ constexpr uint32_t smem_tiles(int epi) { return (epi == 2 ? 5u : 6u) * 2 * kHgABytes; }
-__host__ __device__ constexpr uint32_t smem_bytes(int epi) { return smem_tiles(epi) + kHgEpiWarps * stage_tiles(epi) * kHgStageOut + 1024 + 256; }
+// bytes of input stages: six of 32 KB at bn = 256, more when B is narrower. A second staging tile per warp in the place of the sixth
+// stage cost dW 1 to 6 %.
+constexpr uint32_t kHgSmemTiles = 6 * 2 * kHgABytes;
+constexpr uint32_t kHgSmemBytes = kHgSmemTiles + kHgEpiWarps * kHgStageOut + 1024 + 256;
 
+template <bool V>
+struct Const {
+    static constexpr bool value = V;
+};
 enum { kEpiGrad = 0, kEpiHidden = 1, kEpiWeight = 2, kEpiInt8 = 3, kEpiStats = 4 };
 enum { kMaskNone = 0, kMaskBytes = 1, kMaskBits = 2 };
 
@@ -80,7 +83,7 @@ struct HeadGemm {
     const uint32_t* k_count;   // device: the extent along K (≤ k), or null
     uint32_t bn;               // columns per tile: 256 or 128, kEpiInt8 a multiple of 32 up to 256
     uint32_t stages;
-    uint32_t a_mn, b_mn;       // A / B contiguous along M / N instead of K
+    uint32_t b_mn;             // B contiguous along N instead of K (kEpiWeight: both operands always lie across K; A of the others never)
     uint32_t b_n0, b_k0;       // where this piece of the vocabulary begins in B, along N / along K
     uint32_t a_m0;             // … in A, along M
     uint32_t split;            // kEpiHidden: ranges of K, each with its own output buffer, where that fills the device better (hidden_split); the steps of K that rule is given, 0: never
@@ -140,9 +143,8 @@ __device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, uint32_t sr
     asm volatile("cp.async.bulk.commit_group;" ::: "memory");
 }
 // the oldest of the warp's kTiles staging tiles may be written again (its store has read it)
-template <int kTiles>
 __device__ __forceinline__ void stage_free(int lane) {
-    if (lane == 0) asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(kTiles - 1) : "memory");
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
     __syncwarp();
 }
 // the warp's staging tile is complete: send it off
@@ -440,7 +442,7 @@ __global__ void __launch_bounds__(kHgThreads, 1)
     const uint32_t smem_base = (smem_addr(smem_raw) + 1023u) & ~1023u;
     constexpr uint32_t kCtas = PAIR ? 2 : 1, kRows = kCtas * kHgBM;  // CTAs that share a tile, and its rows
     const uint32_t b_bytes = (p.bn / kCtas) * 128, stage_bytes = kHgABytes + b_bytes;
-    const uint32_t bars = smem_base + smem_tiles(EPI) + kHgEpiWarps * stage_tiles(EPI) * kHgStageOut;
+    const uint32_t bars = smem_base + kHgSmemTiles + kHgEpiWarps * kHgStageOut;
     const uint32_t bar_full = bars, bar_empty = bars + 8 * kHgMaxStages, bar_acc_full = bars + 16 * kHgMaxStages, bar_acc_empty = bar_acc_full + 16, bar_done = bar_acc_empty + 16;
     __shared__ uint32_t tmem_slot;
     __shared__ volatile uint32_t abort_flag;
@@ -510,7 +512,8 @@ __global__ void __launch_bounds__(kHgThreads, 1)
     if (warp < 2) next_kernel_may_start();
     if (warp == 0) {
         // ---- loader (both CTAs) -------------------------------------------------------------------
-        if (lane == 0) {
+        auto load = [&](auto b_across) {
+            constexpr bool b_mn = decltype(b_across)::value;
             const uint32_t full_first = PAIR ? in_first_cta(bar_full) : bar_full;
             uint32_t s = 0, phase = 1u, issued = 0, a_at = smem_base;
             bool ok = true;
@@ -523,13 +526,13 @@ __global__ void __launch_bounds__(kHgThreads, 1)
                     const uint32_t bar = full_first + 8 * s, b_at = a_at + kHgABytes;
                     const int32_t k0 = (int32_t)(kc * kKStep), kb = (int32_t)p.b_k0 + k0;
                     if constexpr (PAIR) {
-                        if (p.a_mn) {  // two boxes of 64 m × 64 k
+                        if constexpr (EPI == kEpiWeight) {  // two boxes of 64 m × 64 k
                             tma_load_2d_pair(a_at, &map_a, m0, k0, bar);
                             tma_load_2d_pair(a_at + 8192, &map_a, m0 + 64, k0, bar);
                         } else {
                             tma_load_2d_pair(a_at, &map_a, k0, m0, bar);
                         }
-                        if (p.b_mn) {
+                        if constexpr (b_mn) {
                             tma_load_2d_pair(b_at, &map_b, n0, kb, bar);
                             if (p.bn == 256) tma_load_2d_pair(b_at + 8192, &map_b, n0 + 64, kb, bar);
                         } else {
@@ -537,7 +540,7 @@ __global__ void __launch_bounds__(kHgThreads, 1)
                         }
                     } else {  // A is contiguous along K in the products that run on single CTAs
                         tma_load_2d(a_at, &map_a, k0, m0, bar);
-                        if (p.b_mn) {
+                        if constexpr (b_mn) {
                             for (uint32_t j = 0; j < p.bn / 64; j++) tma_load_2d(b_at + 8192 * j, &map_b, n0 + (int32_t)(64 * j), kb, bar);
                         } else {
                             tma_load_2d(b_at, &map_b, kb, n0, bar);
@@ -552,19 +555,25 @@ __global__ void __launch_bounds__(kHgThreads, 1)
                 const unsigned long long t_start = global_ns();
                 while (global_ns() - t_start < 2000000ull) {}
             }
+        };
+        if (lane == 0) {
+            if (EPI == kEpiWeight || (!kI8 && p.b_mn)) load(Const<true>());
+            else load(Const<false>());
         }
     } else if (warp == 1) {
         // ---- tensor-core issue (first CTA only) -------------------------------------------------------
-        if (rank == 0 && lane == 0) {
+        auto issue = [&](auto b_across) {
+            constexpr bool a_mn = EPI == kEpiWeight, b_mn = decltype(b_across)::value;
             const uint32_t shape = ((p.bn >> 3) << 17) | ((kRows >> 4) << 24);
             // f32 accumulators of bf16 products, or s32 accumulators of s8 products
-            const uint32_t idesc = kI8 ? ((2u << 4) | (1u << 7) | (1u << 10) | shape) : ((1u << 4) | (1u << 7) | (1u << 10) | (p.a_mn << 15) | (p.b_mn << 16) | shape);
+            const uint32_t idesc = kI8 ? ((2u << 4) | (1u << 7) | (1u << 10) | shape) : ((1u << 4) | (1u << 7) | (1u << 10) | ((a_mn ? 1u : 0u) << 15) | ((b_mn ? 1u : 0u) << 16) | shape);
             // contiguous along K: rows of 128 bytes, groups of 8 rows 1024 bytes apart, 32 bytes of K per product; contiguous along M / N:
             // 64-wide blocks 8 KB apart, groups of 8 k-rows 1024 bytes apart, 16 k-rows per product. One descriptor per operand, the
             // rest are additions to its address field (this thread's instructions between two products are what the tensor pipe waits for)
-            const uint64_t da0 = p.a_mn ? smem_desc_sw128(smem_base, 8192, 1024) : smem_desc_sw128(smem_base, 16, 1024);
-            const uint64_t db0 = p.b_mn ? smem_desc_sw128(smem_base + kHgABytes, 8192, 1024) : smem_desc_sw128(smem_base + kHgABytes, 16, 1024);
-            const uint32_t a_step = (p.a_mn ? 2048u : 32u) >> 4, b_step = (p.b_mn ? 2048u : 32u) >> 4, s_step = stage_bytes >> 4;
+            const uint64_t da0 = a_mn ? smem_desc_sw128(smem_base, 8192, 1024) : smem_desc_sw128(smem_base, 16, 1024);
+            const uint64_t db0 = b_mn ? smem_desc_sw128(smem_base + kHgABytes, 8192, 1024) : smem_desc_sw128(smem_base + kHgABytes, 16, 1024);
+            constexpr uint32_t a_step = (a_mn ? 2048u : 32u) >> 4, b_step = (b_mn ? 2048u : 32u) >> 4;
+            const uint32_t s_step = stage_bytes >> 4;
             auto commit = [](uint32_t bar) {
                 if constexpr (PAIR) tc_commit_pair(bar);
                 else tc_commit(bar);
@@ -602,14 +611,17 @@ __global__ void __launch_bounds__(kHgThreads, 1)
                 n++;
             }
             commit(bar_done);
+        };
+        if (rank == 0 && lane == 0) {
+            if (EPI == kEpiWeight || (!kI8 && p.b_mn)) issue(Const<true>());
+            else issue(Const<false>());
         }
     } else {
         // ---- epilogue (both CTAs): thread = row of the output (of the transposed one for kEpiInt8) ---------
         const uint32_t quarter = (uint32_t)warp & 3u, half = ((uint32_t)warp - 2u) >> 2;
         const uint32_t half_cols = p.bn / 2;  // this warp's columns: [half · bn/2, + bn/2), a multiple of 16
         const int chunks = (int)half_cols / 32;  // four or two of 32 columns in the bf16 products
-        const uint32_t stage_out = smem_base + smem_tiles(EPI) + ((uint32_t)warp - 2u) * stage_tiles(EPI) * kHgStageOut;
-        uint32_t sent = 0;  // staging tiles sent off so far
+        const uint32_t stage_out = smem_base + kHgSmemTiles + ((uint32_t)warp - 2u) * kHgStageOut;
         float alpha = 1.f;
         if constexpr (EPI == kEpiHidden || EPI == kEpiWeight) alpha = p.alpha ? *p.alpha : 1.f;
         // plain loads: the kernel before this one may have written these while this one was starting, so they are not read-only data
@@ -700,7 +712,7 @@ __global__ void __launch_bounds__(kHgThreads, 1)
                     if constexpr (EPI == kEpiGrad) {
                         uint32_t g[16];
                         epi_grad<MASK>(p, live, v, y, r.cf, ys, token, mask.chunk(c), g);
-                        if ((c & 1) == 0) stage_free<1>(lane);
+                        if ((c & 1) == 0) stage_free(lane);
 #pragma unroll
                         for (int j = 0; j < 4; j++) sts_piece(stage_out, lane, 4 * (c & 1) + j, g[4 * j], g[4 * j + 1], g[4 * j + 2], g[4 * j + 3]);
                         if (c & 1) stage_send(&map_out, stage_out, lane, (int32_t)(col0 + 32 * (c - 1)), (int32_t)row0);
@@ -739,15 +751,12 @@ __global__ void __launch_bounds__(kHgThreads, 1)
                         }
                         scale32(z, scale);
                         scale32(z + 32, scale);
-                        const uint32_t tile = stage_out + (sent & 1u) * kHgStageOut, col = col0 + 32 * c;
-                        stage_free<2>(lane);
+                        const uint32_t col = col0 + 32 * c;
+                        stage_free(lane);
 #pragma unroll
                         for (int j = 0; j < 8; j++)
-                            sts_piece(tile, lane, j, pack_bf16(z[8 * j], z[8 * j + 1]), pack_bf16(z[8 * j + 2], z[8 * j + 3]), pack_bf16(z[8 * j + 4], z[8 * j + 5]), pack_bf16(z[8 * j + 6], z[8 * j + 7]));
-                        if (row0 < mm && col < p.n) {
-                            stage_send(&map_out, tile, lane, (int32_t)(p.out_col0 + col), (int32_t)(p.out_row0 + row0));
-                            sent++;
-                        }
+                            sts_piece(stage_out, lane, j, pack_bf16(z[8 * j], z[8 * j + 1]), pack_bf16(z[8 * j + 2], z[8 * j + 3]), pack_bf16(z[8 * j + 4], z[8 * j + 5]), pack_bf16(z[8 * j + 6], z[8 * j + 7]));
+                        if (row0 < mm && col < p.n) stage_send(&map_out, stage_out, lane, (int32_t)(p.out_col0 + col), (int32_t)(p.out_row0 + row0));
                     }
                 } else {
 #pragma unroll 1
@@ -765,14 +774,10 @@ __global__ void __launch_bounds__(kHgThreads, 1)
                     const uint32_t col = col0 + 32 * c;
                     if (EPI == kEpiWeight && p.staged) {
                         scale32(z, scale);
-                        const uint32_t tile = stage_out + (sent & 1u) * kHgStageOut;
-                        stage_free<2>(lane);
+                        stage_free(lane);
 #pragma unroll
-                        for (int j = 0; j < 8; j++) sts_piece(tile, lane, j, __float_as_uint(z[4 * j]), __float_as_uint(z[4 * j + 1]), __float_as_uint(z[4 * j + 2]), __float_as_uint(z[4 * j + 3]));
-                        if (row0 < mm && col < p.n) {
-                            stage_send(&map_out, tile, lane, (int32_t)(p.out_col0 + col), (int32_t)(p.out_row0 + row0));
-                            sent++;
-                        }
+                        for (int j = 0; j < 8; j++) sts_piece(stage_out, lane, j, __float_as_uint(z[4 * j]), __float_as_uint(z[4 * j + 1]), __float_as_uint(z[4 * j + 2]), __float_as_uint(z[4 * j + 3]));
+                        if (row0 < mm && col < p.n) stage_send(&map_out, stage_out, lane, (int32_t)(p.out_col0 + col), (int32_t)(p.out_row0 + row0));
                     } else if (live && col < p.n) {
                         float* part = p.acc + ((uint64_t)w.split * p.acc_rows(mm) + row) * p.n + col;
                         if (p.acc_in) {

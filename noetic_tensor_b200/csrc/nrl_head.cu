@@ -34,7 +34,7 @@ static int need_cc10() {
 template <int EPI, int MASK, bool PAIR>
 static int launch_tiles(const CUtensorMap& ma, const CUtensorMap& mb, const CUtensorMap& mo, HeadGemm p, uint64_t tiles, cudaStream_t st) {
     constexpr unsigned ctas = PAIR ? 2 : 1;
-    p.stages = smem_tiles(EPI) / (kHgABytes + (p.bn / ctas) * 128);
+    p.stages = kHgSmemTiles / (kHgABytes + (p.bn / ctas) * 128);
     if (p.stages > kHgMaxStages) p.stages = kHgMaxStages;
     if (tiles > 0x7fffffffull) return NRL_E_UNSUPPORTED;
     int dev = 0;
@@ -42,12 +42,12 @@ static int launch_tiles(const CUtensorMap& ma, const CUtensorMap& mb, const CUte
     if (e != cudaSuccess) return (int)e;
     static std::atomic<uint64_t> ready{0};  // devices on which this kernel may have its shared memory
     if (dev >= 64 || !(ready.load(std::memory_order_acquire) >> dev & 1u)) {
-        e = cudaFuncSetAttribute(head_gemm_kernel<EPI, MASK, PAIR>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem_bytes(EPI));
+        e = cudaFuncSetAttribute(head_gemm_kernel<EPI, MASK, PAIR>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kHgSmemBytes);
         if (e != cudaSuccess) return (int)e;
         if (dev < 64) ready.fetch_or(1ull << dev, std::memory_order_release);
     }
     const uint64_t most = 2 * kPairs / ctas;
-    return launch_as(ctas, head_gemm_kernel<EPI, MASK, PAIR>, dim3(ctas * (unsigned)(tiles < most ? (tiles ? tiles : 1) : most)), kHgThreads, smem_bytes(EPI), st, ma, mb, mo, p);
+    return launch_as(ctas, head_gemm_kernel<EPI, MASK, PAIR>, dim3(ctas * (unsigned)(tiles < most ? (tiles ? tiles : 1) : most)), kHgThreads, kHgSmemBytes, st, ma, mb, mo, p);
 }
 // on pairs of CTAs or, `single`, on CTAs by themselves
 template <int EPI, int MASK = kMaskNone>
@@ -266,7 +266,7 @@ extern "C" int nrl_readout_bwd(const nrl_readout_bwd_args* a, nrl_stream stream)
             p.n = vd ? a->d : cols;
             p.k = (uint32_t)a->rows;
             p.k_count = hr.count;
-            p.a_mn = p.b_mn = 1u;
+            p.b_mn = 1u;
             p.out = (void*)a->d_weights;
             p.out_pitch = vd ? a->d : a->V;
             p.out_row0 = vd ? v0 : 0u;
