@@ -572,7 +572,8 @@ __global__ void __launch_bounds__(kHgThreads, 1)
             // contiguous along K: rows of 128 bytes, groups of 8 rows 1024 bytes apart, 32 bytes of K per product; contiguous along M / N:
             // 64-wide blocks 8 KB apart, groups of 8 k-rows 1024 bytes apart, 16 k-rows per product. One descriptor per operand, the
             // rest are additions to its address field. This thread's instructions between two products are what the tensor pipe waits for:
-            // a vote or a test of a barrier more per stage cost 2 to 8 %, the descriptors' upper halves kept out of the additions gave 10
+            // a vote or a test of a barrier more per stage cost 2 to 8 %, the descriptors' upper halves kept out of the additions gave 10,
+            // two stages to an iteration 2 (8 bits: 3)
             const uint64_t da0 = a_mn ? smem_desc_sw128(smem_base, 8192, 1024) : smem_desc_sw128(smem_base, 16, 1024);
             const uint64_t db0 = b_mn ? smem_desc_sw128(smem_base + kHgABytes, 8192, 1024) : smem_desc_sw128(smem_base + kHgABytes, 16, 1024);
             constexpr uint32_t a_step = (a_mn ? 2048u : 32u) >> 4, b_step = (b_mn ? 2048u : 32u) >> 4;
@@ -594,6 +595,7 @@ __global__ void __launch_bounds__(kHgThreads, 1)
                 if (!mbar_wait(bar_acc_empty + 8 * acc, ((n >> 1) & 1u) ^ 1u, &abort_flag)) { ok = false; break; }
                 tc_fence_after();
                 const uint32_t d_tmem = tmem + acc * 256;
+#pragma unroll 2
                 for (uint32_t kc = w.k0; kc < w.k1; kc++) {
                     if (!mbar_wait(bar_full + 8 * s, phase, &abort_flag)) { ok = false; break; }
                     tc_fence_after();
