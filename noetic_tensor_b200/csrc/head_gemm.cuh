@@ -343,7 +343,7 @@ __device__ __forceinline__ void epi_stats(const HeadGemm& p, uint32_t v, float y
             W = (W + S * dm) * sc;
             S *= sc;
         }
-        m = cm;
+        m = fmax_nan(m, cm);  // a NaN stays: the sums it went into must not be taken for the other columns'
     }
     const float m2 = -m * c2;
     const f32x2 c22 = pack2(c2, c2), m22 = pack2(m2, m2);
