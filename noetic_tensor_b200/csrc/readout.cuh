@@ -168,7 +168,7 @@ __device__ __forceinline__ void readout_fold_tile(const ReadoutParams& p, uint32
                 ts *= sc;
                 if (EXTRA) qs *= sc;
             }
-            m = cm;
+            m = fmax_nan(m, cm);  // a NaN stays: the sums it went into must not be taken for the other columns'
             if (p.greedy) {  // the first column that holds the new maximum (ties with an earlier chunk never come here)
                 uint32_t first = 31u;
 #pragma unroll
