@@ -12,7 +12,7 @@ the vocabulary makes the loss NaN instead of raising.
 import torch
 
 from . import capi, ops
-from .rl import Head, Loss, _as
+from .rl import Head, Loss, _as, _token_ids
 
 
 class CeOptions:
@@ -47,7 +47,7 @@ def _targets(targets, S, N, V, ignore_index=None, check=True):
         bad = (t < 0) | (t >= V)
         if bad.any():
             raise IndexError(f"one_hot: {int(t[bad][0])} is outside 0..{V}")
-    return t.to(torch.int32).contiguous(), keep
+    return (_as(t, torch.int32) if check else _token_ids(t, V)), keep
 
 
 def _ce(logits, targets, keep, smoothing, reduce):

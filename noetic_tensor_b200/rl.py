@@ -123,11 +123,18 @@ def _as(t, dtype):
     return t if t is None or (t.dtype is dtype and t.is_contiguous()) else t.to(dtype).contiguous()
 
 
+def _token_ids(tokens, V):
+    """Tokens as contiguous int32. An id of 64 bits outside the vocabulary stays outside: its lower 32 bits may be a token."""
+    if tokens is not None and tokens.dtype is torch.int64:
+        tokens = tokens.clamp(-1, V)
+    return _as(tokens, torch.int32)
+
+
 class _HeadRun:
     """A forward of a Head and what its backward needs (not the hidden states when they are checkpointed)."""
 
     def __init__(self, head, tokens, scored, want_entropy, ce_seeds, ce_weights):
-        self.tokens, self.weight, self.kw, self.grad_dtype, self.shape = _as(tokens, torch.int32), head.weight, head.kw, head.grad_dtype, head.hidden.shape
+        self.tokens, self.weight, self.kw, self.grad_dtype, self.shape = _token_ids(tokens, head.V), head.weight, head.kw, head.grad_dtype, head.hidden.shape
         self.fwd = ops.readout_scored_forward(head.hidden, head.weight, tokens=self.tokens, scored=_as(scored, torch.float32), want_entropy=want_entropy, ce_seeds=ce_seeds, ce_weights=ce_weights,
                                               **head.kw)
         self.saved = ops.quantize_rows(head.hidden) if head.checkpoint else head.hidden
@@ -235,7 +242,7 @@ class _TokenLogProbs:
             self.run, self.z = self.z.run(tokens, mask), None
             self.logp = self.run.fwd.logp.reshape(self.lead)
             return
-        self.fwd = ops.row_forward(self.z.flat, tokens=tokens.reshape(-1).to(torch.int32).contiguous(), want_entropy=False, **self.z.kw())
+        self.fwd = ops.row_forward(self.z.flat, tokens=_token_ids(tokens.reshape(-1), self.z.V), want_entropy=False, **self.z.kw())
         self.logp = self.fwd.logp.reshape(self.lead)
 
     def grad_logits(self, g_logp):
@@ -390,7 +397,7 @@ def head_token_log_probs(hidden, weight, tokens, round_bf16=False, vocab_mask=No
     Returns (log-probs [...], entropies [...]). Untracked; needs a compute-capability-10 device."""
     lead = hidden.shape[:-1]
     allow, bits = _vocab_mask_args(vocab_mask, weight.shape[1])
-    o = ops.readout_forward(hidden.reshape(-1, hidden.shape[-1]).contiguous(), weight, tokens=tokens.reshape(-1).to(torch.int32).contiguous(), round_bf16=round_bf16, allow=allow, allow_bits=bits,
+    o = ops.readout_forward(hidden.reshape(-1, hidden.shape[-1]).contiguous(), weight, tokens=_token_ids(tokens.reshape(-1), weight.shape[1]), round_bf16=round_bf16, allow=allow, allow_bits=bits,
                             temperature=temperature)
     ops.check_status(o.status)
     return o.logp.reshape(lead), o.entropy.reshape(lead)
