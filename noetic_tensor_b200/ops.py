@@ -25,7 +25,8 @@ def _p(t):
 
 
 def _stream(dev):
-    return torch._C._cuda_getCurrentRawStream(dev.index)  # the handle of torch.cuda.current_stream(dev)
+    index = torch.cuda.current_device() if dev.index is None else dev.index  # torch.device("cuda") is the current one
+    return torch._C._cuda_getCurrentRawStream(index)  # the handle of torch.cuda.current_stream(dev)
 
 
 def _launch(dev, name, *args):
