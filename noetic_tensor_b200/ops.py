@@ -291,26 +291,31 @@ def clip_fraction(logp, old_logp, advantages, *, mask=None, clip_low, clip_high,
 def reduce_tokens(per, mask, reduction):
     S, B, T = per.shape
     dev = per.device
+    _need(per, torch.float32, per.shape, "per", dev)
+    mask_at = _need_flat(mask, torch.float32, S * B * T, "mask", dev)
     shape = {capi.REDUCE_NONE: (S, B, T), capi.REDUCE_PER_SEQUENCE: (S, B)}.get(reduction, (S,))
     out = torch.empty(shape, dtype=torch.float32, device=dev)
     with torch.cuda.device(dev):
-        capi.check(capi.lib().nrl_reduce_tokens(reduction, S, B, T, _p(per), _p(mask), _p(out), _stream(dev)), "nrl_reduce_tokens")
+        capi.check(capi.lib().nrl_reduce_tokens(reduction, S, B, T, _p(per), mask_at, _p(out), _stream(dev)), "nrl_reduce_tokens")
     return out
 
 
 def reduce_tokens_backward(shape, mask, reduction, g_out):
     S, B, T = shape
     dev = g_out.device
+    mask_at = _need_flat(mask, torch.float32, S * B * T, "mask", dev)
     d = torch.empty(shape, dtype=torch.float32, device=dev)
     with torch.cuda.device(dev):
-        capi.check(capi.lib().nrl_reduce_tokens_bwd(reduction, S, B, T, _p(mask), _p(g_out), _p(d), _stream(dev)), "nrl_reduce_tokens_bwd")
+        capi.check(capi.lib().nrl_reduce_tokens_bwd(reduction, S, B, T, mask_at, _p(g_out), _p(d), _stream(dev)), "nrl_reduce_tokens_bwd")
     return d
 
 
 def mask_rows(x, mask):
+    _need(x, torch.float32, x.shape, "x", x.device)
+    mask_at = _need_flat(mask, torch.float32, x.numel(), "mask", x.device)
     out = torch.empty_like(x)
     with torch.cuda.device(x.device):
-        capi.check(capi.lib().nrl_mask_rows(x.numel(), _p(x), _p(mask), _p(out), _stream(x.device)), "nrl_mask_rows")
+        capi.check(capi.lib().nrl_mask_rows(x.numel(), _p(x), mask_at, _p(out), _stream(x.device)), "nrl_mask_rows")
     return out
 
 

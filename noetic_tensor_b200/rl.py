@@ -6,7 +6,8 @@ Each loss returns a `Loss`: `.value` is the reduced tensor the reference functio
 `(value * upstream).sum().backward()` yields in the reference. Where the reference builds ~40
 tape nodes per PPO step, this path has one forward and one backward pass over the logits.
 
-Masks: `mask` is the scoring mask [S,B,T] of 0/1 floats (src/nn/rl.rs:9-14); `vocab_mask` is
+Masks: `mask` is the scoring mask [S,B,T] of 0/1 floats (src/nn/rl.rs:9-14; other types, bool among them,
+are converted); `vocab_mask` is
 either a float additive mask broadcastable as [1,V] or [rows,V] (the reference's form,
 src/nn/rl.rs:471-486) or a uint8/bool allow-mask of the same shapes.
 """
@@ -254,6 +255,7 @@ class _TokenLogProbs:
 
 
 def token_log_probs(logits, tokens, mask=None):
+    mask = _as(mask, torch.float32)
     t = _TokenLogProbs(logits, tokens, mask)
     value = t.logp if mask is None else ops.mask_rows(t.logp, mask)
 
@@ -274,7 +276,7 @@ _CHECK_NAMES = {
 
 
 def _token_level(kind, logits, tokens, mask, reduction, **kw):
-    lead = logits.shape[:-1]
+    lead, mask = logits.shape[:-1], _as(mask, torch.float32)
     if len(lead) != 3:
         raise ValueError("logp must be [S, B, T]")
     if isinstance(logits, Head) and kind == capi.LOSS_PG and reduction == TOKEN_MEAN and kw["weights"].shape == lead and (mask is None or mask.shape == lead):
@@ -302,7 +304,7 @@ def _token_level(kind, logits, tokens, mask, reduction, **kw):
 
 def _head_policy_gradient(head, tokens, mask, weights):
     """A Head's token-mean policy gradient comes out of the forward call itself, value and gradient."""
-    lead, mask = head.shape[:-1], _as(mask, torch.float32)
+    lead = head.shape[:-1]
     run = head.run(tokens, mask, ce_seeds=lead[0], ce_weights=weights)
     if DEBUG_CHECKS:
         debug_check("policy_gradient_loss", run.fwd.logp.reshape(lead), mask)
@@ -341,7 +343,7 @@ def _row_level(which, logits, ref_logits, mask, reduction):
     z = _tempered(logits)
     if len(z.shape) != 4:
         raise ValueError("logits [S, B, T, V]")
-    lead = z.shape[:-1]
+    lead, mask = z.shape[:-1], _as(mask, torch.float32)
     if isinstance(z, Head):
         if which != "entropy":
             raise ValueError("the exact KL to a reference needs both sides' logits: a Head has none (kl_estimate takes one)")
