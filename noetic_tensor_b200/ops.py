@@ -304,9 +304,10 @@ def reduce_tokens_backward(shape, mask, reduction, g_out):
     S, B, T = shape
     dev = g_out.device
     mask_at = _need_flat(mask, torch.float32, S * B * T, "mask", dev)
+    g_at = _need_flat(g_out, torch.float32, {capi.REDUCE_NONE: S * B * T, capi.REDUCE_PER_SEQUENCE: S * B}.get(reduction, S), "upstream", dev)
     d = torch.empty(shape, dtype=torch.float32, device=dev)
     with torch.cuda.device(dev):
-        capi.check(capi.lib().nrl_reduce_tokens_bwd(reduction, S, B, T, mask_at, _p(g_out), _p(d), _stream(dev)), "nrl_reduce_tokens_bwd")
+        capi.check(capi.lib().nrl_reduce_tokens_bwd(reduction, S, B, T, mask_at, g_at, _p(d), _stream(dev)), "nrl_reduce_tokens_bwd")
     return d
 
 
