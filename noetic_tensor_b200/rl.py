@@ -386,6 +386,8 @@ def _vocab_mask_args(vocab_mask, V):
         return None, None
     if vocab_mask.dtype == torch.int32:
         return None, vocab_mask.reshape(-1, vocab_mask.shape[-1]).contiguous()
+    if vocab_mask.shape[-1:] != (V,):
+        raise ValueError(f"vocab_mask: [..., {V}] or [1, {V}], got {tuple(vocab_mask.shape)}")
     allow = vocab_mask.reshape(-1, V)
     return (allow.view(torch.uint8) if allow.dtype == torch.bool else allow).contiguous(), None
 
