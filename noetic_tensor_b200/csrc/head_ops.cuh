@@ -513,7 +513,7 @@ __global__ void __launch_bounds__(256) quantise_rows_kernel(const void* x, uint6
 __global__ void __launch_bounds__(256) quantise_columns_kernel(const uint16_t* w, uint32_t d, uint32_t V, uint64_t pitch, int8_t* q, float* scales) {
     __shared__ float part[4][64];
     __shared__ float big[64];
-    __shared__ int8_t tile[64][68];
+    __shared__ uint32_t tile[64][17];  // 64 bytes a row and one word more: written by bytes down a column, read by words
     next_kernel_may_start();
     after_previous_kernel();
     const uint32_t c = threadIdx.x & 63, part_of = threadIdx.x >> 6;
@@ -530,13 +530,14 @@ __global__ void __launch_bounds__(256) quantise_columns_kernel(const uint16_t* w
     }
     __syncthreads();
     const Quantiser quantise(big[c]);
+    int8_t* mine = reinterpret_cast<int8_t*>(tile[c]);
     for (uint32_t k0 = 0; k0 < pitch; k0 += 64) {
-        for (uint32_t k = part_of; k < 64; k += 4) tile[c][k] = v < V && k0 + k < d ? (int8_t)quantise(load_x<NRL_BF16>(w, (uint64_t)(k0 + k) * V + v)) : (int8_t)0;
+        for (uint32_t k = part_of; k < 64; k += 4) mine[k] = v < V && k0 + k < d ? (int8_t)quantise(load_x<NRL_BF16>(w, (uint64_t)(k0 + k) * V + v)) : (int8_t)0;
         __syncthreads();
         // 64 rows of 64 bytes, four bytes a thread and step
         for (uint32_t i = threadIdx.x; i < 64 * 16; i += 256) {
             const uint32_t r = i >> 4, k = (i & 15) * 4;
-            if (blockIdx.x * 64 + r < V && k0 + k < pitch) *reinterpret_cast<uint32_t*>(q + (uint64_t)(blockIdx.x * 64 + r) * pitch + k0 + k) = *reinterpret_cast<const uint32_t*>(&tile[r][k]);
+            if (blockIdx.x * 64 + r < V && k0 + k < pitch) *reinterpret_cast<uint32_t*>(q + (uint64_t)(blockIdx.x * 64 + r) * pitch + k0 + k) = tile[r][i & 15];
         }
         __syncthreads();
     }
