@@ -704,6 +704,7 @@ __global__ void __launch_bounds__(kHgThreads, 1)
 #pragma unroll 1
                 for (int c = 0; c < chunks; c++) {
                     float y[32];
+                    __syncwarp();
                     tc_ld32(taddr + 32 * c, reinterpret_cast<uint32_t*>(y));
                     tc_wait_ld();
                     pin32(y);
@@ -744,6 +745,7 @@ __global__ void __launch_bounds__(kHgThreads, 1)
                     for (int c = 0; c < chunks; c += 2) {
                         float z[64];
                         if (there) {
+                            __syncwarp();
                             tc_ld32(taddr + 32 * c, reinterpret_cast<uint32_t*>(z));
                             tc_ld32(taddr + 32 * c + 32, reinterpret_cast<uint32_t*>(z + 32));
                             tc_wait_ld();
@@ -768,6 +770,7 @@ __global__ void __launch_bounds__(kHgThreads, 1)
                 for (int c = 0; c < chunks; c++) {
                     float z[32];
                     if (there) {
+                        __syncwarp();
                         tc_ld32(taddr + 32 * c, reinterpret_cast<uint32_t*>(z));
                         tc_wait_ld();
                         pin32(z);
@@ -826,6 +829,7 @@ __global__ void __launch_bounds__(kHgThreads, 1)
                     float y[16];
                     if (some && ok) {
                         uint32_t z[16];
+                        __syncwarp();
                         tc_ld16(taddr + c, z);
                         tc_wait_ld();
                         pin16(z);

@@ -44,7 +44,8 @@ __device__ __forceinline__ void tc_mma_bf16(uint32_t d_tmem, uint64_t a_desc, ui
         "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
         : "memory");
 }
-// 32 consecutive f32 columns of this thread's lane
+// 32 consecutive f32 columns of this thread's lane. The whole warp executes a load of tensor memory together: behind anything
+// that lanes do differently there is a __syncwarp() before it.
 __device__ __forceinline__ void tc_ld32(uint32_t taddr, uint32_t r[32]) {
     asm volatile(
         "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"

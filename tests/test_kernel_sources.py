@@ -14,3 +14,16 @@ def test_shared_arrays_are_read_as_what_they_are_aligned_for():
     """No array of single bytes in shared memory is read in words: only its type aligns an array."""
     text = source("head_ops.cuh")
     assert not re.findall(r"__shared__\s+u?int8_t", text)
+
+
+def loads_of_tensor_memory(text):
+    """The line before each load (or run of loads) of tensor memory."""
+    lines = [line.strip() for line in text.splitlines() if line.strip()]
+    is_load = [line.startswith(("tc_ld32(", "tc_ld16(")) for line in lines]
+    return [lines[i - 1] for i in range(1, len(lines)) if is_load[i] and not is_load[i - 1]]
+
+
+def test_a_warp_comes_together_before_it_loads_tensor_memory():
+    """tcgen05.ld is executed by a whole warp (.sync.aligned), and the code before it in a loop is not the same in every lane."""
+    before = loads_of_tensor_memory(source("head_gemm.cuh"))
+    assert len(before) == 4 and set(before) == {"__syncwarp();"}
