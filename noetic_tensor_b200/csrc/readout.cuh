@@ -94,6 +94,7 @@ __device__ __forceinline__ void readout_fold_tile(const ReadoutParams& p, uint32
 #pragma unroll 1
     for (int c = 0; c < kRoBN / 32; c++) {
         uint32_t r[32];
+        __syncwarp();
         tc_ld32(taddr + c * 32, r);
         tc_wait_ld();
         const uint32_t col0 = t * kRoBN + c * 32;
@@ -317,7 +318,9 @@ __global__ void __launch_bounds__(kRoThreads, 1) readout_fwd_kernel(const __grid
         bool ok = true;
         for (uint32_t t = t0; t < t1 && ok; t++) {
             const uint32_t n = t - t0, acc = n & 1u;
-            if (!mbar_wait(bar_acc_full + 8 * acc, (n >> 1) & 1u, &abort_flag)) { ok = false; break; }
+            // the warp goes on, or gives up, as one
+            ok = __all_sync(0xffffffffu, mbar_wait(bar_acc_full + 8 * acc, (n >> 1) & 1u, &abort_flag));
+            if (!ok) break;
             tc_fence_after();
             readout_fold_tile<ROUND, EXTRA>(p, tmem + ((quarter * 32u) << 16) + acc * kRoBN, t, row, live, tok, m, S, W, ztok);
             // this accumulator may be overwritten once all four epilogue warps are done with it
@@ -500,7 +503,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kRoThreads, 1)
             float m = NRL_NEG_INF, S = 0.f, W = 0.f, ztok = __int_as_float(0x7fc00000);
             for (uint32_t t = t0; t < t1 && ok; t++, n++) {
                 const uint32_t acc = n & 1u;
-                if (!mbar_wait(bar_acc_full + 8 * acc, (n >> 1) & 1u, &abort_flag)) { ok = false; break; }
+                // the warp goes on, or gives up, as one
+                ok = __all_sync(0xffffffffu, mbar_wait(bar_acc_full + 8 * acc, (n >> 1) & 1u, &abort_flag));
+                if (!ok) break;
                 tc_fence_after();
                 readout_fold_tile<ROUND, EXTRA>(p, tmem + ((quarter * 32u) << 16) + acc * kRoBN, t, row, live, tok, m, S, W, ztok);
                 tc_fence_before();

@@ -27,3 +27,11 @@ def test_a_warp_comes_together_before_it_loads_tensor_memory():
     """tcgen05.ld is executed by a whole warp (.sync.aligned), and the code before it in a loop is not the same in every lane."""
     before = loads_of_tensor_memory(source("head_gemm.cuh"))
     assert len(before) == 4 and set(before) == {"__syncwarp();"}
+    assert loads_of_tensor_memory(source("readout.cuh")) == ["__syncwarp();"]
+
+
+def test_a_warp_gives_up_a_wait_as_one():
+    """Behind a wait for an accumulator the warp's lanes meet again: one that gave up by itself would leave the others waiting for it."""
+    for name, waits in (("head_gemm.cuh", 1), ("readout.cuh", 2)):
+        lines = [line for line in source(name).splitlines() if "mbar_wait(bar_acc_full" in line]
+        assert len(lines) == waits and all("__all_sync(0xffffffffu, mbar_wait(" in line for line in lines)
