@@ -160,9 +160,10 @@ __device__ __forceinline__ void scale32(float* z, float by) {
 #pragma unroll
     for (int i = 0; i < 32; i += 2) unpack2(mul2(pack2(z[i], z[i + 1]), b2), z[i], z[i + 1]);
 }
-// an arrival on a barrier of either CTA of the pair
+// An arrival on a barrier of either CTA of the pair that hands tensor memory back (mbar_try_wait_pair waits for it). A release at
+// this scope waits for what the thread has stored: the statistics of 2048 x 50264 x 512 took 125 us with one, 100 without.
 __device__ __forceinline__ void mbar_arrive_remote(uint32_t bar_cluster_addr) {
-    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar_cluster_addr) : "memory");
+    asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar_cluster_addr) : "memory");
 }
 // keeps what reads z behind this point
 __device__ __forceinline__ void pin32(float* z) {
@@ -592,7 +593,7 @@ __global__ void __launch_bounds__(kHgThreads, 1)
                 const Item w = item(t);
                 if (w.k0 == w.k1) continue;  // an empty sum: the epilogue writes zeros by itself
                 const uint32_t acc = n & 1u;
-                if (!mbar_wait(bar_acc_empty + 8 * acc, ((n >> 1) & 1u) ^ 1u, &abort_flag)) { ok = false; break; }
+                if (!mbar_wait<PAIR>(bar_acc_empty + 8 * acc, ((n >> 1) & 1u) ^ 1u, &abort_flag)) { ok = false; break; }
                 tc_fence_after();
                 const uint32_t d_tmem = tmem + acc * 256;
 #pragma unroll 2

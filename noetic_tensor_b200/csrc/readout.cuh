@@ -467,7 +467,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kRoThreads, 1)
                 if (!item(g, split, rb, t0, t1)) continue;
                 for (uint32_t t = t0; t < t1 && ok; t++, n++) {
                     const uint32_t acc = n & 1u;
-                    if (!mbar_wait(bar_acc_empty + 8 * acc, ((n >> 1) & 1u) ^ 1u, &abort_flag)) { ok = false; break; }
+                    if (!mbar_wait<true>(bar_acc_empty + 8 * acc, ((n >> 1) & 1u) ^ 1u, &abort_flag)) { ok = false; break; }
                     tc_fence_after();
                     const uint32_t d_tmem = tmem + acc * kRoBN;
                     for (uint32_t kc = 0; kc < kchunks; kc++, it++) {

@@ -13,12 +13,27 @@ namespace nrl {
 constexpr unsigned long long kWaitLimitNs = 2000000000ull;  // 2 s: far beyond any legitimate wait here
 
 // ---- raw PTX wrappers -----------------------------------------------------------------------------
-// Bounded wait: false when the CTA aborted or the limit passed (then the abort flag is raised).
+// as mbar_try_wait, for arrivals from both CTAs of a pair that hand tensor memory back. Relaxed: the tcgen05 fences before the arrival
+// and behind the wait order the accesses to tensor memory, and no other data passes with it
+__device__ __forceinline__ bool mbar_try_wait_pair(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.relaxed.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    return ok != 0;
+}
+// Bounded wait: false when the CTA aborted or the limit passed (then the abort flag is raised). PAIR: mbar_try_wait_pair.
+template <bool PAIR = false>
 __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile uint32_t* abort_flag, unsigned long long limit_ns = kWaitLimitNs) {
-    if (mbar_try_wait(bar, parity)) return true;
+    auto arrived = [&] { return PAIR ? mbar_try_wait_pair(bar, parity) : mbar_try_wait(bar, parity); };
+    if (arrived()) return true;
     const unsigned long long t0 = global_ns();
     for (uint32_t i = 1;; i++) {
-        if (mbar_try_wait(bar, parity)) return true;
+        if (arrived()) return true;
         if ((i & 63u) == 0u) {
             if (*abort_flag) return false;
             if (global_ns() - t0 > limit_ns) {

@@ -35,3 +35,13 @@ def test_a_warp_gives_up_a_wait_as_one():
     for name, waits in (("head_gemm.cuh", 1), ("readout.cuh", 2)):
         lines = [line for line in source(name).splitlines() if "mbar_wait(bar_acc_full" in line]
         assert len(lines) == waits and all("__all_sync(0xffffffffu, mbar_wait(" in line for line in lines)
+
+
+def test_what_crosses_between_the_ctas_of_a_pair_says_so():
+    """Arrivals on the other CTA's barrier, and the waits for them, are ordered for the cluster: the default is the own CTA."""
+    for name in ("tcgen05.cuh", "head_gemm.cuh", "readout.cuh"):
+        for arrival in re.findall(r"mbarrier\.arrive[\w.:]*", source(name)):
+            assert "shared::cluster" not in arrival or re.search(r"\.(relaxed|release)\.cluster\.", arrival), arrival
+    assert re.search(r"mbarrier\.try_wait\.parity\.\w+\.cluster\.", source("tcgen05.cuh"))
+    assert re.findall(r"mbar_wait(<\w+>)?\(bar_acc_empty", source("head_gemm.cuh")) == ["<PAIR>"]
+    assert re.findall(r"mbar_wait(<\w+>)?\(bar_acc_empty", source("readout.cuh")) == ["", "<true>"]  # one CTA, a pair
