@@ -133,6 +133,12 @@ __device__ __forceinline__ void tc_mma_i8_pair(uint32_t d_tmem, uint64_t a_desc,
 __device__ __forceinline__ void stg32(void* p, const uint32_t r[8]) {
     asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]) : "memory");
 }
+// four bytes read once, past L1; not as read-only data: the kernel that wrote them may still run when this one starts
+__device__ __forceinline__ uint32_t ldg4(const void* p) {
+    uint32_t v;
+    asm volatile("ld.global.L1::no_allocate.u32 %0, [%1];" : "=r"(v) : "l"(p));
+    return v;
+}
 __device__ __forceinline__ void ldg32(const void* p, uint32_t r[8]) {
     asm volatile("ld.global.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]) : "l"(p) : "memory");
 }
@@ -195,7 +201,7 @@ struct MaskAhead {
         if constexpr (MASK == kMaskBits) {
             const uint32_t* mp = reinterpret_cast<const uint32_t*>(p.allow) + (uint64_t)caller_row * p.allow_stride + (v >> 5);
 #pragma unroll
-            for (int c = 0; c < 4; c++) raw[c] = live && v + 32 * c < p.vocab ? ldg_stream4(mp + c) : 0u;
+            for (int c = 0; c < 4; c++) raw[c] = live && v + 32 * c < p.vocab ? ldg4(mp + c) : 0u;
         } else if constexpr (MASK == kMaskBytes) {
             const uint32_t here = v + 4 * lane;
             const uint32_t lives = __ballot_sync(0xffffffffu, live);
@@ -206,7 +212,7 @@ struct MaskAhead {
                 const uint8_t* q = mp + (uint64_t)row * p.allow_stride;
                 uint32_t x = 0u;
                 if ((lives >> r & 1u) && here < p.vocab) {  // V is a multiple of 8: a lane's four columns exist or do not
-                    if (p.allow_wide) x = ldg_stream4(q);
+                    if (p.allow_wide) x = ldg4(q);
                     else x = (uint32_t)q[0] | (uint32_t)q[1] << 8 | (uint32_t)q[2] << 16 | (uint32_t)q[3] << 24;
                 }
                 raw[r] = x;
@@ -696,7 +702,7 @@ __global__ void __launch_bounds__(kHgThreads, 1)
                 const float ys = p.zscale * kLog2e * r.xs.x;
                 int32_t token = r.token;
                 if (EPI == kEpiStats && live && p.tokens) {
-                    token = __ldg(p.tokens + r.caller_row);
+                    token = p.tokens[r.caller_row];
                     if ((uint32_t)token >= p.vocab) token = -1;  // no such column, not even past the vocabulary's end in its last tile
                 }
                 float m = -FLT_MAX, S = 0.f, W = 0.f, ytok = __int_as_float(0x7fc00000);

@@ -45,3 +45,9 @@ def test_what_crosses_between_the_ctas_of_a_pair_says_so():
     assert re.search(r"mbarrier\.try_wait\.parity\.\w+\.cluster\.", source("tcgen05.cuh"))
     assert re.findall(r"mbar_wait(<\w+>)?\(bar_acc_empty", source("head_gemm.cuh")) == ["<PAIR>"]
     assert re.findall(r"mbar_wait(<\w+>)?\(bar_acc_empty", source("readout.cuh")) == ["", "<true>"]  # one CTA, a pair
+
+
+def test_kernels_that_start_early_read_nothing_as_read_only_data():
+    """Such a kernel is running before the one that writes its inputs has ended, so they change during its lifetime."""
+    for name in ("head_gemm.cuh", "head_ops.cuh"):
+        assert not re.findall(r"__ldg\(|ldg_stream\w*\(|ld\.global\.nc|__restrict__", source(name)), name
