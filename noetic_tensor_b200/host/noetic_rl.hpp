@@ -563,7 +563,7 @@ inline void head_mask(Args& a, const Tensor* vocab_mask, uint64_t rows, uint64_t
     }
     if (vocab_mask->dtype() != DType::U8) throw std::runtime_error("rl: a U8 allow-mask or I32 words of bits");
     const uint64_t n = numel(vocab_mask->shape());
-    if (n != V && n != rows * V) throw std::runtime_error("rl: mask shape");
+    if (vocab_mask->rank() < 1 || vocab_mask->shape().back() != V || (n != V && n != rows * V)) throw std::runtime_error("rl: mask shape");
     a.allow_mask = vocab_mask->dev();
     a.allow_row_stride = n == V ? 0 : V;
 }

@@ -154,6 +154,21 @@ static void test(Form form, double tau, bool checkpoint) {
     held(twice.grad(hw)->to_vec(), both(t.dw), both(t.ew), "d weight, twice");
 }
 
+// a mask whose last axis is not the vocabulary is refused, not regrouped into rows of V
+static void test_mask_shapes() {
+    const Tensor hx = Tensor::from_f32(x, {S, B, T, d}, dev, DType::BF16), hw = Tensor::from_f32(w, {d, V}, dev, DType::BF16);
+    for (const Shape& shape : {Shape{2, V / 2}, Shape{V, 1}, Shape{2 * N, V / 2}, Shape{V, N}}) {
+        const Tensor vm = Tensor::from_u8(std::vector<uint8_t>(numel(shape), 1), shape, dev);
+        bool refused = false;
+        try {
+            rl::head_token_log_probs(hx, hw, IntTensor::from_data(tok, {S, B, T}), nullptr, false, &vm);
+        } catch (const std::exception& e) {
+            refused = std::string(e.what()).find("mask shape") != std::string::npos;
+        }
+        CHECK(refused, "mask of %zu rows of %zu", shape[0], shape[1]);
+    }
+}
+
 int main() {
     int n = 0;
     if (cudaGetDeviceCount(&n) != cudaSuccess || n == 0) {
@@ -162,6 +177,7 @@ int main() {
     }
     make();
     try {
+        test_mask_shapes();
         for (Form f : {kNone, kBytes, kByteRow, kBits, kBitRow})
             for (double tau : {1.0, 0.7, 1.5})
                 for (bool checkpoint : {false, true}) test(f, tau, checkpoint);
