@@ -626,6 +626,9 @@ int nrl_ce_mean(uint64_t s, uint64_t n, nrl_devptr logp, nrl_devptr keep, nrl_de
  * scale per row as nrl_i8_quantize_rows writes them. The logits are then those of values·scale (products of
  * the exact integers, scaled in f32), normalised by the given row statistics — the forward's on the
  * unrounded states — and d_weights is taken with values·scale.
+ * So the probabilities of this gradient add up to 1 only as far as the rounding leaves the logits alone: it is within 1 % (norm) of the
+ * unrounded one for states of about one size, and off by several times the rounding's own share where one channel is far above the others.
+ * Run the forward on the rounded states (nrl_i8_dequantize_rows) to have the value and the gradient of one function.
  *
  * Limits as nrl_readout_fwd: d and V multiples of 8, 16-byte aligned matrices, compute capability 10.x.
  * A product that gives up a bounded wait (an internal error) writes NaN for what it did not reach. */
