@@ -423,9 +423,9 @@ def reduce_tokens_backward_pairs(reduction, S, B, T, seq_begin, n_seq, pairs, ma
 
 
 class Readout:
-    """Outputs of nrl_readout_fwd (fields are None when not requested)."""
+    """Outputs of nrl_readout_fwd (fields are None when not requested); `rounded`: of logits rounded to bf16."""
 
-    __slots__ = ("logp", "entropy", "rowstats", "status", "logits", "tokens")
+    __slots__ = ("logp", "entropy", "rowstats", "status", "logits", "tokens", "rounded")
 
 
 def _readout_masks(a, V, rows, allow, allow_bits, dev):
@@ -467,6 +467,7 @@ def readout_forward(hidden, weights, *, tokens=None, weights_are_vd=False, round
     a.V, a.d, a.rows, a.temperature = V, d, rows, float(temperature)
     a.hidden, a.weights = _p(hidden), _p(weights)
     out = Readout()
+    out.rounded = round_bf16
     out.logp = out.tokens = None
     if uniforms is not None:
         if tokens is not None or greedy:
@@ -688,7 +689,7 @@ def int8_linear(x, w, dtype=torch.float32):
 def readout_backward(hidden, weights, fwd, *, tokens=None, g_logp=None, g_ent=None, weights_are_vd=False, allow=None, allow_bits=None, temperature=1.0, want_hidden=True,
                      want_weights=True, grad_dtype=torch.bfloat16, add_hidden=None, add_weights=None, workspace=None, hidden_shape=None):
     """(d_hidden, d_weights) of Σ g_logp·logp + Σ g_ent·entropy of the results `fwd` of
-    `readout_scored_forward` or `readout_forward` (their `rowstats` and, with `g_ent`, `entropy`), the
+    `readout_scored_forward` or `readout_forward` (their `rowstats` and, with `g_ent`, `entropy`; not of rounded logits), the
     logits computed again in pieces (nrl_readout_bwd). `hidden`: the bf16 [..., d] of the forward call, or
     an Int8Rows checkpoint of it (d_hidden then has `hidden_shape`, default [rows, d]). Gradients are
     `grad_dtype` (bfloat16 or float32); `add_hidden` / `add_weights` are tensors they are added to in place
@@ -706,6 +707,8 @@ def readout_backward(hidden, weights, fwd, *, tokens=None, g_logp=None, g_ent=No
     V = _readout_weight(weights, d, weights_are_vd, dev)
     if grad_dtype is not torch.bfloat16 and grad_dtype is not torch.float32:
         raise TypeError(f"gradients must be bfloat16 or float32, got {grad_dtype}")
+    if type(fwd) is Readout and fwd.rounded:
+        raise ValueError("fwd: of logits rounded to bf16, which have no gradient here")
     own = type(fwd) is ScoredReadout and fwd.rows == rows and fwd._buf.device == dev
     from_loss = 4 * fwd._g if own and g_logp is None and g_ent is None else 0  # where fwd's gradient of the log-probs lies, 0: not used
     if g_logp is None and g_ent is None and not from_loss:
