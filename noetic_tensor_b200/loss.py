@@ -40,6 +40,8 @@ def _targets(targets, S, N, V, ignore_index=None, check=True):
         raise ValueError("targets [S, B, T]")
     keep = None
     if ignore_index is not None:
+        if t.dtype is not torch.int32 or not -(2**31) <= ignore_index < 2**31:
+            t = t.to(torch.int64)  # a comparison takes the scalar as the tensor's type
         ignored = t == ignore_index
         keep = (~ignored).to(torch.float32)
         t = torch.where(ignored, torch.zeros_like(t), t)
