@@ -652,7 +652,7 @@ typedef struct nrl_readout_bwd_args {
     uint64_t hidden_pitch;     /* bytes between int8 rows, a multiple of 16; 0 or d for bf16 */
     nrl_devptr weights;        /* bf16 [d, V], or [V, d] with W_VD */
     nrl_devptr tokens;         /* i32 [rows], with g_logp */
-    nrl_devptr rowstats;       /* f32 [rows, 4] of the forward */
+    nrl_devptr rowstats;       /* f32 [rows, 4] of the forward (not of one with NRL_READOUT_ROUND_BF16: those normalise other logits) */
     nrl_devptr entropy;        /* f32 [rows] of the forward, with g_ent */
     nrl_devptr g_logp;         /* f32 [rows] or 0 */
     nrl_devptr g_ent;          /* f32 [rows] or 0 */

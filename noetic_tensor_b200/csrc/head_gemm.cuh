@@ -23,8 +23,9 @@
 // Bound: the tensor pipe for the large products (1536 rows, V = 32 000, d = 2048: 130 to 138 us each, the pipe busy 76 to 84 % of the
 // time at the clock that power leaves, 1.53 GHz), HBM for the few-row forms (87 rows, V = 151 936, d = 2048: 98 to 115 us for the
 // weight's 622 MB, which each reads once; d_weights writes as much in 158 us, what a fill takes; 8 bits, one token, V = 128 256,
-// d = 4096: 86 us, 6.1 TB/s). Waits are bounded as in the readout forward; a role that gives up raises the pair's abort flag
-// and the tiles not reached are written as NaN.
+// d = 4096: 86 us, 6.1 TB/s). Waits are bounded as in the readout forward; a role that gives up raises its
+// CTA's abort flag, on which that CTA's other roles stop (the partner's stop at their own limit), and the tiles not reached are
+// written as NaN.
 #pragma once
 #include "tcgen05.cuh"
 
@@ -114,7 +115,7 @@ struct HeadGemm {
     uint32_t out_f32, out_add; // type of `out`; add to what it holds
     uint32_t out_col0;         // kEpiWeight: first column (or first row, with out_row0) of this piece
     uint32_t out_row0;
-    uint32_t wide;             // rows of out are 32-byte aligned (kEpiInt8: n_scale is 16-byte aligned)
+    uint32_t wide;             // rows of out are 32-byte aligned
     uint32_t staged;           // results leave through shared memory and TMA stores (map_out)
     __host__ __device__ static uint32_t acc_rows(uint32_t rows_in_use) { return (rows_in_use + 255u) & ~255u; }
     // kEpiInt8
@@ -150,7 +151,7 @@ __device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, uint32_t sr
     asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];" ::"l"(map), "r"(x), "r"(y), "r"(src) : "memory");
     asm volatile("cp.async.bulk.commit_group;" ::: "memory");
 }
-// the oldest of the warp's kTiles staging tiles may be written again (its store has read it)
+// the warp's staging tile may be written again (its last store has read it)
 __device__ __forceinline__ void stage_free(int lane) {
     if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
     __syncwarp();

@@ -499,7 +499,6 @@ extern "C" int nrl_i8_matmul(const nrl_i8_matmul_args* a, nrl_stream stream) {
     p.out = (void*)a->out;
     p.out_pitch = a->n;
     p.out_f32 = a->dtype == NRL_F32 ? 1u : 0u;
-    p.wide = a->x_scales % 16 == 0 ? 1u : 0u;
     CUtensorMap mw, mx;
     // the extent along K is k, not the pitch: what lies behind a row's k integers is read as zeros
     rc = encode_2d(&mw, true, a->w, a->k, a->n, a->w_pitch, 128, 128);
