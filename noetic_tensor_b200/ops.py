@@ -702,8 +702,11 @@ def readout_backward(hidden, weights, fwd, *, tokens=None, g_logp=None, g_ent=No
         raise ValueError("readout_backward needs CUDA tensors: this library has no CPU path")
     d = quant.d if quant else x.shape[-1]
     if hidden_shape is None:
-        hidden_shape = torch.Size((x.shape[0], d)) if quant else x.shape
+        hidden_shape = (x.shape[0], d) if quant else x.shape
+    hidden_shape = torch.Size(hidden_shape)
     rows = hidden_shape.numel() // d if d else 0
+    if hidden_shape[-1:] != (d,):
+        raise ValueError(f"hidden_shape: [..., {d}], got {tuple(hidden_shape)}")
     V = _readout_weight(weights, d, weights_are_vd, dev)
     if grad_dtype is not torch.bfloat16 and grad_dtype is not torch.float32:
         raise TypeError(f"gradients must be bfloat16 or float32, got {grad_dtype}")
