@@ -511,7 +511,7 @@ int nrl_check_status(nrl_devptr status, uint64_t rows, nrl_stream stream, uint64
  * `logits_out` (optional, bf16 [rows, V]) receives the rounded logits, for comparisons.
  * Needs compute capability 10.x (NRL_E_UNSUPPORTED otherwise) and
  * nrl_readout_workspace_bytes(rows, V, d, flags) bytes of scratch. status[r]: bit 0 no finite logit, bit 1
- * a NaN, bit 2 the kernel gave up a bounded wait (an internal error: outputs of that row are NaN).
+ * a NaN (or a draw from a row whose maximum is +inf), bit 2 the kernel gave up a bounded wait (an internal error: outputs of that row are NaN).
  * Results are bitwise reproducible run to run. */
 enum {
     NRL_READOUT_W_VD = 1u << 0,

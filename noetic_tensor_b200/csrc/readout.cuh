@@ -539,7 +539,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kRoThreads, 1)
 
 // Merge the column ranges of each row in index order (f64, as the row kernels finalise) and write
 // the outputs: rowstats (m, ln Z, 0, 0), entropy = ln Z − W / Z, logp = z_tok − m − ln Z.
-// `greedy`: tokens is an output, the index kept by the first range (in column order) that reached the row's maximum.
+// `greedy`: tokens is an output, the index kept by the first range (in column order) that reached the row's maximum (with sums; those of
+// an infinite maximum are NaN).
 __global__ void readout_finish_kernel(uint64_t rows, uint32_t nsplit, const float* parts, int32_t* tokens, float* logp, float* entropy, float* rowstats, uint8_t* status, uint32_t greedy) {
     const uint64_t row = (uint64_t)blockIdx.x * blockDim.x + threadIdx.x;
     if (row >= rows) return;
@@ -560,7 +561,7 @@ __global__ void readout_finish_kernel(uint64_t rows, uint32_t nsplit, const floa
     int32_t picked = -1;
     if (greedy) {
         for (uint32_t s = 0; s < nsplit && picked < 0; s++)
-            if (pr[s].x == m && pr[s].y > 0.f) picked = (int32_t)__float_as_uint(pr[s].w);
+            if (pr[s].x == m && pr[s].y != 0.f) picked = (int32_t)__float_as_uint(pr[s].w);
         ztok = m;
     }
     uint32_t st = 0u;
@@ -638,15 +639,18 @@ __global__ void __launch_bounds__(256) readout_pick_kernel(ReadoutParams p, cons
     const float nan = __int_as_float(0x7fc00000);
     ReadoutPick pk;
     pk.resid = 0.0; pk.m = m; pk.lnZ = (float)lnZ; pk.slab = -1; pk.pad = 0u;
-    if (st) {
+    auto refuse = [&](uint32_t why) {
         if (lane == 0) {
             tokens[row] = -1;
             if (logp) logp[row] = nan;
             if (entropy) entropy[row] = nan;
             if (rowstats) reinterpret_cast<float4*>(rowstats)[row] = make_float4(nan, nan, nan, nan);
-            if (status) status[row] = (uint8_t)st;
+            if (status) status[row] = (uint8_t)why;
             picks[row] = pk;
         }
+    };
+    if (st) {
+        refuse(st);
         return;
     }
     const double target = (double)uniforms[row] * Z;
@@ -676,6 +680,10 @@ __global__ void __launch_bounds__(256) readout_pick_kernel(ReadoutParams p, cons
     if (slab < 0) {  // rounding left no crossing: the last slab with mass, its last token with mass
         slab = last_mass;
         pk.resid = 1e300;
+    }
+    if (slab < 0) {  // no mass anywhere: the maximum is +inf, and inf − inf is what every share is made of
+        refuse(2u);
+        return;
     }
     pk.slab = slab;
     if (lane == 0) {
