@@ -20,6 +20,11 @@ def _dt(t):
     raise TypeError(f"logits must be float32 or bfloat16, got {t.dtype}")
 
 
+def nearest_f32(x):
+    """The 32-bit float nearest to `x`, as the library takes it."""
+    return C.c_float(x).value
+
+
 def _p(t):
     return 0 if t is None else t.data_ptr()
 
@@ -518,6 +523,11 @@ def _bwd_workspace_bytes(rows, V, d):
     return capi.lib().nrl_readout_bwd_workspace_bytes(rows, V, d)
 
 
+def _no_zero_temperature(temperature):
+    if nearest_f32(temperature) == 0.0:  # the library's word for "no temperature"
+        raise ValueError(f"temperature {temperature}: 0 in 32 bits (must be positive)")
+
+
 class ScoredReadout:
     """Outputs of nrl_readout_scored_fwd, in one buffer: `rowstats` [rows, 4], `status` uint8 [rows] and,
     when requested (else None), `logp`, `entropy`, `ce_g_logp` [rows] and `ce_loss` [seeds]."""
@@ -563,6 +573,7 @@ def readout_scored_forward(hidden, weights, *, tokens=None, scored=None, want_en
     d, n = hidden.shape[-1], hidden.numel()
     rows = n // d if d else 0
     V = _readout_weight(weights, d, weights_are_vd, dev)
+    _no_zero_temperature(temperature)
     xp, tp, sp = _need_flat(hidden, torch.bfloat16, n, "hidden", dev), _need_flat(tokens, torch.int32, rows, "tokens", dev), _need_flat(scored, torch.float32, rows, "scored", dev)
     out = ScoredReadout(rows, tokens is not None, want_entropy, ce_seeds, dev)
     buf = out._buf.data_ptr()
@@ -710,6 +721,7 @@ def readout_backward(hidden, weights, fwd, *, tokens=None, g_logp=None, g_ent=No
     V = _readout_weight(weights, d, weights_are_vd, dev)
     if grad_dtype is not torch.bfloat16 and grad_dtype is not torch.float32:
         raise TypeError(f"gradients must be bfloat16 or float32, got {grad_dtype}")
+    _no_zero_temperature(temperature)
     if type(fwd) is Readout and fwd.rounded:
         raise ValueError("fwd: of logits rounded to bf16, which have no gradient here")
     own = type(fwd) is ScoredReadout and fwd.rows == rows and fwd._buf.device == dev

@@ -113,8 +113,8 @@ class Head:
     it the loss, NaN, as does a position with no allowed token."""
 
     def __init__(self, hidden, weight, temperature=1.0, vocab_mask=None, weight_is_vd=False, checkpoint=False, grad_dtype=torch.bfloat16):
-        if not (0.0 < temperature < float("inf")):
-            raise ValueError(f"tempered_logits: temperature {temperature} (must be positive)")
+        if not (0.0 < ops.nearest_f32(temperature) < float("inf")):
+            raise ValueError(f"tempered_logits: temperature {temperature} (must be positive, in 32 bits too)")
         if vocab_mask is not None and vocab_mask.dtype not in (torch.uint8, torch.bool, torch.int32):
             raise ValueError("Head: vocab_mask is a uint8/bool allow-mask or int32 words of bits")
         self.V = weight.shape[0 if weight_is_vd else 1]
