@@ -701,7 +701,8 @@ inline Tensor head_logits(const Tensor& hidden, const Int8Weight& weight, DType 
 // head_sample_categorical under the same mask and temperature is scored with.
 inline Tensor head_token_log_probs(const Tensor& hidden, const Tensor& weight, const IntTensor& tokens, Tensor* entropy = nullptr, bool round_bf16 = false, const Tensor* vocab_mask = nullptr,
                                    double temperature = 1.0, bool checkpoint = false) {
-    if (!(temperature > 0.0 && std::isfinite(temperature))) throw std::runtime_error("tempered_logits: temperature must be > 0");
+    // in 32 bits, as the library takes it: 0 would mean "no temperature" there
+    if (!((float)temperature > 0.f && std::isfinite((float)temperature))) throw std::runtime_error("tempered_logits: temperature must be > 0");
     if (hidden.dtype() != DType::BF16 || weight.dtype() != DType::BF16) throw std::runtime_error("head_token_log_probs: BF16 hidden states and weight");
     if (hidden.rank() < 1 || weight.rank() != 2 || weight.shape()[0] != hidden.shape().back()) throw std::runtime_error("head_token_log_probs: hidden [.., d], weight [d, V]");
     const Shape lead(hidden.shape().begin(), hidden.shape().end() - 1);
@@ -750,7 +751,7 @@ inline Tensor head_token_log_probs(const Tensor& hidden, const Tensor& weight, c
 inline IntTensor head_sample_categorical(const Tensor& hidden, const Tensor& weight, const Tensor& uniforms, const Tensor* vocab_mask = nullptr, Tensor* logp = nullptr,
                                          Tensor* entropy = nullptr, double temperature = 1.0) {
     if (!(temperature >= 0.0 && std::isfinite(temperature))) throw std::runtime_error("sample_categorical: temperature (must be >= 0)");
-    const bool greedy = temperature == 0.0;
+    const bool greedy = (float)temperature == 0.f;  // what is 0 in 32 bits too: the library would take it for 1
     if (hidden.dtype() != DType::BF16 || weight.dtype() != DType::BF16) throw std::runtime_error("head_sample_categorical: BF16 hidden states and weight");
     if (hidden.rank() < 1 || weight.rank() != 2 || weight.shape()[0] != hidden.shape().back()) throw std::runtime_error("head_sample_categorical: hidden [.., d], weight [d, V]");
     const Shape lead(hidden.shape().begin(), hidden.shape().end() - 1);

@@ -409,6 +409,8 @@ def head_token_log_probs(hidden, weight, tokens, round_bf16=False, vocab_mask=No
     rollout drawn by `head_sample_categorical` under the same mask and temperature is scored with.
     Returns (log-probs [...], entropies [...]). Untracked; needs a compute-capability-10 device."""
     lead = hidden.shape[:-1]
+    if not (0.0 < ops.nearest_f32(temperature) < float("inf")):
+        raise ValueError(f"tempered_logits: temperature {temperature} (must be positive, in 32 bits too)")
     allow, bits = _vocab_mask_args(vocab_mask, weight.shape[1])
     o = ops.readout_forward(hidden.reshape(-1, hidden.shape[-1]).contiguous(), weight, tokens=_token_ids(tokens.reshape(-1), weight.shape[1]), round_bf16=round_bf16, allow=allow, allow_bits=bits,
                             temperature=temperature)
@@ -429,7 +431,7 @@ def head_sample_categorical(hidden, weight, uniforms, vocab_mask=None, temperatu
     x = hidden.reshape(-1, hidden.shape[-1]).contiguous()
     if not (temperature >= 0.0 and temperature == temperature and temperature != float("inf")):
         raise ValueError("sample_categorical: temperature (must be >= 0)")
-    if uniforms is None or temperature == 0.0:
+    if uniforms is None or ops.nearest_f32(temperature) == 0.0:  # the library takes 0 for no temperature
         o = ops.readout_forward(x, weight, greedy=True, allow=allow, allow_bits=bits)
     else:
         o = ops.readout_forward(x, weight, uniforms=uniforms.reshape(-1).contiguous(), allow=allow, allow_bits=bits, temperature=temperature)

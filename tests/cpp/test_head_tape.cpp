@@ -169,6 +169,21 @@ static void test_mask_shapes() {
     }
 }
 
+// a temperature that is 0 in 32 bits: no temperature to score with, and the first maximum when drawing
+static void test_temperatures() {
+    const Tensor hx = Tensor::from_f32(x, {S, B, T, d}, dev, DType::BF16), hw = Tensor::from_f32(w, {d, V}, dev, DType::BF16), u = Tensor::from_f32(std::vector<float>(N, 0.5f), {S, B, T}, dev);
+    for (double tau : {0.0, 1e-50}) {
+        bool refused = false;
+        try {
+            rl::head_token_log_probs(hx, hw, IntTensor::from_data(tok, {S, B, T}), nullptr, false, nullptr, tau);
+        } catch (const std::exception& e) {
+            refused = std::string(e.what()).find("temperature") != std::string::npos;
+        }
+        CHECK(refused, "temperature %g", tau);
+        CHECK(rl::head_sample_categorical(hx, hw, u, nullptr, nullptr, nullptr, tau).data == rl::head_sample_categorical(hx, hw, u, nullptr, nullptr, nullptr, 1e-3).data, "temperature %g", tau);
+    }
+}
+
 int main() {
     int n = 0;
     if (cudaGetDeviceCount(&n) != cudaSuccess || n == 0) {
@@ -178,6 +193,7 @@ int main() {
     make();
     try {
         test_mask_shapes();
+        test_temperatures();
         for (Form f : {kNone, kBytes, kByteRow, kBits, kBitRow})
             for (double tau : {1.0, 0.7, 1.5})
                 for (bool checkpoint : {false, true}) test(f, tau, checkpoint);
