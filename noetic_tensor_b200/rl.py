@@ -97,7 +97,7 @@ class Head:
     tempered ones (src/nn/rl.rs:475-486); the mask is a uint8/bool allow-mask [..., V] or [1, V], or int32
     words of one bit per token. With `checkpoint` a loss keeps the hidden states for its backward as 8-bit
     integers with a scale per position (half the memory) instead of keeping `hidden`. `grad_dtype`:
-    bfloat16 or float32.
+    bfloat16 or float32 (d(logits) is rounded to bf16 on the way to either).
 
     The checkpoint's gradient takes the logits of the rounded states and the normaliser of the unrounded ones, those of
     the loss's value, so its probabilities add up to 1 only as far as the rounding leaves the logits alone. Hidden
